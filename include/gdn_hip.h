@@ -409,6 +409,34 @@ int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_tensor* k_cach
                                    int32_t num_splits, float scale, void* stream);
 
 /*
+ * Append of new tokens to the paged caches, with the position rotation of q
+ * and k on the way (the reference rotates in torch,
+ * layers/rotary_embedding.py:20-31, and writes no cache).
+ *   k, v (T, Hkv, D); k_cache, v_cache (num_blocks, page, Hkv, D), written in
+ *   place; block_tables (N, max_blocks) i32|i64; context_lens (N,) the lengths
+ *   with the new tokens, as the paged attention ops take them; q, out
+ *   (T, Hq, D), both or neither; cu_seqlens (N+1,), or NULL for one token per
+ *   sequence (T = N); cos, sin (P, rot / 2) fp32, both or neither.
+ * bf16 or fp16 throughout, D = 64, 128 or 256, rot a multiple of 16 up to D;
+ * unit inner strides, 16-byte aligned rows.
+ * Token i of sequence n sits at position p = context_lens[n] - len_n + i, in
+ * slot p % page of block block_tables[n][p / page].  With (a, b) the dims
+ * (j, j + rot / 2), or (2 j, 2 j + 1) when interleaved != 0, j < rot / 2, of q
+ * and k: (a, b) <- (a cos[p][j] - b sin[p][j], b cos[p][j] + a sin[p][j]) in
+ * fp32, rounded once; the other dims and v are copied.  out may be q itself.
+ * A token in no sequence, or at a position below 0, past the table's
+ * max_blocks * page or past the P rows of the rotation, is not appended and
+ * its out row is zero; a table entry outside [0, num_blocks) is not written
+ * either (its tokens' out rows are rotated as usual).  Nothing else in the
+ * caches is touched.  The tokens' slots must be distinct.
+ * GDN_ERR_RANGE when max_blocks * page >= 2^31.
+ */
+int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+                    const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
+                    gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos, const gdn_tensor* sin,
+                    int32_t interleaved, void* stream);
+
+/*
  * Measurement utility, no counterpart in the reference: copies nbytes (a
  * multiple of 16; both pointers 16-byte aligned) from src to dst with a plain
  * streaming kernel (16-byte non-temporal loads and stores, grid-stride loop

@@ -10,6 +10,7 @@ from .full_attention import (
     flash_attention_prefill,
     paged_flash_attention_decode,
     paged_flash_attention_prefill,
+    paged_kv_append,
 )
 from .norm import RMSNormGated
 from .gated_delta_rule import (
@@ -26,6 +27,7 @@ __all__ = [
     "flash_attention_prefill",
     "paged_flash_attention_decode",
     "paged_flash_attention_prefill",
+    "paged_kv_append",
     "chunk_gated_delta_rule_fwd",
     "gated_delta_net_decode_step",
     "recurrent_gated_delta_rule",

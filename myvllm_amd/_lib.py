@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "paged_attention_decode_workspace_size",
     "paged_attention_decode",
     "paged_attention_decode_noalloc",
+    "paged_kv_append",
     "gdn_hbm_copy",
     "gdn_strerror",
     "gdn_abi_version",
@@ -165,6 +166,8 @@ def load() -> ctypes.CDLL:
         lib.paged_attention_decode.restype = ctypes.c_int
         lib.paged_attention_decode.argtypes = [_PT] * 7 + [ctypes.c_int32, ctypes.c_float, ctypes.c_void_p]
         lib.paged_attention_decode_noalloc.restype = ctypes.c_int
+        lib.paged_kv_append.restype = ctypes.c_int
+        lib.paged_kv_append.argtypes = [_PT] * 11 + [ctypes.c_int32, ctypes.c_void_p]
         lib.gdn_hbm_copy.restype = ctypes.c_int
         lib.gdn_hbm_copy.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
                                      ctypes.c_void_p]

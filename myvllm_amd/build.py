@@ -28,6 +28,7 @@ SOURCES = [
     "gdn_norm.hip",
     "linear.hip",
     "attention.hip",
+    "kv_append.hip",
     "hbm_copy.hip",
     "gdn_capi.cpp",
 ]

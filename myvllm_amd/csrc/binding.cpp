@@ -180,6 +180,7 @@ typedef Entry<15, 6, int32_t, float> PagedDecodeNoalloc;
 typedef Entry<16, 13, int32_t, float, float> DecodeFusedNorm;
 typedef Entry<17, 3> Linear;
 typedef Entry<18, 10, float, int32_t, int32_t> ChunkPrefillSplitEx;
+typedef Entry<19, 11, int32_t> KvAppend;
 typedef Size<0, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> ChunkPrefillSize;
 typedef Size<1, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> PagedPrefillSize;
 typedef Size<2, int64_t, int64_t, int64_t, int32_t> PagedDecodeSize;
@@ -210,6 +211,7 @@ const Bound kBound[] = {
     GDN_BOUND("paged_attention_prefill_split", PagedPrefillSplit),
     GDN_BOUND("paged_attention_decode", PagedDecode),
     GDN_BOUND("paged_attention_decode_noalloc", PagedDecodeNoalloc),
+    GDN_BOUND("paged_kv_append", KvAppend),
     GDN_BOUND("gdn_chunk_prefill_workspace_size", ChunkPrefillSize),
     GDN_BOUND("paged_attention_prefill_workspace_size", PagedPrefillSize),
     GDN_BOUND("paged_attention_decode_workspace_size", PagedDecodeSize),

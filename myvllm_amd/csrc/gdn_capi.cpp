@@ -52,6 +52,11 @@ hipError_t attn_paged_decode_launch(const gdn_tensor* q, const gdn_tensor* kc, c
                                     int32_t splits, float scale, hipStream_t st);
 hipError_t attn_decode_scratch(hipStream_t st, float** ptr);
 int32_t attn_decode_start_price();
+int64_t paged_kv_append_waves(int64_t T, int64_t rows, int64_t D);
+hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* kc, gdn_tensor* vc,
+                                  const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* q, gdn_tensor* out,
+                                  const gdn_tensor* cu, const gdn_tensor* cos, const gdn_tensor* sin, int interleaved,
+                                  hipStream_t st);
 hipError_t hbm_stream_copy_launch(const void* src, void* dst, int64_t nbytes, int32_t blocks, hipStream_t st);
 
 #define GDN_EXPORT extern "C" __attribute__((visibility("default")))
@@ -718,6 +723,66 @@ GDN_EXPORT int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_ten
   }
   return launch_rc(attn_paged_decode_launch(q, k_cache, v_cache, block_tables, context_lens, out, ws, num_splits,
                                             scale, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+                               const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
+                               gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos,
+                               const gdn_tensor* sin, int32_t interleaved, void* stream) {
+  GDN_TRY(check_desc(k, 3));
+  GDN_TRY(check_desc(v, 3));
+  GDN_TRY(check_desc(block_tables, 2));
+  const int64_t T = k->shape[0], Hkv = k->shape[1], D = k->shape[2], N = block_tables->shape[0];
+  GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, N));
+  for (int i = 0; i < 3; ++i)
+    if (v->shape[i] != k->shape[i]) return GDN_ERR_SHAPE;
+  if (k_cache->shape[2] != Hkv || k_cache->shape[3] != D) return GDN_ERR_SHAPE;
+  if (Hkv <= 0) return GDN_ERR_HEADS;
+  if (k->dtype != GDN_DTYPE_BF16 && k->dtype != GDN_DTYPE_F16) return GDN_ERR_DTYPE;
+  if (v->dtype != k->dtype || k_cache->dtype != k->dtype || v_cache->dtype != k->dtype) return GDN_ERR_DTYPE;
+  if (D != 64 && D != 128 && D != 256) return GDN_ERR_HEAD_DIM;
+  if (k->stride[2] != 1 || v->stride[2] != 1 || k_cache->stride[3] != 1 || v_cache->stride[3] != 1)
+    return GDN_ERR_STRIDE;
+  if (T > 0 && (!vec_ok(k, 16) || !vec_ok(v, 16))) return GDN_ERR_ALIGN;
+  if (numel(k_cache) > 0 && (!vec_ok(k_cache, 16) || !vec_ok(v_cache, 16))) return GDN_ERR_ALIGN;
+  int64_t Hq = 0;
+  if (!q != !out) return GDN_ERR_NULL;
+  if (q) {
+    GDN_TRY(check_desc(q, 3));
+    GDN_TRY(check_desc(out, 3));
+    Hq = q->shape[1];
+    if (q->shape[0] != T || q->shape[2] != D) return GDN_ERR_SHAPE;
+    for (int i = 0; i < 3; ++i)
+      if (out->shape[i] != q->shape[i]) return GDN_ERR_SHAPE;
+    if (Hq <= 0) return GDN_ERR_HEADS;
+    if (q->dtype != k->dtype || out->dtype != k->dtype) return GDN_ERR_DTYPE;
+    if (q->stride[2] != 1 || out->stride[2] != 1) return GDN_ERR_STRIDE;
+    if (T > 0 && (!vec_ok(q, 16) || !vec_ok(out, 16))) return GDN_ERR_ALIGN;
+  }
+  if (cu_seqlens) {
+    GDN_TRY(check_desc(cu_seqlens, 1));
+    if (cu_seqlens->shape[0] != N + 1) return GDN_ERR_SHAPE;
+    if (!is_index(cu_seqlens->dtype)) return GDN_ERR_DTYPE;
+    if (cu_seqlens->stride[0] != 1) return GDN_ERR_STRIDE;
+  } else if (T != N) {
+    return GDN_ERR_SHAPE;
+  }
+  if (!cos != !sin) return GDN_ERR_NULL;
+  if (cos) {
+    GDN_TRY(check_desc(cos, 2));
+    GDN_TRY(check_desc(sin, 2));
+    const int64_t half = cos->shape[1];
+    if (sin->shape[0] != cos->shape[0] || sin->shape[1] != half || half <= 0 || half % 8 != 0 || 2 * half > D)
+      return GDN_ERR_SHAPE;
+    if (cos->dtype != GDN_DTYPE_F32 || sin->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
+    if (cos->stride[1] != 1 || sin->stride[1] != 1) return GDN_ERR_STRIDE;
+    if (numel(cos) > 0 && (!vec_ok(cos, 16) || !vec_ok(sin, 16))) return GDN_ERR_ALIGN;
+  }
+  if (block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31)) return GDN_ERR_RANGE;
+  if (Hq + 2 * Hkv > kMaxGrid / 2 || T > kMaxGrid / 2 || paged_kv_append_waves(T, Hq + 2 * Hkv, D) > kMaxGrid / 2)
+    return GDN_ERR_RANGE;
+  return launch_rc(paged_kv_append_launch(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos,
+                                          sin, interleaved, reinterpret_cast<hipStream_t>(stream)));
 }
 
 GDN_EXPORT int gdn_hbm_copy(const void* src, void* dst, int64_t nbytes, int32_t blocks, void* stream) {

@@ -252,3 +252,51 @@ def paged_flash_attention_prefill(
         _lib.call("paged_attention_prefill", q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens, o,
                   int(max_seqlen), float(scale))
     return _finish(out, o)
+
+
+def paged_kv_append(
+    q: torch.Tensor | None,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    interleaved: bool = False,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Puts the new tokens' k, v (T, Hkv, D) into the paged caches and rotates
+    q and k on the way: the step before the paged attention ops, with their
+    tables and lengths.  ``context_lens`` (N,) counts the new tokens, so token i
+    of sequence n sits at position ``context_lens[n] - len_n + i``; without
+    ``cu_seqlens`` every sequence has one token (a decode step).
+
+    ``cos`` and ``sin`` (positions, rot / 2), fp32, turn the first ``rot`` dims
+    of q and k (halves ``(j, j + rot / 2)`` as the reference's
+    ``layers/rotary_embedding.py:20-31``, or neighbours ``(2 j, 2 j + 1)`` when
+    ``interleaved``); without them nothing is rotated.  Returns the rotated q
+    (None for ``q=None``), into ``out`` where given, which may be q itself.
+
+    A token in no sequence or at a position without a table column or a row of
+    the rotation is not appended and its row of q is zero; table entries
+    outside ``[0, num_blocks)`` are not written.  No host sync.  The caches are
+    written where they lie, so their rows must be 16-byte aligned."""
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
+    if q is None and out is not None:
+        raise ValueError("out is the rotated q's: none without q")
+    dev = _lib.require_device(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
+    k, v = _lib.vec16(k), _lib.vec16(v)
+    cos, sin = (None if t is None else _lib.vec16(t) for t in (cos, sin))
+    o = None
+    if q is not None:
+        # (rows aligned already are rotated where they lie when out is q)
+        o = _out_for(out, q.shape, q.dtype, dev)
+        q = _lib.vec16(q)
+    _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
+              int(bool(interleaved)))
+    return None if o is None else _finish(out, o)

@@ -116,3 +116,44 @@ def attention_loop_ref(q, k, v, scale, pos, causal):
             for dv in range(Dv):
                 out[i, h, dv] = sum(w[t] * float(v[keys[t], kh, dv]) for t in range(len(keys))) / z
     return out
+
+
+def rotate_ref(x, cos, sin, interleaved=False):
+    """x (n, H, D) with the first 2 * cos.shape[1] dims turned by row i of
+    cos, sin (n, rot / 2): halves (``layers/rotary_embedding.py:20-31``) or
+    neighbours; fp64."""
+    x = x.double().clone()
+    half = cos.shape[1]
+    a, b = (slice(0, 2 * half, 2), slice(1, 2 * half, 2)) if interleaved else (slice(0, half), slice(half, 2 * half))
+    xa, xb, c, s = x[..., a].clone(), x[..., b].clone(), cos.double()[:, None], sin.double()[:, None]
+    x[..., a] = xa * c - xb * s
+    x[..., b] = xb * c + xa * s
+    return x
+
+
+def paged_kv_append_ref(q, k, v, k_cache, v_cache, block_tables, context_lens, cu_seqlens=None, cos=None, sin=None,
+                        interleaved=False):
+    """Token by token: token i of sequence n to position ctx_n - len_n + i.
+    Writes the fp64 ``k_cache``, ``v_cache`` in place; returns q rotated (fp64,
+    rows of tokens without a position zero)."""
+    bs = k_cache.shape[1]
+    N = block_tables.shape[0]
+    cu = list(range(N + 1)) if cu_seqlens is None else [int(c) for c in cu_seqlens]
+    limit = block_tables.shape[1] * bs
+    if cos is not None:
+        limit = min(limit, cos.shape[0])
+    out = torch.zeros(k.shape[0], 0 if q is None else q.shape[1], k.shape[2], dtype=torch.float64)
+    for n in range(N):
+        for t in range(cu[n], cu[n + 1]):
+            p = int(context_lens[n]) - cu[n + 1] + t
+            if not 0 <= p < limit:
+                continue
+            turn = (lambda x: rotate_ref(x[t:t + 1], cos[p:p + 1], sin[p:p + 1], interleaved)[0]) \
+                if cos is not None else (lambda x: x[t].double())
+            if q is not None:
+                out[t] = turn(q)
+            blk = int(block_tables[n, p // bs])
+            if 0 <= blk < k_cache.shape[0]:
+                k_cache[blk, p % bs] = turn(k)
+                v_cache[blk, p % bs] = v[t].double()
+    return None if q is None else out
