@@ -1,0 +1,127 @@
+// What the full-attention kernels share: the MFMA shapes per 16-bit type, the
+// transposed LDS read, key and value rows of packed and paged sources.
+#pragma once
+
+#include "gdn_common.h"
+
+namespace {
+
+template <typename T> struct Mma;
+template <> struct Mma<bf16_t> {
+  typedef bf16x8 v8;
+  typedef bf16x4 v4;
+  static GDN_DEVICE f32x16 m32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static GDN_DEVICE f32x4 m16k32(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static GDN_DEVICE f32x4 m16k16(v4 a, v4 b, f32x4 c) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mma<f16_t> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+  static GDN_DEVICE f32x16 m32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static GDN_DEVICE f32x4 m16k32(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static GDN_DEVICE f32x4 m16k16(v4 a, v4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short __attribute__((address_space(3))) lds_short;
+typedef s16x4_t __attribute__((address_space(3))) lds_s16x4_t;
+
+// ds_read_b64_tr_b16: in each 16-lane group, lane i supplies the address of
+// 4 consecutive 16-bit elements of row (i >> 2), columns 4 (i & 3) .. +3, of
+// a 4 x 16 block, and receives column i of that block (rows 0..3).
+template <typename V4> GDN_DEVICE V4 tr4(const void* p) {
+  return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p)));
+}
+
+GDN_DEVICE float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max(x[l], x[l ^ 32]) in every lane l: one v_permlane32_swap of x with
+// itself (lanes 0..31 of one copy trade places with lanes 32..63 of the
+// other, so each lane then holds both of the pair's values), no LDS round
+// trip as a ds_bpermute would take.  (The two results are copied to scalars
+// before they are reinterpreted: this clang reads the first element of the
+// vector for __builtin_bit_cast(float, sw[1]).)  The maximum is a select:
+// fmaxf would first quiet both operands, two more instructions on the
+// softmax's dependency chain (the scores are never NaN).
+GDN_DEVICE float max_lane_pair32(float x) {
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t ua = sw[0], ub = sw[1];
+  const float a = __builtin_bit_cast(float, ua), b = __builtin_bit_cast(float, ub);
+  return a > b ? a : b;
+}
+
+GDN_DEVICE int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// An index at a wave-uniform position read through the scalar data cache (a
+// constant-address-space load): its wait is on the scalar/LDS counter, so it
+// does not drain the vector loads in flight.  Only for read-only inputs.
+typedef const int32_t __attribute__((address_space(4))) * const_i32_ptr;
+typedef const int64_t __attribute__((address_space(4))) * const_i64_ptr;
+GDN_DEVICE int64_t load_index_scalar(const void* p, int64_t i, bool is64) {
+  return is64 ? __builtin_bit_cast(const_i64_ptr, p)[i] : (int64_t)__builtin_bit_cast(const_i32_ptr, p)[i];
+}
+
+// Row j of a key or value source: packed varlen rows (row s0 + j) or paged
+// rows (block table[n][j / page], slot j % page).  nullptr past the valid
+// range or for a table entry outside [0, num_blocks): such rows read as zero.
+struct KvSource {
+  const char* base;
+  int64_t sb, st, sh;  // byte strides: block (paged), row, head
+};
+
+struct PagedTable {
+  const void* table;
+  int64_t row_stride, cols, num_blocks;
+  int32_t page;
+  bool is64;
+};
+
+template <bool PAGED>
+GDN_DEVICE const char* kv_row(const KvSource& s, const PagedTable& tb, int64_t n, int64_t s0, int64_t j, int kvh) {
+  if (PAGED) {
+    const int64_t col = j / tb.page;
+    if (col >= tb.cols) return nullptr;
+    const int64_t blk = load_index(tb.table, n * tb.row_stride + col, tb.is64);
+    if (blk < 0 || blk >= tb.num_blocks) return nullptr;
+    return s.base + blk * s.sb + (j - col * tb.page) * s.st + kvh * s.sh;
+  } else {
+    return s.base + (s0 + j) * s.st + kvh * s.sh;
+  }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+KvSource kv_source(const gdn_tensor* t, bool paged) {
+  const int64_t es = t->dtype == GDN_DTYPE_F32 ? 4 : 2;
+  KvSource s;
+  s.base = reinterpret_cast<const char*>(t->data);
+  if (paged) {
+    s.sb = t->stride[0] * es;
+    s.st = t->stride[1] * es;
+    s.sh = t->stride[2] * es;
+  } else {
+    s.sb = 0;
+    s.st = t->stride[0] * es;
+    s.sh = t->stride[1] * es;
+  }
+  return s;
+}
+
+PagedTable paged_table(const gdn_tensor* tab, const gdn_tensor* kc) {
+  PagedTable p;
+  p.table = tab->data;
+  p.row_stride = tab->stride[0];
+  p.cols = tab->shape[1];
+  p.num_blocks = kc->shape[0];
+  p.page = (int32_t)kc->shape[1];
+  p.is64 = tab->dtype == GDN_DTYPE_I64;
+  return p;
+}
+
+int heads_per_group(int R) { return R % 4 == 0 ? 4 : (R % 2 == 0 ? 2 : 1); }
+
+}  // namespace
