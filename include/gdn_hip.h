@@ -409,6 +409,53 @@ int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_tensor* k_cach
                                    int32_t num_splits, float scale, void* stream);
 
 /*
+ * The three attention ops with another form of scores (no counterpart in the
+ * reference).  With x = scale q.k of the query at position i and the key at j:
+ *   softcap > 0: x <- softcap tanh(x / softcap), softcap at most 4096;
+ *   slopes (Hq,) fp32: x <- x - slopes[h] |i - j| for query head h;
+ *   prefix_lens (N,) i32|i64, causal only: keys j < prefix_lens[n] are visible
+ *   to every query of sequence n, the others as ever (j <= i).
+ * softcap 0 and NULL leave each of them out.  All else is as for the plain ops
+ * above: arguments, head dims (64, 128 or 256), errors, the workspaces of the
+ * paged ones (NULL: the prefill is not split) and their sizes.  GDN_ERR_ARG for
+ * a softcap out of range (the tanh is within 2e-7 softcap) and for prefix_lens
+ * without causal.
+ */
+int flash_attention_varlen_scored(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v,
+                                  const gdn_tensor* cu_seqlens, gdn_tensor* out, const gdn_tensor* slopes,
+                                  const gdn_tensor* prefix_lens, int64_t max_seqlen, float scale, float softcap,
+                                  int32_t causal, void* stream);
+int paged_attention_prefill_scored(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                   const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                   const gdn_tensor* cu_seqlens, gdn_tensor* out, gdn_tensor* workspace,
+                                   const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_t max_seqlen,
+                                   float scale, float softcap, void* stream);
+int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                  const gdn_tensor* block_tables, const gdn_tensor* context_lens, gdn_tensor* out,
+                                  gdn_tensor* workspace, const gdn_tensor* slopes, int32_t num_splits, float scale,
+                                  float softcap, void* stream);
+
+/*
+ * paged_attention_decode for sequences that begin with the same keys (no
+ * counterpart in the reference): the same result, with those keys read once
+ * per group.
+ *   prefix_lens (G,) i32|i64; cu_groups (G+1,) i32|i64, non-decreasing, or NULL
+ *   for one group (G = 1): the sequences [cu_groups[g], cu_groups[g + 1]) hold
+ *   the same first prefix_lens[g] keys and values.  They are read through the
+ *   block table of the first of them that is that long; a shorter sequence, and
+ *   one in no group, is read through its own table alone.
+ *   num_splits 2..256, as for paged_attention_decode, for each sequence's own
+ *   keys.  workspace: 1-D fp32, 16-byte aligned, overwritten, of
+ *   paged_attention_decode_shared_workspace_size elements.
+ */
+int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_q_heads,
+                                                     int64_t num_kv_heads, int64_t head_dim, int32_t num_splits);
+int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                  const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                  const gdn_tensor* prefix_lens, const gdn_tensor* cu_groups, gdn_tensor* out,
+                                  gdn_tensor* workspace, int32_t num_splits, float scale, void* stream);
+
+/*
  * Append of new tokens to the paged caches, with the position rotation of q
  * and k on the way (the reference rotates in torch,
  * layers/rotary_embedding.py:20-31, and writes no cache).

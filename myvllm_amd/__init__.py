@@ -9,6 +9,7 @@ from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .full_attention import (
     flash_attention_prefill,
     paged_flash_attention_decode,
+    paged_flash_attention_decode_shared,
     paged_flash_attention_prefill,
     paged_kv_append,
 )
@@ -26,6 +27,7 @@ __all__ = [
     "chunk_gated_delta_rule",
     "flash_attention_prefill",
     "paged_flash_attention_decode",
+    "paged_flash_attention_decode_shared",
     "paged_flash_attention_prefill",
     "paged_kv_append",
     "chunk_gated_delta_rule_fwd",

@@ -58,6 +58,11 @@ EXPORTED_SYMBOLS = (
     "paged_attention_decode_workspace_size",
     "paged_attention_decode",
     "paged_attention_decode_noalloc",
+    "flash_attention_varlen_scored",
+    "paged_attention_prefill_scored",
+    "paged_attention_decode_scored",
+    "paged_attention_decode_shared",
+    "paged_attention_decode_shared_workspace_size",
     "paged_kv_append",
     "gdn_hbm_copy",
     "gdn_strerror",
@@ -166,6 +171,16 @@ def load() -> ctypes.CDLL:
         lib.paged_attention_decode.restype = ctypes.c_int
         lib.paged_attention_decode.argtypes = [_PT] * 7 + [ctypes.c_int32, ctypes.c_float, ctypes.c_void_p]
         lib.paged_attention_decode_noalloc.restype = ctypes.c_int
+        F, I, L, P = ctypes.c_float, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+        for fn, types in (
+            ("flash_attention_varlen_scored", [_PT] * 7 + [L, F, F, I, P]),
+            ("paged_attention_prefill_scored", [_PT] * 10 + [L, F, F, P]),
+            ("paged_attention_decode_scored", [_PT] * 8 + [I, F, F, P]),
+            ("paged_attention_decode_shared", [_PT] * 9 + [I, F, P]),
+        ):
+            getattr(lib, fn).restype, getattr(lib, fn).argtypes = ctypes.c_int, types
+        lib.paged_attention_decode_shared_workspace_size.restype = L
+        lib.paged_attention_decode_shared_workspace_size.argtypes = [L] * 5 + [I]
         lib.paged_kv_append.restype = ctypes.c_int
         lib.paged_kv_append.argtypes = [_PT] * 11 + [ctypes.c_int32, ctypes.c_void_p]
         lib.gdn_hbm_copy.restype = ctypes.c_int

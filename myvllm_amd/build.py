@@ -28,16 +28,18 @@ SOURCES = [
     "gdn_norm.hip",
     "linear.hip",
     "attention.hip",
+    "attention_scored.hip",
+    "attention_shared.hip",
     "kv_append.hip",
     "hbm_copy.hip",
     "gdn_capi.cpp",
 ]
 
 ARCH = "gfx950"
-# Per-source flags.  attention.hip: keep MFMA accumulators in architectural
+# Per-source flags.  attention*.hip: keep MFMA accumulators in architectural
 # VGPRs; with the default AGPR form the D=256 prefill tile (128 accumulator
 # registers) was shuttled between AGPRs and VGPRs on every key tile.
-SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in SOURCES if s.startswith("attention")}
 # Packed-FP32 VALU ops are disabled for all device code (they are generated
 # from plain float2 arithmetic at -O3 otherwise).
 COMMON_FLAGS = [

@@ -93,6 +93,56 @@ GDN_DEVICE const char* kv_row(const KvSource& s, const PagedTable& tb, int64_t n
   }
 }
 
+// What a prefill or decode kernel computes.
+enum AttnForm {
+  kPlain,
+  kScored,  // capped or biased scores, prefix masks
+  kShared,  // decode of sequences that share their first keys: those (prefill kernel), and the others (decode kernel)
+};
+
+// The groups of sequences of a shared decode: group g is sequences
+// [groups[g], groups[g + 1]) (all of them without `groups`), whose first
+// lens[g] keys are the same.
+struct SharedArgs {
+  const void *groups, *lens;
+  int32_t n;
+  bool groups64, lens64;
+};
+struct SharedGroup {
+  int64_t b0, b1, keys;  // sequences, and the keys that are read once for all of them
+};
+// The keys are taken in whole 16-key steps, so that each sequence's own keys
+// begin at one; a group of one sequence shares nothing.
+GDN_DEVICE SharedGroup shared_group(const SharedArgs& s, int64_t g, int64_t B, int64_t cap) {
+  SharedGroup r{0, B, 0};
+  if (s.groups) {
+    r.b0 = clamp64(load_index(s.groups, g, s.groups64), 0, B);
+    r.b1 = clamp64(load_index(s.groups, g + 1, s.groups64), r.b0, B);
+  }
+  if (r.b1 - r.b0 > 1) r.keys = clamp64(load_index(s.lens, g, s.lens64), 0, cap) & ~int64_t(15);
+  return r;
+}
+// The group that holds sequence b, or -1.
+GDN_DEVICE int32_t shared_group_of(const SharedArgs& s, int64_t b, int64_t B) {
+  if (!s.groups) return s.n > 0 ? 0 : -1;
+  int32_t lo = 0, hi = s.n;
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) / 2;
+    if (load_index(s.groups, mid, s.groups64) <= b) lo = mid;
+    else hi = mid;
+  }
+  if (s.n < 1) return -1;
+  const SharedGroup r = shared_group(s, lo, B, 0);
+  return b >= r.b0 && b < r.b1 ? lo : -1;
+}
+// The keys of sequence b, of length L, that its group reads for it: all of the
+// group's, or none where the sequence is shorter than they are.
+GDN_DEVICE int64_t shared_keys_of(const SharedArgs& s, int64_t b, int64_t L, int64_t B, int64_t cap) {
+  const int32_t g = shared_group_of(s, b, B);
+  const int64_t keys = g < 0 ? 0 : shared_group(s, g, B, cap).keys;
+  return L >= keys ? keys : 0;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 KvSource kv_source(const gdn_tensor* t, bool paged) {

@@ -49,7 +49,16 @@ struct DecodeArgs {
   float c;
   bool ctx64;
   bool prices_inline;  // the decode waves compute Q themselves (small batches)
+  // kScored: as in the prefill's arguments
+  float cap_in, cap_out;
+  const float* slopes;
+  SharedArgs sh;  // kShared: a sequence's keys here are those past its group's
 };
+
+// The first of the keys that the decode kernel reads for sequence b.
+template <AttnForm FORM> GDN_DEVICE int64_t decode_first_key(const DecodeArgs& a, int64_t b, int64_t L, int64_t cap) {
+  return FORM == kShared ? shared_keys_of(a.sh, b, L, a.B, cap) : 0;
+}
 
 // Price prefix of the batch for the split decode: Q[b] = sum over b' < b of
 // the price of b' (ceil(L_b' / 16) + kDecodeStartPrice, or 0 with no keys),
@@ -58,6 +67,7 @@ struct DecodeArgs {
 // sequences, the run sums are scanned across the block, and each thread writes
 // its run's prefixes.  (Q[B] < 2^31: the entry point checks
 // B * (ceil(capacity / 16) + kDecodeStartPrice).)
+template <AttnForm FORM>
 __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeArgs a) {
   __shared__ int32_t wsum[16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -65,7 +75,9 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
   const int per = (a.B + 1023) / 1024;
   const int64_t b0 = (int64_t)tid * per;
   auto price_of = [&](int64_t b) -> int32_t {
-    const int32_t t = b < a.B ? (int32_t)((clamp64(load_index(a.ctx, b, a.ctx64), 0, cap) + 15) / 16) : 0;
+    if (b >= a.B) return 0;
+    const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
+    const int32_t t = (int32_t)((L - decode_first_key<FORM>(a, b, L, cap) + 15) / 16);
     return t > 0 ? t + kDecodeStartPrice : 0;
   };
   int32_t sum = 0;
@@ -96,7 +108,7 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
 template <typename T, int D>
 constexpr size_t decode_lds_per_wave() { return (size_t)16 * (D + 16) * sizeof(T) + (size_t)(D / 32) * 64 * 16; }
 
-template <typename T, int D, bool PAGE16>
+template <typename T, int D, bool PAGE16, AttnForm FORM = kPlain>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_kernel(const DecodeArgs a) {
   typedef Mma<T> M;
   typedef typename M::v8 v8;
@@ -123,10 +135,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const char* kvv = a.v.base + kvh * a.v.sh;
   const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;
   const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
+  // scored: the scores become exponents of 2 in the tile, which the softmax scales by 1
+  const float cs = FORM == kScored ? 1.f : c;
+  const float slope = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e : 0.f;
 
   // keys [k_lo, k_hi) of sequence b (k_lo a multiple of 16); the result goes
   // to the output (slot < 0) or to workspace slot `slot`
-  auto piece = [&](int64_t b, int64_t k_lo, int64_t k_hi, int64_t slot) {
+  auto piece = [&](int64_t b, int64_t k_lo, int64_t k_hi, int64_t slot, int64_t last_key) {
     const int ntiles = k_hi > k_lo ? (int)((k_hi - k_lo + 15) / 16) : 0;
     // query fragments (B operand of S^T): lane holds head column lane % 16,
     // dims 32 s + 8 grp .. +7; kept in LDS to leave registers for two tiles
@@ -242,6 +257,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // keys 4 grp + r of the tile) and O^T += V^T P^T
     auto accumulate = [&](int t, f32x4 s) {
       const uint32_t j0 = (uint32_t)k_lo + 16u * (uint32_t)t;  // (key positions fit 32 bits)
+      if constexpr (FORM == kScored) {
+        // as in the prefill; the query sits at its sequence's last key
+        if (a.cap_out > 0.f) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[r] = __builtin_fmaf(-2.f * a.cap_out,
+                                  __builtin_amdgcn_rcpf(1.f + exp2_fast(s[r] * c * a.cap_in)), a.cap_out);
+        } else {
+          s *= c;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[r] = __builtin_fmaf(slope, (float)((int32_t)(j0 + 4u * grp + r) - (int32_t)last_key), s[r]);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (j0 + 4u * grp + r >= (uint32_t)k_hi) s[r] = -INFINITY;
@@ -251,10 +280,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       // by 2^8, and then to the maximum over the four lanes, taken only on
       // that rare path (the same decisions and bases as taking it every tile)
       const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-      if (__builtin_amdgcn_ballot_w64(mx * c > m_used + 8.f) != 0) {
+      if (__builtin_amdgcn_ballot_w64(mx * cs > m_used + 8.f) != 0) {
         float mg = fmaxf(mx, __shfl_xor(mx, 16));
         mg = fmaxf(mg, __shfl_xor(mg, 32));
-        const float mn = fmaxf(m_used, mg * c);
+        const float mn = fmaxf(m_used, mg * cs);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
 #pragma unroll
         for (int d = 0; d < NDT; ++d) oacc[d] *= alpha;
@@ -265,7 +294,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       v4 pf;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = exp2_fast(__builtin_fmaf(s[r], c, nb));
+        const float p = exp2_fast(__builtin_fmaf(s[r], cs, nb));
         lsum += p;
         pf[r] = (T)p;
       }
@@ -334,7 +363,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       // writes the prefix for the combine
       auto price = [&](int32_t i) -> int32_t {
         if (i >= a.B) return 0;
-        const int32_t t = (int32_t)((clamp64(load_index(a.ctx, i, a.ctx64), 0, cap) + 15) / 16);
+        const int64_t L = clamp64(load_index(a.ctx, i, a.ctx64), 0, cap);
+        const int32_t t = (int32_t)((L - decode_first_key<FORM>(a, i, L, cap) + 15) / 16);
         return t > 0 ? t + SP : 0;
       };
       int32_t tot = 0;
@@ -401,16 +431,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     int64_t k_lo = 0, k_hi = L, slot = -1;
     bool any = true;
     if (a.splits > 1) {
-      const int32_t tb = (int32_t)((L + 15) / 16);  // the sequence's tiles
+      const int64_t first = decode_first_key<FORM>(a, b, L, cap);
+      const int32_t tb = (int32_t)((L - first + 15) / 16);  // the sequence's tiles
       qn = qb + (tb > 0 ? tb + SP : 0);
       const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
       const int32_t t0 = r0 < 0 ? 0 : (r0 > tb ? tb : r0), t1 = r1 < 0 ? 0 : (r1 > tb ? tb : r1);
-      k_lo = 16 * (int64_t)t0;
-      k_hi = 16 * (int64_t)t1 < L ? 16 * (int64_t)t1 : L;
+      k_lo = first + 16 * (int64_t)t0;
+      k_hi = first + 16 * (int64_t)t1 < L ? first + 16 * (int64_t)t1 : L;
       any = t1 > t0;
-      if (t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
+      // (shared: every piece is merged with the group's)
+      if (FORM == kShared || t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
     }
-    if (any) piece(b, k_lo, k_hi, slot);
+    if (any) piece(b, k_lo, k_hi, slot, L - 1);
     if (a.splits == 1 || qn >= x1) break;
     ++b;
     qb = qn;
@@ -484,24 +516,25 @@ __global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArg
   for (int e = 0; e < E; ++e) op[e] = (T)(acc[e] * inv);
 }
 
-template <typename T, int D>
+template <typename T, int D, AttnForm FORM = kPlain>
 hipError_t launch_decode_t(const DecodeArgs& a, hipStream_t st) {
   const int hgroups = (a.Hq / a.Hkv + 15) / 16;
   const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / a.kvw * hgroups), (unsigned)a.B);
   const size_t lds = (size_t)a.kvw * decode_lds_per_wave<T, D>();
   if (a.splits > 1 && !a.prices_inline) {
-    attn_decode_prices_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
+    attn_decode_prices_kernel<FORM><<<dim3(1), dim3(1024), 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   if (a.tab.page % 16 == 0 && a.k.sb < (int64_t(1) << 32) && a.v.sb < (int64_t(1) << 32) &&
       a.tab.cols * a.tab.page < (int64_t(1) << 31) && a.tab.num_blocks < (int64_t(1) << 31))
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, true>), grid, dim3(64 * a.kvw), lds, st, a);
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, true, FORM>), grid, dim3(64 * a.kvw), lds, st, a);
   else
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, false>), grid, dim3(64 * a.kvw), lds, st, a);
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, false, FORM>), grid, dim3(64 * a.kvw), lds, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((attn_decode_combine_kernel<T, D>), dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st, a);
+  if constexpr (FORM != kShared)  // (whose pieces are merged with the groups')
+    hipLaunchKernelGGL((attn_decode_combine_kernel<T, D>), dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st, a);
   return hipGetLastError();
 }
 

@@ -35,6 +35,13 @@ struct AttnArgs {
   int64_t rows;
   int32_t extra;
   float* part;
+  // kScored: 2 / cap of the tanh cap and cap * log2(e) (cap 0: none), slopes of
+  // the distance bias (Hq,), and keys of each sequence that all its queries see
+  float cap_in, cap_out;
+  const float* slopes;
+  const void* pfx;
+  bool pfx64;
+  SharedArgs sh;  // kShared
 };
 
 // Floats of one piece's partial: per wave, the accumulators of its 32 queries
@@ -301,6 +308,114 @@ GDN_DEVICE SplitPiece split_piece(const AttnArgs& a, const SplitPlan& sp, int sh
   return {-1, 0, 0};
 }
 
+// kShared: the rows of the prefill tile are the queries of a group, one per
+// sequence, times the R query heads of a kv head: row r is head r % R of
+// sequence b0 + r / R.  Its keys are cut into pieces of `tiles` key tiles (the
+// same for all groups), one workgroup for each (kv head, group, piece, 128
+// rows), in that order.
+// Lane i prices i + 1 times `mult` pieces of the longest group, in 1/32 of a
+// key-tile step: the rounds of workgroups that run at once, kFixed steps each;
+// the partials' traffic, D / 128 of 1/32 step per workgroup; the merge's chain
+// over a row's pieces.  Whole numbers: the prefill and the combine kernel agree.
+struct SharedRows {
+  int32_t rt, n;  // blocks of 128 rows, key tiles
+};
+template <int BN>
+GDN_DEVICE SharedRows shared_rows(const AttnArgs& a, const SharedGroup& g) {
+  const int32_t rows = (int32_t)(g.b1 - g.b0) * (a.Hq / a.Hkv);
+  return g.keys > 0 ? SharedRows{(rows + 127) >> 7, (int32_t)((g.keys + BN - 1) / BN)} : SharedRows{0, 0};
+}
+template <int BN>
+GDN_DEVICE SharedRows shared_rows_lane(const AttnArgs& a, int c) {
+  const int g = c + (threadIdx.x & 63);
+  return g < a.sh.n ? shared_rows<BN>(a, shared_group(a.sh, g, a.T, a.tab.cols * a.tab.page)) : SharedRows{0, 0};
+}
+GDN_DEVICE int shared_pieces(int n, int tiles, float inv) { return n > 0 ? split_further(n, tiles, inv) + 1 : 0; }
+template <int D, int BN>
+GDN_DEVICE int shared_tiles(const AttnArgs& a) {
+  constexpr int kSlots = D == 256 ? 256 : D == 128 ? 512 : 768, kFixed = 10;
+  const int lane = threadIdx.x & 63;
+  int top = 0, rt = 0;
+  for (int c = 0; c < a.sh.n; c += 64) {
+    const SharedRows q = shared_rows_lane<BN>(a, c);
+    top = q.n > top ? q.n : top;
+    rt += wave_sum(q.rt);
+  }
+  const int nmax = wave_top(top);
+  if (nmax == 0 || (int64_t)rt * a.Hkv > (1 << 20)) return kWholeRows;
+  const int mult = (kSlots + 64 * rt * a.Hkv - 1) / (64 * rt * a.Hkv), want = (lane + 1) * mult;
+  int tiles = (nmax + want - 1) / want;
+  tiles += tiles & 1;
+  const float inv = __builtin_amdgcn_rcpf((float)tiles);
+  int x = 0;
+  for (int c = 0; c < a.sh.n; c += 64) {
+    const SharedRows q = shared_rows_lane<BN>(a, c);
+    const int m = a.sh.n - c < 64 ? a.sh.n - c : 64;
+    for (int j = 0; j < m; ++j)
+      x += __mul24(__builtin_amdgcn_readlane(q.rt, j), shared_pieces(__builtin_amdgcn_readlane(q.n, j), tiles, inv));
+  }
+  const int64_t wgs = (int64_t)x * a.Hkv;
+  x = wgs < 1 << 24 ? (int)wgs : 1 << 24;
+  const int most = shared_pieces(nmax, tiles, inv);
+  const int64_t cost = 32 * (int64_t)((x + kSlots - 1) / kSlots) * (kFixed + tiles) + (int64_t)x * D / 128 + 3 * most;
+  const int c24 = x <= a.extra && cost < 1 << 24 ? (int)cost : 1 << 24;
+  const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
+  return __builtin_amdgcn_readlane(x, best) <= a.extra ? __builtin_amdgcn_readlane(tiles, best) : kWholeRows;
+}
+
+// Workgroup `id` of the shared prefill.  Consecutive ids go to the 8 XCDs in
+// turn, so an eighth of the list is dealt to each: the row blocks over the same
+// keys then run on one XCD and read them from its L2.
+struct SharedWork {
+  int64_t lead, b0;  // the sequence through whose table the keys are read (-1: nothing to do), the group's first
+  int64_t keys;
+  int32_t rows, tile, tile0, tiles, kvh;
+  uint32_t slot;
+};
+template <int D, int BN>
+GDN_DEVICE SharedWork shared_work(const AttnArgs& a, uint32_t id) {
+  SharedWork r{};
+  r.lead = -1;
+  r.tiles = shared_tiles<D, BN>(a);
+  if (r.tiles == kWholeRows) return r;
+  const float inv = __builtin_amdgcn_rcpf((float)r.tiles);
+  int per_head = 0;
+  for (int c = 0; c < a.sh.n; c += 64) {
+    const SharedRows q = shared_rows_lane<BN>(a, c);
+    per_head += wave_sum(q.rt * shared_pieces(q.n, r.tiles, inv));
+  }
+  const uint32_t all = (uint32_t)per_head * a.Hkv, per = (all + 7) / 8;
+  r.slot = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || r.slot >= all) return r;
+  r.kvh = (int)(r.slot / (uint32_t)per_head);
+  int left = (int)r.slot - r.kvh * per_head;
+  for (int c = 0; c < a.sh.n; c += 64) {
+    const SharedRows q = shared_rows_lane<BN>(a, c);
+    const int x = q.rt * shared_pieces(q.n, r.tiles, inv), sum = wave_inclusive_scan_i32(x), u = left - (sum - x);
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(u >= 0 && u < x);
+    if (mine) {
+      const int l = __builtin_ctzll(mine), rt = __builtin_amdgcn_readlane(q.rt, l);
+      const int v = __builtin_amdgcn_readlane(u, l), piece = v / rt;
+      r.tile = v - piece * rt;
+      r.tile0 = piece * r.tiles;
+      const SharedGroup g = shared_group(a.sh, c + l, a.T, a.tab.cols * a.tab.page);
+      r.b0 = g.b0;
+      r.keys = g.keys;
+      r.rows = (int32_t)(g.b1 - g.b0) * (a.Hq / a.Hkv);
+      // (a sequence shorter than the shared keys may have no table; one of the
+      // others has all of them, or no row of the group is read)
+      for (int64_t b = g.b0; b < g.b1 && r.lead < 0; b += 64) {
+        const int64_t i = b + (threadIdx.x & 63);
+        const uint64_t ok = __builtin_amdgcn_ballot_w64(i < g.b1 && load_index(a.ctx, i, a.ctx64) >= g.keys);
+        if (ok) r.lead = b + __builtin_ctzll(ok);
+      }
+      return r;
+    }
+    left -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return r;
+}
+
 // Output rows that no sequence covers -- [0, cu[0]) and [cu[N], T), clamped
 // like seq_range -- are zero, as the reference allocates o zero-filled
 // (ops/full_attention.py:467).  The workgroups past the last tile, `wg` of `n`,
@@ -344,7 +459,7 @@ GDN_DEVICE void zero_rows_tail(const AttnArgs& a, uint32_t wg, uint32_t n) {
 // keys held to 256 registers 259; eight chunks over up to 4,096 cached keys
 // 563 -> 329 us (345).  D = 64: 180 -> 165 us.  D = 96 (vision): 64 keys 142,
 // 32 keys 157, three waves per SIMD 158 (32 keys) and 197 (64, spills).
-template <typename T, int D, int BN, int PG, bool SPLIT, int DQ = 0>
+template <typename T, int D, int BN, int PG, bool SPLIT, int DQ = 0, AttnForm FORM = kPlain>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prefill_kernel(const AttnArgs a) {
   constexpr bool PAGED = PG != 0;
   // DQ > 0: head dims of a.dim <= DQ <= D elements (packed rows only), a
@@ -357,6 +472,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   constexpr bool RAG = DQ > 0;
   static_assert(!RAG || (PG == 0 && DQ <= D && DQ % 16 == 0), "ragged head dims are packed rows");
   static_assert(!SPLIT || PG >= 2, "split rows are paged rows of whole 16-row groups");
+  static_assert(FORM == kPlain || !RAG, "scored and shared rows are of the kernels' own head dims");
+  static_assert(FORM != kShared || (PAGED && !SPLIT), "shared keys are paged, in pieces of their own");
   typedef Mma<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v4 v4;
@@ -417,44 +534,73 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       piece = p.piece;
     }
   }
-  if (!further) {
-    st = attn_tile_lookup<D, PAGED, SPLIT>(a, 32 * qsubs, row_id / hg, lookup);
-    // (no tile is left past the grid's rows unless the offsets decrease: nothing
-    // is kept for it in the workspace)
-    if (SPLIT && row_id >= srows && st.seq >= 0) return;
-    if (st.seq < 0) {
-      const uint32_t tiles = srows / hg + 1;
-      zero_rows_tail<T>(a, (uint32_t)st.tile * hg + row_id % hg, (tiles - (row_id / hg - (uint32_t)st.tile)) * hg);
-      return;
-    }
-  }
-  const int64_t n = st.seq;
-  const int y = (int)(row_id % hg);
-  const int kvh = y / groups;
-  const int head = kvh * R + (y % groups) * gh + (w % gh);
-
-  int64_t s0, s1;
-  seq_range(a.cu, a.cu64, n, a.T, s0, s1);
-  const int64_t len = s1 - s0;
-  const int64_t ntile = (len + 32 * qsubs - 1) / (32 * qsubs);
-  const int64_t qb = (ntile - 1 - st.tile) * 32 * qsubs;  // last query tiles first
-
-  int64_t Lk, off;
-  if (PAGED) {
-    const int64_t ctx = load_index(a.ctx, n, a.ctx64);
-    Lk = clamp64(ctx, 0, a.tab.cols * a.tab.page);
-    off = ctx - len;  // position of query 0
-  } else {
-    Lk = len;
+  // the tile's rows: s0 + (qb ...) of its sequence, `len` of them, or rows (qb
+  // ...) of its group; their keys, and the position of row 0
+  int64_t n, s0, len, qb, Lk, off;
+  int kvh, head;
+  int64_t pfx = 0;  // keys that every row sees
+  int64_t sb0 = 0;
+  int stile0 = 0;
+  if constexpr (FORM == kShared) {
+    const SharedWork sw = shared_work<D, BN>(a, blockIdx.x);
+    if (sw.lead < 0) return;
+    n = sw.lead;
+    sb0 = sw.b0;
+    s0 = 0;
+    len = sw.rows;
+    qb = 128 * (int64_t)sw.tile;
+    Lk = sw.keys;
     off = 0;
+    kvh = sw.kvh;
+    head = kvh * R;
+    slot = sw.slot;
+    stile0 = sw.tile0;
+    ptiles = sw.tiles;
+  } else {
+    if (!further) {
+      st = attn_tile_lookup<D, PAGED, SPLIT>(a, 32 * qsubs, row_id / hg, lookup);
+      // (no tile is left past the grid's rows unless the offsets decrease: nothing
+      // is kept for it in the workspace)
+      if (SPLIT && row_id >= srows && st.seq >= 0) return;
+      if (st.seq < 0) {
+        const uint32_t tiles = srows / hg + 1;
+        zero_rows_tail<T>(a, (uint32_t)st.tile * hg + row_id % hg, (tiles - (row_id / hg - (uint32_t)st.tile)) * hg);
+        return;
+      }
+    }
+    n = st.seq;
+    const int y = (int)(row_id % hg);
+    kvh = y / groups;
+    head = kvh * R + (y % groups) * gh + (w % gh);
+
+    int64_t s1;
+    seq_range(a.cu, a.cu64, n, a.T, s0, s1);
+    len = s1 - s0;
+    const int64_t ntile = (len + 32 * qsubs - 1) / (32 * qsubs);
+    qb = (ntile - 1 - st.tile) * 32 * qsubs;  // last query tiles first
+
+    if (PAGED) {
+      const int64_t ctx = load_index(a.ctx, n, a.ctx64);
+      Lk = clamp64(ctx, 0, a.tab.cols * a.tab.page);
+      off = ctx - len;  // position of query 0
+    } else {
+      Lk = len;
+      off = 0;
+    }
+    if (FORM == kScored && a.pfx) pfx = load_index(a.pfx, n, a.pfx64);
   }
+  // (causal: the keys that the rows before row `end` see)
+  auto seen = [&](int64_t end) __attribute__((always_inline)) {
+    const int64_t e = off + end;
+    return clamp64(FORM == kScored && e < pfx ? pfx : e, 0, Lk);
+  };
   const int64_t q0 = qb + (w / gh) * 32;
   const int64_t wg_qend = qb + 32 * qsubs < len ? qb + 32 * qsubs : len;
   const int64_t w_qend = q0 + 32 < len ? q0 + 32 : len;
-  const int64_t kend_row = a.causal ? clamp64(off + wg_qend, 0, Lk) : Lk;
-  const int64_t kend_roww = q0 >= len ? 0 : (a.causal ? clamp64(off + w_qend, 0, Lk) : Lk);
+  const int64_t kend_row = FORM != kShared && a.causal ? seen(wg_qend) : Lk;
+  const int64_t kend_roww = q0 >= len ? 0 : (FORM != kShared && a.causal ? seen(w_qend) : Lk);
   // this piece's key tiles [tile0, ntiles); keys past its end are not loaded
-  const int tile0 = SPLIT ? piece * ptiles : 0;
+  const int tile0 = FORM == kShared ? stile0 : SPLIT ? piece * ptiles : 0;
   if (SPLIT && piece > 0 && (int64_t)tile0 * BN >= kend_row) return;
   int64_t kend = kend_row, kend_w = kend_roww;
   bool whole = true;  // the row is one piece
@@ -464,7 +610,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     kend = kend_row > end ? end : kend_row;
     kend_w = kend_roww > end ? end : kend_roww;
   };
-  if (SPLIT && further) cut(ptiles);
+  if (FORM == kShared || (SPLIT && further)) cut(ptiles);
 
   // query fragments (B operand of S^T = K Q^T): lane holds query q0 + lane % 32,
   // dims 16 ks + 8 (lane / 32) .. +7
@@ -477,7 +623,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   v8 qf[NKS];
   {
     static_assert(!RAG || q_pieces_inside(DQ), "query pieces are read inside their row");
-    const T* qp = reinterpret_cast<const T*>(a.q) + (s0 + (qvalid ? qi : 0)) * a.q_st + (int64_t)head * a.q_sh;
+    const int64_t row = qvalid ? qi : 0;
+    const uint32_t sb = FORM == kShared ? (uint32_t)row / (uint32_t)R : 0u, sh = FORM == kShared ? (uint32_t)row - sb * R : 0u;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (FORM == kShared ? sb0 + sb : s0 + row) * a.q_st +
+                  (int64_t)(FORM == kShared ? head + (int)sh : head) * a.q_sh;
 #pragma unroll
     for (int s = 0; s < NKS; ++s)
       qf[s] = *reinterpret_cast<const v8*>(qp + (RAG ? q_piece(s, hh, a.dim) : 16 * s + 8 * hh));
@@ -557,7 +706,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       }
     }
   };
-  if (SPLIT) {
+  if (SPLIT || FORM == kShared) {
     gcol = (uint32_t)tile0 * NG / gpp;
     grem = (uint32_t)tile0 * NG - gcol * gpp;
   }
@@ -664,8 +813,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   // a key tile needs the mask when it reaches past the keys (t BN + BN > Lk)
   // or, causal, past the wave's first query (t BN + BN - 1 > off + q0):
   // t BN > mthr, one 32-bit test per tile (key positions stay below 2^31)
-  const int mthr = (int)clamp64(a.causal ? (Lk - BN < off + q0 - BN + 1 ? Lk - BN : off + q0 - BN + 1) : Lk - BN, -1,
-                                0x7fffffff);
+  const int64_t first = FORM == kScored && off + q0 + 1 < pfx ? pfx : off + q0 + 1;  // keys that the first query sees
+  const int mthr = (int)clamp64(FORM != kShared && a.causal && first < Lk ? first - BN : Lk - BN, -1, 0x7fffffff);
+  const int qpos = FORM == kScored ? (int)clamp64(off + qi, INT32_MIN, INT32_MAX) : 0;
+  const float slope = FORM == kScored && a.slopes ? -a.slopes[head] * kLog2e : 0.f;
   // `mid` (the next tiles' LDS stores and global loads) is issued right after
   // the score MFMAs, so that its issue overlaps their execution; a wave with
   // no keys left in this tile still runs it
@@ -673,6 +824,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     if ((int64_t)t * BN < kend_w) {
       const T* K = ks[buf];
       const T* V = vs[buf];
+      // (scored: the scores become exponents of 2 below, so the softmax scales them by 1)
+      const float cs = FORM == kScored ? 1.f : c;
       f32x16 s[NA];
 #pragma unroll
       for (int aa = 0; aa < NA; ++aa) {
@@ -698,10 +851,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         }
       }
       mid();
+      if constexpr (FORM == kScored) {
+        // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), within 2e-7
+        // cap; the distance is exact, a whole number below 2^24 (rounded past it)
+        if (a.cap_out > 0.f) {
+          const float ci = c * a.cap_in;
+#pragma unroll
+          for (int aa = 0; aa < NA; ++aa)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[aa][r] = __builtin_fmaf(-2.f * a.cap_out,
+                                        __builtin_amdgcn_rcpf(1.f + exp2_fast(s[aa][r] * ci)), a.cap_out);
+        } else {
+#pragma unroll
+          for (int aa = 0; aa < NA; ++aa) s[aa] *= c;
+        }
+        if (a.slopes) {
+          const float d0 = (float)(int)((uint32_t)(t * BN + 4 * hh) - (uint32_t)qpos);
+#pragma unroll
+          for (int aa = 0; aa < NA; ++aa)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[aa][r] = __builtin_fmaf(slope, __builtin_fabsf(d0 + (float)(32 * aa + 8 * (r >> 2) + (r & 3))), s[aa][r]);
+        }
+      }
       // mask keys past the sequence / context and, if causal, past the query
       const int64_t tk0 = (int64_t)t * BN;
       if (t * BN > mthr) {
-        const int64_t lim = (a.causal ? (off + qi + 1 < Lk ? off + qi + 1 : Lk) : Lk) - tk0;
+        const int64_t own = FORM == kScored && off + qi + 1 < pfx ? pfx : off + qi + 1;
+        const int64_t lim = (FORM != kShared && a.causal && own < Lk ? own : Lk) - tk0;
         const int rel = (int)clamp64(lim, -1, BN);  // keys of the tile at or past rel are masked
 #pragma unroll
         for (int aa = 0; aa < NA; ++aa)
@@ -720,8 +898,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       for (int aa = 0; aa < NA; ++aa)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[aa][r]);
-      if (__builtin_amdgcn_ballot_w64(mx * c > m_used + 8.f) != 0) {
-        const float mn = fmaxf(m_used, max_lane_pair32(mx) * c);
+      if (__builtin_amdgcn_ballot_w64(mx * cs > m_used + 8.f) != 0) {
+        const float mn = fmaxf(m_used, max_lane_pair32(mx) * cs);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
 #pragma unroll
         for (int d = 0; d < NDT; ++d) oacc[d] *= alpha;
@@ -736,7 +914,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
           v8 pf;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float p = exp2_fast(__builtin_fmaf(s[aa][8 * h2 + e], c, nb));
+            const float p = exp2_fast(__builtin_fmaf(s[aa][8 * h2 + e], cs, nb));
             lsum += p;
             pf[e] = (T)p;
           }
@@ -819,8 +997,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   }
 
   const float lt = lsum + __shfl_xor(lsum, 32);
-  if constexpr (SPLIT) {
-    if (!whole) {
+  if constexpr (SPLIT || FORM == kShared) {
+    if (FORM == kShared || !whole) {
       float* pw = a.part + (int64_t)slot * prefill_part_floats<D>() + w * prefill_part_wave<D>();
 #pragma unroll
       for (int d = 0; d < NDT; ++d)
@@ -880,7 +1058,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
 // 4 waves x 32 queries as the prefill kernel, each lane reading back its own
 // accumulator pieces of DG 32-dim blocks.  Rows of one piece were written by
 // the prefill itself.
-template <typename T, int D, int BN, int DG>
+template <typename T, int D, int BN, int DG, AttnForm FORM = kPlain>
 __global__ __launch_bounds__(256) void attn_prefill_combine_kernel(const AttnArgs a) {
   typedef typename Mma<T>::v4 v4;
   __shared__ int32_t lookup[8];
@@ -903,7 +1081,12 @@ __global__ __launch_bounds__(256) void attn_prefill_combine_kernel(const AttnArg
   const int64_t ctx = load_index(a.ctx, st.seq, a.ctx64);
   const int64_t Lk = clamp64(ctx, 0, a.tab.cols * a.tab.page);
   const int64_t wg_qend = qb + 32 * qsubs < len ? qb + 32 * qsubs : len;
-  const int64_t kend = clamp64(ctx - len + wg_qend, 0, Lk);
+  int64_t end = ctx - len + wg_qend;
+  if (FORM == kScored && a.pfx) {
+    const int64_t pfx = load_index(a.pfx, st.seq, a.pfx64);
+    end = end < pfx ? pfx : end;
+  }
+  const int64_t kend = clamp64(end, 0, Lk);
   const int64_t pk = (int64_t)sp.tiles * BN;
   const int np = (int)((kend + pk - 1) / pk);
   const int64_t qi = qb + (w / gh) * 32 + (lane & 31);
@@ -948,7 +1131,14 @@ __global__ __launch_bounds__(256) void attn_prefill_combine_kernel(const AttnArg
   }
 }
 
-template <typename T, int D, int BN, bool PAGED, int DQ = 0>
+// Whether the kernels that look a page up once per 16 rows serve the caches:
+// whole 16-row groups per page, 32-bit table arithmetic.
+bool whole_groups(const AttnArgs& a) {
+  return a.tab.page % 16 == 0 && a.k.sb < (int64_t(1) << 32) && a.v.sb < (int64_t(1) << 32) && a.tab.cols > 0 &&
+         a.tab.cols * a.tab.page < (int64_t(1) << 31) && a.tab.num_blocks < (int64_t(1) << 31);
+}
+
+template <typename T, int D, int BN, bool PAGED, int DQ = 0, AttnForm FORM = kPlain>
 hipError_t launch_prefill_t(const AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
   const int qsubs = 4 / a.gh;
   // without sequences there are only rows to zero
@@ -961,28 +1151,26 @@ hipError_t launch_prefill_t(const AttnArgs& a, int64_t nseq, int64_t max_len, hi
   const int64_t tiles = a.T / (32 * qsubs) + nseq + 1;
   const dim3 grid((unsigned)(tiles * (a.Hq / a.gh)));
   if constexpr (!PAGED) {
-    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 0, false, DQ>), grid, dim3(256), 0, st, a);
-  } else if (a.tab.page % 16 == 0 && a.k.sb < (int64_t(1) << 32) && a.v.sb < (int64_t(1) << 32) && a.tab.cols > 0 &&
-             a.tab.cols * a.tab.page < (int64_t(1) << 31) && a.tab.num_blocks < (int64_t(1) << 31)) {
-    // whole 16-row groups per page, 32-bit table arithmetic
+    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 0, false, DQ, FORM>), grid, dim3(256), 0, st, a);
+  } else if (whole_groups(a)) {
     if (a.extra > 0) {
       const dim3 sgrid((unsigned)(a.rows + a.Hq / a.gh + a.extra));
       constexpr int DG = D == 256 ? 2 : 1;  // 32-dim blocks per combine workgroup
       if (a.tab.is64)
-        hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, true>), sgrid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, true, 0, FORM>), sgrid, dim3(256), 0, st, a);
       else
-        hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, true>), sgrid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, true, 0, FORM>), sgrid, dim3(256), 0, st, a);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       // (many rows fill the chip by themselves)
-      hipLaunchKernelGGL((attn_prefill_combine_kernel<T, D, BN, DG>),
+      hipLaunchKernelGGL((attn_prefill_combine_kernel<T, D, BN, DG, FORM>),
                          dim3((unsigned)a.rows, a.rows >= 256 ? 1 : D / (32 * DG)), dim3(256), 0, st, a);
     } else if (a.tab.is64)
-      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, false>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, false, 0, FORM>), grid, dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, false>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, false, 0, FORM>), grid, dim3(256), 0, st, a);
   } else
-    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 1, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 1, false, 0, FORM>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -998,10 +1186,10 @@ hipError_t launch_prefill_t(const AttnArgs& a, int64_t nseq, int64_t max_len, hi
 bool few_workgroups(const AttnArgs& a, int64_t nseq, int64_t max_len) {
   return max_len > 256 && (a.T / (32 * (4 / a.gh)) + nseq) * (a.Hq / a.gh) <= (a.causal ? 736 : 672);
 }
-template <typename T, int DQ>
+template <typename T, int DQ, AttnForm FORM = kPlain>
 hipError_t launch_prefill_64(const AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
-  return few_workgroups(a, nseq, max_len) ? launch_prefill_t<T, 64, 64, false, DQ>(a, nseq, max_len, st)
-                                          : launch_prefill_t<T, 64, 32, false, DQ>(a, nseq, max_len, st);
+  return few_workgroups(a, nseq, max_len) ? launch_prefill_t<T, 64, 64, false, DQ, FORM>(a, nseq, max_len, st)
+                                          : launch_prefill_t<T, 64, 32, false, DQ, FORM>(a, nseq, max_len, st);
 }
 
 // Whether a paged prefill over at most `cap` keys per sequence runs split, and

@@ -181,9 +181,14 @@ typedef Entry<16, 13, int32_t, float, float> DecodeFusedNorm;
 typedef Entry<17, 3> Linear;
 typedef Entry<18, 10, float, int32_t, int32_t> ChunkPrefillSplitEx;
 typedef Entry<19, 11, int32_t> KvAppend;
+typedef Entry<20, 7, int64_t, float, float, int32_t> AttnVarlenScored;
+typedef Entry<21, 10, int64_t, float, float> PagedPrefillScored;
+typedef Entry<22, 8, int32_t, float, float> PagedDecodeScored;
+typedef Entry<23, 9, int32_t, float> PagedDecodeShared;
 typedef Size<0, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> ChunkPrefillSize;
 typedef Size<1, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> PagedPrefillSize;
 typedef Size<2, int64_t, int64_t, int64_t, int32_t> PagedDecodeSize;
+typedef Size<3, int64_t, int64_t, int64_t, int64_t, int64_t, int32_t> PagedDecodeSharedSize;
 
 struct Bound {
   const char* name;
@@ -212,6 +217,11 @@ const Bound kBound[] = {
     GDN_BOUND("paged_attention_decode", PagedDecode),
     GDN_BOUND("paged_attention_decode_noalloc", PagedDecodeNoalloc),
     GDN_BOUND("paged_kv_append", KvAppend),
+    GDN_BOUND("flash_attention_varlen_scored", AttnVarlenScored),
+    GDN_BOUND("paged_attention_prefill_scored", PagedPrefillScored),
+    GDN_BOUND("paged_attention_decode_scored", PagedDecodeScored),
+    GDN_BOUND("paged_attention_decode_shared", PagedDecodeShared),
+    GDN_BOUND("paged_attention_decode_shared_workspace_size", PagedDecodeSharedSize),
     GDN_BOUND("gdn_chunk_prefill_workspace_size", ChunkPrefillSize),
     GDN_BOUND("paged_attention_prefill_workspace_size", PagedPrefillSize),
     GDN_BOUND("paged_attention_decode_workspace_size", PagedDecodeSize),

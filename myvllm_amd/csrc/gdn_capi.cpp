@@ -52,6 +52,25 @@ hipError_t attn_paged_decode_launch(const gdn_tensor* q, const gdn_tensor* kc, c
                                     int32_t splits, float scale, hipStream_t st);
 hipError_t attn_decode_scratch(hipStream_t st, float** ptr);
 int32_t attn_decode_start_price();
+hipError_t attn_varlen_scored_launch(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v,
+                                     const gdn_tensor* cu, gdn_tensor* out, const gdn_tensor* slopes,
+                                     const gdn_tensor* pfx, int64_t max_seqlen, float scale, float cap, int causal,
+                                     hipStream_t st);
+hipError_t attn_paged_scored_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                    const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* cu,
+                                    gdn_tensor* out, float* workspace, const gdn_tensor* slopes,
+                                    const gdn_tensor* pfx, int64_t max_seqlen, float scale, float cap,
+                                    hipStream_t st);
+hipError_t attn_decode_scored_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                     const gdn_tensor* tab, const gdn_tensor* ctx, gdn_tensor* out, float* workspace,
+                                     const gdn_tensor* slopes, int32_t splits, float scale, float cap,
+                                     hipStream_t st);
+int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
+int64_t attn_shared_partials(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
+hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                     const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
+                                     const gdn_tensor* groups, gdn_tensor* out, float* workspace, int64_t own,
+                                     int32_t splits, float scale, hipStream_t st);
 int64_t paged_kv_append_waves(int64_t T, int64_t rows, int64_t D);
 hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* kc, gdn_tensor* vc,
                                   const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* q, gdn_tensor* out,
@@ -548,8 +567,8 @@ GDN_EXPORT int gdn_gating(const gdn_tensor* a, const gdn_tensor* b, const gdn_te
 }
 
 namespace {
-int varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v, const gdn_tensor* cu_seqlens,
-                   gdn_tensor* out, int64_t max_seqlen, float scale, int32_t causal, void* stream, bool any_dim) {
+int check_varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v, const gdn_tensor* cu_seqlens,
+                         const gdn_tensor* out, int64_t max_seqlen, bool any_dim) {
   GDN_TRY(check_desc(q, 3));
   GDN_TRY(check_desc(k, 3));
   GDN_TRY(check_desc(v, 3));
@@ -571,8 +590,34 @@ int varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v
   const int64_t es = elem_size(k->dtype);
   if (std::max<int64_t>(max_seqlen, 64) * std::max(k->stride[0], v->stride[0]) * es >= (int64_t(1) << 31))
     return GDN_ERR_RANGE;
+  return GDN_OK;
+}
+
+int varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v, const gdn_tensor* cu_seqlens,
+                   gdn_tensor* out, int64_t max_seqlen, float scale, int32_t causal, void* stream, bool any_dim) {
+  GDN_TRY(check_varlen_prefill(q, k, v, cu_seqlens, out, max_seqlen, any_dim));
   return launch_rc(attn_varlen_prefill_launch(q, k, v, cu_seqlens, out, max_seqlen, scale, causal,
                                               reinterpret_cast<hipStream_t>(stream)));
+}
+
+// Score forms: the cap, slopes (Hq,) fp32 and prefix lengths (N,).
+int check_scores(const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_t Hq, int64_t N, float softcap,
+                 bool causal) {
+  if (!(softcap >= 0.f && softcap <= 4096.f)) return GDN_ERR_ARG;
+  if (slopes) {
+    GDN_TRY(check_desc(slopes, 1));
+    if (slopes->shape[0] != Hq) return GDN_ERR_SHAPE;
+    if (slopes->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
+    if (slopes->stride[0] != 1) return GDN_ERR_STRIDE;
+  }
+  if (prefix_lens) {
+    if (!causal) return GDN_ERR_ARG;
+    GDN_TRY(check_desc(prefix_lens, 1));
+    if (prefix_lens->shape[0] != N) return GDN_ERR_SHAPE;
+    if (!is_index(prefix_lens->dtype)) return GDN_ERR_DTYPE;
+    if (prefix_lens->stride[0] != 1) return GDN_ERR_STRIDE;
+  }
+  return GDN_OK;
 }
 }  // namespace
 
@@ -589,10 +634,10 @@ GDN_EXPORT int flash_attention_varlen_any_dim(const gdn_tensor* q, const gdn_ten
 }
 
 namespace {
-// Checks and launch of the paged prefill; without a workspace its rows are not split.
-int paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
-                  const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
-                  gdn_tensor* out, const gdn_tensor* workspace, int64_t max_seqlen, float scale, void* stream) {
+// Checks of the paged prefill; *ws: its workspace, null where its rows are not split.
+int check_paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                        const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
+                        const gdn_tensor* out, const gdn_tensor* workspace, int64_t max_seqlen, float** ws) {
   GDN_TRY(check_desc(q, 3));
   GDN_TRY(check_desc(out, 3));
   GDN_TRY(check_desc(cu_seqlens, 1));
@@ -611,7 +656,7 @@ int paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tens
   if (k_cache->shape[1] * std::max(k_cache->stride[1], v_cache->stride[1]) * es >= (int64_t(1) << 31) ||
       block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31))
     return GDN_ERR_RANGE;
-  float* ws = nullptr;
+  *ws = nullptr;
   if (workspace) {
     GDN_TRY(check_desc(workspace, 1));
     if (workspace->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
@@ -621,9 +666,18 @@ int paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tens
     if (workspace->shape[0] < need) return GDN_ERR_SHAPE;
     if (need > 0) {
       if (!aligned(workspace, 16)) return GDN_ERR_ALIGN;
-      ws = reinterpret_cast<float*>(workspace->data);
+      *ws = reinterpret_cast<float*>(workspace->data);
     }
   }
+  return GDN_OK;
+}
+
+int paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                  const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
+                  gdn_tensor* out, const gdn_tensor* workspace, int64_t max_seqlen, float scale, void* stream) {
+  float* ws;
+  GDN_TRY(check_paged_prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, workspace, max_seqlen,
+                              &ws));
   return launch_rc(attn_paged_prefill_launch(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, ws,
                                              max_seqlen, scale, reinterpret_cast<hipStream_t>(stream)));
 }
@@ -689,21 +743,29 @@ int check_paged_decode(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn
 }
 }  // namespace
 
+namespace {
+// The workspace of a split decode, of at least `need` floats (null for one split).
+int decode_workspace(const gdn_tensor* workspace, int64_t need, int32_t num_splits, int64_t B, float** ws) {
+  *ws = nullptr;
+  if (num_splits <= 1) return GDN_OK;
+  GDN_TRY(check_desc(workspace, 1));
+  if (workspace->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
+  if (workspace->stride[0] != 1) return GDN_ERR_STRIDE;
+  if (workspace->shape[0] < need) return GDN_ERR_SHAPE;
+  if (B > 0 && !aligned(workspace, 16)) return GDN_ERR_ALIGN;
+  *ws = reinterpret_cast<float*>(workspace->data);
+  return GDN_OK;
+}
+}  // namespace
+
 GDN_EXPORT int paged_attention_decode(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                                       const gdn_tensor* block_tables, const gdn_tensor* context_lens, gdn_tensor* out,
                                       gdn_tensor* workspace, int32_t num_splits, float scale, void* stream) {
   GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits));
-  const int64_t B = q->shape[0];
-  float* ws = nullptr;
-  if (num_splits > 1) {
-    GDN_TRY(check_desc(workspace, 1));
-    if (workspace->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
-    if (workspace->stride[0] != 1) return GDN_ERR_STRIDE;
-    if (workspace->shape[0] < paged_attention_decode_workspace_size(B, q->shape[1], q->shape[2], num_splits))
-      return GDN_ERR_SHAPE;
-    if (B > 0 && !aligned(workspace, 16)) return GDN_ERR_ALIGN;
-    ws = reinterpret_cast<float*>(workspace->data);
-  }
+  float* ws;
+  GDN_TRY(decode_workspace(workspace, paged_attention_decode_workspace_size(q->shape[0], q->shape[1], q->shape[2],
+                                                                            num_splits),
+                           num_splits, q->shape[0], &ws));
   return launch_rc(attn_paged_decode_launch(q, k_cache, v_cache, block_tables, context_lens, out, ws, num_splits,
                                             scale, reinterpret_cast<hipStream_t>(stream)));
 }
@@ -723,6 +785,87 @@ GDN_EXPORT int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_ten
   }
   return launch_rc(attn_paged_decode_launch(q, k_cache, v_cache, block_tables, context_lens, out, ws, num_splits,
                                             scale, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int flash_attention_varlen_scored(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v,
+                                             const gdn_tensor* cu_seqlens, gdn_tensor* out, const gdn_tensor* slopes,
+                                             const gdn_tensor* prefix_lens, int64_t max_seqlen, float scale,
+                                             float softcap, int32_t causal, void* stream) {
+  GDN_TRY(check_varlen_prefill(q, k, v, cu_seqlens, out, max_seqlen, false));
+  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, softcap, causal != 0));
+  return launch_rc(attn_varlen_scored_launch(q, k, v, cu_seqlens, out, slopes, prefix_lens, max_seqlen, scale, softcap,
+                                             causal, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_attention_prefill_scored(const gdn_tensor* q, const gdn_tensor* k_cache,
+                                              const gdn_tensor* v_cache, const gdn_tensor* block_tables,
+                                              const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
+                                              gdn_tensor* out, gdn_tensor* workspace, const gdn_tensor* slopes,
+                                              const gdn_tensor* prefix_lens, int64_t max_seqlen, float scale,
+                                              float softcap, void* stream) {
+  float* ws;
+  GDN_TRY(check_paged_prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, workspace, max_seqlen,
+                              &ws));
+  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, softcap, true));
+  return launch_rc(attn_paged_scored_launch(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, ws,
+                                            slopes, prefix_lens, max_seqlen, scale, softcap,
+                                            reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tensor* k_cache,
+                                             const gdn_tensor* v_cache, const gdn_tensor* block_tables,
+                                             const gdn_tensor* context_lens, gdn_tensor* out, gdn_tensor* workspace,
+                                             const gdn_tensor* slopes, int32_t num_splits, float scale, float softcap,
+                                             void* stream) {
+  GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits));
+  GDN_TRY(check_scores(slopes, nullptr, q->shape[1], q->shape[0], softcap, true));
+  float* ws;
+  GDN_TRY(decode_workspace(workspace, paged_attention_decode_workspace_size(q->shape[0], q->shape[1], q->shape[2],
+                                                                            num_splits),
+                           num_splits, q->shape[0], &ws));
+  return launch_rc(attn_decode_scored_launch(q, k_cache, v_cache, block_tables, context_lens, out, ws, slopes,
+                                             num_splits, scale, softcap, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs, int64_t num_groups,
+                                                                int64_t num_q_heads, int64_t num_kv_heads,
+                                                                int64_t head_dim, int32_t num_splits) {
+  if (num_seqs < 0 || num_groups < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return 0;
+  return paged_attention_decode_workspace_size(num_seqs, num_q_heads, head_dim, num_splits) +
+         attn_shared_partials(num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim);
+}
+
+GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache,
+                                             const gdn_tensor* v_cache, const gdn_tensor* block_tables,
+                                             const gdn_tensor* context_lens, const gdn_tensor* prefix_lens,
+                                             const gdn_tensor* cu_groups, gdn_tensor* out, gdn_tensor* workspace,
+                                             int32_t num_splits, float scale, void* stream) {
+  if (num_splits < 2) return GDN_ERR_RANGE;
+  GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits));
+  GDN_TRY(check_desc(prefix_lens, 1));
+  const int64_t B = q->shape[0], Hq = q->shape[1], D = q->shape[2], Hkv = k_cache->shape[2], G = prefix_lens->shape[0];
+  if (!is_index(prefix_lens->dtype)) return GDN_ERR_DTYPE;
+  if (prefix_lens->stride[0] != 1) return GDN_ERR_STRIDE;
+  if (cu_groups) {
+    GDN_TRY(check_desc(cu_groups, 1));
+    if (cu_groups->shape[0] != G + 1) return GDN_ERR_SHAPE;
+    if (!is_index(cu_groups->dtype)) return GDN_ERR_DTYPE;
+    if (cu_groups->stride[0] != 1) return GDN_ERR_STRIDE;
+  } else if (G != 1) {
+    return GDN_ERR_SHAPE;
+  }
+  // rows, key positions and workgroups are counted in 32 bits
+  if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ ||
+      block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31) ||
+      attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20))
+    return GDN_ERR_RANGE;
+  const int64_t own = paged_attention_decode_workspace_size(B, Hq, D, num_splits);
+  float* ws;
+  GDN_TRY(decode_workspace(workspace, own + attn_shared_partials(B, G, Hq, Hkv, D), num_splits, B, &ws));
+  return launch_rc(attn_decode_shared_launch(q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups,
+                                             out, ws, own, num_splits, scale, reinterpret_cast<hipStream_t>(stream)));
 }
 
 GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,

@@ -14,6 +14,11 @@ the output's dim stride is the dim stride (``:76``), the non-causal path masks
 keys past the sequence end, and the paged prefill reads its work list and
 ``cu_seqlens`` correctly (``:378-380``); a query with no visible key gives a
 zero row instead of 0/0.
+
+The three ops take other forms of scores as keywords (``softcap``,
+``alibi_slopes``, ``prefix_lens``), and beside them stand the append that fills
+the caches (:func:`paged_kv_append`) and the decode of sequences that share
+their first keys (:func:`paged_flash_attention_decode_shared`).
 """
 from __future__ import annotations
 
@@ -62,19 +67,35 @@ def flash_attention_prefill(
     is_causal: bool,
     max_seqlen: int | None = None,
     out: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    prefix_lens: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Varlen attention over packed sequences: q (T, Hq, D), k, v (T, Hkv, D) ->
     (T, Hq, D).  ``max_seqlen`` (the longest sequence) is read from
-    ``cu_seqlens`` when not given, one host sync as in the reference (``:139``)."""
+    ``cu_seqlens`` when not given, one host sync as in the reference (``:139``).
+
+    Other forms of scores x = scale q.k, applied in this order: ``softcap``
+    (above 0, at most 4096): x <- softcap tanh(x / softcap); ``alibi_slopes``
+    (Hq,) fp32: x <- x - slope_h |i - j|; ``prefix_lens`` (N,), causal only: the
+    first ``prefix_lens[n]`` keys are visible to every query of sequence n.  A
+    packed batch is its own document mask: each document a sequence."""
     if q.shape[1] != num_heads or k.shape[1] != num_kv_heads or q.shape[2] != head_dim or v.shape[2] != head_v_dim:
         raise ValueError("q/k/v shapes disagree with num_heads/num_kv_heads/head_dim/head_v_dim")
-    dev = _lib.require_device(q, k, v, cu_seqlens)
+    dev = _lib.require_device(q, k, v, cu_seqlens, alibi_slopes, prefix_lens)
     if max_seqlen is None:
         max_seqlen = _max_seqlen(cu_seqlens)
     own = head_dim in _KERNEL_HEAD_DIMS and head_v_dim == head_dim
-    if not own and not _direct_head_dim(q, k, v, head_dim, head_v_dim, max_seqlen):
-        return _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out)
+    scored = _scored(softcap, alibi_slopes, prefix_lens)
+    if not own and (scored or not _direct_head_dim(q, k, v, head_dim, head_v_dim, max_seqlen)):
+        return _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out,
+                               softcap=softcap, alibi_slopes=alibi_slopes, prefix_lens=prefix_lens)
     q, k, v = _lib.vec16(q), _lib.vec16(k), _lib.vec16(v)
+    if scored:
+        o = _out_for(out, (q.shape[0], q.shape[1], head_v_dim), q.dtype, dev)
+        _lib.call("flash_attention_varlen_scored", q, k, v, cu_seqlens, o, alibi_slopes, prefix_lens, int(max_seqlen),
+                  float(scale), float(softcap or 0.0), int(bool(is_causal)))
+        return _finish(out, o)
     o = _out_for(out if own or _apart(out, q, k, v) else None, (q.shape[0], q.shape[1], head_v_dim), q.dtype, dev)
     _lib.call("flash_attention_varlen" if own else "flash_attention_varlen_any_dim", q, k, v, cu_seqlens, o,
               int(max_seqlen), float(scale), int(bool(is_causal)))
@@ -82,6 +103,10 @@ def flash_attention_prefill(
 
 
 _KERNEL_HEAD_DIMS = (64, 128, 256)
+
+
+def _scored(softcap, alibi_slopes, prefix_lens=None) -> bool:
+    return softcap is not None or alibi_slopes is not None or prefix_lens is not None
 
 
 def _direct_head_dim(q, k, v, head_dim, head_v_dim, max_seqlen) -> bool:
@@ -106,7 +131,7 @@ def _apart(out, q, k, v) -> bool:
             and out.untyped_storage().data_ptr() not in {t.untyped_storage().data_ptr() for t in (q, k, v)})
 
 
-def _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out):
+def _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out, **form):
     """Head dims no kernel reads as they lie (:func:`_direct_head_dim`) run
     zero-padded to the next of 64, 128 and 256: zero dims add nothing to q.k
     and give zero output columns, which are dropped.  The padded copies cost
@@ -116,7 +141,7 @@ def _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal,
         raise ValueError(f"head dims {head_dim}/{head_v_dim} above {_KERNEL_HEAD_DIMS[-1]} are not supported")
     pad = lambda t: torch.nn.functional.pad(t, (0, Dp - t.shape[-1]))
     o = flash_attention_prefill(pad(q), pad(k), pad(v), cu_seqlens, scale, q.shape[1], k.shape[1], Dp, Dp, is_causal,
-                                max_seqlen=max_seqlen)
+                                max_seqlen=max_seqlen, **form)
     return _finish(out, o[..., :head_v_dim]) if out is not None else o[..., :head_v_dim]
 
 
@@ -151,13 +176,16 @@ def paged_flash_attention_decode(
     block_size: int,
     num_splits: int | None = None,
     out: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """One query per sequence over its paged cache: q (B, Hq, D), caches
     (num_blocks, block_size, Hkv, D), block_tables (B, max_blocks),
-    context_lens (B,) -> (B, Hq, D).  No host sync."""
+    context_lens (B,) -> (B, Hq, D).  No host sync.  ``softcap`` and
+    ``alibi_slopes`` as in :func:`flash_attention_prefill`."""
     if k_cache.shape[1] != block_size:
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
-    dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens)
+    dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens, alibi_slopes)
     B, Hq, Dh = q.shape
     if num_splits is None:
         num_splits = decode_num_splits(B, Hq, k_cache.shape[2], block_tables.shape[1] * block_size)
@@ -167,8 +195,56 @@ def paged_flash_attention_decode(
         ws = torch.empty(n_ws, dtype=torch.float32, device=dev)
     q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
     o = _out_for(out, (B, Hq, v_cache.shape[-1]), q.dtype, dev)
-    _lib.call("paged_attention_decode", q, k_cache, v_cache, block_tables, context_lens, o, ws, int(num_splits),
-              float(scale))
+    if _scored(softcap, alibi_slopes):
+        _lib.call("paged_attention_decode_scored", q, k_cache, v_cache, block_tables, context_lens, o, ws,
+                  alibi_slopes, int(num_splits), float(scale), float(softcap or 0.0))
+    else:
+        _lib.call("paged_attention_decode", q, k_cache, v_cache, block_tables, context_lens, o, ws, int(num_splits),
+                  float(scale))
+    return _finish(out, o)
+
+
+def paged_flash_attention_decode_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    scale: float,
+    block_size: int,
+    cu_groups: torch.Tensor | None = None,
+    num_splits: int | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_flash_attention_decode` for sequences that begin with the
+    same keys (a common prompt): the same result, with those keys read once per
+    group and not once per sequence.
+
+    The sequences ``[cu_groups[g], cu_groups[g + 1])`` (all of them without
+    ``cu_groups``, then ``prefix_lens`` has one element) hold the same first
+    ``prefix_lens[g]`` keys and values, counted in ``context_lens`` as any
+    others.  Their tables name pages that hold them, as a rule the same ones;
+    they are read through the table of the group's first sequence that is long
+    enough.  A shorter sequence, and one in no group, is read through its own
+    table alone.  No host sync; where the workspace is not to be had it runs as
+    the plain decode."""
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
+    dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups)
+    B, Hq, Dh = q.shape
+    if num_splits is None:
+        num_splits = max(2, decode_num_splits(B, Hq, k_cache.shape[2], block_tables.shape[1] * block_size))
+    n_ws = _lib.workspace_size("paged_attention_decode_shared_workspace_size", B, prefix_lens.numel(), Hq,
+                               k_cache.shape[2], Dh, int(num_splits))
+    q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
+    o = _out_for(out, (B, Hq, v_cache.shape[-1]), q.dtype, dev)
+    try:
+        ws = torch.empty(n_ws, dtype=torch.float32, device=dev)
+    except torch.OutOfMemoryError:
+        return paged_flash_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scale, block_size, out=out)
+    _lib.call("paged_attention_decode_shared", q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups,
+              o, ws, int(num_splits), float(scale))
     return _finish(out, o)
 
 
@@ -229,6 +305,9 @@ def paged_flash_attention_prefill(
     page_block_size: int,
     max_seqlen: int | None = None,
     out: torch.Tensor | None = None,
+    softcap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    prefix_lens: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Prefill over a paged cache that already holds the new keys: query i of
     sequence n sits at position ``context_lens[n] - len_n + i`` and attends
@@ -236,16 +315,22 @@ def paged_flash_attention_prefill(
     per-16-row work list) is accepted for interface parity and not needed:
     the kernel tiles the queries itself from ``cu_seqlens``.  Few new tokens
     over a long cache are split over the keys as well; the partials then take a
-    temporary workspace of up to 512 MiB, without which nothing is split."""
+    temporary workspace of up to 512 MiB, without which nothing is split.
+    ``softcap``, ``alibi_slopes`` and ``prefix_lens`` as in
+    :func:`flash_attention_prefill`, positions and keys counted over the cache."""
     if k_cache.shape[1] != page_block_size:
         raise ValueError(f"page_block_size {page_block_size} != k_cache.shape[1] {k_cache.shape[1]}")
-    dev = _lib.require_device(q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens)
+    dev = _lib.require_device(q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens, alibi_slopes,
+                              prefix_lens)
     if max_seqlen is None:
         max_seqlen = _max_seqlen(cu_seqlens)
     q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
     o = _out_for(out, (q.shape[0], q.shape[1], v_cache.shape[-1]), q.dtype, dev)
     ws = _prefill_workspace(q, k_cache, v_cache, page_block_tables, cu_seqlens, page_block_size)
-    if ws is not None:
+    if _scored(softcap, alibi_slopes, prefix_lens):
+        _lib.call("paged_attention_prefill_scored", q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens,
+                  o, ws, alibi_slopes, prefix_lens, int(max_seqlen), float(scale), float(softcap or 0.0))
+    elif ws is not None:
         _lib.call("paged_attention_prefill_split", q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens, o,
                   ws, int(max_seqlen), float(scale))
     else:

@@ -157,3 +157,20 @@ def paged_kv_append_ref(q, k, v, k_cache, v_cache, block_tables, context_lens, c
                 k_cache[blk, p % bs] = turn(k)
                 v_cache[blk, p % bs] = v[t].double()
     return None if q is None else out
+
+
+def attention_weights_ref(q_rows, k_seq, pos, scale, causal=True, softcap=None, slopes=None, prefix=0):
+    """Scores x (n, Hq, m) of q_rows (n, Hq, D) at positions ``pos`` over keys
+    0..m-1 with cap, distance bias and prefix mask, -inf where masked, and the
+    softmax weights (zero rows where nothing is visible); fp64."""
+    r = q_rows.shape[1] // k_seq.shape[1]
+    pos = torch.as_tensor(pos)
+    x = torch.einsum("nhd,mhd->nhm", q_rows.double(), k_seq.double().repeat_interleave(r, 1)) * scale
+    if softcap:
+        x = softcap * torch.tanh(x / softcap)
+    j = torch.arange(k_seq.shape[0])
+    if slopes is not None:
+        x = x - slopes.double()[None, :, None] * (pos[:, None] - j).abs()[:, None]
+    if causal:
+        x = x.masked_fill(((j > pos[:, None]) & (j >= prefix))[:, None], float("-inf"))
+    return x, torch.softmax(x, -1).nan_to_num(0.0)
