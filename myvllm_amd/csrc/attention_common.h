@@ -100,48 +100,20 @@ enum AttnForm {
   kShared,  // decode of sequences that share their first keys: those (prefill kernel), and the others (decode kernel)
 };
 
-// The groups of sequences of a shared decode: group g is sequences
-// [groups[g], groups[g + 1]) (all of them without `groups`), whose first
-// lens[g] keys are the same.
-struct SharedArgs {
-  const void *groups, *lens;
-  int32_t n;
-  bool groups64, lens64;
+// What a shared decode's first launch writes down (attention_shared.hip).  Of a
+// sequence: the keys that its group reads for it (its own begin there), its
+// group's pieces (0 where it is not read with the group) and 128-row blocks,
+// rt << 11 | pieces; the group's first slot of a kv head, and the sequence's
+// first row in the group.
+struct SharedSeq {
+  int32_t first, pieces, slot, row;
 };
-struct SharedGroup {
-  int64_t b0, b1, keys;  // sequences, and the keys that are read once for all of them
+// Of a workgroup: the sequence through whose table the keys are read (-1: no
+// work), the group's first sequence and rows, the workgroup's first row, its
+// keys [32 tile0, keys), kv head and slot of the partials.
+struct SharedWork {
+  int32_t lead, b0, rows, row, tile0, keys, kvh, slot;
 };
-// The keys are taken in whole 16-key steps, so that each sequence's own keys
-// begin at one; a group of one sequence shares nothing.
-GDN_DEVICE SharedGroup shared_group(const SharedArgs& s, int64_t g, int64_t B, int64_t cap) {
-  SharedGroup r{0, B, 0};
-  if (s.groups) {
-    r.b0 = clamp64(load_index(s.groups, g, s.groups64), 0, B);
-    r.b1 = clamp64(load_index(s.groups, g + 1, s.groups64), r.b0, B);
-  }
-  if (r.b1 - r.b0 > 1) r.keys = clamp64(load_index(s.lens, g, s.lens64), 0, cap) & ~int64_t(15);
-  return r;
-}
-// The group that holds sequence b, or -1.
-GDN_DEVICE int32_t shared_group_of(const SharedArgs& s, int64_t b, int64_t B) {
-  if (!s.groups) return s.n > 0 ? 0 : -1;
-  int32_t lo = 0, hi = s.n;
-  while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) / 2;
-    if (load_index(s.groups, mid, s.groups64) <= b) lo = mid;
-    else hi = mid;
-  }
-  if (s.n < 1) return -1;
-  const SharedGroup r = shared_group(s, lo, B, 0);
-  return b >= r.b0 && b < r.b1 ? lo : -1;
-}
-// The keys of sequence b, of length L, that its group reads for it: all of the
-// group's, or none where the sequence is shorter than they are.
-GDN_DEVICE int64_t shared_keys_of(const SharedArgs& s, int64_t b, int64_t L, int64_t B, int64_t cap) {
-  const int32_t g = shared_group_of(s, b, B);
-  const int64_t keys = g < 0 ? 0 : shared_group(s, g, B, cap).keys;
-  return L >= keys ? keys : 0;
-}
 
 constexpr float kLog2e = 1.4426950408889634f;
 

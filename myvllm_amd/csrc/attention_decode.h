@@ -52,13 +52,8 @@ struct DecodeArgs {
   // kScored: as in the prefill's arguments
   float cap_in, cap_out;
   const float* slopes;
-  SharedArgs sh;  // kShared: a sequence's keys here are those past its group's
+  const SharedSeq* seqs;  // kShared: a sequence's keys here are those past its group's
 };
-
-// The first of the keys that the decode kernel reads for sequence b.
-template <AttnForm FORM> GDN_DEVICE int64_t decode_first_key(const DecodeArgs& a, int64_t b, int64_t L, int64_t cap) {
-  return FORM == kShared ? shared_keys_of(a.sh, b, L, a.B, cap) : 0;
-}
 
 // Price prefix of the batch for the split decode: Q[b] = sum over b' < b of
 // the price of b' (ceil(L_b' / 16) + kDecodeStartPrice, or 0 with no keys),
@@ -67,7 +62,6 @@ template <AttnForm FORM> GDN_DEVICE int64_t decode_first_key(const DecodeArgs& a
 // sequences, the run sums are scanned across the block, and each thread writes
 // its run's prefixes.  (Q[B] < 2^31: the entry point checks
 // B * (ceil(capacity / 16) + kDecodeStartPrice).)
-template <AttnForm FORM>
 __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeArgs a) {
   __shared__ int32_t wsum[16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -75,9 +69,7 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
   const int per = (a.B + 1023) / 1024;
   const int64_t b0 = (int64_t)tid * per;
   auto price_of = [&](int64_t b) -> int32_t {
-    if (b >= a.B) return 0;
-    const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
-    const int32_t t = (int32_t)((L - decode_first_key<FORM>(a, b, L, cap) + 15) / 16);
+    const int32_t t = b < a.B ? (int32_t)((clamp64(load_index(a.ctx, b, a.ctx64), 0, cap) + 15) / 16) : 0;
     return t > 0 ? t + kDecodeStartPrice : 0;
   };
   int32_t sum = 0;
@@ -108,8 +100,9 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
 template <typename T, int D>
 constexpr size_t decode_lds_per_wave() { return (size_t)16 * (D + 16) * sizeof(T) + (size_t)(D / 32) * 64 * 16; }
 
-template <typename T, int D, bool PAGE16, AttnForm FORM = kPlain>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_kernel(const DecodeArgs a) {
+// One wave of it: wave wv of block (bx, by, bz), with decode_lds_per_wave() of LDS.
+template <typename T, int D, bool PAGE16, AttnForm FORM>
+GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_t bx, uint32_t by, uint32_t bz) {
   typedef Mma<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v4 v4;
@@ -118,16 +111,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   constexpr int NDT = D / 16;
   constexpr int CH = D / 8;
   constexpr int NLD = 16 * CH / 64;
-  extern __shared__ __align__(16) char decode_smem[];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   // this wave's LDS: the V tile, then its query fragments
-  T* vs = reinterpret_cast<T*>(decode_smem + wv * decode_lds_per_wave<T, D>());
+  T* vs = reinterpret_cast<T*>(lds);
   v8* qs = reinterpret_cast<v8*>(vs + 16 * LDV);
   const int64_t cap = a.tab.cols * a.tab.page;
 
   const int R = a.Hq / a.Hkv, hgroups = (R + 15) / 16;
-  const int kvh = (blockIdx.y / hgroups) * a.kvw + wv;
-  const int hcol = (blockIdx.y % hgroups) * 16 + (lane & 15);
+  const int kvh = (by / hgroups) * a.kvw + wv;
+  const int hcol = (by % hgroups) * 16 + (lane & 15);
   const bool hvalid = hcol < R;
   const int head = kvh * R + (hvalid ? hcol : 0);
   const int grp = lane >> 4;
@@ -352,10 +344,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   // with one split, unit z is sequence z; else unit u holds the batch's
   // prices [x0, x1) (they fit 31 bits, which the entry point checks)
   constexpr int32_t SP = kDecodeStartPrice;
-  int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
+  int32_t b = bz, x0 = 0, x1 = 0, qb = 0;
   if (a.splits > 1) {
     const int64_t U = (int64_t)a.B * a.units;
-    const int64_t u = (int64_t)blockIdx.z * a.units + blockIdx.x;
+    const int64_t u = (int64_t)bz * a.units + bx;
     if (a.prices_inline) {
       // small batch: every wave sums the prices itself (a lane per sequence,
       // 64 at a time), then finds the sequence holding price x0 in a second
@@ -363,8 +355,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       // writes the prefix for the combine
       auto price = [&](int32_t i) -> int32_t {
         if (i >= a.B) return 0;
-        const int64_t L = clamp64(load_index(a.ctx, i, a.ctx64), 0, cap);
-        const int32_t t = (int32_t)((L - decode_first_key<FORM>(a, i, L, cap) + 15) / 16);
+        const int32_t t = (int32_t)((clamp64(load_index(a.ctx, i, a.ctx64), 0, cap) + 15) / 16);
         return t > 0 ? t + SP : 0;
       };
       int32_t tot = 0;
@@ -374,7 +365,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       tot = __builtin_amdgcn_readfirstlane(tot);
       x0 = (int32_t)(u * tot / U);
       x1 = (int32_t)((u + 1) * tot / U);
-      const bool writer = u == 0 && blockIdx.y == 0 && wv == 0;
+      const bool writer = u == 0 && by == 0 && wv == 0;
       if (writer && lane == 0) a.prices[a.B] = tot;
       if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
       int32_t run = 0;
@@ -431,7 +422,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     int64_t k_lo = 0, k_hi = L, slot = -1;
     bool any = true;
     if (a.splits > 1) {
-      const int64_t first = decode_first_key<FORM>(a, b, L, cap);
+      const int64_t first = FORM == kShared ? a.seqs[b].first : 0;
       const int32_t tb = (int32_t)((L - first + 15) / 16);  // the sequence's tiles
       qn = qb + (tb > 0 ? tb + SP : 0);
       const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
@@ -440,13 +431,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       k_hi = first + 16 * (int64_t)t1 < L ? first + 16 * (int64_t)t1 : L;
       any = t1 > t0;
       // (shared: every piece is merged with the group's)
-      if (FORM == kShared || t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
+      if (FORM == kShared || t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)bz * a.units + bx;
     }
     if (any) piece(b, k_lo, k_hi, slot, L - 1);
     if (a.splits == 1 || qn >= x1) break;
     ++b;
     qb = qn;
   }
+}
+
+template <typename T, int D, bool PAGE16, AttnForm FORM = kPlain>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_kernel(const DecodeArgs a) {
+  extern __shared__ __align__(16) char decode_smem[];
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  attn_decode_wave<T, D, PAGE16, FORM>(a, decode_smem + wv * decode_lds_per_wave<T, D>(), wv, blockIdx.x, blockIdx.y,
+                                       blockIdx.z);
 }
 
 // Merge of the pieces of one (sequence, query head): one wave, D / 64
@@ -522,7 +521,7 @@ hipError_t launch_decode_t(const DecodeArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / a.kvw * hgroups), (unsigned)a.B);
   const size_t lds = (size_t)a.kvw * decode_lds_per_wave<T, D>();
   if (a.splits > 1 && !a.prices_inline) {
-    attn_decode_prices_kernel<FORM><<<dim3(1), dim3(1024), 0, st>>>(a);
+    attn_decode_prices_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -533,8 +532,7 @@ hipError_t launch_decode_t(const DecodeArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((attn_decode_kernel<T, D, false, FORM>), grid, dim3(64 * a.kvw), lds, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  if constexpr (FORM != kShared)  // (whose pieces are merged with the groups')
-    hipLaunchKernelGGL((attn_decode_combine_kernel<T, D>), dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st, a);
+  hipLaunchKernelGGL((attn_decode_combine_kernel<T, D>), dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st, a);
   return hipGetLastError();
 }
 

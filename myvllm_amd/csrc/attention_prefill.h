@@ -12,7 +12,9 @@
 
 #include <algorithm>
 
-#include "attention_common.h"
+#include <type_traits>
+
+#include "attention_decode.h"
 
 namespace {
 
@@ -41,7 +43,14 @@ struct AttnArgs {
   const float* slopes;
   const void* pfx;
   bool pfx64;
-  SharedArgs sh;  // kShared
+};
+
+// kShared: the shared keys' workgroups, and the decode of the sequences' own
+// keys, which takes the grid's first own_wgs workgroups (a multiple of 8)
+struct SharedAttnArgs : AttnArgs {
+  const SharedWork* work;
+  DecodeArgs own;
+  uint32_t own_wgs;
 };
 
 // Floats of one piece's partial: per wave, the accumulators of its 32 queries
@@ -308,114 +317,6 @@ GDN_DEVICE SplitPiece split_piece(const AttnArgs& a, const SplitPlan& sp, int sh
   return {-1, 0, 0};
 }
 
-// kShared: the rows of the prefill tile are the queries of a group, one per
-// sequence, times the R query heads of a kv head: row r is head r % R of
-// sequence b0 + r / R.  Its keys are cut into pieces of `tiles` key tiles (the
-// same for all groups), one workgroup for each (kv head, group, piece, 128
-// rows), in that order.
-// Lane i prices i + 1 times `mult` pieces of the longest group, in 1/32 of a
-// key-tile step: the rounds of workgroups that run at once, kFixed steps each;
-// the partials' traffic, D / 128 of 1/32 step per workgroup; the merge's chain
-// over a row's pieces.  Whole numbers: the prefill and the combine kernel agree.
-struct SharedRows {
-  int32_t rt, n;  // blocks of 128 rows, key tiles
-};
-template <int BN>
-GDN_DEVICE SharedRows shared_rows(const AttnArgs& a, const SharedGroup& g) {
-  const int32_t rows = (int32_t)(g.b1 - g.b0) * (a.Hq / a.Hkv);
-  return g.keys > 0 ? SharedRows{(rows + 127) >> 7, (int32_t)((g.keys + BN - 1) / BN)} : SharedRows{0, 0};
-}
-template <int BN>
-GDN_DEVICE SharedRows shared_rows_lane(const AttnArgs& a, int c) {
-  const int g = c + (threadIdx.x & 63);
-  return g < a.sh.n ? shared_rows<BN>(a, shared_group(a.sh, g, a.T, a.tab.cols * a.tab.page)) : SharedRows{0, 0};
-}
-GDN_DEVICE int shared_pieces(int n, int tiles, float inv) { return n > 0 ? split_further(n, tiles, inv) + 1 : 0; }
-template <int D, int BN>
-GDN_DEVICE int shared_tiles(const AttnArgs& a) {
-  constexpr int kSlots = D == 256 ? 256 : D == 128 ? 512 : 768, kFixed = 10;
-  const int lane = threadIdx.x & 63;
-  int top = 0, rt = 0;
-  for (int c = 0; c < a.sh.n; c += 64) {
-    const SharedRows q = shared_rows_lane<BN>(a, c);
-    top = q.n > top ? q.n : top;
-    rt += wave_sum(q.rt);
-  }
-  const int nmax = wave_top(top);
-  if (nmax == 0 || (int64_t)rt * a.Hkv > (1 << 20)) return kWholeRows;
-  const int mult = (kSlots + 64 * rt * a.Hkv - 1) / (64 * rt * a.Hkv), want = (lane + 1) * mult;
-  int tiles = (nmax + want - 1) / want;
-  tiles += tiles & 1;
-  const float inv = __builtin_amdgcn_rcpf((float)tiles);
-  int x = 0;
-  for (int c = 0; c < a.sh.n; c += 64) {
-    const SharedRows q = shared_rows_lane<BN>(a, c);
-    const int m = a.sh.n - c < 64 ? a.sh.n - c : 64;
-    for (int j = 0; j < m; ++j)
-      x += __mul24(__builtin_amdgcn_readlane(q.rt, j), shared_pieces(__builtin_amdgcn_readlane(q.n, j), tiles, inv));
-  }
-  const int64_t wgs = (int64_t)x * a.Hkv;
-  x = wgs < 1 << 24 ? (int)wgs : 1 << 24;
-  const int most = shared_pieces(nmax, tiles, inv);
-  const int64_t cost = 32 * (int64_t)((x + kSlots - 1) / kSlots) * (kFixed + tiles) + (int64_t)x * D / 128 + 3 * most;
-  const int c24 = x <= a.extra && cost < 1 << 24 ? (int)cost : 1 << 24;
-  const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
-  return __builtin_amdgcn_readlane(x, best) <= a.extra ? __builtin_amdgcn_readlane(tiles, best) : kWholeRows;
-}
-
-// Workgroup `id` of the shared prefill.  Consecutive ids go to the 8 XCDs in
-// turn, so an eighth of the list is dealt to each: the row blocks over the same
-// keys then run on one XCD and read them from its L2.
-struct SharedWork {
-  int64_t lead, b0;  // the sequence through whose table the keys are read (-1: nothing to do), the group's first
-  int64_t keys;
-  int32_t rows, tile, tile0, tiles, kvh;
-  uint32_t slot;
-};
-template <int D, int BN>
-GDN_DEVICE SharedWork shared_work(const AttnArgs& a, uint32_t id) {
-  SharedWork r{};
-  r.lead = -1;
-  r.tiles = shared_tiles<D, BN>(a);
-  if (r.tiles == kWholeRows) return r;
-  const float inv = __builtin_amdgcn_rcpf((float)r.tiles);
-  int per_head = 0;
-  for (int c = 0; c < a.sh.n; c += 64) {
-    const SharedRows q = shared_rows_lane<BN>(a, c);
-    per_head += wave_sum(q.rt * shared_pieces(q.n, r.tiles, inv));
-  }
-  const uint32_t all = (uint32_t)per_head * a.Hkv, per = (all + 7) / 8;
-  r.slot = (id & 7) * per + (id >> 3);
-  if ((id >> 3) >= per || r.slot >= all) return r;
-  r.kvh = (int)(r.slot / (uint32_t)per_head);
-  int left = (int)r.slot - r.kvh * per_head;
-  for (int c = 0; c < a.sh.n; c += 64) {
-    const SharedRows q = shared_rows_lane<BN>(a, c);
-    const int x = q.rt * shared_pieces(q.n, r.tiles, inv), sum = wave_inclusive_scan_i32(x), u = left - (sum - x);
-    const uint64_t mine = __builtin_amdgcn_ballot_w64(u >= 0 && u < x);
-    if (mine) {
-      const int l = __builtin_ctzll(mine), rt = __builtin_amdgcn_readlane(q.rt, l);
-      const int v = __builtin_amdgcn_readlane(u, l), piece = v / rt;
-      r.tile = v - piece * rt;
-      r.tile0 = piece * r.tiles;
-      const SharedGroup g = shared_group(a.sh, c + l, a.T, a.tab.cols * a.tab.page);
-      r.b0 = g.b0;
-      r.keys = g.keys;
-      r.rows = (int32_t)(g.b1 - g.b0) * (a.Hq / a.Hkv);
-      // (a sequence shorter than the shared keys may have no table; one of the
-      // others has all of them, or no row of the group is read)
-      for (int64_t b = g.b0; b < g.b1 && r.lead < 0; b += 64) {
-        const int64_t i = b + (threadIdx.x & 63);
-        const uint64_t ok = __builtin_amdgcn_ballot_w64(i < g.b1 && load_index(a.ctx, i, a.ctx64) >= g.keys);
-        if (ok) r.lead = b + __builtin_ctzll(ok);
-      }
-      return r;
-    }
-    left -= __builtin_amdgcn_readlane(sum, 63);
-  }
-  return r;
-}
-
 // Output rows that no sequence covers -- [0, cu[0]) and [cu[N], T), clamped
 // like seq_range -- are zero, as the reference allocates o zero-filled
 // (ops/full_attention.py:467).  The workgroups past the last tile, `wg` of `n`,
@@ -460,7 +361,8 @@ GDN_DEVICE void zero_rows_tail(const AttnArgs& a, uint32_t wg, uint32_t n) {
 // 563 -> 329 us (345).  D = 64: 180 -> 165 us.  D = 96 (vision): 64 keys 142,
 // 32 keys 157, three waves per SIMD 158 (32 keys) and 197 (64, spills).
 template <typename T, int D, int BN, int PG, bool SPLIT, int DQ = 0, AttnForm FORM = kPlain>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prefill_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prefill_kernel(
+    const std::conditional_t<FORM == kShared, SharedAttnArgs, AttnArgs> a) {
   constexpr bool PAGED = PG != 0;
   // DQ > 0: head dims of a.dim <= DQ <= D elements (packed rows only), a
   // multiple of 8.  The rows are read as they lie and the 16-byte pieces past
@@ -542,20 +444,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   int64_t sb0 = 0;
   int stile0 = 0;
   if constexpr (FORM == kShared) {
-    const SharedWork sw = shared_work<D, BN>(a, blockIdx.x);
+    if (blockIdx.x < a.own_wgs) {
+      // a wave per kv head and unit, `kvw` of them a block of the decode's grid;
+      // two waves' LDS lies in the key tiles, two in the value tiles
+      static_assert(2 * decode_lds_per_wave<T, D>() <= sizeof(ks) && sizeof(ks) <= sizeof(vs), "the decode's LDS");
+      const uint32_t kvw = a.own.kvw, v = blockIdx.x * (4 / kvw) + w / kvw;
+      const uint32_t nx = a.own.units, ny = a.own.Hkv / kvw * ((R + 15) / 16), bz = v / (nx * ny);
+      if (bz < (uint32_t)a.own.B)
+        attn_decode_wave<T, D, (PG >= 2), kShared>(
+            a.own, reinterpret_cast<char*>(w < 2 ? ks[0] : vs[0]) + (w & 1) * decode_lds_per_wave<T, D>(), w % kvw,
+            v % nx, v / nx % ny, bz);
+      return;
+    }
+    const SharedWork sw = a.work[blockIdx.x - a.own_wgs];
     if (sw.lead < 0) return;
     n = sw.lead;
     sb0 = sw.b0;
     s0 = 0;
     len = sw.rows;
-    qb = 128 * (int64_t)sw.tile;
+    qb = sw.row;
     Lk = sw.keys;
     off = 0;
     kvh = sw.kvh;
     head = kvh * R;
     slot = sw.slot;
     stile0 = sw.tile0;
-    ptiles = sw.tiles;
   } else {
     if (!further) {
       st = attn_tile_lookup<D, PAGED, SPLIT>(a, 32 * qsubs, row_id / hg, lookup);
@@ -610,7 +523,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     kend = kend_row > end ? end : kend_row;
     kend_w = kend_roww > end ? end : kend_roww;
   };
-  if (FORM == kShared || (SPLIT && further)) cut(ptiles);
+  if (SPLIT && further) cut(ptiles);
 
   // query fragments (B operand of S^T = K Q^T): lane holds query q0 + lane % 32,
   // dims 16 ks + 8 (lane / 32) .. +7

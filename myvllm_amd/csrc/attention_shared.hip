@@ -1,67 +1,273 @@
 // Paged decode of sequences that begin with the same keys: the softmax over
 // all keys of a sequence is merged from the one over the shared keys and the one
-// over its own, (O, m, l) each.
+// over its own, (O, m, l) each: m = max, l = sum l_i 2^(m_i - m), O likewise.
 //
-// The shared keys run through the prefill kernel (attention_prefill.h, kShared):
-// the queries of a group, sequences x heads of one kv head, are the rows of its
-// MFMA tile, so the group's K and V are read once per 128 of them instead of once
-// per sequence.  Each sequence's own keys run through the decode kernel
-// (attention_decode.h, kShared).  Both leave unnormalised pieces, which the
-// kernel below merges.
+// Three launches.  A plan, from the lengths on the device: one workgroup.  Then,
+// in one grid, the shared keys through the prefill kernel (attention_prefill.h,
+// kShared), the queries of a group, sequences x heads of a kv head, being the
+// rows of its MFMA tile, so that the group's K and V are read once per 128 of
+// them instead of once per sequence; and each sequence's own keys through the
+// decode kernel (attention_decode.h, kShared) on the workgroups beside them: the
+// one is bound by MFMA and LDS, the other by HBM.  The third merges their
+// unnormalised pieces.
 #include "attention_decode.h"
 #include "attention_prefill.h"
 
 namespace {
 
+constexpr int kSharedTile = 32;  // keys of a tile of the prefill kernel
+template <int D> constexpr int kSharedSlots = D == 256 ? 256 : D == 128 ? 512 : 768;  // workgroups that run at once
+constexpr int kMaxPieces11 = 2047;  // pieces of a row, held in 11 bits
+
+struct SharedGroup {
+  int32_t keys, b0, rows;   // keys that are read once for all, first sequence, rows (sequences x heads of a kv head)
+  int32_t rt, pieces;       // 128-row blocks, pieces of the keys
+  int32_t slot, lead, pad;  // first slot of a kv head; the sequence through whose table the keys are read
+};
+
+struct SharedPlanArgs {
+  const void *ctx, *groups, *lens;
+  bool ctx64, groups64, lens64;
+  int32_t B, n, R, Hkv;  // n groups
+  int64_t cap;
+  int32_t slots, own_wgs, grid;  // slots of the partials; workgroups of the own keys, and of the shared ones
+  int32_t* prices;
+  int32_t* per_head;  // slots of a kv head
+  SharedSeq* seqs;
+  SharedGroup* group;
+  SharedWork* work;
+};
+
+// Sequences and keys of group g.  The keys are taken in whole 16-key steps, so
+// that each sequence's own begin at one; a group of one sequence shares nothing.
+GDN_DEVICE SharedGroup shared_group(const SharedPlanArgs& a, int64_t g) {
+  SharedGroup r{};
+  int64_t b0 = 0, b1 = a.B;
+  const int64_t keys = load_index(a.lens, g, a.lens64);
+  if (a.groups) {
+    b0 = load_index(a.groups, g, a.groups64);
+    b1 = load_index(a.groups, g + 1, a.groups64);
+  }
+  b0 = clamp64(b0, 0, a.B);
+  b1 = clamp64(b1, b0, a.B);
+  r.b0 = (int32_t)b0;
+  r.rows = (int32_t)(b1 - b0) * a.R;
+  r.keys = b1 - b0 > 1 ? (int32_t)(clamp64(keys, 0, a.cap) & ~int64_t(15)) : 0;
+  r.rt = r.keys > 0 ? (r.rows + 127) >> 7 : 0;
+  return r;
+}
+// The group that may hold sequence b: the last g with groups[g] <= b.
+GDN_DEVICE int32_t shared_group_of(const SharedPlanArgs& a, int64_t b) {
+  int32_t lo = 0, hi = a.n;
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) / 2;
+    if (load_index(a.groups, mid, a.groups64) <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+// The keys of sequence b that its group reads for it: all of the group's, or
+// none where it is shorter than they are or in no group.
+GDN_DEVICE int32_t shared_first(const SharedPlanArgs& a, int32_t b, int64_t L) {
+  if (a.n < 1) return 0;
+  const SharedGroup g = shared_group(a, shared_group_of(a, b));
+  return b >= g.b0 && b - g.b0 < g.rows / a.R && L >= g.keys ? g.keys : 0;
+}
+
+// Key tiles per piece of the shared keys (all wave's lanes; 0: no shared keys).
+// Lane i prices i + 1 times `mult` pieces of the longest group, in 1/8 of a
+// key-tile step of one workgroup: the end of the last piece where F workgroups
+// are free at once and `own` of them after the own keys' time, each piece taking
+// kFixed steps and its tiles; the partials' traffic; the merge's chain.
+template <int D>
+GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
+  constexpr int kSlots = kSharedSlots<D>, kFixed = 8, kOwn = 8;
+  const int lane = threadIdx.x & 63;
+  auto group = [&](int c) { return c + lane < a.n ? shared_group(a, c + lane) : SharedGroup{}; };
+  int top = 0, rt = 0;
+  for (int c = 0; c < a.n; c += 64) {
+    const SharedGroup g = group(c);
+    const int n = (g.keys + kSharedTile - 1) / kSharedTile;
+    top = n > top ? n : top;
+    rt += wave_sum(g.rt);
+  }
+  const int nmax = wave_top(top);
+  if (nmax == 0) return 0;
+  const int64_t least = (int64_t)rt * a.Hkv;
+  const int mult = least < kSlots ? (kSlots + 64 * (int)least - 1) / (64 * (int)least) : 1, want = (lane + 1) * mult;
+  int tiles = (nmax + want - 1) / want;
+  tiles += tiles & 1;
+  const float inv = __builtin_amdgcn_rcpf((float)tiles);
+  int64_t wgs = 0;
+  for (int c = 0; c < a.n; c += 64) {
+    const SharedGroup g = group(c);
+    const int m = a.n - c < 64 ? a.n - c : 64;
+    for (int j = 0; j < m; ++j) {
+      const int n = (__builtin_amdgcn_readlane(g.keys, j) + kSharedTile - 1) / kSharedTile;
+      wgs += __mul24(__builtin_amdgcn_readlane(g.rt, j), n > 0 ? split_further(n, tiles, inv) + 1 : 0);
+    }
+  }
+  wgs *= a.Hkv;
+  const bool fits = wgs <= a.slots;
+  const int x = fits ? (int)wgs : 0, len = 8 * (kFixed + tiles);
+  const int own = a.own_wgs < kSlots ? a.own_wgs : kSlots, F = kSlots - own;
+  const int64_t t64 = (int64_t)prices * a.Hkv * D / 11000;  // (5.2 TB/s of K and V)
+  const int t = t64 < 8 * kOwn ? 8 * kOwn : t64 < 1 << 22 ? (int)t64 : 1 << 22;
+  int M = len * ((x + kSlots - 1) / kSlots) + (F == 0 ? t : 0);
+  for (int i = 0; i < 64 && F > 0; ++i) {
+    const int after = M > t ? (M - t) / len : 0;
+    if ((M / len) * F + after * own >= x) break;
+    const int next = (M / len + 1) * len, next_own = t + (after + 1) * len;
+    M = next < next_own ? next : next_own;
+  }
+  const int64_t cost = (int64_t)M + (int64_t)x * D / 1400 + (nmax / tiles) / 4;
+  const int c24 = fits && cost < 1 << 24 ? (int)cost : 1 << 24;
+  // (the smallest, of equals the one with fewer pieces; one piece always fits)
+  const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
+  return __builtin_amdgcn_readlane(fits ? tiles : 0, best);
+}
+
+// Sum over the threads before this one; *all: over all 1,024.
+GDN_DEVICE int32_t block_exclusive(int32_t x, int32_t* wsum, int32_t* all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int32_t inc = wave_inclusive_scan_i32(x);
+  __syncthreads();
+  if (lane == 63) wsum[w] = inc;
+  __syncthreads();
+  int32_t base = 0, sum = 0;
+  for (int i = 0; i < 16; ++i) {
+    base += i < w ? wsum[i] : 0;
+    sum += wsum[i];
+  }
+  *all = sum;
+  return base + inc - x;
+}
+
+// The plan: the price prefix of the own keys (as attn_decode_prices_kernel's),
+// the groups' pieces and slots, and what each sequence and workgroup reads.
+// Consecutive workgroups go to the 8 XCDs in turn, so an eighth of the slots,
+// ordered (kv head, group, piece, block), is dealt to each: the blocks over the
+// same keys run on one XCD and read them from its L2.
+template <int D>
+__global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs a) {
+  __shared__ int32_t wsum[16], tiles_lds;
+  const int tid = threadIdx.x, per = (a.B + 1023) / 1024;
+  auto price_of = [&](int32_t b) -> int32_t {
+    if (b >= a.B) return 0;
+    const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, a.cap);
+    const int32_t t = (int32_t)((L - shared_first(a, b, L) + 15) / 16);
+    return t > 0 ? t + kDecodeStartPrice : 0;
+  };
+  int32_t sum = 0, total;
+  for (int i = 0; i < per; ++i) sum += price_of(tid * per + i);
+  int32_t run = block_exclusive(sum, wsum, &total);
+  for (int i = 0; i < per; ++i) {
+    const int32_t b = tid * per + i;
+    if (b >= a.B) break;
+    a.prices[b] = run;
+    run += per == 1 ? sum : price_of(b);
+  }
+  if (tid == 0) a.prices[a.B] = total;
+  if (tid < 64) {
+    const int t = shared_tiles<D>(a, total);
+    if (tid == 0) tiles_lds = t;
+  }
+  __syncthreads();
+
+  // groups: pieces, slots, and the first sequence that is as long as the shared
+  // keys (a padding one may have no table)
+  const int tiles = tiles_lds;
+  const float inv = __builtin_amdgcn_rcpf((float)tiles);
+  int32_t slots = 0;
+  for (int32_t c = 0; c < a.n; c += 1024) {
+    SharedGroup g{};
+    if (c + tid < a.n) {
+      g = shared_group(a, c + tid);
+      if (tiles > 0 && g.keys > 0) g.pieces = split_further((g.keys + kSharedTile - 1) / kSharedTile, tiles, inv) + 1;
+      const int32_t nb = g.pieces > 0 ? g.rows / a.R : 0;
+      g.lead = -1;
+      for (int32_t b = 0; b < nb && g.lead < 0; b += 4) {
+        bool ok[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ok[e] = load_index(a.ctx, g.b0 + (b + e < nb ? b + e : 0), a.ctx64) >= g.keys;
+        g.lead = ok[0] ? b : ok[1] ? b + 1 : ok[2] ? b + 2 : ok[3] ? b + 3 : -1;
+      }
+      // (past the end the first sequence was looked at again: not long enough)
+      if (g.lead >= 0) g.lead += g.b0;
+    }
+    int32_t all;
+    const int32_t before = block_exclusive(g.rt * g.pieces, wsum, &all);
+    g.slot = slots + before;
+    if (c + tid < a.n) a.group[c + tid] = g;
+    slots += all;
+  }
+  if (tid == 0) *a.per_head = slots;
+  __syncthreads();
+
+  for (int32_t b = tid; b < a.B; b += 1024) {
+    SharedSeq s{};
+    if (a.n > 0) {
+      const SharedGroup g = a.group[shared_group_of(a, b)];
+      const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, a.cap);
+      const bool in = b >= g.b0 && b - g.b0 < g.rows / a.R && L >= g.keys;
+      s = SharedSeq{in ? g.keys : 0, g.rt << 11 | (in ? g.pieces : 0), g.slot, (b - g.b0) * a.R};
+    }
+    a.seqs[b] = s;
+  }
+  const uint32_t all = (uint32_t)slots * a.Hkv, xcd = (all + 7) / 8;
+  for (uint32_t id = tid; id < (uint32_t)a.grid; id += 1024) {
+    SharedWork k{};
+    k.lead = -1;
+    const uint32_t slot = (id & 7) * xcd + (id >> 3);
+    if ((id >> 3) < xcd && slot < all) {
+      k.kvh = (int32_t)(slot / (uint32_t)slots);
+      const int32_t left = (int32_t)slot - k.kvh * slots;
+      int32_t lo = 0, hi = a.n;  // the last group with slot <= left (one without slots has the next one's)
+      while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) / 2;
+        if (a.group[mid].slot <= left) lo = mid;
+        else hi = mid;
+      }
+      const SharedGroup g = a.group[lo];
+      const int32_t piece = (left - g.slot) / g.rt, end = (piece + 1) * tiles * kSharedTile;
+      k = SharedWork{g.lead, g.b0, g.rows, 128 * (left - g.slot - piece * g.rt), piece * tiles,
+                     end < g.keys ? end : g.keys, k.kvh, (int32_t)slot};
+    }
+    a.work[id] = k;
+  }
+}
+
 // Merge of the pieces of 32 rows (sequence, head of a kv head) and 32 dims, laid
 // out as the prefill kernel's accumulators: lane l has row l % 32 and 4 x 4 dims.
 // The four waves take every fourth piece, the shared ones first, and merge
 // through LDS.
-template <typename T, int D, int BN>
-__global__ __launch_bounds__(256) void shared_decode_combine_kernel(const AttnArgs a, const DecodeArgs d) {
+template <typename T, int D>
+__global__ __launch_bounds__(256) void shared_decode_combine_kernel(const SharedAttnArgs a, const int32_t* per_head) {
   typedef typename Mma<T>::v4 v4;
   __shared__ float part[4][18][64];
+  const DecodeArgs& d = a.own;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int R = a.Hq / a.Hkv, kvh = blockIdx.z, hh = lane >> 5;
+  const int R = a.Hq / a.Hkv, kvh = blockIdx.z, hh = lane >> 5, dim0 = 32 * blockIdx.y;
   const uint32_t nrows = (uint32_t)a.T * R, row = blockIdx.x * 32 + (lane & 31);
   const bool valid = row < nrows;
-  const uint32_t b = (valid ? row : 0u) / R;
-  const int head = kvh * R + (int)((valid ? row : 0u) - b * R);
-  const int64_t cap = a.tab.cols * a.tab.page, L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
-
+  const uint32_t b = (valid ? row : 0u) / (uint32_t)R, h = (valid ? row : 0u) - b * R;
+  const int head = kvh * R + (int)h;
+  const SharedSeq q = d.seqs[b];
+  const int64_t Pt = d.prices[d.B], qb = d.prices[b], qn = d.prices[b + 1], U = (int64_t)d.B * d.units;
   // shared pieces: np of them, rt slots apart
-  int np = 0, rt = 0, first = 0, pl = 0;
-  const int tiles = shared_tiles<D, BN>(a);
-  if (tiles != kWholeRows) {
-    const float inv = __builtin_amdgcn_rcpf((float)tiles);
-    const int g = shared_group_of(a.sh, b, a.T);
-    int per_head = 0;
-    for (int c = 0; c < a.sh.n; c += 64) {
-      const SharedRows q = shared_rows_lane<BN>(a, c);
-      const int x = q.rt * shared_pieces(q.n, tiles, inv), m = a.sh.n - c < 64 ? a.sh.n - c : 64;
-      per_head += wave_sum(x);
-      for (int j = 0; j < m; ++j) first += c + j < g ? __builtin_amdgcn_readlane(x, j) : 0;
-    }
-    if (valid && g >= 0) {
-      const SharedGroup sg = shared_group(a.sh, g, a.T, cap);
-      const SharedRows q = shared_rows<BN>(a, sg);
-      const int r = (int)row - (int)sg.b0 * R;
-      np = sg.keys > 0 && L >= sg.keys ? shared_pieces(q.n, tiles, inv) : 0;
-      rt = q.rt;
-      first += kvh * per_head + (r >> 7);
-      pl = (int)prefill_part_wave<D>() * ((r >> 5) & 3) + (r & 31) + 32 * hh;  // (m's offset less 32 D)
-    }
-  }
+  const int np = valid ? q.pieces & kMaxPieces11 : 0, rt = q.pieces >> 11, r = q.row + (int)h;
+  const int64_t first = (int64_t)kvh * *per_head + q.slot + (r >> 7);
+  const float* const mine = a.part + prefill_part_wave<D>() * ((r >> 5) & 3);
+  const int pl = (r & 31) + 32 * hh;  // the row's lane there
   // own pieces: units u0 .. u0 + ns - 1
-  const int64_t U = (int64_t)d.B * d.units, Pt = d.prices[d.B], qb = d.prices[b], qn = d.prices[b + 1];
   int64_t u0 = 0;
   int ns = 0;
   if (valid && qn > qb) {
     u0 = ((qb + kDecodeStartPrice + 1) * U - 1) / Pt;
     ns = (int)((qn * U - 1) / Pt - u0) + 1;
   }
+  const bool all_units = Pt >= U;  // every unit has a price range, and a piece
 
-  const int dim0 = 32 * blockIdx.y;
   f32x4 acc[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -70,13 +276,12 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const AttnAr
 #pragma unroll 2
   for (int i = w; i < most; i += 4) {
     const int64_t u = u0 + i - np;
-    // (a unit without a price range, where there are more units than prices, has no piece)
-    const bool own = i >= np, any = i < np + ns && (!own || (u + 1) * Pt / U > u * Pt / U);
-    if (!any) continue;
+    const bool own = i >= np;
+    if (i >= np + ns || (own && !all_units && (u + 1) * Pt / U <= u * Pt / U)) continue;
     const float* pp = own ? d.part + ((b + u) * d.Hq + head) * (int64_t)(D + 4)
-                          : a.part + (first + (int64_t)i * rt) * prefill_part_floats<D>();
-    const float m = own ? pp[D] : pp[pl + 32 * D], lp = own ? pp[D + 1] : pp[pl + 32 * D + 64];
-    const float* po = own ? pp + dim0 + 4 * hh : pp + (pl - pl % 64) + 8 * 32 * (int)blockIdx.y * 4 + 4 * (pl % 64);
+                          : mine + (first + (int64_t)i * rt) * prefill_part_floats<D>();
+    const float m = pp[own ? D : 32 * D + pl], lp = pp[own ? D + 1 : 32 * D + 64 + pl];
+    const float* po = pp + (own ? dim0 + 4 * hh : 32 * dim0 + 4 * pl);
     f32x4 o[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) o[g] = *reinterpret_cast<const f32x4*>(po + (own ? 8 : 256) * g);
@@ -113,63 +318,73 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const AttnAr
     *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + b * a.o_st + (int64_t)head * a.o_sh + dim0 + 8 * w + 4 * hh) = ov;
 }
 
+// The workspace, in floats: the decode's, the plan, the shared pieces' partials.
 // Workgroups that the shared keys may take: one per 128 rows of a group and kv
 // head, up to four times as many or one round of the chip in pieces, within
 // 512 MiB of partials.
-int64_t shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
-  const int64_t most = std::min(groups, B / 2);  // (groups of two sequences at least)
+struct SharedSpace {
+  int64_t slots, grid, own, seqs, group, work, part, all;
+};
+SharedSpace shared_space(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t D, int64_t own) {
+  SharedSpace s{};
+  const int64_t most = std::min(n, B / 2);  // (groups of two sequences at least)
   const int64_t base = Hkv * (B * (Hq / Hkv) / 128 + most), chip = D == 256 ? 256 : D == 128 ? 512 : 768;
   const int64_t fit = (int64_t(1) << 27) / (4 * (32 * D + 128));
-  return most > 0 ? std::max(base, std::min(std::max(4 * base, chip), fit)) : 0;
+  s.slots = most > 0 ? std::max(base, std::min(std::max(4 * base, chip), fit)) : 0;
+  s.grid = (s.slots + 7) / 8 * 8;
+  s.own = own;
+  s.seqs = own + 4;  // (per_head before them)
+  s.group = s.seqs + B * 4;
+  s.work = s.group + n * 8;
+  s.part = s.work + s.grid * 8;
+  s.all = s.part + s.slots * 4 * (32 * D + 128);
+  return s;
 }
 
 template <typename T, int D>
-hipError_t launch_shared(const AttnArgs& a, const DecodeArgs& d, hipStream_t st) {
-  constexpr int BN = 32;
-  if (a.extra > 0) {
-    const dim3 grid((unsigned)((a.extra + 7) / 8 * 8));
-    if (!whole_groups(a))
-      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 1, false, 0, kShared>), grid, dim3(256), 0, st, a);
-    else if (a.tab.is64)
-      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, false, 0, kShared>), grid, dim3(256), 0, st, a);
-    else
-      hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, false, 0, kShared>), grid, dim3(256), 0, st, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  const hipError_t e = launch_decode_t<T, D, kShared>(d, st);
+hipError_t launch_shared(const SharedAttnArgs& a, const SharedPlanArgs& p, hipStream_t st) {
+  constexpr int BN = kSharedTile;
+  shared_plan_kernel<D><<<dim3(1), dim3(1024), 0, st>>>(p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const dim3 grid(a.own_wgs + (unsigned)p.grid);
+  if (!whole_groups(a))
+    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 1, false, 0, kShared>), grid, dim3(256), 0, st, a);
+  else if (a.tab.is64)
+    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 3, false, 0, kShared>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_prefill_kernel<T, D, BN, 2, false, 0, kShared>), grid, dim3(256), 0, st, a);
+  e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t rows = a.T * (a.Hq / a.Hkv);
-  hipLaunchKernelGGL((shared_decode_combine_kernel<T, D, BN>),
-                     dim3((unsigned)((rows + 31) / 32), D / 32, (unsigned)a.Hkv), dim3(256), 0, st, a, d);
+  hipLaunchKernelGGL((shared_decode_combine_kernel<T, D>),
+                     dim3((unsigned)((rows + 31) / 32), D / 32, (unsigned)a.Hkv), dim3(256), 0, st, a, p.per_head);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
-  return shared_slots(B, groups, Hq, Hkv, D);
+  return shared_space(B, groups, Hq, Hkv, D, 0).slots;
 }
 
-int64_t attn_shared_partials(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
-  return shared_slots(B, groups, Hq, Hkv, D) * 4 * (32 * D + 128);
+int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t own) {
+  return shared_space(B, groups, Hq, Hkv, D, own).all;
 }
 
-// workspace: the decode kernel's, `own` floats, then the shared pieces'
+// workspace: attn_shared_floats() of them, the first `own` the decode kernel's
 hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                      const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
                                      const gdn_tensor* groups, gdn_tensor* out, float* workspace, int64_t own,
                                      int32_t splits, float scale, hipStream_t st) {
   if (q->shape[0] == 0) return hipSuccess;
-  DecodeArgs d = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
-  d.sh.lens = lens->data;
-  d.sh.lens64 = lens->dtype == GDN_DTYPE_I64;
-  d.sh.n = (int32_t)lens->shape[0];
-  if (groups) {
-    d.sh.groups = groups->data;
-    d.sh.groups64 = groups->dtype == GDN_DTYPE_I64;
-  }
-  AttnArgs a{};
+  const int64_t n = lens->shape[0], D = q->shape[2];
+  const SharedSpace sp = shared_space(q->shape[0], n, q->shape[1], kc->shape[2], D, own);
+  SharedAttnArgs a{};
+  DecodeArgs& d = a.own;
+  d = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
+  d.prices_inline = false;
+  d.seqs = reinterpret_cast<const SharedSeq*>(workspace + sp.seqs);
   a.q = d.q;
   a.q_st = d.q_ss;
   a.q_sh = d.q_sh;
@@ -186,17 +401,40 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   a.Hq = d.Hq;
   a.Hkv = d.Hkv;
   a.gh = 1;  // a wave per 32 rows
-  a.dim = (int32_t)q->shape[2];
+  a.dim = (int32_t)D;
   a.c = d.c;
-  a.sh = d.sh;
-  a.part = workspace + own;
-  a.extra = (int32_t)shared_slots(d.B, d.sh.n, d.Hq, d.Hkv, a.dim);
-  if (q->dtype == GDN_DTYPE_BF16) {
-    if (a.dim == 64) return launch_shared<bf16_t, 64>(a, d, st);
-    if (a.dim == 128) return launch_shared<bf16_t, 128>(a, d, st);
-    return launch_shared<bf16_t, 256>(a, d, st);
+  a.part = workspace + sp.part;
+  a.work = reinterpret_cast<const SharedWork*>(workspace + sp.work);
+  const int64_t blocks = (int64_t)d.B * d.units * (d.Hkv / d.kvw) * ((d.Hq / d.Hkv + 15) / 16);
+  a.own_wgs = (uint32_t)((blocks * d.kvw + 31) / 32 * 8);
+  SharedPlanArgs p{};
+  p.ctx = d.ctx;
+  p.ctx64 = d.ctx64;
+  p.lens = lens->data;
+  p.lens64 = lens->dtype == GDN_DTYPE_I64;
+  if (groups) {
+    p.groups = groups->data;
+    p.groups64 = groups->dtype == GDN_DTYPE_I64;
   }
-  if (a.dim == 64) return launch_shared<f16_t, 64>(a, d, st);
-  if (a.dim == 128) return launch_shared<f16_t, 128>(a, d, st);
-  return launch_shared<f16_t, 256>(a, d, st);
+  p.B = d.B;
+  p.n = (int32_t)n;
+  p.R = d.Hq / d.Hkv;
+  p.Hkv = d.Hkv;
+  p.cap = d.tab.cols * d.tab.page;
+  p.slots = (int32_t)sp.slots;
+  p.grid = (int32_t)sp.grid;
+  p.own_wgs = (int32_t)a.own_wgs;
+  p.prices = d.prices;
+  p.per_head = reinterpret_cast<int32_t*>(workspace + sp.own);
+  p.seqs = reinterpret_cast<SharedSeq*>(workspace + sp.seqs);
+  p.group = reinterpret_cast<SharedGroup*>(workspace + sp.group);
+  p.work = reinterpret_cast<SharedWork*>(workspace + sp.work);
+  if (q->dtype == GDN_DTYPE_BF16) {
+    if (D == 64) return launch_shared<bf16_t, 64>(a, p, st);
+    if (D == 128) return launch_shared<bf16_t, 128>(a, p, st);
+    return launch_shared<bf16_t, 256>(a, p, st);
+  }
+  if (D == 64) return launch_shared<f16_t, 64>(a, p, st);
+  if (D == 128) return launch_shared<f16_t, 128>(a, p, st);
+  return launch_shared<f16_t, 256>(a, p, st);
 }

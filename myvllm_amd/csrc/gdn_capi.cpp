@@ -66,7 +66,7 @@ hipError_t attn_decode_scored_launch(const gdn_tensor* q, const gdn_tensor* kc, 
                                      const gdn_tensor* slopes, int32_t splits, float scale, float cap,
                                      hipStream_t st);
 int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
-int64_t attn_shared_partials(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
+int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t own);
 hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                      const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
                                      const gdn_tensor* groups, gdn_tensor* out, float* workspace, int64_t own,
@@ -833,8 +833,8 @@ GDN_EXPORT int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs
   if (num_seqs < 0 || num_groups < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return paged_attention_decode_workspace_size(num_seqs, num_q_heads, head_dim, num_splits) +
-         attn_shared_partials(num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim);
+  return attn_shared_floats(num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim,
+                            paged_attention_decode_workspace_size(num_seqs, num_q_heads, head_dim, num_splits));
 }
 
 GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache,
@@ -859,11 +859,12 @@ GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tens
   // rows, key positions and workgroups are counted in 32 bits
   if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ ||
       block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31) ||
-      attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20))
+      attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20) ||
+      B * (num_splits - 1) > kMaxGrid / 2 / (Hkv * ((Hq / Hkv + 15) / 16)))
     return GDN_ERR_RANGE;
   const int64_t own = paged_attention_decode_workspace_size(B, Hq, D, num_splits);
   float* ws;
-  GDN_TRY(decode_workspace(workspace, own + attn_shared_partials(B, G, Hq, Hkv, D), num_splits, B, &ws));
+  GDN_TRY(decode_workspace(workspace, attn_shared_floats(B, G, Hq, Hkv, D, own), num_splits, B, &ws));
   return launch_rc(attn_decode_shared_launch(q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups,
                                              out, ws, own, num_splits, scale, reinterpret_cast<hipStream_t>(stream)));
 }

@@ -95,15 +95,16 @@ def test_shared_range():
 
 
 def test_shared_workspace():
-    """The decode's own, then 128 rows of D + 4 floats per workgroup of shared keys; none for single sequences."""
+    """The decode's own, the plan, 128 rows of D + 4 floats per workgroup of shared keys; none for single sequences."""
     size = _lib.load().paged_attention_decode_shared_workspace_size
     own = _lib.load().paged_attention_decode_workspace_size
-    assert size(1, 1, 16, 2, 256, 4) == own(1, 16, 256, 4)
-    assert size(64, 0, 16, 2, 256, 4) == own(64, 16, 256, 4)
-    assert size(4, 1, 16, 2, 256, 4) - own(4, 16, 256, 4) == 256 * 128 * 260
+    plan = lambda B, G, wgs: 4 + 4 * B + 8 * G + 8 * (-(-wgs // 8) * 8)  # noqa: E731
+    assert size(1, 1, 16, 2, 256, 4) == own(1, 16, 256, 4) + plan(1, 1, 0)
+    assert size(64, 0, 16, 2, 256, 4) == own(64, 16, 256, 4) + plan(64, 0, 0)
+    assert size(4, 1, 16, 2, 256, 4) - own(4, 16, 256, 4) == 256 * 128 * 260 + plan(4, 1, 256)
     assert size(4, 1, 16, 2, 96, 4) == 0 and size(4, 1, 16, 3, 64, 4) == 0
     rows = 2 * (65535 * 8 // 128 + 1)
-    assert size(65535, 1, 16, 2, 256, 2) - own(65535, 16, 256, 2) == rows * 128 * 260
+    assert size(65535, 1, 16, 2, 256, 2) - own(65535, 16, 256, 2) == rows * 128 * 260 + plan(65535, 1, rows)
 
 
 def test_python_refusals():
