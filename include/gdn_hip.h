@@ -444,16 +444,15 @@ int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tensor* k_cache
  *   the same first prefix_lens[g] keys and values.  They are read through the
  *   block table of the first of them that is that long; a shorter sequence, and
  *   one in no group, is read through its own table alone.
- *   num_splits 2..256, as for paged_attention_decode, for each sequence's own
- *   keys.  workspace: 1-D fp32, 16-byte aligned, overwritten, of
+ *   workspace: 1-D fp32, 16-byte aligned, overwritten, of
  *   paged_attention_decode_shared_workspace_size elements.
  */
 int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_q_heads,
-                                                     int64_t num_kv_heads, int64_t head_dim, int32_t num_splits);
+                                                     int64_t num_kv_heads, int64_t head_dim);
 int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                                   const gdn_tensor* block_tables, const gdn_tensor* context_lens,
                                   const gdn_tensor* prefix_lens, const gdn_tensor* cu_groups, gdn_tensor* out,
-                                  gdn_tensor* workspace, int32_t num_splits, float scale, void* stream);
+                                  gdn_tensor* workspace, float scale, void* stream);
 
 /*
  * Append of new tokens to the paged caches, with the position rotation of q

@@ -176,11 +176,11 @@ def load() -> ctypes.CDLL:
             ("flash_attention_varlen_scored", [_PT] * 7 + [L, F, F, I, P]),
             ("paged_attention_prefill_scored", [_PT] * 10 + [L, F, F, P]),
             ("paged_attention_decode_scored", [_PT] * 8 + [I, F, F, P]),
-            ("paged_attention_decode_shared", [_PT] * 9 + [I, F, P]),
+            ("paged_attention_decode_shared", [_PT] * 9 + [F, P]),
         ):
             getattr(lib, fn).restype, getattr(lib, fn).argtypes = ctypes.c_int, types
         lib.paged_attention_decode_shared_workspace_size.restype = L
-        lib.paged_attention_decode_shared_workspace_size.argtypes = [L] * 5 + [I]
+        lib.paged_attention_decode_shared_workspace_size.argtypes = [L] * 5
         lib.paged_kv_append.restype = ctypes.c_int
         lib.paged_kv_append.argtypes = [_PT] * 11 + [ctypes.c_int32, ctypes.c_void_p]
         lib.gdn_hbm_copy.restype = ctypes.c_int

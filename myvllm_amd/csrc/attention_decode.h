@@ -45,14 +45,16 @@ struct DecodeArgs {
   float* part;     // (B + U = B splits, Hq, D + 4): O, m, l per piece (rows padded to 16 bytes)
   int32_t* prices;  // (B + 1): the price prefix Q (splits > 1)
   int32_t B, Hq, Hkv, splits, kvw;
-  int32_t units;  // splits > 1: units per sequence, splits - 1 (U = B units)
+  int32_t units;  // splits > 1: units per sequence, splits - 1 (U = B units); shared: of waves in the grid
   float c;
   bool ctx64;
   bool prices_inline;  // the decode waves compute Q themselves (small batches)
   // kScored: as in the prefill's arguments
   float cap_in, cap_out;
   const float* slopes;
-  const SharedSeq* seqs;  // kShared: a sequence's keys here are those past its group's
+  // kShared: a sequence's keys here are those past its group's, dealt over head[1] units
+  const SharedSeq* seqs;
+  const int32_t* head;
 };
 
 // Price prefix of the batch for the split decode: Q[b] = sum over b' < b of
@@ -100,9 +102,8 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
 template <typename T, int D>
 constexpr size_t decode_lds_per_wave() { return (size_t)16 * (D + 16) * sizeof(T) + (size_t)(D / 32) * 64 * 16; }
 
-// One wave of it: wave wv of block (bx, by, bz), with decode_lds_per_wave() of LDS.
-template <typename T, int D, bool PAGE16, AttnForm FORM>
-GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_t bx, uint32_t by, uint32_t bz) {
+template <typename T, int D, bool PAGE16, AttnForm FORM = kPlain>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_kernel(const DecodeArgs a) {
   typedef Mma<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v4 v4;
@@ -111,15 +112,16 @@ GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_
   constexpr int NDT = D / 16;
   constexpr int CH = D / 8;
   constexpr int NLD = 16 * CH / 64;
-  const int lane = threadIdx.x & 63;
+  extern __shared__ __align__(16) char decode_smem[];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // this wave's LDS: the V tile, then its query fragments
-  T* vs = reinterpret_cast<T*>(lds);
+  T* vs = reinterpret_cast<T*>(decode_smem + wv * decode_lds_per_wave<T, D>());
   v8* qs = reinterpret_cast<v8*>(vs + 16 * LDV);
   const int64_t cap = a.tab.cols * a.tab.page;
 
   const int R = a.Hq / a.Hkv, hgroups = (R + 15) / 16;
-  const int kvh = (by / hgroups) * a.kvw + wv;
-  const int hcol = (by % hgroups) * 16 + (lane & 15);
+  const int kvh = (blockIdx.y / hgroups) * a.kvw + wv;
+  const int hcol = (blockIdx.y % hgroups) * 16 + (lane & 15);
   const bool hvalid = hcol < R;
   const int head = kvh * R + (hvalid ? hcol : 0);
   const int grp = lane >> 4;
@@ -344,10 +346,10 @@ GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_
   // with one split, unit z is sequence z; else unit u holds the batch's
   // prices [x0, x1) (they fit 31 bits, which the entry point checks)
   constexpr int32_t SP = kDecodeStartPrice;
-  int32_t b = bz, x0 = 0, x1 = 0, qb = 0;
+  int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
   if (a.splits > 1) {
     const int64_t U = (int64_t)a.B * a.units;
-    const int64_t u = (int64_t)bz * a.units + bx;
+    const int64_t u = (int64_t)blockIdx.z * a.units + blockIdx.x;
     if (a.prices_inline) {
       // small batch: every wave sums the prices itself (a lane per sequence,
       // 64 at a time), then finds the sequence holding price x0 in a second
@@ -365,7 +367,7 @@ GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_
       tot = __builtin_amdgcn_readfirstlane(tot);
       x0 = (int32_t)(u * tot / U);
       x1 = (int32_t)((u + 1) * tot / U);
-      const bool writer = u == 0 && by == 0 && wv == 0;
+      const bool writer = u == 0 && blockIdx.y == 0 && wv == 0;
       if (writer && lane == 0) a.prices[a.B] = tot;
       if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
       int32_t run = 0;
@@ -422,30 +424,20 @@ GDN_DEVICE void attn_decode_wave(const DecodeArgs& a, char* lds, int wv, uint32_
     int64_t k_lo = 0, k_hi = L, slot = -1;
     bool any = true;
     if (a.splits > 1) {
-      const int64_t first = FORM == kShared ? a.seqs[b].first : 0;
-      const int32_t tb = (int32_t)((L - first + 15) / 16);  // the sequence's tiles
+      const int32_t tb = (int32_t)((L + 15) / 16);  // the sequence's tiles
       qn = qb + (tb > 0 ? tb + SP : 0);
       const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
       const int32_t t0 = r0 < 0 ? 0 : (r0 > tb ? tb : r0), t1 = r1 < 0 ? 0 : (r1 > tb ? tb : r1);
-      k_lo = first + 16 * (int64_t)t0;
-      k_hi = first + 16 * (int64_t)t1 < L ? first + 16 * (int64_t)t1 : L;
+      k_lo = 16 * (int64_t)t0;
+      k_hi = 16 * (int64_t)t1 < L ? 16 * (int64_t)t1 : L;
       any = t1 > t0;
-      // (shared: every piece is merged with the group's)
-      if (FORM == kShared || t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)bz * a.units + bx;
+      if (t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
     }
     if (any) piece(b, k_lo, k_hi, slot, L - 1);
     if (a.splits == 1 || qn >= x1) break;
     ++b;
     qb = qn;
   }
-}
-
-template <typename T, int D, bool PAGE16, AttnForm FORM = kPlain>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_kernel(const DecodeArgs a) {
-  extern __shared__ __align__(16) char decode_smem[];
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  attn_decode_wave<T, D, PAGE16, FORM>(a, decode_smem + wv * decode_lds_per_wave<T, D>(), wv, blockIdx.x, blockIdx.y,
-                                       blockIdx.z);
 }
 
 // Merge of the pieces of one (sequence, query head): one wave, D / 64

@@ -14,7 +14,7 @@
 
 #include <type_traits>
 
-#include "attention_decode.h"
+#include "attention_own.h"
 
 namespace {
 
@@ -445,15 +445,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   int stile0 = 0;
   if constexpr (FORM == kShared) {
     if (blockIdx.x < a.own_wgs) {
-      // a wave per kv head and unit, `kvw` of them a block of the decode's grid;
-      // two waves' LDS lies in the key tiles, two in the value tiles
-      static_assert(2 * decode_lds_per_wave<T, D>() <= sizeof(ks) && sizeof(ks) <= sizeof(vs), "the decode's LDS");
-      const uint32_t kvw = a.own.kvw, v = blockIdx.x * (4 / kvw) + w / kvw;
-      const uint32_t nx = a.own.units, ny = a.own.Hkv / kvw * ((R + 15) / 16), bz = v / (nx * ny);
-      if (bz < (uint32_t)a.own.B)
-        attn_decode_wave<T, D, (PG >= 2), kShared>(
-            a.own, reinterpret_cast<char*>(w < 2 ? ks[0] : vs[0]) + (w & 1) * decode_lds_per_wave<T, D>(), w % kvw,
-            v % nx, v / nx % ny, bz);
+      // a wave per unit, 16 query heads and kv head (the heads of a unit together:
+      // their rows lie side by side); two waves' LDS lies in the key tiles, two in
+      // the value tiles
+      static_assert(2 * own_lds_per_wave<T, D>() <= sizeof(ks) && sizeof(ks) <= sizeof(vs), "the own keys' LDS");
+      const uint32_t id = blockIdx.x * 4 + w, ny = a.Hkv * ((R + 15) / 16), u = id / ny, y = id - u * ny;
+      if (u < (uint32_t)a.own.units)
+        attn_own_wave<T, D, (PG >= 2)>(a.own,
+                                       reinterpret_cast<char*>(w < 2 ? ks[0] : vs[0]) + (w & 1) * own_lds_per_wave<T, D>(),
+                                       u, y % a.Hkv, y / a.Hkv);
       return;
     }
     const SharedWork sw = a.work[blockIdx.x - a.own_wgs];

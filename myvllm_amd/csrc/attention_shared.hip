@@ -18,6 +18,7 @@ namespace {
 constexpr int kSharedTile = 32;  // keys of a tile of the prefill kernel
 template <int D> constexpr int kSharedSlots = D == 256 ? 256 : D == 128 ? 512 : 768;  // workgroups that run at once
 constexpr int kMaxPieces11 = 2047;  // pieces of a row, held in 11 bits
+constexpr int kOwnPrices = 5;
 
 struct SharedGroup {
   int32_t keys, b0, rows;   // keys that are read once for all, first sequence, rows (sequences x heads of a kv head)
@@ -31,8 +32,9 @@ struct SharedPlanArgs {
   int32_t B, n, R, Hkv;  // n groups
   int64_t cap;
   int32_t slots, own_wgs, grid;  // slots of the partials; workgroups of the own keys, and of the shared ones
+  int32_t units;                 // of the own keys, at most
   int32_t* prices;
-  int32_t* per_head;  // slots of a kv head
+  int32_t* head;  // slots of a kv head, units of the own keys
   SharedSeq* seqs;
   SharedGroup* group;
   SharedWork* work;
@@ -113,12 +115,14 @@ GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
   const int own = a.own_wgs < kSlots ? a.own_wgs : kSlots, F = kSlots - own;
   const int64_t t64 = (int64_t)prices * a.Hkv * D / 11000;  // (5.2 TB/s of K and V)
   const int t = t64 < 8 * kOwn ? 8 * kOwn : t64 < 1 << 22 ? (int)t64 : 1 << 22;
-  int M = len * ((x + kSlots - 1) / kSlots) + (F == 0 ? t : 0);
-  for (int i = 0; i < 64 && F > 0; ++i) {
-    const int after = M > t ? (M - t) / len : 0;
-    if ((M / len) * F + after * own >= x) break;
-    const int next = (M / len + 1) * len, next_own = t + (after + 1) * len;
+  // M: where k rounds of the free workgroups and j of the others make x
+  int k = (x + kSlots - 1) / kSlots, j = 0, M = len * k + (F == 0 ? t : 0);
+  while (F > 0 && __builtin_amdgcn_ballot_w64(k * F + j * own < x)) {
+    if (k * F + j * own >= x) continue;
+    const int next = (k + 1) * len, next_own = t + (j + 1) * len;
     M = next < next_own ? next : next_own;
+    k += next <= next_own;
+    j += next_own <= next;
   }
   const int64_t cost = (int64_t)M + (int64_t)x * D / 1400 + (nmax / tiles) / 4;
   const int c24 = fits && cost < 1 << 24 ? (int)cost : 1 << 24;
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
     if (b >= a.B) return 0;
     const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, a.cap);
     const int32_t t = (int32_t)((L - shared_first(a, b, L) + 15) / 16);
-    return t > 0 ? t + kDecodeStartPrice : 0;
+    return t > 0 ? t + kOwnStartPrice : 0;
   };
   int32_t sum = 0, total;
   for (int i = 0; i < per; ++i) sum += price_of(tid * per + i);
@@ -201,7 +205,12 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
     if (c + tid < a.n) a.group[c + tid] = g;
     slots += all;
   }
-  if (tid == 0) *a.per_head = slots;
+  if (tid == 0) {
+    a.head[0] = slots;
+    // (a unit of at least kOwnPrices: shorter ones only leave more to merge)
+    const int32_t u = total / kOwnPrices;
+    a.head[1] = u < 1 ? 1 : u < a.units ? u : a.units;
+  }
   __syncthreads();
 
   for (int32_t b = tid; b < a.B; b += 1024) {
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
 // The four waves take every fourth piece, the shared ones first, and merge
 // through LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void shared_decode_combine_kernel(const SharedAttnArgs a, const int32_t* per_head) {
+__global__ __launch_bounds__(256) void shared_decode_combine_kernel(const SharedAttnArgs a) {
   typedef typename Mma<T>::v4 v4;
   __shared__ float part[4][18][64];
   const DecodeArgs& d = a.own;
@@ -253,17 +262,17 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const Shared
   const uint32_t b = (valid ? row : 0u) / (uint32_t)R, h = (valid ? row : 0u) - b * R;
   const int head = kvh * R + (int)h;
   const SharedSeq q = d.seqs[b];
-  const int64_t Pt = d.prices[d.B], qb = d.prices[b], qn = d.prices[b + 1], U = (int64_t)d.B * d.units;
+  const int64_t Pt = d.prices[d.B], qb = d.prices[b], qn = d.prices[b + 1], U = d.head[1];
   // shared pieces: np of them, rt slots apart
   const int np = valid ? q.pieces & kMaxPieces11 : 0, rt = q.pieces >> 11, r = q.row + (int)h;
-  const int64_t first = (int64_t)kvh * *per_head + q.slot + (r >> 7);
+  const int64_t first = (int64_t)kvh * d.head[0] + q.slot + (r >> 7);
   const float* const mine = a.part + prefill_part_wave<D>() * ((r >> 5) & 3);
   const int pl = (r & 31) + 32 * hh;  // the row's lane there
   // own pieces: units u0 .. u0 + ns - 1
   int64_t u0 = 0;
   int ns = 0;
   if (valid && qn > qb) {
-    u0 = ((qb + kDecodeStartPrice + 1) * U - 1) / Pt;
+    u0 = ((qb + kOwnStartPrice + 1) * U - 1) / Pt;
     ns = (int)((qn * U - 1) / Pt - u0) + 1;
   }
   const bool all_units = Pt >= U;  // every unit has a price range, and a piece
@@ -322,18 +331,25 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const Shared
 // Workgroups that the shared keys may take: one per 128 rows of a group and kv
 // head, up to four times as many or one round of the chip in pieces, within
 // 512 MiB of partials.
+// The own keys are dealt over U units: 384 waves with the heads (96 CUs at
+// D = 256; a CU reads some 42 GB/s whatever its waves have in flight, so HBM's
+// rate takes half the chip), and one per four sequences at least, which it takes
+// a while to begin with.  256 sequences behind 16,384 keys / 64 behind 8,192 with
+// 128 waves 403 / 70 us, 256 226 / 51, 384 179 / 44, 512 190 / 46.
 struct SharedSpace {
-  int64_t slots, grid, own, seqs, group, work, part, all;
+  int64_t units, slots, grid, prices, head, seqs, group, work, part, all;
 };
-SharedSpace shared_space(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t D, int64_t own) {
+SharedSpace shared_space(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t D) {
   SharedSpace s{};
+  s.units = std::max(std::max<int64_t>(384 / (Hkv * ((Hq / Hkv + 15) / 16)), 1), (B + 3) / 4);
   const int64_t most = std::min(n, B / 2);  // (groups of two sequences at least)
   const int64_t base = Hkv * (B * (Hq / Hkv) / 128 + most), chip = D == 256 ? 256 : D == 128 ? 512 : 768;
   const int64_t fit = (int64_t(1) << 27) / (4 * (32 * D + 128));
   s.slots = most > 0 ? std::max(base, std::min(std::max(4 * base, chip), fit)) : 0;
   s.grid = (s.slots + 7) / 8 * 8;
-  s.own = own;
-  s.seqs = own + 4;  // (per_head before them)
+  s.prices = (B + s.units) * Hq * (D + 4);
+  s.head = s.prices + (B + 1 + 3) / 4 * 4;
+  s.seqs = s.head + 4;
   s.group = s.seqs + B * 4;
   s.work = s.group + n * 8;
   s.part = s.work + s.grid * 8;
@@ -358,32 +374,36 @@ hipError_t launch_shared(const SharedAttnArgs& a, const SharedPlanArgs& p, hipSt
   if (e != hipSuccess) return e;
   const int64_t rows = a.T * (a.Hq / a.Hkv);
   hipLaunchKernelGGL((shared_decode_combine_kernel<T, D>),
-                     dim3((unsigned)((rows + 31) / 32), D / 32, (unsigned)a.Hkv), dim3(256), 0, st, a, p.per_head);
+                     dim3((unsigned)((rows + 31) / 32), D / 32, (unsigned)a.Hkv), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
-  return shared_space(B, groups, Hq, Hkv, D, 0).slots;
+  return shared_space(B, groups, Hq, Hkv, D).slots;
 }
 
-int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t own) {
-  return shared_space(B, groups, Hq, Hkv, D, own).all;
+int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
+  return shared_space(B, groups, Hq, Hkv, D).all;
 }
 
-// workspace: attn_shared_floats() of them, the first `own` the decode kernel's
+// workspace: attn_shared_floats() of them
 hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                      const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
-                                     const gdn_tensor* groups, gdn_tensor* out, float* workspace, int64_t own,
-                                     int32_t splits, float scale, hipStream_t st) {
+                                     const gdn_tensor* groups, gdn_tensor* out, float* workspace, float scale,
+                                     hipStream_t st) {
   if (q->shape[0] == 0) return hipSuccess;
   const int64_t n = lens->shape[0], D = q->shape[2];
-  const SharedSpace sp = shared_space(q->shape[0], n, q->shape[1], kc->shape[2], D, own);
+  const SharedSpace sp = shared_space(q->shape[0], n, q->shape[1], kc->shape[2], D);
   SharedAttnArgs a{};
   DecodeArgs& d = a.own;
-  d = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
-  d.prices_inline = false;
+  d = decode_args(q, kc, vc, tab, ctx, out, nullptr, 1, scale);
+  d.splits = 2;  // (more than one)
+  d.units = (int32_t)sp.units;
+  d.part = workspace;
+  d.prices = reinterpret_cast<int32_t*>(workspace + sp.prices);
+  d.head = reinterpret_cast<const int32_t*>(workspace + sp.head);
   d.seqs = reinterpret_cast<const SharedSeq*>(workspace + sp.seqs);
   a.q = d.q;
   a.q_st = d.q_ss;
@@ -405,8 +425,8 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   a.c = d.c;
   a.part = workspace + sp.part;
   a.work = reinterpret_cast<const SharedWork*>(workspace + sp.work);
-  const int64_t blocks = (int64_t)d.B * d.units * (d.Hkv / d.kvw) * ((d.Hq / d.Hkv + 15) / 16);
-  a.own_wgs = (uint32_t)((blocks * d.kvw + 31) / 32 * 8);
+  const int64_t waves = sp.units * d.Hkv * ((d.Hq / d.Hkv + 15) / 16);
+  a.own_wgs = (uint32_t)((waves + 31) / 32 * 8);
   SharedPlanArgs p{};
   p.ctx = d.ctx;
   p.ctx64 = d.ctx64;
@@ -425,7 +445,8 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   p.grid = (int32_t)sp.grid;
   p.own_wgs = (int32_t)a.own_wgs;
   p.prices = d.prices;
-  p.per_head = reinterpret_cast<int32_t*>(workspace + sp.own);
+  p.units = d.units;
+  p.head = reinterpret_cast<int32_t*>(workspace + sp.head);
   p.seqs = reinterpret_cast<SharedSeq*>(workspace + sp.seqs);
   p.group = reinterpret_cast<SharedGroup*>(workspace + sp.group);
   p.work = reinterpret_cast<SharedWork*>(workspace + sp.work);

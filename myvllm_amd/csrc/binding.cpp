@@ -184,11 +184,11 @@ typedef Entry<19, 11, int32_t> KvAppend;
 typedef Entry<20, 7, int64_t, float, float, int32_t> AttnVarlenScored;
 typedef Entry<21, 10, int64_t, float, float> PagedPrefillScored;
 typedef Entry<22, 8, int32_t, float, float> PagedDecodeScored;
-typedef Entry<23, 9, int32_t, float> PagedDecodeShared;
+typedef Entry<23, 9, float> PagedDecodeShared;
 typedef Size<0, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> ChunkPrefillSize;
 typedef Size<1, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> PagedPrefillSize;
 typedef Size<2, int64_t, int64_t, int64_t, int32_t> PagedDecodeSize;
-typedef Size<3, int64_t, int64_t, int64_t, int64_t, int64_t, int32_t> PagedDecodeSharedSize;
+typedef Size<3, int64_t, int64_t, int64_t, int64_t, int64_t> PagedDecodeSharedSize;
 
 struct Bound {
   const char* name;

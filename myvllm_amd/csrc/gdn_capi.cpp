@@ -66,11 +66,11 @@ hipError_t attn_decode_scored_launch(const gdn_tensor* q, const gdn_tensor* kc, 
                                      const gdn_tensor* slopes, int32_t splits, float scale, float cap,
                                      hipStream_t st);
 int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
-int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t own);
+int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
 hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                      const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
-                                     const gdn_tensor* groups, gdn_tensor* out, float* workspace, int64_t own,
-                                     int32_t splits, float scale, hipStream_t st);
+                                     const gdn_tensor* groups, gdn_tensor* out, float* workspace, float scale,
+                                     hipStream_t st);
 int64_t paged_kv_append_waves(int64_t T, int64_t rows, int64_t D);
 hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* kc, gdn_tensor* vc,
                                   const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* q, gdn_tensor* out,
@@ -829,21 +829,19 @@ GDN_EXPORT int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tens
 
 GDN_EXPORT int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs, int64_t num_groups,
                                                                 int64_t num_q_heads, int64_t num_kv_heads,
-                                                                int64_t head_dim, int32_t num_splits) {
+                                                                int64_t head_dim) {
   if (num_seqs < 0 || num_groups < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads % num_kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return attn_shared_floats(num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim,
-                            paged_attention_decode_workspace_size(num_seqs, num_q_heads, head_dim, num_splits));
+  return attn_shared_floats(num_seqs, num_groups, num_q_heads, num_kv_heads, head_dim);
 }
 
 GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache,
                                              const gdn_tensor* v_cache, const gdn_tensor* block_tables,
                                              const gdn_tensor* context_lens, const gdn_tensor* prefix_lens,
                                              const gdn_tensor* cu_groups, gdn_tensor* out, gdn_tensor* workspace,
-                                             int32_t num_splits, float scale, void* stream) {
-  if (num_splits < 2) return GDN_ERR_RANGE;
-  GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits));
+                                             float scale, void* stream) {
+  GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, 2));
   GDN_TRY(check_desc(prefix_lens, 1));
   const int64_t B = q->shape[0], Hq = q->shape[1], D = q->shape[2], Hkv = k_cache->shape[2], G = prefix_lens->shape[0];
   if (!is_index(prefix_lens->dtype)) return GDN_ERR_DTYPE;
@@ -859,14 +857,12 @@ GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tens
   // rows, key positions and workgroups are counted in 32 bits
   if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ ||
       block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31) ||
-      attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20) ||
-      B * (num_splits - 1) > kMaxGrid / 2 / (Hkv * ((Hq / Hkv + 15) / 16)))
+      attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20))
     return GDN_ERR_RANGE;
-  const int64_t own = paged_attention_decode_workspace_size(B, Hq, D, num_splits);
   float* ws;
-  GDN_TRY(decode_workspace(workspace, attn_shared_floats(B, G, Hq, Hkv, D, own), num_splits, B, &ws));
+  GDN_TRY(decode_workspace(workspace, attn_shared_floats(B, G, Hq, Hkv, D), 2, B, &ws));
   return launch_rc(attn_decode_shared_launch(q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups,
-                                             out, ws, own, num_splits, scale, reinterpret_cast<hipStream_t>(stream)));
+                                             out, ws, scale, reinterpret_cast<hipStream_t>(stream)));
 }
 
 GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,

@@ -214,7 +214,6 @@ def paged_flash_attention_decode_shared(
     scale: float,
     block_size: int,
     cu_groups: torch.Tensor | None = None,
-    num_splits: int | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """:func:`paged_flash_attention_decode` for sequences that begin with the
@@ -233,10 +232,8 @@ def paged_flash_attention_decode_shared(
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups)
     B, Hq, Dh = q.shape
-    if num_splits is None:
-        num_splits = max(2, decode_num_splits(B, Hq, k_cache.shape[2], block_tables.shape[1] * block_size))
     n_ws = _lib.workspace_size("paged_attention_decode_shared_workspace_size", B, prefix_lens.numel(), Hq,
-                               k_cache.shape[2], Dh, int(num_splits))
+                               k_cache.shape[2], Dh)
     q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
     o = _out_for(out, (B, Hq, v_cache.shape[-1]), q.dtype, dev)
     try:
@@ -244,7 +241,7 @@ def paged_flash_attention_decode_shared(
     except torch.OutOfMemoryError:
         return paged_flash_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scale, block_size, out=out)
     _lib.call("paged_attention_decode_shared", q, k_cache, v_cache, block_tables, context_lens, prefix_lens, cu_groups,
-              o, ws, int(num_splits), float(scale))
+              o, ws, float(scale))
     return _finish(out, o)
 
 

@@ -57,10 +57,10 @@ def test_decode_refusals(change, code):
 
 
 def shared_args():
-    n = _lib.load().paged_attention_decode_shared_workspace_size(4, 2, 4, 2, 64, 3)
+    n = _lib.load().paged_attention_decode_shared_workspace_size(4, 2, 4, 2, 64)
     return dict(q=Z(4, 4, 64, dtype=BF), kc=Z(6, 16, 2, 64, dtype=BF), vc=Z(6, 16, 2, 64, dtype=BF),
                 tab=Z(4, 3, dtype=I32), ctx=Z(4, dtype=I32), lens=Z(2, dtype=I32), groups=Z(3, dtype=I32),
-                out=Z(4, 4, 64, dtype=BF), ws=Z(n), splits=3)
+                out=Z(4, 4, 64, dtype=BF), ws=Z(n))
 
 
 @cpu_only
@@ -70,7 +70,7 @@ def shared_args():
         (dict(lens=None), NULL), (dict(lens=Z(2)), DTYPE), (dict(lens=Z(4, dtype=I32)[::2]), STRIDE),
         (dict(lens=Z(1, 2, dtype=I32)), NDIM), (dict(lens=Z(3, dtype=I32)), SHAPE), (dict(groups=None), SHAPE),
         (dict(groups=Z(3)), DTYPE), (dict(groups=Z(6, dtype=I32)[::2]), STRIDE), (dict(groups=Z(2, dtype=I32)), SHAPE),
-        (dict(splits=1), RANGE), (dict(splits=257), RANGE), (dict(ws=None), NULL), (dict(ws=Z(8)), SHAPE),
+        (dict(ws=None), NULL), (dict(ws=Z(8)), SHAPE),
         (dict(ws=Z(2 * 10**7, dtype=BF)), DTYPE), (dict(ws=Z(2 * 10**7)[1:]), ALIGN), (dict(ws=Z(2, 2 * 10**7)), NDIM),
         (dict(q=Z(4, 3, 64, dtype=BF), out=Z(4, 3, 64, dtype=BF)), HEADS), (dict(ctx=Z(3, dtype=I32)), SHAPE),
         (dict(out=Z(4, 4, 64)), DTYPE), (dict(kc=Z(6, 16, 2, 72, dtype=BF), vc=Z(6, 16, 2, 72, dtype=BF)), SHAPE),
@@ -78,33 +78,37 @@ def shared_args():
 )
 def test_shared_refusals(change, code):
     a = shared_args() | change
-    splits = a.pop("splits")
-    assert _lib.load().paged_attention_decode_shared(*(D(t) for t in a.values()), splits, 1.0, None) == code
+    assert _lib.load().paged_attention_decode_shared(*(D(t) for t in a.values()), 1.0, None) == code
 
 
 @cpu_only
 def test_shared_range():
     """2^27 columns of 16 keys are 2^31 positions (refused before any HIP call)."""
     a = shared_args()
-    splits = a.pop("splits")
     tab = _lib.describe(a.pop("tab"))
     tab.shape[1] = 2**27
     d = [D(t) for t in a.values()]
     d.insert(3, ctypes.byref(tab))
-    assert _lib.load().paged_attention_decode_shared(*d, splits, 1.0, None) == RANGE
+    assert _lib.load().paged_attention_decode_shared(*d, 1.0, None) == RANGE
 
 
 def test_shared_workspace():
-    """The decode's own, the plan, 128 rows of D + 4 floats per workgroup of shared keys; none for single sequences."""
+    """Partials of the own keys' pieces (a slot per sequence and unit) and their
+    prices, the plan, 128 rows of D + 4 floats per workgroup of shared keys
+    (none for single sequences)."""
     size = _lib.load().paged_attention_decode_shared_workspace_size
-    own = _lib.load().paged_attention_decode_workspace_size
-    plan = lambda B, G, wgs: 4 + 4 * B + 8 * G + 8 * (-(-wgs // 8) * 8)  # noqa: E731
-    assert size(1, 1, 16, 2, 256, 4) == own(1, 16, 256, 4) + plan(1, 1, 0)
-    assert size(64, 0, 16, 2, 256, 4) == own(64, 16, 256, 4) + plan(64, 0, 0)
-    assert size(4, 1, 16, 2, 256, 4) - own(4, 16, 256, 4) == 256 * 128 * 260 + plan(4, 1, 256)
-    assert size(4, 1, 16, 2, 96, 4) == 0 and size(4, 1, 16, 3, 64, 4) == 0
+
+    def want(B, G, Hq, D, units, wgs):
+        return ((B + units) * Hq * (D + 4) + (B + 4) // 4 * 4 + 4 + 4 * B + 8 * G + 8 * (-(-wgs // 8) * 8)
+                + wgs * 128 * (D + 4))
+
+    assert size(1, 1, 16, 2, 256) == want(1, 1, 16, 256, 192, 0)
+    assert size(64, 0, 16, 2, 256) == want(64, 0, 16, 256, 192, 0)
+    assert size(4, 1, 16, 2, 256) == want(4, 1, 16, 256, 192, 256)
+    assert size(4, 1, 128, 2, 64) == want(4, 1, 128, 64, 48, 768)
+    assert size(4, 1, 16, 2, 96) == 0 and size(4, 1, 16, 3, 64) == 0
     rows = 2 * (65535 * 8 // 128 + 1)
-    assert size(65535, 1, 16, 2, 256, 2) - own(65535, 16, 256, 2) == rows * 128 * 260 + plan(65535, 1, rows)
+    assert size(65535, 1, 16, 2, 256) == want(65535, 1, 16, 256, 16384, rows)
 
 
 def test_python_refusals():

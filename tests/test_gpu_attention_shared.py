@@ -47,12 +47,11 @@ def make(groups, Hq, Hkv, D, page=16, dtype=BF, index=torch.int32, seed=0, cols=
                 prefix_lens=torch.tensor([p for p, _ in groups], dtype=index)), torch.tensor(cu, dtype=index)
 
 
-def check(dev, c, cu, scale=None, rows=None, plain=True, splits=None):
+def check(dev, c, cu, scale=None, rows=None, plain=True):
     d = {n: t.to(dev) for n, t in c.items()}
     page, D = c["k_cache"].shape[1], c["q"].shape[2]
     scale = D**-0.5 if scale is None else scale
-    out = paged_flash_attention_decode_shared(*d.values(), scale, page, cu_groups=None if cu is None else cu.to(dev),
-                                              num_splits=splits)
+    out = paged_flash_attention_decode_shared(*d.values(), scale, page, cu_groups=None if cu is None else cu.to(dev))
     for b in range(len(c["q"])) if rows is None else rows:
         L = int(c["context_lens"][b])
         k, v = (gather_paged(c[n], c["block_tables"][b], L) for n in ("k_cache", "v_cache"))
@@ -124,11 +123,13 @@ def test_scales(dev, scale):
     check(dev, c, cu, scale=scale, plain=False)
 
 
-@pytest.mark.parametrize("splits", [2, 7, 256])
-def test_splits(dev, splits):
-    c, cu = make([(500, [600, 3, 0, 90])], 16, 2, 256, seed=6)
-    print(f"shared decode splits={splits}", flush=True)
-    check(dev, c, cu, splits=splits)
+@pytest.mark.parametrize("D, page, index", [(64, 16, torch.int32), (64, 48, torch.int64), (128, 32, torch.int32),
+                                            (256, 16, torch.int64)])
+def test_long_own_keys(dev, D, page, index):
+    """Many kv heads leave few units: pieces of over 1,024 own keys, whose pages are looked up in batches."""
+    c, cu = make([(100, [3000, 17, 2500, 1])], 64, 64, D, page, index=index, seed=6)
+    print(f"shared decode, long own keys D={D} page={page}", flush=True)
+    check(dev, c, cu)
 
 
 def test_many_sequences(dev):
