@@ -14,7 +14,10 @@ constexpr int32_t kOwnStartPrice = 4;
 template <typename T, int D> constexpr size_t own_lds_per_wave() { return (size_t)32 * (D + 8) * sizeof(T); }
 
 // Unit u's pieces for kv head kvh and query heads 16 hg .. + 15 of it, each to its
-// workspace slot b + u.  As attn_decode_kernel, but made for one wave per SIMD,
+// workspace slot b + u.  A CU reads 36 to 45 GB/s of HBM whatever its waves have
+// in flight and however early they read their fragments (548 MB: 32 CUs 377 us,
+// 64 205, 96 159), so what counts is that the waves are on many CUs and never
+// idle.  As attn_decode_kernel, but made for one wave per SIMD,
 // which is all that runs beside the shared keys' tiles at D = 256: 32 keys per
 // step, two 16-key halves whose score MFMAs are independent and whose P V is one
 // 16x16x32 MFMA per 16 dims (the k-slot 8 g + j of lane group g is key 4 g + j of
@@ -64,8 +67,8 @@ GDN_DEVICE void attn_own_wave(const DecodeArgs& a, char* lds, int64_t u, int kvh
       const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_ss + (int64_t)head * a.q_sh + 8 * grp;
 #pragma unroll
       for (int s = 0; s < NKS; ++s) {
-        const v8 q = hvalid ? *reinterpret_cast<const v8*>(qp + 32 * s) : v8{};
-        qf[s] = a.c > 0.f ? q : (a.c < 0.f ? -q : v8{});  // (c > 0 below)
+        const v8 q = *reinterpret_cast<const v8*>(qp + 32 * s);  // (an invalid column's is dropped at the end)
+        qf[s] = a.c > 0.f ? q : (a.c < 0.f ? -q : v8{});         // (c > 0 below)
       }
     }
     // tile t is 16-key group k_lo / 16 + t, in page g / gpp at slot 16 (g % gpp);
