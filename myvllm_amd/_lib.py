@@ -252,6 +252,12 @@ def vec16_ok(t: torch.Tensor) -> bool:
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all((t.stride(i) * es) % 16 == 0 for i in range(t.dim() - 1))
 
 
+def vec16_all(*tensors: torch.Tensor | None) -> bool:
+    """:func:`vec16_ok` of all of them (None aside), in one call."""
+    ok = (_fast or _load_fast()).vec16_ok(*tensors)
+    return ok if ok is not None else all(t is None or vec16_ok(t) for t in tensors)
+
+
 def vec16(t: torch.Tensor) -> torch.Tensor:
     """t itself when the kernels can read it with 16-byte vector accesses, else a
     contiguous copy (also of a contiguous one at a misaligned address): the

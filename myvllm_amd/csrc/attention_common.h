@@ -115,6 +115,38 @@ struct SharedWork {
   int32_t lead, b0, rows, row, tile0, keys, kvh, slot;
 };
 
+// A capped score, cap tanh(x) of x = scale s / cap, is cap - 2 cap / (1 + e^(2 x)),
+// and a constant on all scores of a row does not change its softmax: the raw score
+// s becomes -1 / (1 + 2^(k s)), k = 2 log2(e) scale / cap, which 2 cap log2(e)
+// scales to an exponent of 2, within 2e-7 cap.
+GDN_DEVICE float cap_score(float s, float k) {
+  return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s * k));
+}
+
+// The same as tanh(x) / 2 - 1 / 2 by an odd polynomial of degree 9 for |x| <= 3/4
+// (|s| <= lim; fitted for the least largest error there, 1.9e-7): full-rate
+// instructions instead of the exponential and the reciprocal, and a test of the
+// tile.  It pays where several waves share a SIMD's transcendental unit: D = 64,
+// six prompts capped and biased under a prefix mask 72 -> 65 us, capped alone 57
+// -> 56; D = 128 526 -> 533, D = 256, where a wave has its SIMD to itself, 481 ->
+// 496.
+struct CapNear {
+  float lim, p0, p1, p2, p3, p4;
+  GDN_DEVICE void set(float k) {
+    const float h = k * 0.34657359f, u = h * h;  // x = h s (ln 2 / 2: k is 2 log2(e) scale / cap)
+    lim = h < 1e4f ? 0.75f / h : -1.f;
+    p0 = 0.5f * 0.99999723f * h;
+    p1 = 0.5f * -0.33323076f * h * u;
+    p2 = 0.5f * 0.13226092f * h * u * u;
+    p3 = 0.5f * -0.04928045f * h * u * u * u;
+    p4 = 0.5f * 0.01231883f * h * u * u * u * u;
+  }
+  GDN_DEVICE float operator()(float s) const {
+    const float u = s * s;
+    return __builtin_fmaf(s, __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p4, u, p3), u, p2), u, p1), u, p0), -0.5f);
+  }
+};
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 KvSource kv_source(const gdn_tensor* t, bool paged) {

@@ -128,10 +128,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const char* kvk = a.k.base + kvh * a.k.sh;
   const char* kvv = a.v.base + kvh * a.v.sh;
   const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;
-  const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
-  // scored: the scores become exponents of 2 in the tile, which the softmax scales by 1
-  const float cs = FORM == kScored ? 1.f : c;
-  const float slope = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
+  // (scored: as in the prefill)
+  const float capk = FORM == kScored ? c * a.cap_in : 0.f;
+  if (FORM == kScored && a.cap_out > 0.f) c = a.cap_out;
+  const float sraw = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e / c : 0.f;
 
   // keys [k_lo, k_hi) of sequence b (k_lo a multiple of 16); the result goes
   // to the output (slot < 0) or to workspace slot `slot`
@@ -252,18 +253,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     auto accumulate = [&](int t, f32x4 s) {
       const uint32_t j0 = (uint32_t)k_lo + 16u * (uint32_t)t;  // (key positions fit 32 bits)
       if constexpr (FORM == kScored) {
-        // as in the prefill; the query sits at its sequence's last key
         if (a.cap_out > 0.f) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[r] = __builtin_fmaf(-2.f * a.cap_out,
-                                  __builtin_amdgcn_rcpf(1.f + exp2_fast(s[r] * c * a.cap_in)), a.cap_out);
-        } else {
-          s *= c;
+          for (int r = 0; r < 4; ++r) s[r] = cap_score(s[r], capk);
         }
+        // (the query sits at its sequence's last key)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          s[r] = __builtin_fmaf(slope, (float)((int32_t)(j0 + 4u * grp + r) - (int32_t)last_key), s[r]);
+          s[r] = __builtin_fmaf(sraw, (float)((int32_t)(j0 + 4u * grp + r) - (int32_t)last_key), s[r]);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -274,10 +271,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       // by 2^8, and then to the maximum over the four lanes, taken only on
       // that rare path (the same decisions and bases as taking it every tile)
       const float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-      if (__builtin_amdgcn_ballot_w64(mx * cs > m_used + 8.f) != 0) {
+      if (__builtin_amdgcn_ballot_w64(mx * c > m_used + 8.f) != 0) {
         float mg = fmaxf(mx, __shfl_xor(mx, 16));
         mg = fmaxf(mg, __shfl_xor(mg, 32));
-        const float mn = fmaxf(m_used, mg * cs);
+        const float mn = fmaxf(m_used, mg * c);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
 #pragma unroll
         for (int d = 0; d < NDT; ++d) oacc[d] *= alpha;
@@ -288,7 +285,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       v4 pf;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = exp2_fast(__builtin_fmaf(s[r], cs, nb));
+        const float p = exp2_fast(__builtin_fmaf(s[r], c, nb));
         lsum += p;
         pf[r] = (T)p;
       }

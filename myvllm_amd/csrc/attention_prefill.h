@@ -37,7 +37,7 @@ struct AttnArgs {
   int64_t rows;
   int32_t extra;
   float* part;
-  // kScored: 2 / cap of the tanh cap and cap * log2(e) (cap 0: none), slopes of
+  // kScored: 2 / cap of the tanh cap and 2 cap log2(e) (0: none), slopes of
   // the distance bias (Hq,), and keys of each sequence that all its queries see
   float cap_in, cap_out;
   const float* slopes;
@@ -729,16 +729,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   const int64_t first = FORM == kScored && off + q0 + 1 < pfx ? pfx : off + q0 + 1;  // keys that the first query sees
   const int mthr = (int)clamp64(FORM != kShared && a.causal && first < Lk ? first - BN : Lk - BN, -1, 0x7fffffff);
   const int qpos = FORM == kScored ? (int)clamp64(off + qi, INT32_MIN, INT32_MAX) : 0;
-  const float slope = FORM == kScored && a.slopes ? -a.slopes[head] * kLog2e : 0.f;
+  // tiles up to key `lin` have no visible key past the wave's first query
+  const int lin = FORM == kScored ? (a.causal && pfx <= 0 ? INT32_MAX : (int)clamp64(off + q0 - BN + 1, -1, INT32_MAX)) : 0;
+  const float slope = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e : 0.f;  // in exponents of 2
   // `mid` (the next tiles' LDS stores and global loads) is issued right after
   // the score MFMAs, so that its issue overlaps their execution; a wave with
   // no keys left in this tile still runs it
+  // scored rows: what c scales is the capped score where there is a cap, and the
+  // bias goes on it in the same units (c > 0 from stage_q on)
+  float capk = 0.f, sraw = 0.f, slope4 = 0.f;
+  CapNear cn{};
+  auto score_consts = [&]() __attribute__((always_inline)) {
+    if (a.cap_out > 0.f) {
+      capk = c * a.cap_in;
+      cn.set(capk);
+      c = a.cap_out;
+    }
+    sraw = slope / c;
+    slope4 = slope * (float)(4 * hh);
+  };
   auto compute = [&](int t, int buf, auto&& mid) {
     if ((int64_t)t * BN < kend_w) {
       const T* K = ks[buf];
       const T* V = vs[buf];
-      // (scored: the scores become exponents of 2 below, so the softmax scales them by 1)
-      const float cs = FORM == kScored ? 1.f : c;
       f32x16 s[NA];
 #pragma unroll
       for (int aa = 0; aa < NA; ++aa) {
@@ -764,28 +777,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         }
       }
       mid();
+      // scored: the bias of the tile's first key at this lane's query, where the
+      // distance from it adds to the scores
+      float bias = 0.f;
       if constexpr (FORM == kScored) {
-        // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), within 2e-7
-        // cap; the distance is exact, a whole number below 2^24 (rounded past it)
-        if (a.cap_out > 0.f) {
-          const float ci = c * a.cap_in;
+        constexpr bool NEAR = D == 64;
+        // one straight run per combination: cap (0 none, 1 any score, 2 near), then
+        // bias (0 none, 1 linear, 2 by |i - j|)
+        const float d0 = (float)(int)((uint32_t)(t * BN) - (uint32_t)qpos);
+        auto form = [&](auto cap, auto dist) __attribute__((always_inline)) {
 #pragma unroll
           for (int aa = 0; aa < NA; ++aa)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[aa][r] = __builtin_fmaf(-2.f * a.cap_out,
-                                        __builtin_amdgcn_rcpf(1.f + exp2_fast(s[aa][r] * ci)), a.cap_out);
-        } else {
+            for (int r = 0; r < 16; ++r) {
+              const float j = (float)(32 * aa + 8 * (r >> 2) + (r & 3));
+              float x = s[aa][r];
+              if constexpr (cap == 1) x = cap_score(x, capk);
+              if constexpr (cap == 2) x = cn(x);
+              if constexpr (dist == 1) x = __builtin_fmaf(sraw, j, x);
+              if constexpr (dist == 2) x = __builtin_fmaf(-sraw, __builtin_fabsf(d0 + (float)(4 * hh) + j), x);
+              s[aa][r] = x;
+            }
+          if constexpr (dist == 1) bias = __builtin_fmaf(slope, d0, slope4);
+        };
+        typedef std::integral_constant<int, 0> I0;
+        typedef std::integral_constant<int, 1> I1;
+        typedef std::integral_constant<int, 2> I2;
+        const int dist = !a.slopes ? 0 : t * BN <= lin ? 1 : 2;  // (1: no visible key past the queries, |i - j| = i - j)
+        bool near = false;
+        if (NEAR && a.cap_out > 0.f) {
+          float top = 0.f;
 #pragma unroll
-          for (int aa = 0; aa < NA; ++aa) s[aa] *= c;
+          for (int aa = 0; aa < NA; ++aa)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, __builtin_fabsf(s[aa][r]));
+          near = __builtin_amdgcn_ballot_w64(top > cn.lim) == 0;
         }
-        if (a.slopes) {
-          const float d0 = (float)(int)((uint32_t)(t * BN + 4 * hh) - (uint32_t)qpos);
-#pragma unroll
-          for (int aa = 0; aa < NA; ++aa)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[aa][r] = __builtin_fmaf(slope, __builtin_fabsf(d0 + (float)(32 * aa + 8 * (r >> 2) + (r & 3))), s[aa][r]);
+        if (NEAR && near) {
+          if (dist == 0) form(I2(), I0());
+          else if (dist == 1) form(I2(), I1());
+          else form(I2(), I2());
+        } else if (a.cap_out > 0.f) {
+          if (dist == 0) form(I1(), I0());
+          else if (dist == 1) form(I1(), I1());
+          else form(I1(), I2());
+        } else if (dist == 1) {
+          form(I0(), I1());
+        } else if (dist == 2) {
+          form(I0(), I2());
         }
       }
       // mask keys past the sequence / context and, if causal, past the query
@@ -811,8 +850,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       for (int aa = 0; aa < NA; ++aa)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[aa][r]);
-      if (__builtin_amdgcn_ballot_w64(mx * cs > m_used + 8.f) != 0) {
-        const float mn = fmaxf(m_used, max_lane_pair32(mx) * cs);
+      // (scored: P in bf16 and the sums hold far larger and smaller values, and a
+      // bias that rises towards the query would move the base on every tile)
+      constexpr bool WIDE = FORM == kScored && std::is_same<T, bf16_t>::value;
+      constexpr float RISE = WIDE ? 64.f : 8.f;
+      if (__builtin_amdgcn_ballot_w64(FORM == kScored ? __builtin_fmaf(mx, c, bias) > m_used + RISE : mx * c > m_used + RISE) != 0) {
+        const float mn = FORM == kScored ? fmaxf(m_used, max_lane_pair32(__builtin_fmaf(mx, c, bias)) + (WIDE && a.slopes ? 48.f : 0.f))
+                                         : fmaxf(m_used, max_lane_pair32(mx) * c);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
 #pragma unroll
         for (int d = 0; d < NDT; ++d) oacc[d] *= alpha;
@@ -827,7 +871,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
           v8 pf;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float p = exp2_fast(__builtin_fmaf(s[aa][8 * h2 + e], cs, nb));
+            const float p = exp2_fast(__builtin_fmaf(s[aa][8 * h2 + e], c, FORM == kScored ? nb + bias : nb));
             lsum += p;
             pf[e] = (T)p;
           }
@@ -877,6 +921,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   }
   const int ntiles = (int)((kend + BN - 1) / BN);
   stage_q();  // (waits for the query loads with tile 0's loads in flight)
+  if constexpr (FORM == kScored) score_consts();
   store_tile(0, kA, vA);
   load_tile(tile0 + 1, kB, vB);
   load_tile(tile0 + 2, kA, vA);

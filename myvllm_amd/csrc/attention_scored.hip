@@ -9,7 +9,7 @@ namespace {
 template <typename A> void set_scores(A& a, const gdn_tensor* slopes, float cap) {
   a.slopes = slopes ? reinterpret_cast<const float*>(slopes->data) : nullptr;
   a.cap_in = cap > 0.f ? 2.f / cap : 0.f;
-  a.cap_out = cap > 0.f ? cap * kLog2e : 0.f;
+  a.cap_out = cap > 0.f ? 2.f * cap * kLog2e : 0.f;
 }
 
 template <typename T, bool PAGED>

@@ -143,17 +143,22 @@ PyObject* same_device(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(dev);
 }
 
-// Whether the kernels can read a tensor with 16-byte accesses (unit inner
-// stride, 16-byte aligned data and outer strides); None if it is not a plain one.
-PyObject* vec16_ok(PyObject*, PyObject* o) {
-  if (!plain(o)) Py_RETURN_NONE;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  const int64_t n = t.dim();
-  if (n == 0) Py_RETURN_NONE;
+// Whether the kernels can read tensors (None aside) with 16-byte accesses (unit
+// inner stride, 16-byte aligned data and outer strides); None if one is not a
+// plain one.
+PyObject* vec16_ok(PyObject*, PyObject* const* args, Py_ssize_t count) {
   try {
-    bool ok = t.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    const int64_t es = (int64_t)t.element_size();
-    for (int64_t i = 0; ok && i < n - 1; ++i) ok = t.stride(i) * es % 16 == 0;
+    bool ok = true;
+    for (Py_ssize_t k = 0; k < count; ++k) {
+      if (args[k] == Py_None) continue;
+      if (!plain(args[k])) Py_RETURN_NONE;
+      const at::Tensor& t = THPVariable_Unpack(args[k]);
+      const int64_t n = t.dim();
+      if (n == 0) Py_RETURN_NONE;
+      ok = ok && t.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+      const int64_t es = (int64_t)t.element_size();
+      for (int64_t i = 0; ok && i < n - 1; ++i) ok = t.stride(i) * es % 16 == 0;
+    }
     return PyBool_FromLong(ok);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -252,7 +257,7 @@ PyMODINIT_FUNC PyInit__gdn_binding() {
   };
   for (const Bound& b : kBound) add(b.name, reinterpret_cast<void*>(b.call), METH_FASTCALL);
   add("same_device", reinterpret_cast<void*>(same_device), METH_FASTCALL);
-  add("vec16_ok", reinterpret_cast<void*>(vec16_ok), METH_O);
+  add("vec16_ok", reinterpret_cast<void*>(vec16_ok), METH_FASTCALL);
   add("bind", reinterpret_cast<void*>(bind), METH_O);
   g_methods[k] = PyMethodDef{nullptr, nullptr, 0, nullptr};
   return PyModule_Create(&g_module);

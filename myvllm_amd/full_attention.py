@@ -372,13 +372,10 @@ def paged_kv_append(
     if q is None and out is not None:
         raise ValueError("out is the rotated q's: none without q")
     dev = _lib.require_device(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
-    k, v = _lib.vec16(k), _lib.vec16(v)
-    cos, sin = (None if t is None else _lib.vec16(t) for t in (cos, sin))
-    o = None
-    if q is not None:
-        # (rows aligned already are rotated where they lie when out is q)
-        o = _out_for(out, q.shape, q.dtype, dev)
-        q = _lib.vec16(q)
+    if not _lib.vec16_all(q, k, v, cos, sin):
+        q, k, v, cos, sin = (t if t is None else _lib.vec16(t) for t in (q, k, v, cos, sin))
+    # (rows aligned already are rotated where they lie when out is q)
+    o = None if q is None else _out_for(out, q.shape, q.dtype, dev)
     _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
               int(bool(interleaved)))
     return None if o is None else _finish(out, o)

@@ -90,6 +90,16 @@ def test_varlen_scales(dev, scale, cap, slope):
     check_varlen(dev, case, True, kw, dict(softcap=cap, slopes=slopes), [0, 0])
 
 
+@pytest.mark.parametrize("cap, dtype", [(40.0, BF), (40.0, HF), (6.0, HF), (1.0, BF)])
+def test_varlen_small_head_dim_caps(dev, cap, dtype):
+    """At D = 64 tiles whose scores stay below 3/4 of the cap go another way: all, some and none of them."""
+    case = attn_varlen_case([400, 33], seed=11, Hq=4, Hkv=2, D=64, dtype=dtype)
+    print(f"scored D=64 cap={cap} {dtype}", flush=True)
+    for slopes in (None, alibi(4)):
+        kw = dict(softcap=cap, alibi_slopes=None if slopes is None else slopes.to(dev))
+        check_varlen(dev, case, True, kw, dict(softcap=cap, slopes=slopes), [0, 0])
+
+
 def test_varlen_other_head_dim_strides_and_out(dev):
     """A head dim that runs padded; views of a packed projection into a given tensor."""
     case = attn_varlen_case([50, 20], seed=3, Hq=4, Hkv=4, D=72)
