@@ -231,8 +231,9 @@ def call(fn: str, *args) -> None:
     lib = _lib or load()
     code = getattr(_fast, fn)(*args)
     if code is None:
-        code = getattr(lib, fn)(*(describe(a) if isinstance(a, torch.Tensor) else a for a in args),
-                                stream_handle(args[0].device))
+        with torch.cuda.device(args[0].device):
+            code = getattr(lib, fn)(*(describe(a) if isinstance(a, torch.Tensor) else a for a in args),
+                                    stream_handle(args[0].device))
     if code:
         raise GdnError(fn, code, strerror(code))
 

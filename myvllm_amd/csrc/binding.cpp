@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -86,6 +87,8 @@ struct Entry {
     if (!t.is_cuda()) Py_RETURN_NONE;
     std::tuple<X...> x;
     if (!(convert<X>(args[N + J], std::get<J>(x)) && ...)) return nullptr;
+    // (a default stream is the null one, which means the current device's)
+    const c10::DeviceGuard guard(t.device());
     void* const stream = c10::hip::getCurrentHIPStream(t.device().index()).stream();
     typedef gdn_tensor* Ptr;
     int rc;
