@@ -18,7 +18,7 @@ namespace {
 constexpr int kSharedTile = 32;  // keys of a tile of the prefill kernel
 template <int D> constexpr int kSharedSlots = D == 256 ? 256 : D == 128 ? 512 : 768;  // workgroups that run at once
 constexpr int kMaxPieces11 = 2047;  // pieces of a row, held in 11 bits
-constexpr int kOwnPrices = 5;
+constexpr int kOwnPrices = 3;
 
 struct SharedGroup {
   int32_t keys, b0, rows;   // keys that are read once for all, first sequence, rows (sequences x heads of a kv head)
