@@ -411,7 +411,7 @@ int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_tensor* k_cach
 /*
  * The three attention ops with another form of scores (no counterpart in the
  * reference).  With x = scale q.k of the query at position i and the key at j:
- *   softcap > 0: x <- softcap tanh(x / softcap), softcap at most 4096;
+ *   softcap != 0, from 1e-3 to 4096: x <- softcap tanh(x / softcap);
  *   slopes (Hq,) fp32: x <- x - slopes[h] |i - j| for query head h;
  *   prefix_lens (N,) i32|i64, causal only: keys j < prefix_lens[n] are visible
  *   to every query of sequence n, the others as ever (j <= i).

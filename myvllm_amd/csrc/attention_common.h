@@ -143,7 +143,8 @@ struct CapNear {
   }
   GDN_DEVICE float operator()(float s) const {
     const float u = s * s;
-    return __builtin_fmaf(s, __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p4, u, p3), u, p2), u, p1), u, p0), -0.5f);
+    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p4, u, p3), u, p2), u, p1), u, p0);
+    return __builtin_fmaf(s, p, -0.5f);
   }
 };
 

@@ -436,8 +436,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       piece = p.piece;
     }
   }
-  // the tile's rows: s0 + (qb ...) of its sequence, `len` of them, or rows (qb
-  // ...) of its group; their keys, and the position of row 0
+  // rows from qb on of the `len` of a sequence that begins at s0 (shared: of a
+  // group that begins at sequence sb0), their keys, and the position of row 0
   int64_t n, s0, len, qb, Lk, off;
   int kvh, head;
   int64_t pfx = 0;  // keys that every row sees
@@ -452,7 +452,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       const uint32_t id = blockIdx.x * 4 + w, ny = a.Hkv * ((R + 15) / 16), u = id / ny, y = id - u * ny;
       if (u < (uint32_t)a.own.units)
         attn_own_wave<T, D, (PG >= 2)>(a.own,
-                                       reinterpret_cast<char*>(w < 2 ? ks[0] : vs[0]) + (w & 1) * own_lds_per_wave<T, D>(),
+                                       reinterpret_cast<char*>(w < 2 ? ks[0] : vs[0]) +
+                                           (w & 1) * own_lds_per_wave<T, D>(),
                                        u, y % a.Hkv, y / a.Hkv);
       return;
     }
@@ -537,9 +538,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   {
     static_assert(!RAG || q_pieces_inside(DQ), "query pieces are read inside their row");
     const int64_t row = qvalid ? qi : 0;
-    const uint32_t sb = FORM == kShared ? (uint32_t)row / (uint32_t)R : 0u, sh = FORM == kShared ? (uint32_t)row - sb * R : 0u;
+    // (shared: row r is head r % R of sequence r / R)
+    const uint32_t sb = FORM == kShared ? (uint32_t)row / (uint32_t)R : 0u;
     const T* qp = reinterpret_cast<const T*>(a.q) + (FORM == kShared ? sb0 + sb : s0 + row) * a.q_st +
-                  (int64_t)(FORM == kShared ? head + (int)sh : head) * a.q_sh;
+                  (int64_t)(FORM == kShared ? head + (int)((uint32_t)row - sb * R) : head) * a.q_sh;
 #pragma unroll
     for (int s = 0; s < NKS; ++s)
       qf[s] = *reinterpret_cast<const v8*>(qp + (RAG ? q_piece(s, hh, a.dim) : 16 * s + 8 * hh));
@@ -730,7 +732,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   const int mthr = (int)clamp64(FORM != kShared && a.causal && first < Lk ? first - BN : Lk - BN, -1, 0x7fffffff);
   const int qpos = FORM == kScored ? (int)clamp64(off + qi, INT32_MIN, INT32_MAX) : 0;
   // tiles up to key `lin` have no visible key past the wave's first query
-  const int lin = FORM == kScored ? (a.causal && pfx <= 0 ? INT32_MAX : (int)clamp64(off + q0 - BN + 1, -1, INT32_MAX)) : 0;
+  const int lin = FORM != kScored            ? 0
+                  : a.causal && pfx <= 0 ? INT32_MAX
+                                         : (int)clamp64(off + q0 - BN + 1, -1, INT32_MAX);
   const float slope = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e : 0.f;  // in exponents of 2
   // `mid` (the next tiles' LDS stores and global loads) is issued right after
   // the score MFMAs, so that its issue overlaps their execution; a wave with
@@ -803,7 +807,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         typedef std::integral_constant<int, 0> I0;
         typedef std::integral_constant<int, 1> I1;
         typedef std::integral_constant<int, 2> I2;
-        const int dist = !a.slopes ? 0 : t * BN <= lin ? 1 : 2;  // (1: no visible key past the queries, |i - j| = i - j)
+        // (1: no visible key past the queries, so |i - j| is i - j)
+        const int dist = !a.slopes ? 0 : t * BN <= lin ? 1 : 2;
         bool near = false;
         if (NEAR && a.cap_out > 0.f) {
           float top = 0.f;
@@ -850,12 +855,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       for (int aa = 0; aa < NA; ++aa)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[aa][r]);
-      // (scored: P in bf16 and the sums hold far larger and smaller values, and a
-      // bias that rises towards the query would move the base on every tile)
+      // (A bias that rises towards the query would move the base on every tile:
+      // with P in bf16, of fp32's range, it moves 2^56 ahead of the maximum, which
+      // then rises up to 2^24 above it.)
       constexpr bool WIDE = FORM == kScored && std::is_same<T, bf16_t>::value;
-      constexpr float RISE = WIDE ? 64.f : 8.f;
-      if (__builtin_amdgcn_ballot_w64(FORM == kScored ? __builtin_fmaf(mx, c, bias) > m_used + RISE : mx * c > m_used + RISE) != 0) {
-        const float mn = FORM == kScored ? fmaxf(m_used, max_lane_pair32(__builtin_fmaf(mx, c, bias)) + (WIDE && a.slopes ? 48.f : 0.f))
+      const float top = FORM == kScored ? __builtin_fmaf(mx, c, bias) : mx * c;
+      if (__builtin_amdgcn_ballot_w64(top > m_used + (WIDE ? 24.f : 8.f)) != 0) {
+        const float mn = FORM == kScored ? fmaxf(m_used, max_lane_pair32(top) + (WIDE && a.slopes ? 56.f : 0.f))
                                          : fmaxf(m_used, max_lane_pair32(mx) * c);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
 #pragma unroll

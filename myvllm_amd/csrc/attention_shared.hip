@@ -324,7 +324,8 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const Shared
 #pragma unroll
   for (int e = 0; e < 4; ++e) ov[e] = (T)(o[e] * inv);
   if (valid)
-    *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + b * a.o_st + (int64_t)head * a.o_sh + dim0 + 8 * w + 4 * hh) = ov;
+    *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + b * a.o_st + (int64_t)head * a.o_sh + dim0 + 8 * w + 4 * hh) =
+        ov;
 }
 
 // The workspace, in floats: the decode's, the plan, the shared pieces' partials.

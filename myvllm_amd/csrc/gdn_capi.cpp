@@ -603,7 +603,8 @@ int varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v
 // Score forms: the cap, slopes (Hq,) fp32 and prefix lengths (N,).
 int check_scores(const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_t Hq, int64_t N, float softcap,
                  bool causal) {
-  if (!(softcap >= 0.f && softcap <= 4096.f)) return GDN_ERR_ARG;
+  // (below, the scores' scale leaves fp32; above, the tanh is not exact enough)
+  if (softcap != 0.f && !(softcap >= 1e-3f && softcap <= 4096.f)) return GDN_ERR_ARG;
   if (slopes) {
     GDN_TRY(check_desc(slopes, 1));
     if (slopes->shape[0] != Hq) return GDN_ERR_SHAPE;

@@ -76,7 +76,7 @@ def flash_attention_prefill(
     ``cu_seqlens`` when not given, one host sync as in the reference (``:139``).
 
     Other forms of scores x = scale q.k, applied in this order: ``softcap``
-    (above 0, at most 4096): x <- softcap tanh(x / softcap); ``alibi_slopes``
+    (1e-3 to 4096): x <- softcap tanh(x / softcap); ``alibi_slopes``
     (Hq,) fp32: x <- x - slope_h |i - j|; ``prefix_lens`` (N,), causal only: the
     first ``prefix_lens[n]`` keys are visible to every query of sequence n.  A
     packed batch is its own document mask: each document a sequence."""

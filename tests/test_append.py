@@ -15,8 +15,8 @@ BF = torch.bfloat16
 
 
 def args(D=128, T=5, N=2):
-    return dict(k=Z(T, 2, D, dtype=BF), v=Z(T, 2, D, dtype=BF), kc=Z(6, 16, 2, D, dtype=BF), vc=Z(6, 16, 2, D, dtype=BF),
-                tab=Z(N, 3, dtype=torch.int32), ctx=Z(N, dtype=torch.int32), q=Z(T, 4, D, dtype=BF),
+    return dict(k=Z(T, 2, D, dtype=BF), v=Z(T, 2, D, dtype=BF), kc=Z(6, 16, 2, D, dtype=BF),
+                vc=Z(6, 16, 2, D, dtype=BF), tab=Z(N, 3, dtype=torch.int32), ctx=Z(N, dtype=torch.int32), q=Z(T, 4, D, dtype=BF),
                 out=Z(T, 4, D, dtype=BF), cu=Z(N + 1, dtype=torch.int32), cos=Z(48, 32), sin=Z(48, 32))
 
 

@@ -19,8 +19,8 @@ def D(t):
 
 SCORES = [
     (dict(slopes=Z(3)), SHAPE), (dict(slopes=Z(4, dtype=BF)), DTYPE), (dict(slopes=Z(8)[::2]), STRIDE),
-    (dict(slopes=Z(4, 1)), NDIM), (dict(cap=-1.0), ARG), (dict(cap=4097.0), ARG), (dict(cap=math.nan), ARG),
-    (dict(cap=math.inf), ARG),
+    (dict(slopes=Z(4, 1)), NDIM), (dict(cap=-1.0), ARG), (dict(cap=4097.0), ARG), (dict(cap=9e-4), ARG),
+    (dict(cap=math.nan), ARG), (dict(cap=math.inf), ARG),
 ]
 MASKS = [(dict(pfx=Z(3, dtype=I32)), SHAPE), (dict(pfx=Z(2)), DTYPE), (dict(pfx=Z(4, dtype=I32)[::2]), STRIDE)]
 
@@ -128,8 +128,8 @@ def test_reference_scores():
     x, p = attention_weights_ref(q, k, [0, 2, 4], 0.5, softcap=1.5, slopes=torch.tensor([0.25, 2.0]), prefix=2)
     for n, i in enumerate((0, 2, 4)):
         for h, s in enumerate((0.25, 2.0)):
-            w = [1.5 * math.tanh(0.5 * float(q[n, h] @ k[j, 0]) / 1.5) - s * abs(i - j) if j <= i or j < 2 else -math.inf
-                 for j in range(5)]
+            w = [1.5 * math.tanh(0.5 * float(q[n, h] @ k[j, 0]) / 1.5) - s * abs(i - j)
+                 if j <= i or j < 2 else -math.inf for j in range(5)]
             assert x[n, h].tolist() == pytest.approx(w)
             z = sum(math.exp(v) for v in w)
             assert p[n, h].tolist() == pytest.approx([math.exp(v) / z for v in w])

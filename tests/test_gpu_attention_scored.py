@@ -69,7 +69,7 @@ def test_varlen_both_directions(dev, D):
 
 
 @pytest.mark.parametrize("scale, cap, slope", [(4.0, 2.0, 0.0), (4.0, 4096.0, 0.5), (-0.3, 5.0, 0.1), (0.0, 1.0, 0.25),
-                                               (0.1, None, -0.02), (0.05, 0.25, 30.0), (1e30, 50.0, 0.0)])
+                                               (0.1, None, -0.02), (0.05, 0.25, 30.0), (1.0, 1e-3, 0.0), (1e30, 50.0, 0.0)])
 def test_varlen_scales(dev, scale, cap, slope):
     """Saturated, hardly capped, folded signs, growing with distance, one key wide."""
     case = attn_varlen_case([65, 200], seed=7, Hq=4, Hkv=2, D=128)
