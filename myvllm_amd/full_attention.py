@@ -371,11 +371,13 @@ def paged_kv_append(
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     if q is None and out is not None:
         raise ValueError("out is the rotated q's: none without q")
-    dev = _lib.require_device(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
+    tensors = (k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
+    if not _lib.same_device(*tensors):
+        _lib.require_device(*tensors)
     if not _lib.vec16_all(q, k, v, cos, sin):
         q, k, v, cos, sin = (t if t is None else _lib.vec16(t) for t in (q, k, v, cos, sin))
     # (rows aligned already are rotated where they lie when out is q)
-    o = None if q is None else _out_for(out, q.shape, q.dtype, dev)
+    o = None if q is None else torch.empty_like(q) if out is None else _out_for(out, q.shape, q.dtype, q.device)
     _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
               int(bool(interleaved)))
-    return None if o is None else _finish(out, o)
+    return o if out is None else _finish(out, o)
