@@ -131,7 +131,8 @@ GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
   return __builtin_amdgcn_readlane(fits ? tiles : 0, best);
 }
 
-// Sum over the threads before this one; *all: over all 1,024.
+// Sum over the threads before this one; *all: over all NT.
+template <int NT>
 GDN_DEVICE int32_t block_exclusive(int32_t x, int32_t* wsum, int32_t* all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int32_t inc = wave_inclusive_scan_i32(x);
@@ -139,7 +140,8 @@ GDN_DEVICE int32_t block_exclusive(int32_t x, int32_t* wsum, int32_t* all) {
   if (lane == 63) wsum[w] = inc;
   __syncthreads();
   int32_t base = 0, sum = 0;
-  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
     base += i < w ? wsum[i] : 0;
     sum += wsum[i];
   }
@@ -152,10 +154,10 @@ GDN_DEVICE int32_t block_exclusive(int32_t x, int32_t* wsum, int32_t* all) {
 // Consecutive workgroups go to the 8 XCDs in turn, so an eighth of the slots,
 // ordered (kv head, group, piece, block), is dealt to each: the blocks over the
 // same keys run on one XCD and read them from its L2.
-template <int D>
-__global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs a) {
-  __shared__ int32_t wsum[16], tiles_lds;
-  const int tid = threadIdx.x, per = (a.B + 1023) / 1024;
+template <int D, int NT>
+__global__ __launch_bounds__(NT) void shared_plan_kernel(const SharedPlanArgs a) {
+  __shared__ int32_t wsum[NT / 64], tiles_lds;
+  const int tid = threadIdx.x, per = (a.B + NT - 1) / NT;
   auto price_of = [&](int32_t b) -> int32_t {
     if (b >= a.B) return 0;
     const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, a.cap);
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
   };
   int32_t sum = 0, total;
   for (int i = 0; i < per; ++i) sum += price_of(tid * per + i);
-  int32_t run = block_exclusive(sum, wsum, &total);
+  int32_t run = block_exclusive<NT>(sum, wsum, &total);
   for (int i = 0; i < per; ++i) {
     const int32_t b = tid * per + i;
     if (b >= a.B) break;
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
   const int tiles = tiles_lds;
   const float inv = __builtin_amdgcn_rcpf((float)tiles);
   int32_t slots = 0;
-  for (int32_t c = 0; c < a.n; c += 1024) {
+  for (int32_t c = 0; c < a.n; c += NT) {
     SharedGroup g{};
     if (c + tid < a.n) {
       g = shared_group(a, c + tid);
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
       if (g.lead >= 0) g.lead += g.b0;
     }
     int32_t all;
-    const int32_t before = block_exclusive(g.rt * g.pieces, wsum, &all);
+    const int32_t before = block_exclusive<NT>(g.rt * g.pieces, wsum, &all);
     g.slot = slots + before;
     if (c + tid < a.n) a.group[c + tid] = g;
     slots += all;
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
   }
   __syncthreads();
 
-  for (int32_t b = tid; b < a.B; b += 1024) {
+  for (int32_t b = tid; b < a.B; b += NT) {
     SharedSeq s{};
     if (a.n > 0) {
       const SharedGroup g = a.group[shared_group_of(a, b)];
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(1024) void shared_plan_kernel(const SharedPlanArgs 
     a.seqs[b] = s;
   }
   const uint32_t all = (uint32_t)slots * a.Hkv, xcd = (all + 7) / 8;
-  for (uint32_t id = tid; id < (uint32_t)a.grid; id += 1024) {
+  for (uint32_t id = tid; id < (uint32_t)a.grid; id += NT) {
     SharedWork k{};
     k.lead = -1;
     const uint32_t slot = (id & 7) * xcd + (id >> 3);
@@ -361,7 +363,10 @@ SharedSpace shared_space(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t 
 template <typename T, int D>
 hipError_t launch_shared(const SharedAttnArgs& a, const SharedPlanArgs& p, hipStream_t st) {
   constexpr int BN = kSharedTile;
-  shared_plan_kernel<D><<<dim3(1), dim3(1024), 0, st>>>(p);
+  if (p.B <= 256)
+    shared_plan_kernel<D, 256><<<dim3(1), dim3(256), 0, st>>>(p);
+  else
+    shared_plan_kernel<D, 1024><<<dim3(1), dim3(1024), 0, st>>>(p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(a.own_wgs + (unsigned)p.grid);
