@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kSharedTile = 32;  // keys of a tile of the prefill kernel
 template <int D> constexpr int kSharedSlots = D == 256 ? 256 : D == 128 ? 512 : 768;  // workgroups that run at once
+constexpr int kQueues = 32;         // of workgroups: 8 XCDs x 4 shader engines
 constexpr int kMaxPieces11 = 2047;  // pieces of a row, held in 11 bits
 constexpr int kOwnPrices = 3;
 
@@ -31,8 +32,8 @@ struct SharedPlanArgs {
   bool ctx64, groups64, lens64;
   int32_t B, n, R, Hkv;  // n groups
   int64_t cap;
-  int32_t slots, own_wgs, grid;  // slots of the partials; workgroups of the own keys, and of the shared ones
-  int32_t units;                 // of the own keys, at most
+  int32_t slots, grid;    // slots of the partials; workgroups of the shared keys
+  int32_t units, waves;  // of the own keys: units at most, waves of each
   int32_t* prices;
   int32_t* head;  // slots of a kv head, units of the own keys
   SharedSeq* seqs;
@@ -76,25 +77,47 @@ GDN_DEVICE int32_t shared_first(const SharedPlanArgs& a, int32_t b, int64_t L) {
   return b >= g.b0 && b - g.b0 < g.rows / a.R && L >= g.keys ? g.keys : 0;
 }
 
-// Key tiles per piece of the shared keys (all wave's lanes; 0: no shared keys).
-// Lane i prices i + 1 times `mult` pieces of the longest group, in 1/8 of a
-// key-tile step of one workgroup: the end of the last piece where F workgroups
-// are free at once and `own` of them after the own keys' time, each piece taking
-// kFixed steps and its tiles; the partials' traffic; the merge's chain.
+// How the chip is shared out, by one wave: units of the own keys, and key tiles
+// per piece of the shared ones (0: there are none).
+// The own keys get the part of the workgroups that their part of the work is, in
+// key-tile steps of a workgroup (a price is 16 keys of one wave, four of which
+// a workgroup reads in 1.2 steps), at least kOwnPrices to a unit.
+// Consecutive workgroups go to 32 queues of 8 CUs in turn, so both parts are whole
+// workgroups of every queue (one more than fits waits for a whole round: 64
+// sequences with 64 own keys each 51 us where 40 is due).
+// For the pieces lane i prices i + 1 times `mult` of the longest group, in 1/8 of
+// a step: the end of the last one where F workgroups of a queue are free at once
+// and `own` of them after the own keys' time, each piece taking kFixed steps and its tiles; the
+// partials' traffic; the merge's chain.
+struct SharedPlan {
+  int32_t tiles, units;
+};
 template <int D>
-GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
-  constexpr int kSlots = kSharedSlots<D>, kFixed = 8, kOwn = 8;
+GDN_DEVICE SharedPlan shared_tiles(const SharedPlanArgs& a, int prices) {
+  constexpr int kSlots = kSharedSlots<D>, kDeep = kSlots / kQueues, kFixed = 8, kOwnFixed = 8;
   const int lane = threadIdx.x & 63;
   auto group = [&](int c) { return c + lane < a.n ? shared_group(a, c + lane) : SharedGroup{}; };
   int top = 0, rt = 0;
+  float steps = 0.f;  // of the shared keys, per kv head
   for (int c = 0; c < a.n; c += 64) {
     const SharedGroup g = group(c);
     const int n = (g.keys + kSharedTile - 1) / kSharedTile;
     top = n > top ? n : top;
     rt += wave_sum(g.rt);
+    steps += (float)g.rt * (float)n;
   }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) steps += __shfl_xor(steps, d);
+  steps *= (float)a.Hkv;
+  const float own_steps = 0.3f * (float)prices * (float)a.waves;
+  const int most_units = prices / kOwnPrices < a.units ? prices / kOwnPrices : a.units;
+  int own = (int)(kDeep * own_steps / (own_steps + steps) + 0.5f);
+  own = own > 1 ? own : 1;
+  int units = kQueues * 4 * own / a.waves;
+  units = units < most_units ? units : most_units;
+  units = units > 1 ? units : 1;
   const int nmax = wave_top(top);
-  if (nmax == 0) return 0;
+  if (nmax == 0) return {0, most_units > 1 ? most_units : 1};
   const int64_t least = (int64_t)rt * a.Hkv;
   const int mult = least < kSlots ? (kSlots + 64 * (int)least - 1) / (64 * (int)least) : 1, want = (lane + 1) * mult;
   int tiles = (nmax + want - 1) / want;
@@ -111,12 +134,14 @@ GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
   }
   wgs *= a.Hkv;
   const bool fits = wgs <= a.slots;
-  const int x = fits ? (int)wgs : 0, len = 8 * (kFixed + tiles);
-  const int own = a.own_wgs < kSlots ? a.own_wgs : kSlots, F = kSlots - own;
-  const int64_t t64 = (int64_t)prices * a.Hkv * D / 11000;  // (5.2 TB/s of K and V)
-  const int t = t64 < 8 * kOwn ? 8 * kOwn : t64 < 1 << 22 ? (int)t64 : 1 << 22;
+  const int x = fits ? ((int)wgs + kQueues - 1) / kQueues : 0, len = 8 * (kFixed + tiles);
+  const int64_t busy = ((int64_t)units * a.waves + 4 * kQueues - 1) / (4 * kQueues);
+  own = busy < kDeep ? (int)busy : kDeep;
+  const int F = kDeep - own;
+  const float each = 8.f * kOwnFixed + 9.6f * (float)prices / (float)units;
+  const int t = each < 0x1p22f ? (int)each : 1 << 22;
   // M: where k rounds of the free workgroups and j of the others make x
-  int k = (x + kSlots - 1) / kSlots, j = 0, M = len * k + (F == 0 ? t : 0);
+  int k = (x + kDeep - 1) / kDeep, j = 0, M = len * k + (F == 0 ? t : 0);
   while (F > 0 && __builtin_amdgcn_ballot_w64(k * F + j * own < x)) {
     if (k * F + j * own >= x) continue;
     const int next = (k + 1) * len, next_own = t + (j + 1) * len;
@@ -124,11 +149,11 @@ GDN_DEVICE int shared_tiles(const SharedPlanArgs& a, int prices) {
     k += next <= next_own;
     j += next_own <= next;
   }
-  const int64_t cost = (int64_t)M + (int64_t)x * D / 1400 + (nmax / tiles) / 4;
+  const int64_t cost = (int64_t)M + (int64_t)x * kQueues * D / 1400 + (nmax / tiles) / 4;
   const int c24 = fits && cost < 1 << 24 ? (int)cost : 1 << 24;
   // (the smallest, of equals the one with fewer pieces; one piece always fits)
   const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
-  return __builtin_amdgcn_readlane(fits ? tiles : 0, best);
+  return {__builtin_amdgcn_readlane(fits ? tiles : 0, best), units};
 }
 
 // Sum over the threads before this one; *all: over all NT.
@@ -175,8 +200,11 @@ __global__ __launch_bounds__(NT) void shared_plan_kernel(const SharedPlanArgs a)
   }
   if (tid == 0) a.prices[a.B] = total;
   if (tid < 64) {
-    const int t = shared_tiles<D>(a, total);
-    if (tid == 0) tiles_lds = t;
+    const SharedPlan p = shared_tiles<D>(a, total);
+    if (tid == 0) {
+      tiles_lds = p.tiles;
+      a.head[1] = p.units;
+    }
   }
   __syncthreads();
 
@@ -207,12 +235,7 @@ __global__ __launch_bounds__(NT) void shared_plan_kernel(const SharedPlanArgs a)
     if (c + tid < a.n) a.group[c + tid] = g;
     slots += all;
   }
-  if (tid == 0) {
-    a.head[0] = slots;
-    // (a unit of at least kOwnPrices: shorter ones only leave more to merge)
-    const int32_t u = total / kOwnPrices;
-    a.head[1] = u < 1 ? 1 : u < a.units ? u : a.units;
-  }
+  if (tid == 0) a.head[0] = slots;
   __syncthreads();
 
   for (int32_t b = tid; b < a.B; b += NT) {
@@ -334,17 +357,15 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const Shared
 // Workgroups that the shared keys may take: one per 128 rows of a group and kv
 // head, up to four times as many or one round of the chip in pieces, within
 // 512 MiB of partials.
-// The own keys are dealt over U units: 384 waves with the heads (96 CUs at
-// D = 256; a CU reads some 42 GB/s whatever its waves have in flight, so HBM's
-// rate takes half the chip), and one per four sequences at least, which it takes
-// a while to begin with.  256 sequences behind 16,384 keys / 64 behind 8,192 with
-// 128 waves 403 / 70 us, 256 226 / 51, 384 179 / 44, 512 190 / 46.
+// The own keys are dealt over at most 512 waves' units with the heads (half the
+// chip at D = 256, which reads at HBM's rate), and one per four sequences at least,
+// which it takes a while to begin with.
 struct SharedSpace {
   int64_t units, slots, grid, prices, head, seqs, group, work, part, all;
 };
 SharedSpace shared_space(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t D) {
   SharedSpace s{};
-  s.units = std::max(std::max<int64_t>(384 / (Hkv * ((Hq / Hkv + 15) / 16)), 1), (B + 3) / 4);
+  s.units = std::max(std::max<int64_t>(512 / (Hkv * ((Hq / Hkv + 15) / 16)), 1), (B + 3) / 4);
   const int64_t most = std::min(n, B / 2);  // (groups of two sequences at least)
   const int64_t base = Hkv * (B * (Hq / Hkv) / 128 + most), chip = D == 256 ? 256 : D == 128 ? 512 : 768;
   const int64_t fit = (int64_t(1) << 27) / (4 * (32 * D + 128));
@@ -431,8 +452,8 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   a.c = d.c;
   a.part = workspace + sp.part;
   a.work = reinterpret_cast<const SharedWork*>(workspace + sp.work);
-  const int64_t waves = sp.units * d.Hkv * ((d.Hq / d.Hkv + 15) / 16);
-  a.own_wgs = (uint32_t)((waves + 31) / 32 * 8);
+  const int64_t waves = (int64_t)d.Hkv * ((d.Hq / d.Hkv + 15) / 16);
+  a.own_wgs = (uint32_t)((sp.units * waves + 31) / 32 * 8);
   SharedPlanArgs p{};
   p.ctx = d.ctx;
   p.ctx64 = d.ctx64;
@@ -449,9 +470,9 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   p.cap = d.tab.cols * d.tab.page;
   p.slots = (int32_t)sp.slots;
   p.grid = (int32_t)sp.grid;
-  p.own_wgs = (int32_t)a.own_wgs;
   p.prices = d.prices;
   p.units = d.units;
+  p.waves = (int32_t)waves;
   p.head = reinterpret_cast<int32_t*>(workspace + sp.head);
   p.seqs = reinterpret_cast<SharedSeq*>(workspace + sp.seqs);
   p.group = reinterpret_cast<SharedGroup*>(workspace + sp.group);

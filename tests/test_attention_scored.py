@@ -102,10 +102,10 @@ def test_shared_workspace():
         return ((B + units) * Hq * (D + 4) + (B + 4) // 4 * 4 + 4 + 4 * B + 8 * G + 8 * (-(-wgs // 8) * 8)
                 + wgs * 128 * (D + 4))
 
-    assert size(1, 1, 16, 2, 256) == want(1, 1, 16, 256, 192, 0)
-    assert size(64, 0, 16, 2, 256) == want(64, 0, 16, 256, 192, 0)
-    assert size(4, 1, 16, 2, 256) == want(4, 1, 16, 256, 192, 256)
-    assert size(4, 1, 128, 2, 64) == want(4, 1, 128, 64, 48, 768)
+    assert size(1, 1, 16, 2, 256) == want(1, 1, 16, 256, 256, 0)
+    assert size(64, 0, 16, 2, 256) == want(64, 0, 16, 256, 256, 0)
+    assert size(4, 1, 16, 2, 256) == want(4, 1, 16, 256, 256, 256)
+    assert size(4, 1, 128, 2, 64) == want(4, 1, 128, 64, 64, 768)
     assert size(4, 1, 16, 2, 96) == 0 and size(4, 1, 16, 3, 64) == 0
     rows = 2 * (65535 * 8 // 128 + 1)
     assert size(65535, 1, 16, 2, 256) == want(65535, 1, 16, 256, 16384, rows)
