@@ -87,8 +87,8 @@ GDN_DEVICE int32_t shared_first(const SharedPlanArgs& a, int32_t b, int64_t L) {
 // sequences with 64 own keys each 51 us where 40 is due).
 // For the pieces lane i prices i + 1 times `mult` of the longest group, in 1/8 of
 // a step: the end of the last one where F workgroups of a queue are free at once
-// and `own` of them after the own keys' time, each piece taking kFixed steps and its tiles; the
-// partials' traffic; the merge's chain.
+// and `own` of them after the own keys' time, each piece taking kFixed steps and
+// its tiles; the partials' traffic; the merge's chain.
 struct SharedPlan {
   int32_t tiles, units;
 };
@@ -109,15 +109,15 @@ GDN_DEVICE SharedPlan shared_tiles(const SharedPlanArgs& a, int prices) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) steps += __shfl_xor(steps, d);
   steps *= (float)a.Hkv;
-  const float own_steps = 0.3f * (float)prices * (float)a.waves;
   const int most_units = prices / kOwnPrices < a.units ? prices / kOwnPrices : a.units;
+  const int nmax = wave_top(top);
+  if (nmax == 0) return {0, most_units > 1 ? most_units : 1};
+  const float own_steps = 0.3f * (float)prices * (float)a.waves;
   int own = (int)(kDeep * own_steps / (own_steps + steps) + 0.5f);
   own = own > 1 ? own : 1;
   int units = kQueues * 4 * own / a.waves;
   units = units < most_units ? units : most_units;
   units = units > 1 ? units : 1;
-  const int nmax = wave_top(top);
-  if (nmax == 0) return {0, most_units > 1 ? most_units : 1};
   const int64_t least = (int64_t)rt * a.Hkv;
   const int mult = least < kSlots ? (kSlots + 64 * (int)least - 1) / (64 * (int)least) : 1, want = (lane + 1) * mult;
   int tiles = (nmax + want - 1) / want;
