@@ -39,6 +39,8 @@
  *  - flash_attention_varlen  <- flash_attention_prefill, ops/full_attention.py:114-173
  *  - paged_attention_prefill <- paged_flash_attention_prefill, ops/full_attention.py:454-512
  *  - paged_attention_decode  <- paged_flash_attention_decode, ops/full_attention.py:282-335
+ *  - *_scored, paged_attention_decode_shared, paged_kv_append: beside those, no
+ *    counterpart in the reference
  */
 #ifndef GDN_HIP_H_
 #define GDN_HIP_H_
