@@ -155,9 +155,11 @@ GDN_DEVICE SharedPlan shared_tiles(const SharedPlanArgs& a, int prices) {
   }
   const int64_t cost = (int64_t)M + (int64_t)x * kQueues * D / 1400 + (nmax / tiles) / 4;
   const int c24 = fits && cost < 1 << 24 ? (int)cost : 1 << 24;
-  // (the smallest, of equals the one with fewer pieces; one piece always fits)
+  // (the smallest, of equals the one with fewer pieces; the fewest always fit, and
+  // are taken too where the price of keys past 2^24 wraps)
   const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
-  return {__builtin_amdgcn_readlane(fits ? tiles : 0, best), units};
+  const int fit = fits ? tiles : 0, cheap = __builtin_amdgcn_readlane(fit, best);
+  return {cheap > 0 ? cheap : __builtin_amdgcn_readlane(fit, 0), units};
 }
 
 // Sum over the threads before this one; *all: over all NT.

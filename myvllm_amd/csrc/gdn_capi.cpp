@@ -855,9 +855,10 @@ GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tens
   } else if (G != 1) {
     return GDN_ERR_SHAPE;
   }
-  // rows, key positions and workgroups are counted in 32 bits
+  // rows, key positions (up to one piece past the last) and workgroups are
+  // counted in 32 bits
   if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ ||
-      block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31) ||
+      block_tables->shape[1] * k_cache->shape[1] > (int64_t(1) << 30) ||
       attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20))
     return GDN_ERR_RANGE;
   float* ws;
