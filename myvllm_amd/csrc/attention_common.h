@@ -126,25 +126,25 @@ GDN_DEVICE float cap_score(float s, float k) {
 // The same as tanh(x) / 2 - 1 / 2 by an odd polynomial of degree 9 for |x| <= 3/4
 // (|s| <= lim; fitted for the least largest error there, 1.9e-7): full-rate
 // instructions instead of the exponential and the reciprocal, and a test of the
-// tile.  It pays where several waves share a SIMD's transcendental unit: D = 64,
-// six prompts capped and biased under a prefix mask 72 -> 65 us, capped alone 57
-// -> 56; D = 128 526 -> 533, D = 256, where a wave has its SIMD to itself, 481 ->
-// 496.
+// tile.  It is evaluated in x = h s: folded into the coefficients, the powers of h
+// leave fp32's range (h^9 below 1e-4).  It pays where several waves share a SIMD's
+// transcendental unit: D = 64, six prompts capped and biased under a prefix mask
+// 72 -> 65 us, capped alone 57 -> 56; D = 128 526 -> 533, D = 256, where a wave has
+// its SIMD to itself, 481 -> 496.
 struct CapNear {
-  float lim, p0, p1, p2, p3, p4;
+  float lim, h;
   GDN_DEVICE void set(float k) {
-    const float h = k * 0.34657359f, u = h * h;  // x = h s (ln 2 / 2: k is 2 log2(e) scale / cap)
-    lim = h < 1e4f ? 0.75f / h : -1.f;
-    p0 = 0.5f * 0.99999723f * h;
-    p1 = 0.5f * -0.33323076f * h * u;
-    p2 = 0.5f * 0.13226092f * h * u * u;
-    p3 = 0.5f * -0.04928045f * h * u * u * u;
-    p4 = 0.5f * 0.01231883f * h * u * u * u * u;
+    h = k * 0.34657359f;  // x = h s (ln 2 / 2: k is 2 log2(e) scale / cap)
+    lim = h < 1e30f ? 0.75f / h : -1.f;
   }
   GDN_DEVICE float operator()(float s) const {
-    const float u = s * s;
-    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(p4, u, p3), u, p2), u, p1), u, p0);
-    return __builtin_fmaf(s, p, -0.5f);
+    const float x = s * h, u = x * x;
+    float p = 0.5f * 0.01231883f;
+    p = __builtin_fmaf(p, u, 0.5f * -0.04928045f);
+    p = __builtin_fmaf(p, u, 0.5f * 0.13226092f);
+    p = __builtin_fmaf(p, u, 0.5f * -0.33323076f);
+    p = __builtin_fmaf(p, u, 0.5f * 0.99999723f);
+    return __builtin_fmaf(x, p, -0.5f);
   }
 };
 
