@@ -448,7 +448,8 @@ int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tensor* k_cache
  *   one in no group, is read through its own table alone.
  *   workspace: 1-D fp32, 16-byte aligned, overwritten, of
  *   paged_attention_decode_shared_workspace_size elements.
- * Tables of up to 2^30 key positions.
+ * Tables of up to 2^30 key positions, N (tiles of 16 keys of a table + 4) below
+ * 2^31 (GDN_ERR_RANGE).
  */
 int64_t paged_attention_decode_shared_workspace_size(int64_t num_seqs, int64_t num_groups, int64_t num_q_heads,
                                                      int64_t num_kv_heads, int64_t head_dim);

@@ -417,6 +417,8 @@ int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, in
   return shared_space(B, groups, Hq, Hkv, D).slots;
 }
 
+int32_t attn_shared_start_price() { return kOwnStartPrice; }
+
 int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D) {
   return shared_space(B, groups, Hq, Hkv, D).all;
 }

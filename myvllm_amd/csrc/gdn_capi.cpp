@@ -67,6 +67,7 @@ hipError_t attn_decode_scored_launch(const gdn_tensor* q, const gdn_tensor* kc, 
                                      hipStream_t st);
 int64_t attn_shared_slots(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
 int64_t attn_shared_floats(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D);
+int32_t attn_shared_start_price();
 hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                      const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* lens,
                                      const gdn_tensor* groups, gdn_tensor* out, float* workspace, float scale,
@@ -855,10 +856,12 @@ GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tens
   } else if (G != 1) {
     return GDN_ERR_SHAPE;
   }
-  // rows, key positions (up to one piece past the last) and workgroups are
-  // counted in 32 bits
-  if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ ||
-      block_tables->shape[1] * k_cache->shape[1] > (int64_t(1) << 30) ||
+  // rows, key positions (up to one piece past the last), prices of the own keys
+  // (whose start costs more than the plain decode's) and workgroups are counted in
+  // 32 bits
+  const int64_t cap = block_tables->shape[1] * k_cache->shape[1];
+  if (B * Hq > kMaxGrid / 2 || Hkv > kMaxGridYZ || G > kMaxGridYZ || cap > (int64_t(1) << 30) ||
+      B * ((cap + 15) / 16 + attn_shared_start_price()) >= (int64_t(1) << 31) ||
       attn_shared_slots(B, G, Hq, Hkv, D) >= (int64_t(1) << 20))
     return GDN_ERR_RANGE;
   float* ws;
