@@ -421,7 +421,9 @@ int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_tensor* k_cach
  * above: arguments, head dims (64, 128 or 256), errors, the workspaces of the
  * paged ones (NULL: the prefill is not split) and their sizes.  GDN_ERR_ARG for
  * a softcap out of range (the tanh is within 2e-7 softcap) and for prefix_lens
- * without causal.
+ * without causal.  In bf16 with slopes a prefill may lose values below 1e-21 in
+ * rows whose highest score is that of a key so far off that its bias is tens of
+ * units.
  */
 int flash_attention_varlen_scored(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v,
                                   const gdn_tensor* cu_seqlens, gdn_tensor* out, const gdn_tensor* slopes,
