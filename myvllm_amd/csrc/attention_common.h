@@ -118,13 +118,16 @@ struct SharedWork {
 // A capped score, cap tanh(x) of x = scale s / cap, is cap - 2 cap / (1 + e^(2 x)),
 // and a constant on all scores of a row does not change its softmax: the raw score
 // s becomes -1 / (1 + 2^(k s)), k = 2 log2(e) scale / cap, which 2 cap log2(e)
-// scales to an exponent of 2, within 2e-7 cap.
+// scales to an exponent of 2.  Within 3e-7 cap of the tanh of its fp32 argument:
+// twice the exponential's ulp (2^-23 y (1 - y), y the quotient), the sum's half
+// (2^-24 y^2) and the reciprocal's (2^-24).
 GDN_DEVICE float cap_score(float s, float k) {
   return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s * k));
 }
 
-// The same as tanh(x) / 2 - 1 / 2 by an odd polynomial of degree 9 for |x| <= 3/4
-// (|s| <= lim; fitted for the least largest error there, 1.9e-7): full-rate
+// The same as tanh(x) / 2 - 1 / 2 by an odd polynomial of degree 9 for |x| <= 0.7
+// (|s| <= lim; fitted for the least largest error there, 9.4e-8, 1.9e-7 with the
+// fp32 roundings; to 3/4 it would be 2.9e-7): full-rate
 // instructions instead of the exponential and the reciprocal, and a test of the
 // tile.  It is evaluated in x = h s: folded into the coefficients, the powers of h
 // leave fp32's range (h^9 below 1e-4).  It pays where several waves share a SIMD's
@@ -135,15 +138,15 @@ struct CapNear {
   float lim, h;
   GDN_DEVICE void set(float k) {
     h = k * 0.34657359f;  // x = h s (ln 2 / 2: k is 2 log2(e) scale / cap)
-    lim = h < 1e30f ? 0.75f / h : -1.f;
+    lim = h < 1e30f ? 0.7f / h : -1.f;
   }
   GDN_DEVICE float operator()(float s) const {
     const float x = s * h, u = x * x;
-    float p = 0.5f * 0.01231883f;
-    p = __builtin_fmaf(p, u, 0.5f * -0.04928045f);
-    p = __builtin_fmaf(p, u, 0.5f * 0.13226092f);
-    p = __builtin_fmaf(p, u, 0.5f * -0.33323076f);
-    p = __builtin_fmaf(p, u, 0.5f * 0.99999723f);
+    float p = 0.5f * 0.01319420f;
+    p = __builtin_fmaf(p, u, 0.5f * -0.05019528f);
+    p = __builtin_fmaf(p, u, 0.5f * 0.13257456f);
+    p = __builtin_fmaf(p, u, 0.5f * -0.33326975f);
+    p = __builtin_fmaf(p, u, 0.5f * 0.99999851f);
     return __builtin_fmaf(x, p, -0.5f);
   }
 };
