@@ -475,7 +475,8 @@ int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tensor* k_cache
  * slot p % page of block block_tables[n][p / page].  With (a, b) the dims
  * (j, j + rot / 2), or (2 j, 2 j + 1) when interleaved != 0, j < rot / 2, of q
  * and k: (a, b) <- (a cos[p][j] - b sin[p][j], b cos[p][j] + a sin[p][j]) in
- * fp32, rounded once; the other dims and v are copied.  out may be q itself.
+ * fp32, rounded once; the other dims and v are copied.  out may be q itself, else
+ * it lies in memory of its own.
  * A token in no sequence, or at a position below 0, past the table's
  * max_blocks * page or past the P rows of the rotation, is not appended and
  * its out row is zero; a table entry outside [0, num_blocks) is not written

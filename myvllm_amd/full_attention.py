@@ -131,6 +131,17 @@ def _apart(out, q, k, v) -> bool:
             and out.untyped_storage().data_ptr() not in {t.untyped_storage().data_ptr() for t in (q, k, v)})
 
 
+def _crosses(out, q, k, v) -> bool:
+    """Whether a result of q's form written to `out` row by row, each after its own
+    row of q is read, could land on other rows of q, k or v first: `out` in their
+    memory, and not q itself."""
+    if out is q or out.shape != q.shape or out.dtype != q.dtype:
+        return False  # (another shape or type is refused further on)
+    if out.data_ptr() == q.data_ptr() and out.stride() == q.stride():
+        return False
+    return out.untyped_storage().data_ptr() in {t.untyped_storage().data_ptr() for t in (q, k, v)}
+
+
 def _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out, **form):
     """Head dims no kernel reads as they lie (:func:`_direct_head_dim`) run
     zero-padded to the next of 64, 128 and 256: zero dims add nothing to q.k
@@ -361,7 +372,8 @@ def paged_kv_append(
     of q and k (halves ``(j, j + rot / 2)`` as the reference's
     ``layers/rotary_embedding.py:20-31``, or neighbours ``(2 j, 2 j + 1)`` when
     ``interleaved``); without them nothing is rotated.  Returns the rotated q
-    (None for ``q=None``), into ``out`` where given, which may be q itself.
+    (None for ``q=None``), into ``out`` where given, which may be q itself (in other
+    memory of q, k or v it goes through a copy).
 
     A token in no sequence or at a position without a table column or a row of
     the rotation is not appended and its row of q is zero; table entries
@@ -377,7 +389,8 @@ def paged_kv_append(
     if not _lib.vec16_all(q, k, v, cos, sin):
         q, k, v, cos, sin = (t if t is None else _lib.vec16(t) for t in (q, k, v, cos, sin))
     # (rows aligned already are rotated where they lie when out is q)
-    o = None if q is None else torch.empty_like(q) if out is None else _out_for(out, q.shape, q.dtype, q.device)
+    o = None if q is None else torch.empty_like(q) if out is None or _crosses(out, q, k, v) else \
+        _out_for(out, q.shape, q.dtype, q.device)
     _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
               int(bool(interleaved)))
     return o if out is None else _finish(out, o)
