@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;
   float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
   // (scored: as in the prefill)
-  const float capk = FORM == kScored ? c * a.cap_in : 0.f;
+  const float capk = FORM == kScored ? fminf(c * a.cap_in, 3e38f) : 0.f;
   if (FORM == kScored && a.cap_out > 0.f) c = a.cap_out;
   const float sraw = FORM == kScored && a.slopes ? a.slopes[head] * kLog2e / c : 0.f;
 

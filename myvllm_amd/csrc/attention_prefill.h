@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   CapNear cn{};
   auto score_consts = [&]() __attribute__((always_inline)) {
     if (a.cap_out > 0.f) {
-      capk = c * a.cap_in;
+      capk = fminf(c * a.cap_in, 3e38f);  // (finite: a score of 0 stays 0)
       cn.set(capk);
       c = a.cap_out;
     }

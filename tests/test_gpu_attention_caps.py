@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from attention_bounds import assert_within, ref_and_bound
-from myvllm_amd import flash_attention_prefill, paged_flash_attention_prefill
+from myvllm_amd import flash_attention_prefill, paged_flash_attention_decode, paged_flash_attention_prefill
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -77,3 +77,25 @@ def test_caps_and_scales_at_64_dims(dev, cap, scale):
     got = run(dev, q, k, v, scale, softcap=cap)
     ref, bound = ref_and_bound(q, k, v, torch.arange(70), scale, BF, softcap=cap)
     assert_within(got, ref, bound)
+
+
+@pytest.mark.parametrize("scale", [1e36, -1e38])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scales_past_the_cap(dev, D, scale):
+    """scale / cap past fp32's range: a score of exactly 0 stays 0, every other one
+    is at the cap's end."""
+    q, k, v = normal(12, 64, 4, D), normal(13, 64, 2, D), normal(14, 64, 2, D)
+    q[::2] = 0
+    print(f"scale={scale} D={D}", flush=True)
+    tab = torch.arange(4, dtype=torch.int32, device=dev)[None]
+    kc, vc = (t.to(dev).reshape(4, 16, 2, D) for t in (k, v))
+    none = (q == 0).all(-1, keepdim=True)
+    for cap in (1e-3, 2.0):
+        got = run(dev, q, k, v, scale, softcap=cap)
+        flat, big = ref_and_bound(q, k, v, torch.arange(64), 0.0, BF)
+        assert_within(torch.where(none.to(dev), got, 0), torch.where(none, flat, 0.0), torch.where(none, big, 0.0))
+        assert torch.isfinite(got).all()
+        one = paged_flash_attention_decode(q[:1].to(dev), kc, vc, tab, torch.tensor([64], dtype=torch.int32, device=dev),
+                                           scale, 16, softcap=cap)
+        mean = v.double().mean(0).repeat_interleave(2, 0)[None]
+        assert_within(one, mean, 2**-7 * v.double().abs().mean(0).repeat_interleave(2, 0)[None])
