@@ -420,8 +420,9 @@ int paged_attention_decode_noalloc(const gdn_tensor* q, const gdn_tensor* k_cach
  * softcap 0 and NULL leave each of them out.  All else is as for the plain ops
  * above: arguments, head dims (64, 128 or 256), errors, the workspaces of the
  * paged ones (NULL: the prefill is not split) and their sizes.  GDN_ERR_ARG for
- * a softcap out of range (the tanh is within 3e-7 softcap) and for prefix_lens
- * without causal.  In bf16 with slopes a prefill may lose values below 1e-21 in
+ * a softcap out of range (the tanh is within 3e-7 softcap), for prefix_lens
+ * without causal, and for slopes without a softcap at a scale below 1e-20 that
+ * is not 0.  In bf16 with slopes a prefill may lose values below 1e-21 in
  * rows whose highest score is that of a key so far off that its bias is tens of
  * units.
  */

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
+#include <cmath>
 #include <stdint.h>
 
 #include "../../include/gdn_hip.h"
@@ -602,8 +603,8 @@ int varlen_prefill(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v
 }
 
 // Score forms: the cap, slopes (Hq,) fp32 and prefix lengths (N,).
-int check_scores(const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_t Hq, int64_t N, float softcap,
-                 bool causal) {
+int check_scores(const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_t Hq, int64_t N, float scale,
+                 float softcap, bool causal) {
   // (below, the scores' scale leaves fp32; above, the tanh is not exact enough)
   if (softcap != 0.f && !(softcap >= 1e-3f && softcap <= 4096.f)) return GDN_ERR_ARG;
   if (slopes) {
@@ -611,6 +612,8 @@ int check_scores(const gdn_tensor* slopes, const gdn_tensor* prefix_lens, int64_
     if (slopes->shape[0] != Hq) return GDN_ERR_SHAPE;
     if (slopes->dtype != GDN_DTYPE_F32) return GDN_ERR_DTYPE;
     if (slopes->stride[0] != 1) return GDN_ERR_STRIDE;
+    // (the bias is held in units of the scale: below, slope x distance over it leaves fp32)
+    if (softcap == 0.f && scale != 0.f && std::fabs(scale) < 1e-20f) return GDN_ERR_ARG;
   }
   if (prefix_lens) {
     if (!causal) return GDN_ERR_ARG;
@@ -794,7 +797,7 @@ GDN_EXPORT int flash_attention_varlen_scored(const gdn_tensor* q, const gdn_tens
                                              const gdn_tensor* prefix_lens, int64_t max_seqlen, float scale,
                                              float softcap, int32_t causal, void* stream) {
   GDN_TRY(check_varlen_prefill(q, k, v, cu_seqlens, out, max_seqlen, false));
-  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, softcap, causal != 0));
+  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, scale, softcap, causal != 0));
   return launch_rc(attn_varlen_scored_launch(q, k, v, cu_seqlens, out, slopes, prefix_lens, max_seqlen, scale, softcap,
                                              causal, reinterpret_cast<hipStream_t>(stream)));
 }
@@ -808,7 +811,7 @@ GDN_EXPORT int paged_attention_prefill_scored(const gdn_tensor* q, const gdn_ten
   float* ws;
   GDN_TRY(check_paged_prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, workspace, max_seqlen,
                               &ws));
-  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, softcap, true));
+  GDN_TRY(check_scores(slopes, prefix_lens, q->shape[1], cu_seqlens->shape[0] - 1, scale, softcap, true));
   return launch_rc(attn_paged_scored_launch(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, ws,
                                             slopes, prefix_lens, max_seqlen, scale, softcap,
                                             reinterpret_cast<hipStream_t>(stream)));
@@ -820,7 +823,7 @@ GDN_EXPORT int paged_attention_decode_scored(const gdn_tensor* q, const gdn_tens
                                              const gdn_tensor* slopes, int32_t num_splits, float scale, float softcap,
                                              void* stream) {
   GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits));
-  GDN_TRY(check_scores(slopes, nullptr, q->shape[1], q->shape[0], softcap, true));
+  GDN_TRY(check_scores(slopes, nullptr, q->shape[1], q->shape[0], scale, softcap, true));
   float* ws;
   GDN_TRY(decode_workspace(workspace, paged_attention_decode_workspace_size(q->shape[0], q->shape[1], q->shape[2],
                                                                             num_splits),

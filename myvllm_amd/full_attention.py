@@ -77,9 +77,10 @@ def flash_attention_prefill(
 
     Other forms of scores x = scale q.k, applied in this order: ``softcap``
     (1e-3 to 4096): x <- softcap tanh(x / softcap); ``alibi_slopes``
-    (Hq,) fp32: x <- x - slope_h |i - j|; ``prefix_lens`` (N,), causal only: the
-    first ``prefix_lens[n]`` keys are visible to every query of sequence n.  A
-    packed batch is its own document mask: each document a sequence."""
+    (Hq,) fp32: x <- x - slope_h |i - j| (without a cap for scales from 1e-20
+    on, or 0); ``prefix_lens`` (N,), causal only: the first ``prefix_lens[n]``
+    keys are visible to every query of sequence n.  A packed batch is its own
+    document mask: each document a sequence."""
     if q.shape[1] != num_heads or k.shape[1] != num_kv_heads or q.shape[2] != head_dim or v.shape[2] != head_v_dim:
         raise ValueError("q/k/v shapes disagree with num_heads/num_kv_heads/head_dim/head_v_dim")
     dev = _lib.require_device(q, k, v, cu_seqlens, alibi_slopes, prefix_lens)
