@@ -138,28 +138,28 @@ GDN_DEVICE SharedPlan shared_tiles(const SharedPlanArgs& a, int prices) {
   }
   wgs *= a.Hkv;
   const bool fits = wgs <= a.slots;
-  const int x = fits ? ((int)wgs + kQueues - 1) / kQueues : 0, len = 8 * (kFixed + tiles);
+  const int x = fits ? ((int)wgs + kQueues - 1) / kQueues : 0;
+  const float len = 8.f * (float)(kFixed + tiles);
   const int64_t busy = ((int64_t)units * a.waves + 4 * kQueues - 1) / (4 * kQueues);
   own = busy < kDeep ? (int)busy : kDeep;
   const int F = kDeep - own;
-  const float each = 8.f * kOwnFixed + 9.6f * (float)prices / (float)units;
-  const int t = each < 0x1p22f ? (int)each : 1 << 22;
+  const float t = 8.f * kOwnFixed + 9.6f * (float)prices / (float)units;
   // M: where k rounds of the free workgroups and j of the others make x
-  int k = (x + kDeep - 1) / kDeep, j = 0, M = len * k + (F == 0 ? t : 0);
+  int k = (x + kDeep - 1) / kDeep, j = 0;
+  float M = len * (float)k + (F == 0 ? t : 0.f);
   while (F > 0 && __builtin_amdgcn_ballot_w64(k * F + j * own < x)) {
     if (k * F + j * own >= x) continue;
-    const int next = (k + 1) * len, next_own = t + (j + 1) * len;
+    const float next = (float)(k + 1) * len, next_own = t + (float)(j + 1) * len;
     M = next < next_own ? next : next_own;
     k += next <= next_own;
     j += next_own <= next;
   }
-  const int64_t cost = (int64_t)M + (int64_t)x * kQueues * D / 1400 + (nmax / tiles) / 4;
-  const int c24 = fits && cost < 1 << 24 ? (int)cost : 1 << 24;
-  // (the smallest, of equals the one with fewer pieces; the fewest always fit, and
-  // are taken too where the price of keys past 2^24 wraps)
+  const float cost = M + (float)x * (kQueues * D / 1400.f) + (float)(nmax / tiles) * 0.25f;
+  const int c24 = fits && cost < 0x1p24f ? (int)cost : 1 << 24;
+  // (the smallest, of equals the one with fewer pieces: the fewest, which always
+  // fit, where all cost 2^24)
   const int best = 63 - (wave_top(((1 << 24) - c24) << 6 | (63 - lane)) & 63);
-  const int fit = fits ? tiles : 0, cheap = __builtin_amdgcn_readlane(fit, best);
-  return {cheap > 0 ? cheap : __builtin_amdgcn_readlane(fit, 0), units};
+  return {__builtin_amdgcn_readlane(fits ? tiles : 0, best), units};
 }
 
 // Sum over the threads before this one; *all: over all NT.
