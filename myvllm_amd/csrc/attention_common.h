@@ -97,7 +97,7 @@ GDN_DEVICE const char* kv_row(const KvSource& s, const PagedTable& tb, int64_t n
 enum AttnForm {
   kPlain,
   kScored,  // capped or biased scores, prefix masks
-  kShared,  // decode of sequences that share their first keys: those (prefill kernel), and the others (decode kernel)
+  kShared,  // decode of sequences that share their first keys: those (prefill kernel), and the others (attention_own.h)
 };
 
 // What a shared decode's first launch writes down (attention_shared.hip).  Of a

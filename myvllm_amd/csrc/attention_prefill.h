@@ -190,7 +190,7 @@ template <int BN>
 GDN_DEVICE SplitSeq split_seq(const AttnArgs& a, const SplitPlan& sp, int c, int sh) {
   return c == 0 ? sp.q : split_seq<BN>(a, c + (threadIdx.x & 63), sh);
 }
-// floor((n - 1) / tiles), at most some 64: the float quotient is within one of it
+// floor((n - 1) / tiles), at most 2^20: the float quotient is within one of it
 GDN_DEVICE int split_further(int n, int tiles, float inv) {
   const int last = n > 0 ? n - 1 : 0;
   int u = (int)((float)last * inv);

@@ -6,11 +6,11 @@
 // in one grid, the shared keys through the prefill kernel (attention_prefill.h,
 // kShared), the queries of a group, sequences x heads of a kv head, being the
 // rows of its MFMA tile, so that the group's K and V are read once per 128 of
-// them instead of once per sequence; and each sequence's own keys through the
-// decode kernel (attention_decode.h, kShared) on the workgroups beside them: the
-// one is bound by MFMA and LDS, the other by HBM.  The third merges their
-// unnormalised pieces.  256 sequences of 16 / 2 heads of 256, 16,384 shared keys
-// and 128 to 2,048 of their own (565 MB, 73 GFLOP): 8 + 174 + 9 us, 178 in a row;
+// them instead of once per sequence; and each sequence's own keys, a wave at a
+// time (attention_own.h), on the workgroups beside them: the one is bound by MFMA
+// and LDS, the other by HBM.  The third merges their unnormalised pieces.  256
+// sequences of 16 / 2 heads of 256, 16,384 shared keys and 128 to 2,048 of their
+// own (565 MB, 73 GFLOP): 8 + 174 + 9 us, 178 in a row;
 // 64 behind 8,192 (89 MB) 6 + 30 + 7, 43; 4 behind 1,000 6 + 11 + 6, 23.  With the
 // plan worked out by every workgroup and the own keys in a launch of their own
 // 243, 69 and 33.
@@ -434,7 +434,6 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
   SharedAttnArgs a{};
   DecodeArgs& d = a.own;
   d = decode_args(q, kc, vc, tab, ctx, out, nullptr, 1, scale);
-  d.splits = 2;  // (more than one)
   d.units = (int32_t)sp.units;
   d.part = workspace;
   d.prices = reinterpret_cast<int32_t*>(workspace + sp.prices);
