@@ -361,8 +361,10 @@ __global__ __launch_bounds__(256) void shared_decode_combine_kernel(const Shared
 
 // The workspace, in floats: the decode's, the plan, the shared pieces' partials.
 // Workgroups that the shared keys may take: one per 128 rows of a group and kv
-// head, up to four times as many or one round of the chip in pieces, within
-// 512 MiB of partials.
+// head, however few of them a small group has; in pieces up to four times as many
+// or one round of the chip, the pieces within 512 MiB of partials.  So many groups
+// cost memory: 256 sequences of 16 / 2 heads of 256 in one group 43 MB, in pairs
+// 162; 4,096 of 64 / 8 of 128 710 MB and 1.4 GB.
 // The own keys are dealt over at most 512 waves' units with the heads (half the
 // chip at D = 256, which reads at HBM's rate), and one per four sequences at least,
 // which it takes a while to begin with.
