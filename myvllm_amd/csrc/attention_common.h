@@ -132,7 +132,7 @@ GDN_DEVICE float cap_score(float s, float k) {
 // tile.  It is evaluated in x = h s: folded into the coefficients, the powers of h
 // leave fp32's range (h^9 below 1e-4).  It pays where several waves share a SIMD's
 // transcendental unit: D = 64, six prompts capped and biased under a prefix mask
-// 72 -> 65 us, capped alone 57 -> 56; D = 128 526 -> 533, D = 256, where a wave has
+// 72 -> 66 us, capped alone 57 -> 55; D = 128 526 -> 533, D = 256, where a wave has
 // its SIMD to itself, 481 -> 496.
 struct CapNear {
   float lim, h;

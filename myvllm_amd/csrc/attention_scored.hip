@@ -1,8 +1,8 @@
 // Attention with another form of scores, in the kernels of attention_prefill.h
 // and attention_decode.h: capped by a tanh, biased by the distance of query and
 // key, or with a prefix mask.  Against the plain form (us): 8 causal prompts of 256 to
-// 4,096 tokens, 16 / 2 heads of 256, capped 484 / 417; 4 chunks behind up to 16,384
-// paged keys, 16 / 4 heads of 128, biased 474 / 432; a decode of 64 sequences of
+// 4,096 tokens, 16 / 2 heads of 256, capped 483 / 414; 4 chunks behind up to 16,384
+// paged keys, 16 / 4 heads of 128, biased 481 / 430; a decode of 64 sequences of
 // 1,024 to 8,192 keys, capped, 125 / 120, at 5 TB/s.
 #include "attention_decode.h"
 #include "attention_prefill.h"

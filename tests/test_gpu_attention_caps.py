@@ -95,7 +95,7 @@ def test_scales_past_the_cap(dev, D, scale):
         flat, big = ref_and_bound(q, k, v, torch.arange(64), 0.0, BF)
         assert_within(torch.where(none.to(dev), got, 0), torch.where(none, flat, 0.0), torch.where(none, big, 0.0))
         assert torch.isfinite(got).all()
-        one = paged_flash_attention_decode(q[:1].to(dev), kc, vc, tab, torch.tensor([64], dtype=torch.int32, device=dev),
-                                           scale, 16, softcap=cap)
+        ctx = torch.tensor([64], dtype=torch.int32, device=dev)
+        one = paged_flash_attention_decode(q[:1].to(dev), kc, vc, tab, ctx, scale, 16, softcap=cap)
         mean = v.double().mean(0).repeat_interleave(2, 0)[None]
         assert_within(one, mean, 2**-7 * v.double().abs().mean(0).repeat_interleave(2, 0)[None])

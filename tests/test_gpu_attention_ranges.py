@@ -52,7 +52,7 @@ def test_large_values_and_rising_capped_scores(dev, D, paged):
     k[:, 0, 0] = 7.0 * (torch.arange(256) // 64)
     q, k, v = q.to(BF), k.to(BF), normal(11, 256, 1, D, std=1e33)
     print(f"rising scores D={D} paged={paged}", flush=True)
-    got = run(dev, q, k, v, 2.0, causal=False, softcap=1000.0) if not paged else \
-        run(dev, q, k, v, 2.0, paged=True, softcap=1000.0, prefix_lens=torch.tensor([256], dtype=torch.int32, device=dev))
+    every = dict(prefix_lens=torch.tensor([256], dtype=torch.int32, device=dev)) if paged else dict(causal=False)
+    got = run(dev, q, k, v, 2.0, paged=paged, softcap=1000.0, **every)
     ref, bound = ref_and_bound(q, k, v, torch.arange(len(q)), 2.0, BF, causal=False, softcap=1000.0)
     assert_within(got, ref, bound)
