@@ -140,7 +140,23 @@ def _crosses(out, q, k, v) -> bool:
         return False  # (another shape or type is refused further on)
     if out.data_ptr() == q.data_ptr() and out.stride() == q.stride():
         return False
-    return out.untyped_storage().data_ptr() in {t.untyped_storage().data_ptr() for t in (q, k, v)}
+    return any(_meet(out, t) for t in (q, k, v))
+
+
+def _meet(a, b) -> bool:
+    """Whether two tensors (tokens, heads, dim) of one type may share memory: not
+    where one ends before the other begins, nor as column blocks of one matrix."""
+    es, pa, pb = a.element_size(), a.data_ptr(), b.data_ptr()
+    if a.numel() == 0 or b.numel() == 0 or pa + es * _span(a) <= pb or pb + es * _span(b) <= pa:
+        return False
+    row = a.stride(0) * es
+    at = (pa - pb) % row if row > 0 else 0
+    return not (a.stride(0) == b.stride(0) and es * _span(b[0]) <= at and at + es * _span(a[0]) <= row)
+
+
+def _span(t) -> int:
+    """Elements from a tensor's first to its last."""
+    return 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
 
 
 def _padded_prefill(q, k, v, cu_seqlens, scale, head_dim, head_v_dim, is_causal, max_seqlen, out, **form):
@@ -373,8 +389,8 @@ def paged_kv_append(
     of q and k (halves ``(j, j + rot / 2)`` as the reference's
     ``layers/rotary_embedding.py:20-31``, or neighbours ``(2 j, 2 j + 1)`` when
     ``interleaved``); without them nothing is rotated.  Returns the rotated q
-    (None for ``q=None``), into ``out`` where given, which may be q itself (in other
-    memory of q, k or v it goes through a copy).
+    (None for ``q=None``), into ``out`` where given, which may be q itself (on other
+    rows of q, k or v it goes through a copy).
 
     A token in no sequence or at a position without a table column or a row of
     the rotation is not appended and its row of q is zero; table entries

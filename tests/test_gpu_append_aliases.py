@@ -19,6 +19,15 @@ def test_what_crosses():
     assert _crosses(q[1:], q[:-1], k[1:], v[1:])
     assert _crosses(q.transpose(0, 1)[:, :4], q[:4], k, v)  # q's address, another order of rows
     assert _crosses(k, torch.zeros(9, 4, 64, dtype=BF), k, v)
+    # in one allocation, apart: one after the other, column blocks of one matrix
+    arena = torch.zeros(9 * 4 * 64 * 4, dtype=BF)
+    parts = [t.view(9, 4, 64) for t in arena.chunk(4)]
+    wide = torch.zeros(9, 16, 64, dtype=BF).split([4, 4, 4, 4], 1)
+    for o, *qkv in (parts, wide, wide[::-1], parts[::-1]):
+        assert not _crosses(o, *qkv)
+    late = torch.zeros(10, 16, 64, dtype=BF)  # the next row's column block
+    assert not _crosses(late[1:, 12:], late[:-1, :4], late[:-1, 4:8], late[:-1, 8:12])
+    assert _crosses(late[1:, 10:14], late[:-1, :4], late[:-1, 4:8], late[:-1, 8:12])
     # refused by the entry, not copied over
     assert not _crosses(packed, q, k, v) and not _crosses(one, q, k, v)
     assert not _crosses(k.view(torch.float16), q, k, v)
