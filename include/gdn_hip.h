@@ -39,8 +39,8 @@
  *  - flash_attention_varlen  <- flash_attention_prefill, ops/full_attention.py:114-173
  *  - paged_attention_prefill <- paged_flash_attention_prefill, ops/full_attention.py:454-512
  *  - paged_attention_decode  <- paged_flash_attention_decode, ops/full_attention.py:282-335
- *  - *_scored, paged_attention_decode_shared, paged_kv_append: beside those, no
- *    counterpart in the reference
+ *  - *_scored, *_fp4, paged_attention_decode_shared, paged_kv_append, paged_kv_read,
+ *    cache_copy: beside those, no counterpart in the reference
  */
 #ifndef GDN_HIP_H_
 #define GDN_HIP_H_
@@ -60,6 +60,7 @@ extern "C" {
 #define GDN_DTYPE_F16 2
 #define GDN_DTYPE_I32 3
 #define GDN_DTYPE_I64 4
+#define GDN_DTYPE_U8 5
 
 /* validation codes (negative); positive codes are hipError_t values */
 #define GDN_OK 0
@@ -489,6 +490,79 @@ int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cach
                     const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
                     gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos, const gdn_tensor* sin,
                     int32_t interleaved, void* stream);
+
+/*
+ * paged_kv_append with rotary positions of several axes, caches held in 4 bits, or
+ * both (no counterpart in the reference).
+ *   positions (A, T) i32|i64, 1 <= A <= 4, or NULL: frequency j of a token turns
+ *   by the angle of its axis' position, cos[positions[axis(j)][t]][j].  The axes
+ *   have section0..section3 of the rot / 2 frequencies, in this order (their sum;
+ *   those past A are not read), or, with dealt != 0, in turns while they have some
+ *   left.  A position outside [0, P) on any axis leaves the token out, as a slot
+ *   past the table does; the slot itself follows from context_lens as ever, which
+ *   then may exceed P.  Needs cos and sin.
+ *   k_scales, v_scales, both or neither: k_cache and v_cache are u8
+ *   (num_blocks, page, Hkv, D / 2) and these u8 (num_blocks, Hkv, D / 32, page).  Each
+ *   32 numbers of a row share a scale 2^e, written as the byte e + 127: the smallest e
+ *   with max|x| <= 6 * 2^e, held to -125..125 (bf16) or -13..13 (fp16), which
+ *   keeps every value a normal number of that type.  A number becomes the code (0..7,
+ *   plus 8 for the sign) of the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times the scale,
+ *   of two as near the one with the even code, past 6 scales of 6; the first of two
+ *   codes is in the low half of their byte.  32 numbers with an infinity or a NaN among
+ *   them get the scale byte 255, which reads as NaN.  The numbers are those that a
+ *   16-bit cache would hold; keys are rotated in fp64 for it.  Pages of a multiple of
+ *   16 slots (GDN_ERR_SHAPE); rows of codes 16-byte, scales 4-byte aligned.
+ * All else as for paged_kv_append.  GDN_ERR_ARG for negative sections and sections
+ * that do not add up to rot / 2.
+ */
+int paged_kv_append_ex(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+                       const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
+                       gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos, const gdn_tensor* sin,
+                       const gdn_tensor* positions, gdn_tensor* k_scales, gdn_tensor* v_scales, int32_t interleaved,
+                       int32_t section0, int32_t section1, int32_t section2, int32_t section3, int32_t dealt,
+                       void* stream);
+
+/*
+ * The append's tokens read back: k, v (T, Hkv, D), bf16 or fp16, of caches of that
+ * type, or of caches held in 4 bits (with k_scales and v_scales, as above; values
+ * that a type cannot hold become its infinity).  Tables, lengths and
+ * offsets as for the append; rows without a place, and of table entries outside
+ * [0, num_blocks), are zero.  2 T Hkv below 2^30 (GDN_ERR_RANGE).
+ */
+int paged_kv_read(gdn_tensor* k, gdn_tensor* v, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                  const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
+                  const gdn_tensor* k_scales, const gdn_tensor* v_scales, void* stream);
+
+/*
+ * paged_attention_decode and paged_attention_prefill(_split) over caches held in 4
+ * bits (k_scales, v_scales and the caches as for paged_kv_append_ex): the same results
+ * as over 16-bit caches of the values that the codes stand for, in q's type, which is
+ * to be the type that was appended.  Workspaces and their sizes are the 16-bit ops'; a
+ * NULL workspace leaves the prefill unsplit.  Page strides below 2^32 bytes, and tables
+ * below 2^31 keys (GDN_ERR_RANGE); the prefill's table has a column at least
+ * (GDN_ERR_SHAPE).
+ */
+int paged_attention_decode_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                               const gdn_tensor* k_scales, const gdn_tensor* v_scales, const gdn_tensor* block_tables,
+                               const gdn_tensor* context_lens, gdn_tensor* out, gdn_tensor* workspace,
+                               int32_t num_splits, float scale, void* stream);
+int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                const gdn_tensor* k_scales, const gdn_tensor* v_scales,
+                                const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                const gdn_tensor* cu_seqlens, gdn_tensor* out, gdn_tensor* workspace,
+                                int64_t max_seqlen, float scale, void* stream);
+
+/*
+ * Copies of blocks inside caches (no counterpart in the reference): in every layer of
+ * each cache (layers, blocks, elements of a block), any type, block dst[i] <- block
+ * src[i].  Up to four caches (NULL: none) of one number of blocks.
+ *   pairs (2, n) i32 in HOST memory, read before the call returns: the sources, then
+ *   the places.  Places are distinct and none is a source (GDN_ERR_ARG); ids outside
+ *   the caches are GDN_ERR_RANGE.
+ * The ids travel with the launch, up to 448 pairs each; a captured call replays its own.
+ */
+int cache_copy(gdn_tensor* cache0, gdn_tensor* cache1, gdn_tensor* cache2, gdn_tensor* cache3,
+               const gdn_tensor* pairs, void* stream);
 
 /*
  * Measurement utility, no counterpart in the reference: copies nbytes (a

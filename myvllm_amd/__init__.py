@@ -5,6 +5,7 @@ Public ops keep the names and signatures of yuyifanbupt/myvllm's
 ``myvllm.ops.gated_delta_rule.gated_delta_rule``, ``myvllm.ops.causal_conv1d`` and
 ``myvllm.ops.full_attention``.
 """
+from .cache import LinearAttentionCache, PagedKVCache, cache_copy
 from .causal_conv1d import causal_conv1d_fn, causal_conv1d_update
 from .full_attention import (
     flash_attention_prefill,
@@ -12,6 +13,7 @@ from .full_attention import (
     paged_flash_attention_decode_shared,
     paged_flash_attention_prefill,
     paged_kv_append,
+    paged_kv_read,
 )
 from .norm import RMSNormGated
 from .gated_delta_rule import (
@@ -30,6 +32,10 @@ __all__ = [
     "paged_flash_attention_decode_shared",
     "paged_flash_attention_prefill",
     "paged_kv_append",
+    "paged_kv_read",
+    "cache_copy",
+    "LinearAttentionCache",
+    "PagedKVCache",
     "chunk_gated_delta_rule_fwd",
     "gated_delta_net_decode_step",
     "recurrent_gated_delta_rule",

@@ -33,6 +33,7 @@ DTYPE_CODES = {
     torch.float16: 2,
     torch.int32: 3,
     torch.int64: 4,
+    torch.uint8: 5,
 }
 
 EXPORTED_SYMBOLS = (
@@ -64,6 +65,11 @@ EXPORTED_SYMBOLS = (
     "paged_attention_decode_shared",
     "paged_attention_decode_shared_workspace_size",
     "paged_kv_append",
+    "paged_kv_append_ex",
+    "paged_kv_read",
+    "paged_attention_decode_fp4",
+    "paged_attention_prefill_fp4",
+    "cache_copy",
     "gdn_hbm_copy",
     "gdn_strerror",
     "gdn_abi_version",
@@ -177,6 +183,11 @@ def load() -> ctypes.CDLL:
             ("paged_attention_prefill_scored", [_PT] * 10 + [L, F, F, P]),
             ("paged_attention_decode_scored", [_PT] * 8 + [I, F, F, P]),
             ("paged_attention_decode_shared", [_PT] * 9 + [F, P]),
+            ("paged_kv_append_ex", [_PT] * 14 + [I] * 6 + [P]),
+            ("paged_kv_read", [_PT] * 9 + [P]),
+            ("paged_attention_decode_fp4", [_PT] * 9 + [I, F, P]),
+            ("paged_attention_prefill_fp4", [_PT] * 10 + [L, F, P]),
+            ("cache_copy", [_PT] * 5 + [P]),
         ):
             getattr(lib, fn).restype, getattr(lib, fn).argtypes = ctypes.c_int, types
         lib.paged_attention_decode_shared_workspace_size.restype = L

@@ -30,7 +30,9 @@ SOURCES = [
     "attention.hip",
     "attention_scored.hip",
     "attention_shared.hip",
+    "attention_fp4.hip",
     "kv_append.hip",
+    "cache_copy.hip",
     "hbm_copy.hip",
     "gdn_capi.cpp",
 ]

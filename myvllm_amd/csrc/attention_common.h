@@ -98,6 +98,7 @@ enum AttnForm {
   kPlain,
   kScored,  // capped or biased scores, prefix masks
   kShared,  // decode of sequences that share their first keys: those (prefill kernel), and the others (attention_own.h)
+  kFp4,     // prefill over caches held in 4 bits
 };
 
 // What a shared decode's first launch writes down (attention_shared.hip).  Of a
@@ -154,7 +155,7 @@ struct CapNear {
 constexpr float kLog2e = 1.4426950408889634f;
 
 KvSource kv_source(const gdn_tensor* t, bool paged) {
-  const int64_t es = t->dtype == GDN_DTYPE_F32 ? 4 : 2;
+  const int64_t es = t->dtype == GDN_DTYPE_F32 ? 4 : t->dtype == GDN_DTYPE_U8 ? 1 : 2;
   KvSource s;
   s.base = reinterpret_cast<const char*>(t->data);
   if (paged) {

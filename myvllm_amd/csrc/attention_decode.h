@@ -97,6 +97,108 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
   if (tid == 1023) a.prices[a.B] = base + inc;
 }
 
+// The pieces of a decode workgroup's unit, one after the other:
+// piece(sequence, first key, end of its keys, workspace slot or -1 where it is the
+// whole sequence, the sequence's last key).  first_wave: of the workgroup.
+template <typename Piece>
+GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool first_wave, Piece&& piece) {
+  // with one split, unit z is sequence z; else unit u holds the batch's
+  // prices [x0, x1) (they fit 31 bits, which the entry point checks)
+  constexpr int32_t SP = kDecodeStartPrice;
+  int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
+  if (a.splits > 1) {
+    const int64_t U = (int64_t)a.B * a.units;
+    const int64_t u = (int64_t)blockIdx.z * a.units + blockIdx.x;
+    if (a.prices_inline) {
+      // small batch: every wave sums the prices itself (a lane per sequence,
+      // 64 at a time), then finds the sequence holding price x0 in a second
+      // pass over the exclusive prefix; the first unit's first wave also
+      // writes the prefix for the combine
+      auto price = [&](int32_t i) -> int32_t {
+        if (i >= a.B) return 0;
+        const int32_t t = (int32_t)((clamp64(load_index(a.ctx, i, a.ctx64), 0, cap) + 15) / 16);
+        return t > 0 ? t + SP : 0;
+      };
+      int32_t tot = 0;
+      for (int32_t c0 = 0; c0 < a.B; c0 += 64) tot += price(c0 + lane);
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) tot += __shfl_xor(tot, d);
+      tot = __builtin_amdgcn_readfirstlane(tot);
+      x0 = (int32_t)(u * tot / U);
+      x1 = (int32_t)((u + 1) * tot / U);
+      const bool writer = u == 0 && blockIdx.y == 0 && first_wave;
+      if (writer && lane == 0) a.prices[a.B] = tot;
+      if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
+      int32_t run = 0;
+      for (int32_t c0 = 0; c0 < a.B; c0 += 64) {
+        const int32_t p = price(c0 + lane);
+        int32_t inc = p;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int32_t y = __shfl_up(inc, d);
+          if (lane >= d) inc += y;
+        }
+        const int32_t ex = run + inc - p;  // Q of sequence c0 + lane
+        if (writer && c0 + lane < a.B) a.prices[c0 + lane] = ex;
+        // the lanes with Q <= x0 are a prefix of the chunk's sequences
+        const int32_t cnt = (int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(c0 + lane < a.B && ex <= x0));
+        if (cnt > 0) {
+          b = c0 + cnt - 1;
+          qb = __builtin_amdgcn_readlane(ex, cnt - 1);
+        }
+        run += __builtin_amdgcn_readlane(inc, 63);
+        if (cnt < 64 && !writer) break;  // (the answer is in this chunk)
+      }
+      if (x0 >= x1) return;
+    } else {
+      const int64_t Pt = load_index_scalar(a.prices, a.B, false);
+      x0 = (int32_t)(u * Pt / U);
+      x1 = (int32_t)((u + 1) * Pt / U);
+      if (x0 >= x1) return;  // an empty unit (a smaller total than U): no piece
+      // the sequence holding price x0: the last b < B with Q[b] <= x0 (Q[0] =
+      // 0), by a 64-ary search over the prefix (one probe per lane per
+      // round, Q[lo] <= x0 throughout)
+      int32_t lo = 0, hi = a.B;
+      while (hi - lo > 64) {
+        const int32_t step = (hi - lo + 63) / 64;
+        const int32_t idx = lo + lane * step;
+        const bool le = idx < hi && a.prices[idx] <= x0;
+        lo += ((int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1) * step;
+        hi = lo + step < hi ? lo + step : hi;
+      }
+      const int32_t idx = lo + lane;
+      const bool le = idx < hi && a.prices[idx] <= x0;
+      b = __builtin_amdgcn_readfirstlane(lo + (int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1);
+      qb = (int32_t)load_index_scalar(a.prices, b, false);
+    }
+  }
+  for (;;) {
+    const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
+    // keys of the piece: the whole sequence (one split; a zero row when L =
+    // 0), or its tiles whose prices lie in the unit's range.  A unit that
+    // holds all of a sequence's tiles writes its output row itself (the
+    // combine finds that sequence in one unit and skips it), else the piece
+    // goes to its workspace slot.
+    int32_t qn = 0;
+    int64_t k_lo = 0, k_hi = L, slot = -1;
+    bool any = true;
+    if (a.splits > 1) {
+      const int32_t tb = (int32_t)((L + 15) / 16);  // the sequence's tiles
+      qn = qb + (tb > 0 ? tb + SP : 0);
+      const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
+      const int32_t t0 = r0 < 0 ? 0 : (r0 > tb ? tb : r0), t1 = r1 < 0 ? 0 : (r1 > tb ? tb : r1);
+      k_lo = 16 * (int64_t)t0;
+      k_hi = 16 * (int64_t)t1 < L ? 16 * (int64_t)t1 : L;
+      any = t1 > t0;
+      if (t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
+    }
+    if (any) piece(b, k_lo, k_hi, slot, L - 1);
+    if (a.splits == 1 || qn >= x1) break;
+    ++b;
+    qb = qn;
+  }
+}
+
 // LDS bytes of one decode wave: a 16-row V tile with a 32-byte row skew and
 // the wave's query fragments
 template <typename T, int D>
@@ -340,101 +442,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     }
   };
 
-  // with one split, unit z is sequence z; else unit u holds the batch's
-  // prices [x0, x1) (they fit 31 bits, which the entry point checks)
-  constexpr int32_t SP = kDecodeStartPrice;
-  int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
-  if (a.splits > 1) {
-    const int64_t U = (int64_t)a.B * a.units;
-    const int64_t u = (int64_t)blockIdx.z * a.units + blockIdx.x;
-    if (a.prices_inline) {
-      // small batch: every wave sums the prices itself (a lane per sequence,
-      // 64 at a time), then finds the sequence holding price x0 in a second
-      // pass over the exclusive prefix; the first unit's first wave also
-      // writes the prefix for the combine
-      auto price = [&](int32_t i) -> int32_t {
-        if (i >= a.B) return 0;
-        const int32_t t = (int32_t)((clamp64(load_index(a.ctx, i, a.ctx64), 0, cap) + 15) / 16);
-        return t > 0 ? t + SP : 0;
-      };
-      int32_t tot = 0;
-      for (int32_t c0 = 0; c0 < a.B; c0 += 64) tot += price(c0 + lane);
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) tot += __shfl_xor(tot, d);
-      tot = __builtin_amdgcn_readfirstlane(tot);
-      x0 = (int32_t)(u * tot / U);
-      x1 = (int32_t)((u + 1) * tot / U);
-      const bool writer = u == 0 && blockIdx.y == 0 && wv == 0;
-      if (writer && lane == 0) a.prices[a.B] = tot;
-      if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
-      int32_t run = 0;
-      for (int32_t c0 = 0; c0 < a.B; c0 += 64) {
-        const int32_t p = price(c0 + lane);
-        int32_t inc = p;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int32_t y = __shfl_up(inc, d);
-          if (lane >= d) inc += y;
-        }
-        const int32_t ex = run + inc - p;  // Q of sequence c0 + lane
-        if (writer && c0 + lane < a.B) a.prices[c0 + lane] = ex;
-        // the lanes with Q <= x0 are a prefix of the chunk's sequences
-        const int32_t cnt = (int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(c0 + lane < a.B && ex <= x0));
-        if (cnt > 0) {
-          b = c0 + cnt - 1;
-          qb = __builtin_amdgcn_readlane(ex, cnt - 1);
-        }
-        run += __builtin_amdgcn_readlane(inc, 63);
-        if (cnt < 64 && !writer) break;  // (the answer is in this chunk)
-      }
-      if (x0 >= x1) return;
-    } else {
-      const int64_t Pt = load_index_scalar(a.prices, a.B, false);
-      x0 = (int32_t)(u * Pt / U);
-      x1 = (int32_t)((u + 1) * Pt / U);
-      if (x0 >= x1) return;  // an empty unit (a smaller total than U): no piece
-      // the sequence holding price x0: the last b < B with Q[b] <= x0 (Q[0] =
-      // 0), by a 64-ary search over the prefix (one probe per lane per
-      // round, Q[lo] <= x0 throughout)
-      int32_t lo = 0, hi = a.B;
-      while (hi - lo > 64) {
-        const int32_t step = (hi - lo + 63) / 64;
-        const int32_t idx = lo + lane * step;
-        const bool le = idx < hi && a.prices[idx] <= x0;
-        lo += ((int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1) * step;
-        hi = lo + step < hi ? lo + step : hi;
-      }
-      const int32_t idx = lo + lane;
-      const bool le = idx < hi && a.prices[idx] <= x0;
-      b = __builtin_amdgcn_readfirstlane(lo + (int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1);
-      qb = (int32_t)load_index_scalar(a.prices, b, false);
-    }
-  }
-  for (;;) {
-    const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
-    // keys of the piece: the whole sequence (one split; a zero row when L =
-    // 0), or its tiles whose prices lie in the unit's range.  A unit that
-    // holds all of a sequence's tiles writes its output row itself (the
-    // combine finds that sequence in one unit and skips it), else the piece
-    // goes to its workspace slot.
-    int32_t qn = 0;
-    int64_t k_lo = 0, k_hi = L, slot = -1;
-    bool any = true;
-    if (a.splits > 1) {
-      const int32_t tb = (int32_t)((L + 15) / 16);  // the sequence's tiles
-      qn = qb + (tb > 0 ? tb + SP : 0);
-      const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
-      const int32_t t0 = r0 < 0 ? 0 : (r0 > tb ? tb : r0), t1 = r1 < 0 ? 0 : (r1 > tb ? tb : r1);
-      k_lo = 16 * (int64_t)t0;
-      k_hi = 16 * (int64_t)t1 < L ? 16 * (int64_t)t1 : L;
-      any = t1 > t0;
-      if (t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
-    }
-    if (any) piece(b, k_lo, k_hi, slot, L - 1);
-    if (a.splits == 1 || qn >= x1) break;
-    ++b;
-    qb = qn;
-  }
+  decode_deal(a, cap, lane, wv == 0, piece);
 }
 
 // Merge of the pieces of one (sequence, query head): one wave, D / 64

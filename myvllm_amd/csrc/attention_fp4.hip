@@ -1,0 +1,416 @@
+// Attention over paged caches held in 4 bits (fp4.h): the decode kernel, and the
+// launches of it and of the prefill (attention_prefill.h, kFp4).
+//
+// The codes become 16-bit numbers, exactly, in front of the matrix
+// instructions, so the result is that of the 16-bit attention over the values that
+// the codes stand for.  The scales of a page lie slot by slot for each 32 dims
+// (blocks, heads, D / 32, page): one load gives a lane those of four keys.
+#include "attention_decode.h"
+#include "attention_prefill.h"
+
+namespace {
+
+struct Fp4DecodeArgs : DecodeArgs {
+  ScaleSource ks, vs;
+};
+
+// Decode: a workgroup is four waves, of 4 / KS kv heads (and up to 16 query heads of
+// each); the KS waves of a head take the 32-key tiles of a piece in turn.  Units,
+// pieces and the merge over workgroups are the plain decode's (attention_decode.h).
+//
+// S^T = K Q^T: lane (c, g) holds dims [CB (4 i + g), + CB) of key c of a 16-key group,
+// whole 16-byte loads (a scale each) whose dims the queries' fragments follow.
+// O^T = V^T P^T: lane (c, g) holds dims [VE c, + VE) of the keys 4 g + 0..3 of both
+// groups, which is where S^T leaves their probabilities, so V reaches the matrix
+// instruction without LDS: two numbers of a dim pair at a time are turned into 16
+// bits, and byte permutes pair them by keys.
+template <typename T, int D, int KS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_fp4_kernel(
+    const Fp4DecodeArgs a) {
+  typedef Mma<T> M;
+  typedef typename M::v8 v8;
+  typedef typename M::v4 v4;
+  constexpr int CB = D >= 128 ? 32 : 16;  // dims of one load of K
+  constexpr int NI = D / (4 * CB);        // loads per key and lane
+  constexpr int NQ = CB / 8;              // k-steps per load
+  constexpr int VE = D / 16;              // dims of V per lane
+  constexpr int VW = VE > 8 ? 2 : 1;      // their words
+  constexpr int LDO = D + 4;
+  __shared__ __align__(16) float ob[KS > 1 ? 4 * 16 * LDO : 4];
+  __shared__ float ml[4][2][16];
+
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, grp = lane >> 4, part = wv % KS;
+  const int64_t cap = a.tab.cols * a.tab.page;
+  const int R = a.Hq / a.Hkv, hgroups = (R + 15) / 16;
+  const int kvh = (blockIdx.y / hgroups) * (4 / KS) + wv / KS;
+  const int h0 = (blockIdx.y % hgroups) * 16;
+  const bool hvalid = h0 + c16 < R;
+  const int head = kvh * R + (hvalid ? h0 + c16 : 0);
+  const char* const kbase = a.k.base + kvh * a.k.sh;
+  const char* const vbase = a.v.base + kvh * a.v.sh;
+  const uint8_t* const ksbase = a.ks.base + kvh * a.ks.sh;
+  const uint8_t* const vsbase = a.vs.base + kvh * a.vs.sh;
+  const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;  // (below 2^32, as all of them, checked by the entry)
+  const uint64_t kssb = (uint32_t)a.ks.sb, vssb = (uint32_t)a.vs.sb;
+  const uint32_t kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st, ksd = (uint32_t)a.ks.sd, vsd = (uint32_t)a.vs.sd;
+  const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
+  const uint32_t gpp = (uint32_t)a.tab.page / 16u;
+
+  struct Tile {
+    uint32_t k[2][NI][CB / 8], ks[2][NI];
+    uint32_t v[8][VW], vs[2];
+  };
+
+  auto piece = [&](int64_t b, int64_t k_lo, int64_t k_hi, int64_t slot, int64_t) {
+    const int ntiles = (int)((k_hi - k_lo + 31) / 32);
+    v8 qf[NI][NQ];
+    {
+      const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_ss + (int64_t)head * a.q_sh;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const v8 x = hvalid ? *reinterpret_cast<const v8*>(qp + CB * (4 * i + grp) + 8 * q) : v8{};
+          qf[i][q] = a.c > 0.f ? x : (a.c < 0.f ? -x : v8{});
+        }
+    }
+    const void* trow = reinterpret_cast<const char*>(a.tab.table) + (a.tab.is64 ? 8 : 4) * (b * a.tab.row_stride);
+    const uint32_t g0 = (uint32_t)k_lo / 16u, gend = ((uint32_t)k_hi + 15u) / 16u;
+    auto block_of = [&](uint32_t g) -> int64_t {
+      if (g >= gend) return -1;
+      const int64_t blk = load_index_scalar(trow, gpp == 1u ? g : g / gpp, a.tab.is64);
+      return blk >= 0 && blk < a.tab.num_blocks ? blk : -1;
+    };
+    auto load = [&](int t, const int64_t* blk, Tile& x) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t g = g0 + 2u * (uint32_t)t + h, j0 = 16u * g;
+        const uint32_t r0 = gpp == 1u ? 0u : 16u * (g - (g / gpp) * gpp);
+        const bool ok = blk[h] >= 0;
+        const uint64_t bb = ok ? (uint32_t)blk[h] : 0u;
+        // the ranges end after the group's keys, so codes past them read as 0
+        const uint32_t left = ok && j0 < (uint32_t)k_hi ? (uint32_t)k_hi - j0 : 0u;
+        const uint32_t rows = left > 0u ? r0 + (left < 16u ? left : 16u) : 0u;
+        const __amdgpu_buffer_rsrc_t rk =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + bb * ksb), 0, rows * kst, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + bb * vsb), 0, rows * vst, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)(ksbase + bb * kssb), 0,
+                                                                             left > 0u ? D / 32 * ksd : 0u, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)(vsbase + bb * vssb), 0,
+                                                                             left > 0u ? D / 32 * vsd : 0u, 0x00020000);
+        const uint32_t ko = (r0 + c16) * kst + CB / 2 * grp;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if constexpr (CB == 32) {
+            const uint4 w = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + 64 * i, 0, 0));
+            x.k[h][i][0] = w.x, x.k[h][i][1] = w.y, x.k[h][i][2] = w.z, x.k[h][i][3] = w.w;
+          } else {
+            const uint2 w = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rk, ko, 0, 0));
+            x.k[h][i][0] = w.x, x.k[h][i][1] = w.y;
+          }
+          x.ks[h][i] = __builtin_amdgcn_raw_buffer_load_b8(rks, CB * (4 * i + grp) / 32 * ksd + r0 + c16, 0, 0);
+        }
+        const uint32_t vo = (r0 + 4 * grp) * vst + VE / 2 * c16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t* const w = x.v[4 * h + e];
+          if constexpr (VE == 16) {
+            const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo + e * vst, 0, 0));
+            w[0] = y.x, w[1] = y.y;
+          } else if constexpr (VE == 8) {
+            w[0] = __builtin_amdgcn_raw_buffer_load_b32(rv, vo + e * vst, 0, 0);
+          } else {
+            w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rv, vo + e * vst, 0, 0);
+          }
+        }
+        x.vs[h] = __builtin_amdgcn_raw_buffer_load_b32(rvs, VE * c16 / 32 * vsd + r0 + 4 * grp, 0, 0);
+      }
+    };
+
+    f32x4 oacc[VE];
+#pragma unroll
+    for (int d = 0; d < VE; ++d) oacc[d] = f32x4{};
+    float m_used = -INFINITY, lsum = 0.f, nb = 0.f;  // (as in the plain decode)
+
+    auto compute = [&](int t, const Tile& x) {
+      f32x4 s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = f32x4{};
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const float sc = fp4_scale(x.ks[h][i]);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            s[h] = M::m16k32(__builtin_bit_cast(v8, fp4_eight<T>(x.k[h][i][q], sc)), qf[i][q], s[h]);
+        }
+      }
+      const uint32_t j0 = (uint32_t)k_lo + 32u * (uint32_t)t;
+      uint32_t vs[2] = {x.vs[0], x.vs[1]};
+      if (j0 + 32u > (uint32_t)k_hi) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j0 + 16u * h + 4u * grp + r >= (uint32_t)k_hi) {
+              s[h][r] = -INFINITY;
+              vs[h] &= ~(255u << (8 * r));  // (a stale scale may stand for NaN)
+            }
+      }
+      float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+      mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      if (__builtin_amdgcn_ballot_w64(mx * c > m_used + 8.f) != 0) {
+        float mg = fmaxf(mx, __shfl_xor(mx, 16));
+        mg = fmaxf(mg, __shfl_xor(mg, 32));
+        const float mn = fmaxf(m_used, mg * c);
+        const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
+#pragma unroll
+        for (int d = 0; d < VE; ++d) oacc[d] *= alpha;
+        lsum *= alpha;
+        m_used = mn;
+        nb = mn == -INFINITY ? 0.f : -mn;
+      }
+      v8 pf;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = exp2_fast(__builtin_fmaf(s[h][r], c, nb));
+          lsum += p;
+          pf[4 * h + r] = (T)p;
+        }
+      float sc[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sc[e] = fp4_scale(vs[e >> 2] >> (8 * (e & 3)) & 255u);
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        constexpr int NP = VE > 8 ? 4 : VE / 2;  // pairs of dims in a word
+        uint32_t y[8][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t u = x.v[e][w];
+          y[e][0] = Fp4<T>::template pair<0>(u, sc[e]);
+          y[e][1] = Fp4<T>::template pair<1>(u, sc[e]);
+          if constexpr (NP == 4) {
+            y[e][2] = Fp4<T>::template pair<2>(u, sc[e]);
+            y[e][3] = Fp4<T>::template pair<3>(u, sc[e]);
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const uint32_t sel = o ? 0x07060302u : 0x05040100u;
+            const uint4 vf = {__builtin_amdgcn_perm(y[1][p], y[0][p], sel), __builtin_amdgcn_perm(y[3][p], y[2][p], sel),
+                              __builtin_amdgcn_perm(y[5][p], y[4][p], sel), __builtin_amdgcn_perm(y[7][p], y[6][p], sel)};
+            const int d = 8 * w + 2 * p + o;
+            oacc[d] = M::m16k32(__builtin_bit_cast(v8, vf), pf, oacc[d]);
+          }
+      }
+    };
+
+    // two tiles in flight, their blocks looked up one tile earlier still; loads are
+    // issued unconditionally (past the range they read zeros)
+    Tile xA, xB;
+    int64_t bA[2], bB[2];
+    auto blocks = [&](int t, int64_t* o) {
+      o[0] = block_of(g0 + 2u * (uint32_t)t);
+      o[1] = block_of(g0 + 2u * (uint32_t)t + 1u);
+    };
+    blocks(part, bA);
+    blocks(part + KS, bB);
+    load(part, bA, xA);
+    load(part + KS, bB, xB);
+    blocks(part + 2 * KS, bA);
+    blocks(part + 3 * KS, bB);
+    for (int t = part; t < ntiles; t += 2 * KS) {
+      compute(t, xA);
+      load(t + 2 * KS, bA, xA);
+      blocks(t + 4 * KS, bA);
+      if (t + KS < ntiles) compute(t + KS, xB);
+      load(t + 3 * KS, bB, xB);
+      blocks(t + 5 * KS, bB);
+    }
+
+    float lt = lsum + __shfl_xor(lsum, 16);
+    lt += __shfl_xor(lt, 32);
+    if constexpr (KS == 1) {
+      if (!hvalid) return;
+      const float inv = lt > 0.f ? 1.f / lt : 0.f;
+      float* const pp = a.part + (slot * a.Hq + head) * (int64_t)(D + 4);
+      T* const op = reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)head * a.o_sh;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; j += 4) {
+          const int d = VE * (4 * grp + r) + j;
+          const f32x4 o = {oacc[j][r], oacc[j + 1][r], oacc[j + 2][r], oacc[j + 3][r]};
+          if (slot < 0) *reinterpret_cast<v4*>(op + d) = v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+          else *reinterpret_cast<f32x4*>(pp + d) = o;
+        }
+      if (slot >= 0 && grp == 0) {
+        pp[D] = m_used;
+        pp[D + 1] = lt;
+      }
+    } else {
+      // the head's waves meet in LDS: maxima and sums, then O on the common base
+      const int w0 = wv - part;  // the head's first wave
+      __syncthreads();           // (the previous piece's rows have been read)
+      if (grp == 0) {
+        ml[wv][0][c16] = m_used;
+        ml[wv][1][c16] = lt;
+      }
+      __syncthreads();
+      auto top = [&](int h) {
+        float m = ml[w0][0][h];
+#pragma unroll
+        for (int p = 1; p < KS; ++p) m = fmaxf(m, ml[w0 + p][0][h]);
+        return m;
+      };
+      const float mt = top(c16), f = m_used == -INFINITY ? 0.f : exp2_fast(m_used - mt);
+      float* const mine = ob + (wv * 16 + c16) * LDO;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VE; j += 4)
+          *reinterpret_cast<f32x4*>(mine + VE * (4 * grp + r) + j) =
+              f32x4{oacc[j][r] * f, oacc[j + 1][r] * f, oacc[j + 2][r] * f, oacc[j + 3][r] * f};
+      __syncthreads();
+      constexpr int LR = D / 4;         // lanes per row
+      constexpr int RW = 16 / KS;       // rows per wave
+      static_assert(LR <= 64 && RW % (64 / LR) == 0, "rows of a wave");
+#pragma unroll
+      for (int i = 0; i < RW / (64 / LR); ++i) {
+        const int h = part * RW + i * (64 / LR) + lane / LR, d = 4 * (lane % LR);
+        f32x4 o = *reinterpret_cast<const f32x4*>(ob + (w0 * 16 + h) * LDO + d);
+#pragma unroll
+        for (int p = 1; p < KS; ++p) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(ob + ((w0 + p) * 16 + h) * LDO + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += y[e];
+        }
+        const float m = top(h);
+        float l = 0.f;
+#pragma unroll
+        for (int p = 0; p < KS; ++p) {
+          const float mp = ml[w0 + p][0][h];
+          l += mp == -INFINITY ? 0.f : ml[w0 + p][1][h] * exp2_fast(mp - m);
+        }
+        if (h0 + h >= R) continue;
+        const int hd = kvh * R + h0 + h;
+        if (slot < 0) {
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)hd * a.o_sh + d) =
+              v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+        } else {
+          float* const pp = a.part + (slot * a.Hq + hd) * (int64_t)(D + 4);
+          *reinterpret_cast<f32x4*>(pp + d) = o;
+          if (d == 0) {
+            pp[D] = m;
+            pp[D + 1] = l;
+          }
+        }
+      }
+    }
+  };
+  decode_deal(a, cap, lane, wv == 0, piece);
+}
+
+// Kv heads of a decode workgroup: as many as a 128-byte line of the cache holds rows
+// of, so that a line is read by one XCD (rows of 128, 64 and 32 bytes), if the
+// heads divide by that.
+int fp4_heads(int Hkv, int D) {
+  int n = 256 / D;
+  while (Hkv % n) n /= 2;
+  return n;
+}
+
+template <typename T, int D>
+hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
+  const int heads = fp4_heads(a.Hkv, D), hgroups = (a.Hq / a.Hkv + 15) / 16;
+  const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / heads * hgroups), (unsigned)a.B);
+  if (a.splits > 1 && !a.prices_inline) {
+    attn_decode_prices_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (heads == 1) attn_decode_fp4_kernel<T, D, 4><<<grid, dim3(256), 0, st>>>(a);
+  else if (heads == 2) attn_decode_fp4_kernel<T, D, 2><<<grid, dim3(256), 0, st>>>(a);
+  else attn_decode_fp4_kernel<T, D, 1><<<grid, dim3(256), 0, st>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  attn_decode_combine_kernel<T, D><<<dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
+  constexpr int BN = 32;
+  if (nseq <= 0 || max_len <= 0) {
+    zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu,
+                                                                             a.cu64, a.nseq, a.T);
+    return hipGetLastError();
+  }
+  // (the grids of the 16-bit caches, launch_prefill_t)
+  const int64_t tiles = a.T / (32 * (4 / a.gh)) + nseq + 1;
+  if (a.extra > 0) {
+    const dim3 grid((unsigned)(a.rows + a.Hq / a.gh + a.extra));
+    if (a.tab.is64) attn_prefill_kernel<T, D, BN, 3, true, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+    else attn_prefill_kernel<T, D, BN, 2, true, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    constexpr int DG = D == 256 ? 2 : 1;
+    attn_prefill_combine_kernel<T, D, BN, DG><<<dim3((unsigned)a.rows, a.rows >= 256 ? 1 : D / (32 * DG)), dim3(256), 0,
+                                                st>>>(a);
+    return hipGetLastError();
+  }
+  const dim3 grid((unsigned)(tiles * (a.Hq / a.gh)));
+  if (a.tab.is64) attn_prefill_kernel<T, D, BN, 3, false, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+  else attn_prefill_kernel<T, D, BN, 2, false, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                  const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
+                                  const gdn_tensor* ctx, gdn_tensor* out, float* workspace, int32_t splits, float scale,
+                                  hipStream_t st) {
+  if (q->shape[0] == 0) return hipSuccess;
+  Fp4DecodeArgs a{};
+  static_cast<DecodeArgs&>(a) = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
+  a.ks = scale_source(ks);
+  a.vs = scale_source(vs);
+  const int D = (int)q->shape[2];
+  if (q->dtype == GDN_DTYPE_BF16) {
+    if (D == 64) return launch_decode_fp4<bf16_t, 64>(a, st);
+    if (D == 128) return launch_decode_fp4<bf16_t, 128>(a, st);
+    return launch_decode_fp4<bf16_t, 256>(a, st);
+  }
+  if (D == 64) return launch_decode_fp4<f16_t, 64>(a, st);
+  if (D == 128) return launch_decode_fp4<f16_t, 128>(a, st);
+  return launch_decode_fp4<f16_t, 256>(a, st);
+}
+
+hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                   const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
+                                   const gdn_tensor* ctx, const gdn_tensor* cu, gdn_tensor* out, float* workspace,
+                                   int64_t max_seqlen, float scale, hipStream_t st) {
+  if (q->shape[0] == 0) return hipSuccess;
+  Fp4AttnArgs a{};
+  static_cast<AttnArgs&>(a) = paged_args(q, kc, vc, tab, ctx, cu, out, workspace, scale);
+  a.ks = scale_source(ks);
+  a.vs = scale_source(vs);
+  const int D = (int)q->shape[2];
+  const int64_t N = cu->shape[0] - 1;
+  if (q->dtype == GDN_DTYPE_BF16) {
+    if (D == 64) return launch_prefill_fp4<bf16_t, 64>(a, N, max_seqlen, st);
+    if (D == 128) return launch_prefill_fp4<bf16_t, 128>(a, N, max_seqlen, st);
+    return launch_prefill_fp4<bf16_t, 256>(a, N, max_seqlen, st);
+  }
+  if (D == 64) return launch_prefill_fp4<f16_t, 64>(a, N, max_seqlen, st);
+  if (D == 128) return launch_prefill_fp4<f16_t, 128>(a, N, max_seqlen, st);
+  return launch_prefill_fp4<f16_t, 256>(a, N, max_seqlen, st);
+}

@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "attention_own.h"
+#include "fp4.h"
 
 namespace {
 
@@ -51,6 +52,11 @@ struct SharedAttnArgs : AttnArgs {
   const SharedWork* work;
   DecodeArgs own;
   uint32_t own_wgs;
+};
+
+// kFp4: block scales of the caches' codes
+struct Fp4AttnArgs : AttnArgs {
+  ScaleSource ks, vs;
 };
 
 // Floats of one piece's partial: per wave, the accumulators of its 32 queries
@@ -362,7 +368,8 @@ GDN_DEVICE void zero_rows_tail(const AttnArgs& a, uint32_t wg, uint32_t n) {
 // 32 keys 157, three waves per SIMD 158 (32 keys) and 197 (64, spills).
 template <typename T, int D, int BN, int PG, bool SPLIT, int DQ = 0, AttnForm FORM = kPlain>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prefill_kernel(
-    const std::conditional_t<FORM == kShared, SharedAttnArgs, AttnArgs> a) {
+    const std::conditional_t<FORM == kShared, SharedAttnArgs,
+                             std::conditional_t<FORM == kFp4, Fp4AttnArgs, AttnArgs>> a) {
   constexpr bool PAGED = PG != 0;
   // DQ > 0: head dims of a.dim <= DQ <= D elements (packed rows only), a
   // multiple of 8.  The rows are read as they lie and the 16-byte pieces past
@@ -376,6 +383,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   static_assert(!SPLIT || PG >= 2, "split rows are paged rows of whole 16-row groups");
   static_assert(FORM == kPlain || !RAG, "scored and shared rows are of the kernels' own head dims");
   static_assert(FORM != kShared || (PAGED && !SPLIT), "shared keys are paged, in pieces of their own");
+  // kFp4: a thread loads the codes of QE numbers of a row and their scale byte, and
+  // turns them into 16 bits where the others store their tile to LDS.  So the
+  // tiles in flight take a quarter of the registers, and the products are the
+  // 16-bit cache's.
+  constexpr bool Q4 = FORM == kFp4;
+  constexpr int QE = BN * D / 256, QW = QE >= 8 ? QE / 8 : 1, QL8 = D / QE;  // words of codes, threads per row
+  static_assert(!Q4 || (PG >= 2 && QE >= 8 && QE <= 32 && 32 % QL8 == 0), "codes of up to one block a thread");
   typedef Mma<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v4 v4;
@@ -718,6 +732,100 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       *reinterpret_cast<uint4*>(&vs[buf][row * LDV + 8 * ch]) = vd[i];
     }
   };
+  // (kFp4) this thread's codes and scale of a row of keys or values
+  struct Codes {
+    uint32_t w[QW], s;
+  };
+  typedef std::conditional_t<Q4, Codes, uint4> Reg;
+  constexpr int NREG = Q4 ? 1 : NLD;
+  auto load = [&](int t, Reg* kd, Reg* vd) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      uint32_t nlo[NG], nhi[NG], nsl[NG];
+      bool nin[NG];
+      load_ids(t + 1, nlo, nhi, nin, nsl);
+      // a wave's rows lie in one 16-row group
+      const uint32_t row = (uint32_t)tid / QL8, ch = (uint32_t)tid % QL8;
+      static_assert(64 / QL8 <= 16, "a wave's rows");
+      const int gu = w * (64 / QL8) / 16;
+      uint32_t ulo = idlo[0], uhi = idhi[0], usl = slots[0];
+      bool uin = idin[0];
+#pragma unroll
+      for (int g = 1; g < NG; ++g)
+        if (gu == g) ulo = idlo[g], uhi = idhi[g], usl = slots[g], uin = idin[g];
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)ulo);
+      const uint32_t hi = T64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)uhi) : 0u;
+      const bool valid = uin && hi == 0u && lo < nblk;
+      const uint64_t bb = valid ? lo : 0u;
+      const uint32_t j0 = (uint32_t)t * BN + 16u * gu;
+      const uint32_t ends = usl + (j0 < kend32 ? (kend32 - j0 < 16u ? kend32 - j0 : 16u) : 0u);
+      const __amdgpu_buffer_rsrc_t rk =
+          __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + bb * ksb), 0, valid ? ends * kst : 0u, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv =
+          __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + bb * vsb), 0, valid ? ends * vst : 0u, 0x00020000);
+      // (the scales of rows past the range may be stale: they are read past the
+      // descriptor's end, as 0, or a NaN among them would reach the sums by 0 codes)
+      const uint32_t slot = usl + (row & 15), far = slot < ends ? 0u : 0x80000000u;
+      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(a.ks.base + bb * (uint32_t)a.ks.sb + kvh * a.ks.sh), 0, valid ? D / 32 * (uint32_t)a.ks.sd : 0u, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(a.vs.base + bb * (uint32_t)a.vs.sb + kvh * a.vs.sh), 0, valid ? D / 32 * (uint32_t)a.vs.sd : 0u, 0x00020000);
+      auto codes = [&](__amdgpu_buffer_rsrc_t r, uint32_t o, Codes& c) __attribute__((always_inline)) {
+        if constexpr (QW == 4) {
+          const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+          c.w[0] = x.x, c.w[1] = x.y, c.w[2] = x.z, c.w[3] = x.w;
+        } else if constexpr (QW == 2) {
+          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+          c.w[0] = x.x, c.w[1] = x.y;
+        } else {
+          c.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+        }
+      };
+      codes(rk, slot * kst + ch * (QE / 2), kd[0]);
+      codes(rv, slot * vst + ch * (QE / 2), vd[0]);
+      kd[0].s = __builtin_amdgcn_raw_buffer_load_b8(rks, (ch * QE / 32 * (uint32_t)a.ks.sd + slot) | far, 0, 0);
+      vd[0].s = __builtin_amdgcn_raw_buffer_load_b8(rvs, (ch * QE / 32 * (uint32_t)a.vs.sd + slot) | far, 0, 0);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) idlo[g] = nlo[g], idhi[g] = nhi[g], idin[g] = nin[g], slots[g] = nsl[g];
+    } else {
+      load_tile(t, kd, vd);
+    }
+  };
+  auto store = [&](int buf, const Reg* kd, const Reg* vd) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      const int row = tid / QL8, ch = tid % QL8;
+      // neighbouring lanes write their words in another order each, so that their
+      // 16-byte stores, QE elements apart, fall on different banks
+      const int turn = QW == 4 ? (ch + (ch >> 2)) & 3 : QW == 2 ? ch >> 2 & 1 : 0;
+      auto put = [&](T* at, const Codes& c) __attribute__((always_inline)) {
+        const float s = fp4_scale(c.s);
+        uint32_t x[QW];
+#pragma unroll
+        for (int i = 0; i < QW; ++i) x[i] = c.w[i];
+        if constexpr (QW >= 2) {  // x[i] <- word (i ^ turn)
+#pragma unroll
+          for (int i = 0; i < QW; i += 2) {
+            const uint32_t p = x[i], q = x[i + 1];
+            x[i] = turn & 1 ? q : p;
+            x[i + 1] = turn & 1 ? p : q;
+          }
+        }
+        if constexpr (QW == 4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t p = x[i], q = x[i + 2];
+            x[i] = turn & 2 ? q : p;
+            x[i + 2] = turn & 2 ? p : q;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < QW; ++i) *reinterpret_cast<uint4*>(at + QE * ch + 8 * (i ^ turn)) = fp4_eight<T>(x[i], s);
+      };
+      put(&ks[buf][row * LDK], kd[0]);
+      put(&vs[buf][row * LDV], vd[0]);
+    } else {
+      store_tile(buf, kd, vd);
+    }
+  };
 
   f32x16 oacc[NDT];
 #pragma unroll
@@ -923,8 +1031,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
 
   // tile t computes from LDS buffer t % 2 while tile t + 1 waits in registers
   // and tile t + 2 is in flight: two register sets (A: even tiles, B: odd)
-  uint4 kA[NLD], vA[NLD], kB[NLD], vB[NLD];
-  load_tile(tile0, kA, vA);
+  Reg kA[NREG], vA[NREG], kB[NREG], vB[NREG];
+  load(tile0, kA, vA);
   // (a row's first piece works out where it ends only now, with the first tile's
   // loads in flight: no piece is shorter than that)
   if constexpr (SPLIT) {
@@ -936,9 +1044,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   const int ntiles = (int)((kend + BN - 1) / BN);
   stage_q();  // (waits for the query loads with tile 0's loads in flight)
   if constexpr (FORM == kScored) score_consts();
-  store_tile(0, kA, vA);
-  load_tile(tile0 + 1, kB, vB);
-  load_tile(tile0 + 2, kA, vA);
+  store(0, kA, vA);
+  load(tile0 + 1, kB, vB);
+  load(tile0 + 2, kA, vA);
   __syncthreads();
   // (packed rows: the next tiles' stores and loads go out between the score
   // MFMAs and the softmax; paged rows: after the tile, since their loads
@@ -946,24 +1054,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   for (int t = tile0; t < ntiles; t += 2) {
     if constexpr (PG == 0) {
       compute(t, 0, [&]() __attribute__((always_inline)) {
-        store_tile(1, kB, vB);
-        load_tile(t + 3, kB, vB);
+        store(1, kB, vB);
+        load(t + 3, kB, vB);
       });
       __syncthreads();
       compute(t + 1, 1, [&]() __attribute__((always_inline)) {
-        store_tile(0, kA, vA);
-        load_tile(t + 4, kA, vA);
+        store(0, kA, vA);
+        load(t + 4, kA, vA);
       });
       __syncthreads();
     } else {
       const auto after = []() {};  // (one instantiation of compute for both calls)
       compute(t, 0, after);
-      store_tile(1, kB, vB);
-      load_tile(t + 3, kB, vB);
+      store(1, kB, vB);
+      load(t + 3, kB, vB);
       __syncthreads();
       compute(t + 1, 1, after);
-      store_tile(0, kA, vA);
-      load_tile(t + 4, kA, vA);
+      store(0, kA, vA);
+      load(t + 4, kA, vA);
       __syncthreads();
     }
   }

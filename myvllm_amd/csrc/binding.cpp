@@ -30,6 +30,7 @@ int32_t dtype_code(at::ScalarType t) {
     case at::kHalf: return GDN_DTYPE_F16;
     case at::kInt: return GDN_DTYPE_I32;
     case at::kLong: return GDN_DTYPE_I64;
+    case at::kByte: return GDN_DTYPE_U8;
     default: return -1;
   }
 }
@@ -193,6 +194,11 @@ typedef Entry<20, 7, int64_t, float, float, int32_t> AttnVarlenScored;
 typedef Entry<21, 10, int64_t, float, float> PagedPrefillScored;
 typedef Entry<22, 8, int32_t, float, float> PagedDecodeScored;
 typedef Entry<23, 9, float> PagedDecodeShared;
+typedef Entry<24, 14, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t> KvAppendEx;
+typedef Entry<25, 9> KvRead;
+typedef Entry<26, 9, int32_t, float> PagedDecodeFp4;
+typedef Entry<27, 10, int64_t, float> PagedPrefillFp4;
+typedef Entry<28, 5> CacheCopy;
 typedef Size<0, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> ChunkPrefillSize;
 typedef Size<1, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> PagedPrefillSize;
 typedef Size<2, int64_t, int64_t, int64_t, int32_t> PagedDecodeSize;
@@ -229,6 +235,11 @@ const Bound kBound[] = {
     GDN_BOUND("paged_attention_prefill_scored", PagedPrefillScored),
     GDN_BOUND("paged_attention_decode_scored", PagedDecodeScored),
     GDN_BOUND("paged_attention_decode_shared", PagedDecodeShared),
+    GDN_BOUND("paged_kv_append_ex", KvAppendEx),
+    GDN_BOUND("paged_kv_read", KvRead),
+    GDN_BOUND("paged_attention_decode_fp4", PagedDecodeFp4),
+    GDN_BOUND("paged_attention_prefill_fp4", PagedPrefillFp4),
+    GDN_BOUND("cache_copy", CacheCopy),
     GDN_BOUND("paged_attention_decode_shared_workspace_size", PagedDecodeSharedSize),
     GDN_BOUND("gdn_chunk_prefill_workspace_size", ChunkPrefillSize),
     GDN_BOUND("paged_attention_prefill_workspace_size", PagedPrefillSize),

@@ -8,7 +8,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <stdint.h>
+#include <vector>
 
 #include "../../include/gdn_hip.h"
 
@@ -76,8 +78,23 @@ hipError_t attn_decode_shared_launch(const gdn_tensor* q, const gdn_tensor* kc, 
 int64_t paged_kv_append_waves(int64_t T, int64_t rows, int64_t D);
 hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* kc, gdn_tensor* vc,
                                   const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* q, gdn_tensor* out,
-                                  const gdn_tensor* cu, const gdn_tensor* cos, const gdn_tensor* sin, int interleaved,
+                                  const gdn_tensor* cu, const gdn_tensor* cos, const gdn_tensor* sin,
+                                  const gdn_tensor* pos, gdn_tensor* ks, gdn_tensor* vs, int interleaved,
+                                  const int32_t* sections, bool dealt, hipStream_t st);
+hipError_t paged_kv_read_launch(const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* tab,
+                                const gdn_tensor* ctx, gdn_tensor* k, gdn_tensor* v, const gdn_tensor* cu,
+                                const gdn_tensor* ks, const gdn_tensor* vs, hipStream_t st);
+hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                  const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
+                                  const gdn_tensor* ctx, gdn_tensor* out, float* workspace, int32_t splits, float scale,
                                   hipStream_t st);
+hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                   const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
+                                   const gdn_tensor* ctx, const gdn_tensor* cu, gdn_tensor* out, float* workspace,
+                                   int64_t max_seqlen, float scale, hipStream_t st);
+bool cache_copy_fits(gdn_tensor* const* t, const int64_t* es, int n, int64_t vec);
+hipError_t cache_copy_launch(gdn_tensor* const* t, const int64_t* es, int n, const int32_t* src, const int32_t* dst,
+                             int64_t count, int64_t vec, hipStream_t st);
 hipError_t hbm_stream_copy_launch(const void* src, void* dst, int64_t nbytes, int32_t blocks, hipStream_t st);
 
 #define GDN_EXPORT extern "C" __attribute__((visibility("default")))
@@ -97,6 +114,7 @@ int elem_size(int dt) {
     case GDN_DTYPE_F32: case GDN_DTYPE_I32: return 4;
     case GDN_DTYPE_BF16: case GDN_DTYPE_F16: return 2;
     case GDN_DTYPE_I64: return 8;
+    case GDN_DTYPE_U8: return 1;
     default: return 0;
   }
 }
@@ -302,15 +320,18 @@ constexpr int32_t kMaxDecodeSplits = 256;
 
 // q / out (rows, Hq, D) with the kv tensors' head count and head dim: bf16 or
 // fp16 throughout, D = 64, 128 or 256, unit inner strides, 16-byte rows.
+// (codes: of caches held in 4 bits, two numbers a byte)
 int check_attn_qo(const gdn_tensor* q, const gdn_tensor* out, const gdn_tensor* kv0, const gdn_tensor* kv1,
-                  int64_t Hkv, bool any_dim = false) {
+                  int64_t Hkv, bool any_dim = false, bool codes = false) {
   const int64_t rows = q->shape[0], Hq = q->shape[1], D = q->shape[2];
   if (out->shape[0] != rows || out->shape[1] != Hq || out->shape[2] != D) return GDN_ERR_SHAPE;
   const int kd = kv0->ndim - 1;
-  if (kv0->shape[kd] != D || kv1->shape[kd] != D) return GDN_ERR_SHAPE;
+  const int64_t per = codes ? 2 : 1;
+  const int32_t kv_dtype = codes ? GDN_DTYPE_U8 : q->dtype;
+  if (kv0->shape[kd] * per != D || kv1->shape[kd] * per != D) return GDN_ERR_SHAPE;
   if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0) return GDN_ERR_HEADS;
   if (q->dtype != GDN_DTYPE_BF16 && q->dtype != GDN_DTYPE_F16) return GDN_ERR_DTYPE;
-  if (kv0->dtype != q->dtype || kv1->dtype != q->dtype || out->dtype != q->dtype) return GDN_ERR_DTYPE;
+  if (kv0->dtype != kv_dtype || kv1->dtype != kv_dtype || out->dtype != q->dtype) return GDN_ERR_DTYPE;
   if (any_dim ? (D <= 0 || D > 256 || D % 8 != 0) : (D != 64 && D != 128 && D != 256)) return GDN_ERR_HEAD_DIM;
   if (q->stride[2] != 1 || out->stride[2] != 1 || kv0->stride[kd] != 1 || kv1->stride[kd] != 1)
     return GDN_ERR_STRIDE;
@@ -332,6 +353,36 @@ int check_paged(const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* ta
   if (kc->shape[1] <= 0 || kc->shape[1] > INT32_MAX) return GDN_ERR_SHAPE;
   if (!is_index(tab->dtype) || !is_index(ctx->dtype)) return GDN_ERR_DTYPE;
   if (tab->stride[1] != 1 || ctx->stride[0] != 1) return GDN_ERR_STRIDE;
+  return GDN_OK;
+}
+
+// The block scales (blocks, Hkv, D / 32, page) of caches held in 4 bits, and what
+// the kernels assume of those: whole 16-key groups per page, unit inner strides,
+// rows of codes 16-byte aligned, scales of four slots 4-byte aligned, a block of
+// either below 2^32 bytes away from the next, a page of one kv head below 2^31.
+int check_scales(const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* ks, const gdn_tensor* vs,
+                 const gdn_tensor* tab) {
+  GDN_TRY(check_desc(ks, 4));
+  GDN_TRY(check_desc(vs, 4));
+  if (kc->dtype != GDN_DTYPE_U8 || vc->dtype != GDN_DTYPE_U8 || ks->dtype != GDN_DTYPE_U8 || vs->dtype != GDN_DTYPE_U8)
+    return GDN_ERR_DTYPE;
+  for (const gdn_tensor* t : {ks, vs})
+    if (t->shape[0] != kc->shape[0] || t->shape[1] != kc->shape[2] || t->shape[2] * 16 != kc->shape[3] ||
+        t->shape[3] != kc->shape[1])
+      return GDN_ERR_SHAPE;
+  if (kc->shape[1] % 16 != 0) return GDN_ERR_SHAPE;
+  constexpr int64_t k31 = int64_t(1) << 31, k32 = int64_t(1) << 32;
+  for (const gdn_tensor* t : {kc, vc, ks, vs}) {
+    const bool scales = t == ks || t == vs;
+    if (t->stride[3] != 1) return GDN_ERR_STRIDE;
+    for (int i = 0; i < 3; ++i)
+      if (t->stride[i] < 0) return GDN_ERR_STRIDE;
+    if (numel(t) > 0 && !vec_ok(t, scales ? 4 : 16)) return GDN_ERR_ALIGN;
+    if (t->stride[0] >= k32 || t->stride[1] >= k31 || t->stride[2] >= k31) return GDN_ERR_RANGE;
+    const int64_t span = scales ? t->shape[2] * t->stride[2] + t->shape[3] : t->shape[1] * t->stride[1] + t->shape[3];
+    if (span >= k31) return GDN_ERR_RANGE;
+  }
+  if (kc->shape[0] >= k31 || tab->shape[1] >= k31 || tab->shape[1] * kc->shape[1] >= k31) return GDN_ERR_RANGE;
   return GDN_OK;
 }
 
@@ -642,14 +693,15 @@ namespace {
 // Checks of the paged prefill; *ws: its workspace, null where its rows are not split.
 int check_paged_prefill(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                         const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens,
-                        const gdn_tensor* out, const gdn_tensor* workspace, int64_t max_seqlen, float** ws) {
+                        const gdn_tensor* out, const gdn_tensor* workspace, int64_t max_seqlen, float** ws,
+                        bool codes = false) {
   GDN_TRY(check_desc(q, 3));
   GDN_TRY(check_desc(out, 3));
   GDN_TRY(check_desc(cu_seqlens, 1));
   if (cu_seqlens->shape[0] < 1 || max_seqlen < 0) return GDN_ERR_SHAPE;
   const int64_t N = cu_seqlens->shape[0] - 1;
   GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, N));
-  GDN_TRY(check_attn_qo(q, out, k_cache, v_cache, k_cache->shape[2]));
+  GDN_TRY(check_attn_qo(q, out, k_cache, v_cache, k_cache->shape[2], false, codes));
   if (!is_index(cu_seqlens->dtype)) return GDN_ERR_DTYPE;
   if (cu_seqlens->stride[0] != 1) return GDN_ERR_STRIDE;
   const int64_t R = q->shape[1] / k_cache->shape[2];
@@ -726,12 +778,12 @@ namespace {
 // Checks shared by the two paged decode entries (everything but the workspace).
 int check_paged_decode(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                        const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* out,
-                       int32_t num_splits) {
+                       int32_t num_splits, bool codes = false) {
   GDN_TRY(check_desc(q, 3));
   GDN_TRY(check_desc(out, 3));
   const int64_t B = q->shape[0];
   GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, B));
-  GDN_TRY(check_attn_qo(q, out, k_cache, v_cache, k_cache->shape[2]));
+  GDN_TRY(check_attn_qo(q, out, k_cache, v_cache, k_cache->shape[2], false, codes));
   if (num_splits < 1 || num_splits > kMaxDecodeSplits) return GDN_ERR_RANGE;
   const int64_t Hkv = k_cache->shape[2], R = q->shape[1] / Hkv;
   if (B > kMaxGridYZ || Hkv * ((R + 15) / 16) > kMaxGridYZ) return GDN_ERR_RANGE;
@@ -873,26 +925,48 @@ GDN_EXPORT int paged_attention_decode_shared(const gdn_tensor* q, const gdn_tens
                                              out, ws, scale, reinterpret_cast<hipStream_t>(stream)));
 }
 
-GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
-                               const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
-                               gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos,
-                               const gdn_tensor* sin, int32_t interleaved, void* stream) {
-  GDN_TRY(check_desc(k, 3));
-  GDN_TRY(check_desc(v, 3));
-  GDN_TRY(check_desc(block_tables, 2));
-  const int64_t T = k->shape[0], Hkv = k->shape[1], D = k->shape[2], N = block_tables->shape[0];
-  GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, N));
+namespace {
+// The offsets of a batch of N sequences, or (null) one token each.
+int check_offsets(const gdn_tensor* cu_seqlens, int64_t T, int64_t N) {
+  if (!cu_seqlens) return T == N ? GDN_OK : GDN_ERR_SHAPE;
+  GDN_TRY(check_desc(cu_seqlens, 1));
+  if (cu_seqlens->shape[0] != N + 1) return GDN_ERR_SHAPE;
+  if (!is_index(cu_seqlens->dtype)) return GDN_ERR_DTYPE;
+  return cu_seqlens->stride[0] == 1 ? GDN_OK : GDN_ERR_STRIDE;
+}
+
+// k, v (T, Hkv, D) beside caches of their type, or of codes.
+int check_kv_rows(const gdn_tensor* k, const gdn_tensor* v, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                  bool codes) {
+  const int64_t T = k->shape[0], Hkv = k->shape[1], D = k->shape[2];
   for (int i = 0; i < 3; ++i)
     if (v->shape[i] != k->shape[i]) return GDN_ERR_SHAPE;
-  if (k_cache->shape[2] != Hkv || k_cache->shape[3] != D) return GDN_ERR_SHAPE;
+  if (k_cache->shape[2] != Hkv || k_cache->shape[3] * (codes ? 2 : 1) != D) return GDN_ERR_SHAPE;
   if (Hkv <= 0) return GDN_ERR_HEADS;
   if (k->dtype != GDN_DTYPE_BF16 && k->dtype != GDN_DTYPE_F16) return GDN_ERR_DTYPE;
-  if (v->dtype != k->dtype || k_cache->dtype != k->dtype || v_cache->dtype != k->dtype) return GDN_ERR_DTYPE;
+  const int32_t kv_dtype = codes ? GDN_DTYPE_U8 : k->dtype;
+  if (v->dtype != k->dtype || k_cache->dtype != kv_dtype || v_cache->dtype != kv_dtype) return GDN_ERR_DTYPE;
   if (D != 64 && D != 128 && D != 256) return GDN_ERR_HEAD_DIM;
   if (k->stride[2] != 1 || v->stride[2] != 1 || k_cache->stride[3] != 1 || v_cache->stride[3] != 1)
     return GDN_ERR_STRIDE;
   if (T > 0 && (!vec_ok(k, 16) || !vec_ok(v, 16))) return GDN_ERR_ALIGN;
   if (numel(k_cache) > 0 && (!vec_ok(k_cache, 16) || !vec_ok(v_cache, 16))) return GDN_ERR_ALIGN;
+  return GDN_OK;
+}
+
+int kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+              const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q, gdn_tensor* out,
+              const gdn_tensor* cu_seqlens, const gdn_tensor* cos, const gdn_tensor* sin, const gdn_tensor* positions,
+              gdn_tensor* k_scales, gdn_tensor* v_scales, int32_t interleaved, const int32_t* sections, int32_t dealt,
+              void* stream) {
+  GDN_TRY(check_desc(k, 3));
+  GDN_TRY(check_desc(v, 3));
+  GDN_TRY(check_desc(block_tables, 2));
+  const int64_t T = k->shape[0], Hkv = k->shape[1], D = k->shape[2], N = block_tables->shape[0];
+  GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, N));
+  if (!k_scales != !v_scales) return GDN_ERR_NULL;
+  GDN_TRY(check_kv_rows(k, v, k_cache, v_cache, k_scales != nullptr));
+  if (k_scales) GDN_TRY(check_scales(k_cache, v_cache, k_scales, v_scales, block_tables));
   int64_t Hq = 0;
   if (!q != !out) return GDN_ERR_NULL;
   if (q) {
@@ -907,14 +981,7 @@ GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_ten
     if (q->stride[2] != 1 || out->stride[2] != 1) return GDN_ERR_STRIDE;
     if (T > 0 && (!vec_ok(q, 16) || !vec_ok(out, 16))) return GDN_ERR_ALIGN;
   }
-  if (cu_seqlens) {
-    GDN_TRY(check_desc(cu_seqlens, 1));
-    if (cu_seqlens->shape[0] != N + 1) return GDN_ERR_SHAPE;
-    if (!is_index(cu_seqlens->dtype)) return GDN_ERR_DTYPE;
-    if (cu_seqlens->stride[0] != 1) return GDN_ERR_STRIDE;
-  } else if (T != N) {
-    return GDN_ERR_SHAPE;
-  }
+  GDN_TRY(check_offsets(cu_seqlens, T, N));
   if (!cos != !sin) return GDN_ERR_NULL;
   if (cos) {
     GDN_TRY(check_desc(cos, 2));
@@ -926,11 +993,147 @@ GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_ten
     if (cos->stride[1] != 1 || sin->stride[1] != 1) return GDN_ERR_STRIDE;
     if (numel(cos) > 0 && (!vec_ok(cos, 16) || !vec_ok(sin, 16))) return GDN_ERR_ALIGN;
   }
+  if (positions) {
+    GDN_TRY(check_desc(positions, 2));
+    if (!cos) return GDN_ERR_NULL;
+    if (positions->shape[0] < 1 || positions->shape[0] > 4 || positions->shape[1] != T) return GDN_ERR_SHAPE;
+    if (!is_index(positions->dtype)) return GDN_ERR_DTYPE;
+    if (positions->stride[1] != 1) return GDN_ERR_STRIDE;
+    int64_t sum = 0;
+    for (int64_t i = 0; i < positions->shape[0]; ++i) {
+      if (sections[i] < 0) return GDN_ERR_ARG;
+      sum += sections[i];
+    }
+    if (sum != cos->shape[1]) return GDN_ERR_ARG;
+  }
   if (block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31)) return GDN_ERR_RANGE;
   if (Hq + 2 * Hkv > kMaxGrid / 2 || T > kMaxGrid / 2 || paged_kv_append_waves(T, Hq + 2 * Hkv, D) > kMaxGrid / 2)
     return GDN_ERR_RANGE;
   return launch_rc(paged_kv_append_launch(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos,
-                                          sin, interleaved, reinterpret_cast<hipStream_t>(stream)));
+                                          sin, positions, k_scales, v_scales, interleaved, sections, dealt != 0,
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+}  // namespace
+
+GDN_EXPORT int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+                               const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
+                               gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos,
+                               const gdn_tensor* sin, int32_t interleaved, void* stream) {
+  return kv_append(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin, nullptr, nullptr,
+                   nullptr, interleaved, nullptr, 0, stream);
+}
+
+GDN_EXPORT int paged_kv_append_ex(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cache, gdn_tensor* v_cache,
+                                  const gdn_tensor* block_tables, const gdn_tensor* context_lens, const gdn_tensor* q,
+                                  gdn_tensor* out, const gdn_tensor* cu_seqlens, const gdn_tensor* cos,
+                                  const gdn_tensor* sin, const gdn_tensor* positions, gdn_tensor* k_scales,
+                                  gdn_tensor* v_scales, int32_t interleaved, int32_t section0, int32_t section1,
+                                  int32_t section2, int32_t section3, int32_t dealt, void* stream) {
+  const int32_t sections[4] = {section0, section1, section2, section3};
+  return kv_append(k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin, positions,
+                   k_scales, v_scales, interleaved, sections, dealt, stream);
+}
+
+GDN_EXPORT int paged_kv_read(gdn_tensor* k, gdn_tensor* v, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                             const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                             const gdn_tensor* cu_seqlens, const gdn_tensor* k_scales, const gdn_tensor* v_scales,
+                             void* stream) {
+  GDN_TRY(check_desc(k, 3));
+  GDN_TRY(check_desc(v, 3));
+  GDN_TRY(check_desc(block_tables, 2));
+  const int64_t T = k->shape[0], Hkv = k->shape[1], D = k->shape[2], N = block_tables->shape[0];
+  GDN_TRY(check_paged(k_cache, v_cache, block_tables, context_lens, N));
+  if (!k_scales != !v_scales) return GDN_ERR_NULL;
+  GDN_TRY(check_kv_rows(k, v, k_cache, v_cache, k_scales != nullptr));
+  if (k_scales) GDN_TRY(check_scales(k_cache, v_cache, k_scales, v_scales, block_tables));
+  GDN_TRY(check_offsets(cu_seqlens, T, N));
+  if (block_tables->shape[1] * k_cache->shape[1] >= (int64_t(1) << 31)) return GDN_ERR_RANGE;
+  if (Hkv > kMaxGrid / 4 || T > kMaxGrid / 4 / Hkv || D <= 0) return GDN_ERR_RANGE;  // (2 T Hkv rows below 2^30)
+  return launch_rc(paged_kv_read_launch(k_cache, v_cache, block_tables, context_lens, k, v, cu_seqlens, k_scales,
+                                        v_scales, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_attention_decode_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                          const gdn_tensor* k_scales, const gdn_tensor* v_scales,
+                                          const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                          gdn_tensor* out, gdn_tensor* workspace, int32_t num_splits, float scale,
+                                          void* stream) {
+  GDN_TRY(check_paged_decode(q, k_cache, v_cache, block_tables, context_lens, out, num_splits, true));
+  GDN_TRY(check_scales(k_cache, v_cache, k_scales, v_scales, block_tables));
+  float* ws;
+  GDN_TRY(decode_workspace(workspace, paged_attention_decode_workspace_size(q->shape[0], q->shape[1], q->shape[2],
+                                                                            num_splits),
+                           num_splits, q->shape[0], &ws));
+  return launch_rc(attn_decode_fp4_launch(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, out, ws,
+                                          num_splits, scale, reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                           const gdn_tensor* k_scales, const gdn_tensor* v_scales,
+                                           const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                           const gdn_tensor* cu_seqlens, gdn_tensor* out, gdn_tensor* workspace,
+                                           int64_t max_seqlen, float scale, void* stream) {
+  float* ws;
+  GDN_TRY(check_paged_prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, workspace, max_seqlen,
+                              &ws, true));
+  GDN_TRY(check_scales(k_cache, v_cache, k_scales, v_scales, block_tables));
+  // (the kernel reads the first column of every sequence)
+  if (block_tables->shape[0] > 0 && block_tables->shape[1] == 0) return GDN_ERR_SHAPE;
+  return launch_rc(attn_prefill_fp4_launch(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens,
+                                           cu_seqlens, out, ws, max_seqlen, scale,
+                                           reinterpret_cast<hipStream_t>(stream)));
+}
+
+namespace {
+// Pairs of block ids: all inside the caches, the places distinct and none of them a source.
+int check_pairs(const int32_t* src, const int32_t* dst, int64_t n, int64_t blocks) {
+  for (int64_t i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= blocks || dst[i] < 0 || dst[i] >= blocks) return GDN_ERR_RANGE;
+  if (n <= 32) {
+    for (int64_t i = 0; i < n; ++i)
+      for (int64_t j = 0; j < n; ++j)
+        if (dst[i] == src[j] || (i != j && dst[i] == dst[j])) return GDN_ERR_ARG;
+    return GDN_OK;
+  }
+  try {
+    std::vector<bool> place((size_t)blocks);
+    for (int64_t i = 0; i < n; ++i) {
+      if (place[(size_t)dst[i]]) return GDN_ERR_ARG;
+      place[(size_t)dst[i]] = true;
+    }
+    for (int64_t i = 0; i < n; ++i)
+      if (place[(size_t)src[i]]) return GDN_ERR_ARG;
+  } catch (const std::bad_alloc&) {
+    return (int)hipErrorOutOfMemory;
+  }
+  return GDN_OK;
+}
+}  // namespace
+
+GDN_EXPORT int cache_copy(gdn_tensor* cache0, gdn_tensor* cache1, gdn_tensor* cache2, gdn_tensor* cache3,
+                          const gdn_tensor* pairs, void* stream) {
+  GDN_TRY(check_desc(pairs, 2));
+  if (pairs->shape[0] != 2) return GDN_ERR_SHAPE;
+  if (pairs->dtype != GDN_DTYPE_I32) return GDN_ERR_DTYPE;
+  if (pairs->stride[1] != 1) return GDN_ERR_STRIDE;
+  gdn_tensor* t[4];
+  int64_t es[4], vec = 16;
+  int n = 0;
+  for (gdn_tensor* c : {cache0, cache1, cache2, cache3}) {
+    if (!c) continue;
+    GDN_TRY(check_desc(c, 3));
+    if (n > 0 && c->shape[1] != t[0]->shape[1]) return GDN_ERR_SHAPE;
+    if (c->stride[2] != 1 || c->stride[0] < 0 || c->stride[1] < 0) return GDN_ERR_STRIDE;
+    es[n] = elem_size(c->dtype);
+    if (!vec_ok(c, 16) || c->shape[2] * es[n] % 16 != 0) vec = 1;
+    t[n++] = c;
+  }
+  if (n == 0) return GDN_ERR_NULL;
+  if (!cache_copy_fits(t, es, n, vec)) return GDN_ERR_RANGE;
+  const int32_t* src = reinterpret_cast<const int32_t*>(pairs->data);
+  const int32_t* dst = src + pairs->stride[0];
+  GDN_TRY(check_pairs(src, dst, pairs->shape[1], t[0]->shape[1]));
+  return launch_rc(cache_copy_launch(t, es, n, src, dst, pairs->shape[1], vec, reinterpret_cast<hipStream_t>(stream)));
 }
 
 GDN_EXPORT int gdn_hbm_copy(const void* src, void* dst, int64_t nbytes, int32_t blocks, void* stream) {

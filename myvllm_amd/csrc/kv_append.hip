@@ -18,7 +18,19 @@
 // 1, 2, 3, 5, 6 rows per lane 134, 138, 135, 141, 142.  Plain stores:
 // non-temporal ones take 125 us, but the attention that reads the rows next
 // takes 17 us longer.
-#include "gdn_common.h"
+//
+// AXES: the rotation's positions are the caller's, one per token and axis (time,
+// height and width of an image's patches), and every frequency turns by the
+// position of its own axis: c[j] = cos[p[axis(j)]][j].  The axes of all
+// frequencies are two bits each in the arguments; a lane reads the rows of the
+// axes that its eight frequencies have.
+// FP4: the caches hold codes and block scales (fp4.h) of the rows that the
+// 16-bit cache would hold.  A block's 32 numbers lie in two to four lanes,
+// wherever the rotation's pairs put them, so its largest magnitude is taken by an
+// LDS maximum of the wave.  Keys are rotated in 64 bits there (products of a
+// 16-bit and a 32-bit number are exact in them): next to a border between two
+// codes the last bit of a fp32 sum would choose another one now and then.
+#include "fp4.h"
 
 namespace {
 
@@ -35,7 +47,18 @@ struct AppendArgs {
   int64_t T, nseq, tab_st, cols, num_blocks, limit;  // limit: positions that have a place and an angle
   int32_t page, Hq, Hkv, rot, chunks;                // chunks: waves per token
   bool tab64, ctx64, cu64, interleaved;
+  // AXES: positions (axes, T), their rows of cos and sin, and the axis of each
+  // frequency, eight frequencies a 16-bit half
+  const void* pos;
+  int64_t pos_st, rows;
+  uint32_t axes[8];
+  int32_t naxes;
+  bool pos64;
+  // FP4: the caches' strides are in bytes
+  ScaleSource ks, vs;
 };
+
+constexpr int kMaxAxes = 4;
 
 // The sequence that holds token t, or -1: the last n with cu[n] <= t, by a
 // 64-ary search (one probe per lane and round), if t < cu[n + 1].
@@ -52,7 +75,30 @@ GDN_DEVICE int64_t find_seq(const AppendArgs& a, int64_t t, int lane) {
   return lo < a.nseq ? lo : -1;
 }
 
-template <typename T, int D>
+// The pairs of a lane turned in R's precision, rounded once to T.
+template <typename R, typename T, typename V8>
+GDN_DEVICE void turn(V8& x, V8& y, const float* c, const float* s, bool interleaved) {
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const R a0 = (R)(float)x[2 * j], b0 = (R)(float)x[2 * j + 1];
+      const R a1 = (R)(float)y[2 * j], b1 = (R)(float)y[2 * j + 1];
+      x[2 * j] = (T)(float)(a0 * (R)c[j] - b0 * (R)s[j]);
+      x[2 * j + 1] = (T)(float)(b0 * (R)c[j] + a0 * (R)s[j]);
+      y[2 * j] = (T)(float)(a1 * (R)c[j + 4] - b1 * (R)s[j + 4]);
+      y[2 * j + 1] = (T)(float)(b1 * (R)c[j + 4] + a1 * (R)s[j + 4]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const R p = (R)(float)x[j], q = (R)(float)y[j];
+      x[j] = (T)(float)(p * (R)c[j] - q * (R)s[j]);
+      y[j] = (T)(float)(q * (R)c[j] + p * (R)s[j]);
+    }
+  }
+}
+
+template <typename T, int D, bool AXES = false, bool FP4 = false>
 __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a) {
   typedef T v8 __attribute__((ext_vector_type(8)));
   constexpr int U = D / 16;    // lanes per row
@@ -89,7 +135,15 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
   } else {
     pos = load_index(a.ctx, n, a.ctx64) - 1;
   }
-  const bool placed = pos >= 0 && pos < a.limit;
+  bool placed = pos >= 0 && pos < a.limit;
+  int64_t turns_by[AXES ? kMaxAxes : 1];
+  if constexpr (AXES) {
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x) {
+      turns_by[x] = x < a.naxes ? load_index(a.pos, x * a.pos_st + t, a.pos64) : 0;
+      placed = placed && turns_by[x] >= 0 && turns_by[x] < a.rows;
+    }
+  }
   int64_t block = -1;
   int32_t slot = 0;
   if (placed) {
@@ -99,37 +153,68 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
     if (block >= a.num_blocks) block = -1;
   }
   float c[8], s[8];
-  if (turns && placed) {
+  if (!AXES && turns && placed) {
     Vec8<float>::load(a.cos + pos * a.cos_st + 8 * u, c);
     Vec8<float>::load(a.sin + pos * a.sin_st + 8 * u, s);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
   }
+  if constexpr (AXES) {
+    if (turns && placed) {
+      uint32_t of = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) of = u >> 1 == i ? a.axes[i] : of;
+      of = u & 1 ? of >> 16 : of & 0xFFFFu;
+#pragma unroll
+      for (int x = 0; x < kMaxAxes; ++x) {
+        // (bit 2 j: frequency j has axis x)
+        const uint32_t same = ~(of ^ (0x5555u * (uint32_t)x)), mine = same & (same >> 1) & 0x5555u;
+        if (x >= a.naxes || mine == 0) continue;
+        float cx[8], sx[8];
+        Vec8<float>::load(a.cos + turns_by[x] * a.cos_st + 8 * u, cx);
+        Vec8<float>::load(a.sin + turns_by[x] * a.sin_st + 8 * u, sx);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          c[j] = mine >> (2 * j) & 1u ? cx[j] : c[j];
+          s[j] = mine >> (2 * j) & 1u ? sx[j] : s[j];
+        }
+      }
+    }
+  }
 
+  // (FP4: a largest magnitude per row in flight and block)
+  __shared__ uint32_t tops[FP4 ? 4 * kAppendRows * 32 : 1];
 #pragma unroll
   for (int i = 0; i < kAppendRows; ++i) {
     const int r = r0 + i * RPI;
     if (r >= nrows) continue;
     if (turns && r < nq + a.Hkv) {
-      if (a.interleaved) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a0 = (float)x[i][2 * j], b0 = (float)x[i][2 * j + 1];
-          const float a1 = (float)y[i][2 * j], b1 = (float)y[i][2 * j + 1];
-          x[i][2 * j] = (T)(a0 * c[j] - b0 * s[j]);
-          x[i][2 * j + 1] = (T)(b0 * c[j] + a0 * s[j]);
-          y[i][2 * j] = (T)(a1 * c[j + 4] - b1 * s[j + 4]);
-          y[i][2 * j + 1] = (T)(b1 * c[j + 4] + a1 * s[j + 4]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float p = (float)x[i][j], q = (float)y[i][j];
-          x[i][j] = (T)(p * c[j] - q * s[j]);
-          y[i][j] = (T)(q * c[j] + p * s[j]);
-        }
-      }
+      if (FP4 && r >= nq) turn<double, T>(x[i], y[i], c, s, a.interleaved);
+      else turn<float, T>(x[i], y[i], c, s, a.interleaved);
+    }
+    if (FP4 && r >= nq) {
+      uint32_t* const top = tops + (w * kAppendRows + i) * 32 + lane / U * (D / 32);
+      top[e0 / 32] = 0u;  // (LDS operations of a wave complete in order; both are written by every lane of a row)
+      top[e1 / 32] = 0u;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __hip_atomic_fetch_max(top + e0 / 32, top_of_eight(x[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+      __hip_atomic_fetch_max(top + e1 / 32, top_of_eight(y[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (block < 0) continue;
+      const uint32_t s0 = fp4_scale_byte<T>(top[e0 / 32]), s1 = fp4_scale_byte<T>(top[e1 / 32]);
+      const bool key = r < nq + a.Hkv;
+      const int h = r - nq - (key ? 0 : a.Hkv);
+      uint8_t* const p = reinterpret_cast<uint8_t*>(key ? a.kc : a.vc) + block * (key ? a.kc_sb : a.vc_sb) +
+                         slot * (key ? a.kc_st : a.vc_st) + h * (key ? a.kc_sh : a.vc_sh);
+      const uint32_t w0 = fp4_codes<T>(x[i], s0), w1 = fp4_codes<T>(y[i], s1);
+      *reinterpret_cast<uint32_t*>(p + e0 / 2) = w0;
+      *reinterpret_cast<uint32_t*>(p + e1 / 2) = w1;
+      const ScaleSource& sc = key ? a.ks : a.vs;
+      uint8_t* const q = sc.base + block * sc.sb + h * sc.sh + slot;
+      if (e0 % 32 == 0) q[e0 / 32 * sc.sd] = (uint8_t)s0;
+      if (e1 % 32 == 0) q[e1 / 32 * sc.sd] = (uint8_t)s1;
+      continue;
     }
     T* p;
     if (r < nq) {
@@ -146,16 +231,145 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
   }
 }
 
-template <typename T>
-hipError_t launch_append(const AppendArgs& a, int D, hipStream_t st) {
-  const dim3 grid((unsigned)((a.T * a.chunks + 3) / 4));
-  if (D == 64)
-    paged_kv_append_kernel<T, 64><<<grid, dim3(256), 0, st>>>(a);
-  else if (D == 128)
-    paged_kv_append_kernel<T, 128><<<grid, dim3(256), 0, st>>>(a);
-  else
-    paged_kv_append_kernel<T, 256><<<grid, dim3(256), 0, st>>>(a);
+// Keys and values of tokens read back from the caches, as the append found
+// their places: one wave per kReadRows x (1024 / D) rows, k and v heads of a
+// token in turn, a lane 16 dims of a row.  Rows without a place are zero, and
+// so are those of a table entry outside [0, num_blocks).
+struct ReadArgs {
+  AppendArgs in;  // caches, tables, lengths; T, nseq, Hkv
+  void *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+};
+
+constexpr int kReadRows = 4;
+
+template <typename T, int D, bool FP4>
+__global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
+  const AppendArgs& a = g.in;
+  constexpr int U = D / 16, RPI = 64 / U;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t first = (blockIdx.x * 4 + w) * (kReadRows * RPI), per = 2 * (uint32_t)a.Hkv;  // (rows below 2^31)
+  const uint32_t t0 = first / per;
+  if (t0 >= a.T) return;
+  // the sequence of the wave's first token; a lane whose token is past its end goes on
+  int64_t n0 = t0;
+  if (a.cu) n0 = find_seq(a, t0, lane);
+  const int u = lane % U;
+  uint4 x[kReadRows], y[kReadRows];
+  uint32_t sc[kReadRows];
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    const uint32_t row = first + i * RPI + lane / U, t = row / per, h2 = row - t * per;
+    const bool key = h2 < (uint32_t)a.Hkv;
+    const int64_t h = key ? h2 : h2 - a.Hkv;
+    x[i] = y[i] = uint4{0, 0, 0, 0};
+    sc[i] = 0;
+    if (t >= a.T) continue;
+    int64_t n = n0, pos = -1;
+    if (a.cu) {
+      if (n < 0) n = 0;
+      while (n < a.nseq - 1 && load_index(a.cu, n + 1, a.cu64) <= t) ++n;
+      int64_t s, e;
+      seq_range(a.cu, a.cu64, n, a.T, s, e);
+      if (t >= s && t < e) pos = load_index(a.ctx, n, a.ctx64) - e + t;
+    } else {
+      n = t;
+      pos = load_index(a.ctx, n, a.ctx64) - 1;
+    }
+    if (pos < 0 || pos >= a.limit) continue;
+    const int64_t col = (uint32_t)pos / (uint32_t)a.page, slot = pos - col * a.page;
+    const int64_t block = load_index(a.tab, n * a.tab_st + col, a.tab64);
+    if (block < 0 || block >= a.num_blocks) continue;
+    const char* p = key ? reinterpret_cast<const char*>(a.kc) + block * a.kc_sb + slot * a.kc_st + h * a.kc_sh
+                        : reinterpret_cast<const char*>(a.vc) + block * a.vc_sb + slot * a.vc_st + h * a.vc_sh;
+    if constexpr (FP4) {
+      const uint2 c = *reinterpret_cast<const uint2*>(p + 8 * u);
+      x[i].x = c.x;
+      x[i].y = c.y;
+      const ScaleSource& ss = key ? a.ks : a.vs;
+      sc[i] = ss.base[block * ss.sb + h * ss.sh + (u / 2) * ss.sd + slot];
+    } else {
+      x[i] = *reinterpret_cast<const uint4*>(p + 32 * u);
+      y[i] = *reinterpret_cast<const uint4*>(p + 32 * u + 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    const uint32_t row = first + i * RPI + lane / U, t = row / per, h2 = row - t * per;
+    if (t >= a.T) continue;
+    const bool key = h2 < (uint32_t)a.Hkv;
+    const int64_t h = key ? h2 : h2 - a.Hkv;
+    T* p = key ? reinterpret_cast<T*>(g.k) + t * g.k_st + h * g.k_sh : reinterpret_cast<T*>(g.v) + t * g.v_st + h * g.v_sh;
+    if constexpr (FP4) {
+      const float s = fp4_scale(sc[i]);
+      y[i] = fp4_eight<T>(x[i].y, s);
+      x[i] = fp4_eight<T>(x[i].x, s);
+    }
+    *reinterpret_cast<uint4*>(p + 16 * u) = x[i];
+    *reinterpret_cast<uint4*>(p + 16 * u + 8) = y[i];
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_append(const AppendArgs& a, bool fp4, hipStream_t st) {
+  const dim3 grid((unsigned)((a.T * a.chunks + 3) / 4)), block(256);
+  if (fp4) {
+    if (a.pos) paged_kv_append_kernel<T, D, true, true><<<grid, block, 0, st>>>(a);
+    else paged_kv_append_kernel<T, D, false, true><<<grid, block, 0, st>>>(a);
+  } else {
+    if (a.pos) paged_kv_append_kernel<T, D, true, false><<<grid, block, 0, st>>>(a);
+    else paged_kv_append_kernel<T, D><<<grid, block, 0, st>>>(a);
+  }
   return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_append(const AppendArgs& a, int D, bool fp4, hipStream_t st) {
+  if (D == 64) return launch_append<T, 64>(a, fp4, st);
+  if (D == 128) return launch_append<T, 128>(a, fp4, st);
+  return launch_append<T, 256>(a, fp4, st);
+}
+
+template <typename T, int D>
+hipError_t launch_read(const ReadArgs& g, bool fp4, hipStream_t st) {
+  const int64_t rows = g.in.T * 2 * g.in.Hkv, per = kReadRows * (1024 / D) * 4;
+  const dim3 grid((unsigned)((rows + per - 1) / per)), block(256);
+  if (fp4) paged_kv_read_kernel<T, D, true><<<grid, block, 0, st>>>(g);
+  else paged_kv_read_kernel<T, D, false><<<grid, block, 0, st>>>(g);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_read(const ReadArgs& g, int D, bool fp4, hipStream_t st) {
+  if (D == 64) return launch_read<T, 64>(g, fp4, st);
+  if (D == 128) return launch_read<T, 128>(g, fp4, st);
+  return launch_read<T, 256>(g, fp4, st);
+}
+
+// Caches, tables and lengths of an append or a read; byte strides where `bytes`.
+void set_caches(AppendArgs& a, const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* tab, const gdn_tensor* ctx,
+                const gdn_tensor* cu, int64_t es) {
+  a.kc = kc->data;
+  a.kc_sb = kc->stride[0] * es;
+  a.kc_st = kc->stride[1] * es;
+  a.kc_sh = kc->stride[2] * es;
+  a.vc = vc->data;
+  a.vc_sb = vc->stride[0] * es;
+  a.vc_st = vc->stride[1] * es;
+  a.vc_sh = vc->stride[2] * es;
+  a.num_blocks = kc->shape[0];
+  a.page = (int32_t)kc->shape[1];
+  a.tab = tab->data;
+  a.tab_st = tab->stride[0];
+  a.tab64 = tab->dtype == GDN_DTYPE_I64;
+  a.cols = tab->shape[1];
+  a.limit = a.cols * a.page;
+  a.ctx = ctx->data;
+  a.ctx64 = ctx->dtype == GDN_DTYPE_I64;
+  a.nseq = tab->shape[0];
+  a.Hkv = (int32_t)kc->shape[2];
+  if (cu) {
+    a.cu = cu->data;
+    a.cu64 = cu->dtype == GDN_DTYPE_I64;
+  }
 }
 
 }  // namespace
@@ -165,10 +379,14 @@ int64_t paged_kv_append_waves(int64_t T, int64_t rows, int64_t D) {
   return T * ((rows + per - 1) / per);
 }
 
+// positions (axes, T) and the frequencies of each axis, section after section or
+// (dealt) given to the axes in turn while they have some left; k_scales and
+// v_scales: caches in 4 bits.
 hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* kc, gdn_tensor* vc,
                                   const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* q, gdn_tensor* out,
-                                  const gdn_tensor* cu, const gdn_tensor* cos, const gdn_tensor* sin, int interleaved,
-                                  hipStream_t st) {
+                                  const gdn_tensor* cu, const gdn_tensor* cos, const gdn_tensor* sin,
+                                  const gdn_tensor* pos, gdn_tensor* ks, gdn_tensor* vs, int interleaved,
+                                  const int32_t* sections, bool dealt, hipStream_t st) {
   if (k->shape[0] == 0) return hipSuccess;
   const int D = (int)k->shape[2];
   AppendArgs a{};
@@ -187,39 +405,59 @@ hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_
     a.o_sh = out->stride[1];
     a.Hq = (int32_t)q->shape[1];
   }
-  a.kc = kc->data;
-  a.kc_sb = kc->stride[0];
-  a.kc_st = kc->stride[1];
-  a.kc_sh = kc->stride[2];
-  a.vc = vc->data;
-  a.vc_sb = vc->stride[0];
-  a.vc_st = vc->stride[1];
-  a.vc_sh = vc->stride[2];
-  a.num_blocks = kc->shape[0];
-  a.page = (int32_t)kc->shape[1];
-  a.tab = tab->data;
-  a.tab_st = tab->stride[0];
-  a.tab64 = tab->dtype == GDN_DTYPE_I64;
-  a.cols = tab->shape[1];
-  a.limit = a.cols * a.page;
-  a.ctx = ctx->data;
-  a.ctx64 = ctx->dtype == GDN_DTYPE_I64;
+  set_caches(a, kc, vc, tab, ctx, cu, 1);  // (elements of 16 bits, or bytes of codes)
   a.T = k->shape[0];
-  a.nseq = tab->shape[0];
-  a.Hkv = (int32_t)k->shape[1];
-  if (cu) {
-    a.cu = cu->data;
-    a.cu64 = cu->dtype == GDN_DTYPE_I64;
-  }
   if (cos) {
     a.cos = reinterpret_cast<const float*>(cos->data);
     a.cos_st = cos->stride[0];
     a.sin = reinterpret_cast<const float*>(sin->data);
     a.sin_st = sin->stride[0];
     a.rot = (int32_t)cos->shape[1] * 2;
-    a.limit = cos->shape[0] < a.limit ? cos->shape[0] : a.limit;
+    if (!pos) a.limit = cos->shape[0] < a.limit ? cos->shape[0] : a.limit;
+  }
+  if (pos) {
+    a.pos = pos->data;
+    a.pos_st = pos->stride[0];
+    a.pos64 = pos->dtype == GDN_DTYPE_I64;
+    a.naxes = (int32_t)pos->shape[0];
+    a.rows = cos->shape[0];
+    int32_t left[kMaxAxes];
+    for (int x = 0; x < kMaxAxes; ++x) left[x] = x < a.naxes ? sections[x] : 0;
+    int x = 0;
+    for (int32_t j = 0; j < a.rot / 2; ++j) {  // (the sections' sum, checked by the entry)
+      while (left[x] == 0) x = (x + 1) % kMaxAxes;
+      a.axes[j / 16] |= (uint32_t)x << (2 * (j % 16));
+      --left[x];
+      if (dealt) x = (x + 1) % kMaxAxes;
+    }
+  }
+  if (ks) {
+    a.ks = scale_source(ks);
+    a.vs = scale_source(vs);
   }
   a.chunks = (int32_t)paged_kv_append_waves(1, a.Hq + 2 * a.Hkv, D);
   a.interleaved = interleaved != 0;
-  return k->dtype == GDN_DTYPE_BF16 ? launch_append<bf16_t>(a, D, st) : launch_append<f16_t>(a, D, st);
+  return k->dtype == GDN_DTYPE_BF16 ? launch_append<bf16_t>(a, D, ks != nullptr, st)
+                                    : launch_append<f16_t>(a, D, ks != nullptr, st);
+}
+
+hipError_t paged_kv_read_launch(const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* tab,
+                                const gdn_tensor* ctx, gdn_tensor* k, gdn_tensor* v, const gdn_tensor* cu,
+                                const gdn_tensor* ks, const gdn_tensor* vs, hipStream_t st) {
+  if (k->shape[0] == 0) return hipSuccess;
+  ReadArgs g{};
+  set_caches(g.in, kc, vc, tab, ctx, cu, ks ? 1 : 2);
+  g.in.T = k->shape[0];
+  g.k = k->data;
+  g.k_st = k->stride[0];
+  g.k_sh = k->stride[1];
+  g.v = v->data;
+  g.v_st = v->stride[0];
+  g.v_sh = v->stride[1];
+  if (ks) {
+    g.in.ks = scale_source(ks);
+    g.in.vs = scale_source(vs);
+  }
+  return k->dtype == GDN_DTYPE_BF16 ? launch_read<bf16_t>(g, (int)k->shape[2], ks != nullptr, st)
+                                    : launch_read<f16_t>(g, (int)k->shape[2], ks != nullptr, st);
 }

@@ -19,8 +19,14 @@ The three ops take other forms of scores as keywords (``softcap``,
 ``alibi_slopes``, ``prefix_lens``), and beside them stand the append that fills
 the caches (:func:`paged_kv_append`) and the decode of sequences that share
 their first keys (:func:`paged_flash_attention_decode_shared`).
+
+The append, the paged prefill and the decode also take caches held in 4 bits
+(``k_scales``, ``v_scales``, :func:`paged_kv_append`), a quarter of the memory and
+of the reads.
 """
 from __future__ import annotations
+
+from collections.abc import Sequence
 
 import torch
 
@@ -206,13 +212,19 @@ def paged_flash_attention_decode(
     out: torch.Tensor | None = None,
     softcap: float | None = None,
     alibi_slopes: torch.Tensor | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """One query per sequence over its paged cache: q (B, Hq, D), caches
     (num_blocks, block_size, Hkv, D), block_tables (B, max_blocks),
     context_lens (B,) -> (B, Hq, D).  No host sync.  ``softcap`` and
-    ``alibi_slopes`` as in :func:`flash_attention_prefill`."""
+    ``alibi_slopes`` as in :func:`flash_attention_prefill`; with ``k_scales`` and
+    ``v_scales`` the caches are held in 4 bits (:func:`paged_kv_append`), for plain
+    scores only."""
     if k_cache.shape[1] != block_size:
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
+    if _fp4(k_scales, v_scales, softcap, alibi_slopes):
+        return _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, scale, num_splits, out)
     dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens, alibi_slopes)
     B, Hq, Dh = q.shape
     if num_splits is None:
@@ -229,6 +241,59 @@ def paged_flash_attention_decode(
     else:
         _lib.call("paged_attention_decode", q, k_cache, v_cache, block_tables, context_lens, o, ws, int(num_splits),
                   float(scale))
+    return _finish(out, o)
+
+
+def _fp4(k_scales, v_scales, *forms) -> bool:
+    """Whether a call is over caches held in 4 bits."""
+    if k_scales is None and v_scales is None:
+        return False
+    if k_scales is None or v_scales is None:
+        raise ValueError("k_scales and v_scales come together")
+    if any(f is not None for f in forms):
+        raise ValueError("caches held in 4 bits take plain scores: no softcap, alibi_slopes or prefix_lens")
+    return True
+
+
+def _vec4(t: torch.Tensor) -> torch.Tensor:
+    """Block scales as the kernels read them, four slots at once."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 4 == 0 and all(t.stride(i) % 4 == 0 for i in range(t.dim() - 1))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int) -> int:
+    """:func:`decode_num_splits` of caches held in 4 bits, whose units are
+    workgroups of four waves on 256 / D kv heads (fewer where those do not
+    divide the heads)."""
+    heads = max(1, 256 // max(head_dim, 1))
+    while num_kv_heads % heads:
+        heads //= 2
+    groups = max(num_kv_heads, 1) // heads * ((num_q_heads // max(num_kv_heads, 1) + 15) // 16)
+    rows = max(1, num_seqs * groups)
+    if rows >= _FP4_SPLIT_ROWS:
+        return 1
+    units = max(1, round(_FP4_TARGET_WORKGROUPS / rows))
+    by_keys = -(-max(capacity, 1) // _FP4_MIN_SPLIT_KEYS)
+    return max(1, min(_DECODE_MAX_SPLITS, 1 + min(units, by_keys)))
+
+
+_FP4_TARGET_WORKGROUPS = 512
+_FP4_SPLIT_ROWS = 2048
+_FP4_MIN_SPLIT_KEYS = 256
+
+
+def _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, scale, num_splits, out):
+    dev = _lib.require_device(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens)
+    B, Hq, Dh = q.shape
+    if num_splits is None:
+        num_splits = fp4_decode_num_splits(B, Hq, k_cache.shape[2], Dh, block_tables.shape[1] * k_cache.shape[1])
+    ws = None
+    n_ws = _lib.workspace_size("paged_attention_decode_workspace_size", B, Hq, Dh, int(num_splits))
+    if n_ws > 0:
+        ws = torch.empty(n_ws, dtype=torch.float32, device=dev)
+    o = _out_for(out, (B, Hq, Dh), q.dtype, dev)
+    _lib.call("paged_attention_decode_fp4", _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache), _vec4(k_scales),
+              _vec4(v_scales), block_tables, context_lens, o, ws, int(num_splits), float(scale))
     return _finish(out, o)
 
 
@@ -333,6 +398,8 @@ def paged_flash_attention_prefill(
     softcap: float | None = None,
     alibi_slopes: torch.Tensor | None = None,
     prefix_lens: torch.Tensor | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Prefill over a paged cache that already holds the new keys: query i of
     sequence n sits at position ``context_lens[n] - len_n + i`` and attends
@@ -342,9 +409,14 @@ def paged_flash_attention_prefill(
     over a long cache are split over the keys as well; the partials then take a
     temporary workspace of up to 512 MiB, without which nothing is split.
     ``softcap``, ``alibi_slopes`` and ``prefix_lens`` as in
-    :func:`flash_attention_prefill`, positions and keys counted over the cache."""
+    :func:`flash_attention_prefill`, positions and keys counted over the cache;
+    with ``k_scales`` and ``v_scales`` the caches are held in 4 bits
+    (:func:`paged_kv_append`), for plain scores only."""
     if k_cache.shape[1] != page_block_size:
         raise ValueError(f"page_block_size {page_block_size} != k_cache.shape[1] {k_cache.shape[1]}")
+    if _fp4(k_scales, v_scales, softcap, alibi_slopes, prefix_lens):
+        return _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, page_block_tables, context_lens, cu_seqlens,
+                                  scale, max_seqlen, out)
     dev = _lib.require_device(q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens, alibi_slopes,
                               prefix_lens)
     if max_seqlen is None:
@@ -364,6 +436,19 @@ def paged_flash_attention_prefill(
     return _finish(out, o)
 
 
+def _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens, scale,
+                       max_seqlen, out):
+    dev = _lib.require_device(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens)
+    if max_seqlen is None:
+        max_seqlen = _max_seqlen(cu_seqlens)
+    q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
+    o = _out_for(out, q.shape, q.dtype, dev)
+    ws = _prefill_workspace(q, k_cache, v_cache, block_tables, cu_seqlens, k_cache.shape[1])
+    _lib.call("paged_attention_prefill_fp4", q, k_cache, v_cache, _vec4(k_scales), _vec4(v_scales), block_tables,
+              context_lens, cu_seqlens, o, ws, int(max_seqlen), float(scale))
+    return _finish(out, o)
+
+
 def paged_kv_append(
     q: torch.Tensor | None,
     k: torch.Tensor,
@@ -378,6 +463,11 @@ def paged_kv_append(
     cu_seqlens: torch.Tensor | None = None,
     interleaved: bool = False,
     out: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    sections: Sequence[int] | None = None,
+    sections_interleaved: bool = False,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
 ) -> torch.Tensor | None:
     """Puts the new tokens' k, v (T, Hkv, D) into the paged caches and rotates
     q and k on the way: the step before the paged attention ops, with their
@@ -395,12 +485,34 @@ def paged_kv_append(
     A token in no sequence or at a position without a table column or a row of
     the rotation is not appended and its row of q is zero; table entries
     outside ``[0, num_blocks)`` are not written.  No host sync.  The caches are
-    written where they lie, so their rows must be 16-byte aligned."""
+    written where they lie, so their rows must be 16-byte aligned.
+
+    ``positions`` gives the rotation positions of its own: (T,), or (axes, T) for
+    up to four axes (time, height and width of an image's patches), of which
+    ``sections`` gives each its number of frequencies, rot / 2 together, one section
+    after the other or, with ``sections_interleaved``, dealt to the axes in turn
+    while they have some left.  Frequency j of token t then turns by
+    ``cos[positions[axis(j), t], j]``.  The slots are ``context_lens``' as ever; a
+    position outside the tables leaves the token out.
+
+    ``k_scales`` and ``v_scales``, uint8 (num_blocks, Hkv, D / 32, block_size): the
+    caches are uint8 (num_blocks, block_size, Hkv, D / 2) and hold the rows in 4
+    bits.  Each 32 numbers share a scale 2^e (as the byte e + 127), e the smallest
+    with max|x| <= 6 * 2^e, held to -125..125 (bf16) or -13..13 (fp16); a
+    number is the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times the scale, signed.
+    Numbers next to an infinity or a NaN read as NaN.  ``block_size`` is a multiple
+    of 16 there."""
     if k_cache.shape[1] != block_size:
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     if q is None and out is not None:
         raise ValueError("out is the rotated q's: none without q")
-    tensors = (k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
+    extended = _fp4(k_scales, v_scales) or positions is not None
+    if extended:
+        positions, axes = _axes(positions, sections, cos)
+    elif sections is not None:
+        raise ValueError("sections are those of positions")
+    tensors = (k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin, positions, k_scales,
+               v_scales)
     if not _lib.same_device(*tensors):
         _lib.require_device(*tensors)
     if not _lib.vec16_all(q, k, v, cos, sin):
@@ -408,6 +520,72 @@ def paged_kv_append(
     # (rows aligned already are rotated where they lie when out is q)
     o = None if q is None else torch.empty_like(q) if out is None or _crosses(out, q, k, v) else \
         _out_for(out, q.shape, q.dtype, q.device)
-    _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
-              int(bool(interleaved)))
+    if extended:
+        _lib.call("paged_kv_append_ex", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
+                  positions, k_scales, v_scales, int(bool(interleaved)), *axes, int(bool(sections_interleaved)))
+    else:
+        _lib.call("paged_kv_append", k, v, k_cache, v_cache, block_tables, context_lens, q, o, cu_seqlens, cos, sin,
+                  int(bool(interleaved)))
     return o if out is None else _finish(out, o)
+
+
+def _axes(positions, sections, cos):
+    """positions as (axes, T) and the frequencies of four axes."""
+    if positions is None:
+        if sections is not None:
+            raise ValueError("sections are those of positions")
+        return None, (0, 0, 0, 0)
+    if cos is None:
+        raise ValueError("positions are the rotation's: none without cos and sin")
+    if positions.dim() == 1:
+        positions = positions[None]
+    if sections is None:
+        sections = (cos.shape[1],)
+    if positions.dim() != 2 or not 1 <= positions.shape[0] <= 4 or len(sections) != positions.shape[0]:
+        raise ValueError("positions are (T,) or (axes, T) with one to four axes and as many sections")
+    if sum(sections) != cos.shape[1] or min(sections) < 0:
+        raise ValueError(f"sections {tuple(sections)} are not the {cos.shape[1]} frequencies of cos and sin")
+    if positions.stride(1) != 1:
+        positions = positions.contiguous()
+    return positions, tuple(int(n) for n in sections) + (0,) * (4 - len(sections))
+
+
+def paged_kv_read(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_size: int,
+    num_tokens: int | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+    k_scales: torch.Tensor | None = None,
+    v_scales: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the sequences' last tokens, read back from the paged
+    caches as (T, Hkv, D): what :func:`paged_kv_append` with the same tables,
+    lengths and ``cu_seqlens`` put there (``cu_seqlens`` over the whole
+    contexts reads whole sequences; without it the last token of each).  For a
+    program that moves sequences elsewhere, or changes what a cache is held in.
+
+    ``num_tokens`` (T) is read from ``cu_seqlens`` when not given, one host sync.
+    ``dtype`` is that of caches held in 4 bits (``k_scales``, ``v_scales``): the type
+    that was appended, bf16 when not given.  Tokens without a place, and of table
+    entries outside ``[0, num_blocks)``, are zero rows."""
+    if k_cache.shape[1] != block_size:
+        raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
+    dev = _lib.require_device(k_cache, v_cache, block_tables, context_lens, cu_seqlens, k_scales, v_scales)
+    fp4 = _fp4(k_scales, v_scales)
+    if dtype is None:
+        dtype = torch.bfloat16 if fp4 else k_cache.dtype
+    elif not fp4 and dtype != k_cache.dtype:
+        raise ValueError(f"dtype {dtype} is not the caches' {k_cache.dtype}")
+    if num_tokens is None:
+        num_tokens = int(cu_seqlens[-1].item()) if cu_seqlens is not None else block_tables.shape[0]
+    shape = (num_tokens, k_cache.shape[2], k_cache.shape[3] * (2 if fp4 else 1))
+    k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    if fp4:
+        k_scales, v_scales = _vec4(k_scales), _vec4(v_scales)
+    _lib.call("paged_kv_read", k, v, _lib.vec16(k_cache), _lib.vec16(v_cache), block_tables, context_lens, cu_seqlens,
+              k_scales, v_scales)
+    return k, v
