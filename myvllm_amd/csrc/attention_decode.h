@@ -14,10 +14,10 @@ namespace {
 // O^T = V^T P^T (16x16x16 MFMA).  With one split a unit is one sequence and
 // the wave writes the normalised output.  With num_splits > 1 the batch is
 // dealt evenly over U = B (num_splits - 1) units by price: sequence b costs
-// its 16-key tiles T_b = ceil(L_b / 16) plus kDecodeStartPrice for the start
+// its 16-key tiles T_b = ceil(L_b / 16) plus the start price for the start
 // of a piece (its query load and pipeline fill), 0 if it has no keys; laid
 // end to end the sequences fill prices [0, Q_B), sequence b's tiles at
-// [Q_b + kDecodeStartPrice, Q_{b+1}), and unit u takes the tiles whose prices
+// [Q_b + start price, Q_{b+1}), and unit u takes the tiles whose prices
 // lie in [u Q_B / U, (u+1) Q_B / U).  So every unit streams about the same
 // number of keys whatever the lengths are.  A unit crossing sequence ends
 // runs one piece per sequence.  A piece that is a whole sequence writes its
@@ -32,7 +32,7 @@ namespace {
 // it.  The kvw kv heads of a workgroup (one wave
 // each) read the interleaved head rows of the same cache slots at about the
 // same time, so each page is streamed as one contiguous region.
-constexpr int32_t kDecodeStartPrice = 2;
+constexpr int32_t kDecodeStartPrice = 2;  // (DecodeArgs::start; the decode of 4-bit caches has its own)
 
 struct DecodeArgs {
   const void* q;
@@ -45,6 +45,8 @@ struct DecodeArgs {
   float* part;     // (B + U = B splits, Hq, D + 4): O, m, l per piece (rows padded to 16 bytes)
   int32_t* prices;  // (B + 1): the price prefix Q (splits > 1)
   int32_t B, Hq, Hkv, splits, kvw;
+  int32_t start;  // price of a piece's start
+  double unit_inv;  // splits > 1: 1 / U
   int32_t units;  // splits > 1: units per sequence, splits - 1 (U = B units); shared: of waves in the grid
   float c;
   bool ctx64;
@@ -58,12 +60,12 @@ struct DecodeArgs {
 };
 
 // Price prefix of the batch for the split decode: Q[b] = sum over b' < b of
-// the price of b' (ceil(L_b' / 16) + kDecodeStartPrice, or 0 with no keys),
+// the price of b' (ceil(L_b' / 16) + the start price, or 0 with no keys),
 // Q[B] the total, with L_b the context length clamped to the table's capacity
 // as the decode clamps it.  One workgroup: each thread sums a contiguous run of
 // sequences, the run sums are scanned across the block, and each thread writes
 // its run's prefixes.  (Q[B] < 2^31: the entry point checks
-// B * (ceil(capacity / 16) + kDecodeStartPrice).)
+// B * (ceil(capacity / 16) + start price).)
 __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeArgs a) {
   __shared__ int32_t wsum[16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
   const int64_t b0 = (int64_t)tid * per;
   auto price_of = [&](int64_t b) -> int32_t {
     const int32_t t = b < a.B ? (int32_t)((clamp64(load_index(a.ctx, b, a.ctx64), 0, cap) + 15) / 16) : 0;
-    return t > 0 ? t + kDecodeStartPrice : 0;
+    return t > 0 ? t + a.start : 0;
   };
   int32_t sum = 0;
   for (int i = 0; i < per; ++i) sum += price_of(b0 + i);
@@ -97,6 +99,15 @@ __global__ __launch_bounds__(1024) void attn_decode_prices_kernel(const DecodeAr
   if (tid == 1023) a.prices[a.B] = base + inc;
 }
 
+// floor(n / d) for 0 <= n < 2^56, 0 < d < 2^31, quotients below 2^31 and inv =
+// 1.0 / d: the product is within one of it (a 64-bit division takes 120
+// instructions, which a unit's start waits for).
+GDN_DEVICE int32_t floor_div(int64_t n, int64_t d, double inv) {
+  const int32_t q = (int32_t)((double)n * inv);
+  const int64_t r = n - (int64_t)q * d;
+  return __builtin_amdgcn_readfirstlane(q + (r < 0 ? -1 : r >= d ? 1 : 0));
+}
+
 // The pieces of a decode workgroup's unit, one after the other:
 // piece(sequence, first key, end of its keys, workspace slot or -1 where it is the
 // whole sequence, the sequence's last key).  first_wave: of the workgroup.
@@ -104,7 +115,7 @@ template <typename Piece>
 GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool first_wave, Piece&& piece) {
   // with one split, unit z is sequence z; else unit u holds the batch's
   // prices [x0, x1) (they fit 31 bits, which the entry point checks)
-  constexpr int32_t SP = kDecodeStartPrice;
+  const int32_t SP = a.start;
   int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
   if (a.splits > 1) {
     const int64_t U = (int64_t)a.B * a.units;
@@ -119,25 +130,19 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
         const int32_t t = (int32_t)((clamp64(load_index(a.ctx, i, a.ctx64), 0, cap) + 15) / 16);
         return t > 0 ? t + SP : 0;
       };
-      int32_t tot = 0;
-      for (int32_t c0 = 0; c0 < a.B; c0 += 64) tot += price(c0 + lane);
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) tot += __shfl_xor(tot, d);
-      tot = __builtin_amdgcn_readfirstlane(tot);
-      x0 = (int32_t)(u * tot / U);
-      x1 = (int32_t)((u + 1) * tot / U);
+      const int32_t p0 = price(lane), inc0 = wave_inclusive_scan_i32(p0);
+      int32_t tot = __builtin_amdgcn_readlane(inc0, 63);
+      for (int32_t c0 = 64; c0 < a.B; c0 += 64)
+        tot += __builtin_amdgcn_readlane(wave_inclusive_scan_i32(price(c0 + lane)), 63);
+      x0 = floor_div(u * tot, U, a.unit_inv);
+      x1 = floor_div((u + 1) * tot, U, a.unit_inv);
       const bool writer = u == 0 && blockIdx.y == 0 && first_wave;
       if (writer && lane == 0) a.prices[a.B] = tot;
       if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
       int32_t run = 0;
       for (int32_t c0 = 0; c0 < a.B; c0 += 64) {
-        const int32_t p = price(c0 + lane);
-        int32_t inc = p;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int32_t y = __shfl_up(inc, d);
-          if (lane >= d) inc += y;
-        }
+        const int32_t p = c0 == 0 ? p0 : price(c0 + lane);
+        const int32_t inc = c0 == 0 ? inc0 : wave_inclusive_scan_i32(p);
         const int32_t ex = run + inc - p;  // Q of sequence c0 + lane
         if (writer && c0 + lane < a.B) a.prices[c0 + lane] = ex;
         // the lanes with Q <= x0 are a prefix of the chunk's sequences
@@ -152,8 +157,8 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
       if (x0 >= x1) return;
     } else {
       const int64_t Pt = load_index_scalar(a.prices, a.B, false);
-      x0 = (int32_t)(u * Pt / U);
-      x1 = (int32_t)((u + 1) * Pt / U);
+      x0 = floor_div(u * Pt, U, a.unit_inv);
+      x1 = floor_div((u + 1) * Pt, U, a.unit_inv);
       if (x0 >= x1) return;  // an empty unit (a smaller total than U): no piece
       // the sequence holding price x0: the last b < B with Q[b] <= x0 (Q[0] =
       // 0), by a 64-ary search over the prefix (one probe per lane per
@@ -469,7 +474,8 @@ __global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArg
   float acc[E] = {};
   float l = 0.f;
   if (qn > qb) {  // (else no keys: a zero row)
-    const int64_t u0 = ((qb + kDecodeStartPrice + 1) * U - 1) / Pt, u1 = (qn * U - 1) / Pt;
+    const double inv = 1.0 / (double)Pt;
+    const int64_t u0 = floor_div((qb + a.start + 1) * U - 1, Pt, inv), u1 = floor_div(qn * U - 1, Pt, inv);
     if (u0 == u1) return;  // one unit held the whole sequence and wrote its row
     const bool all_units = Pt >= U;  // every unit has a price range
     const float* base = a.part + ((b + u0) * a.Hq + head) * (int64_t)PS;
@@ -496,13 +502,22 @@ __global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArg
       for (int d = 1; d < 64; d *= 2) ls += __shfl_xor(ls, d);
       l += ls;
       const int cnt = u1 - u0 + 1 - c0 < 64 ? (int)(u1 - u0 + 1 - c0) : 64;
-      for (int j = 0; j < cnt; ++j) {
-        const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), j));
-        const float* pp = base + (c0 + j) * rs + E * lane;
+      // (eight pieces' rows in flight; past the last one, its row once more with weight 0)
+      for (int j0 = 0; j0 < cnt; j0 += 8) {
+        float v[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float v = pp[e];
-          acc[e] += wj == 0.f ? 0.f : wj * v;  // (an empty unit's slot holds stale data)
+        for (int k = 0; k < 8; ++k) {
+          const float* pp = base + (c0 + (j0 + k < cnt ? j0 + k : cnt - 1)) * rs + E * lane;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[k][e] = pp[e];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int j = j0 + k < cnt ? j0 + k : cnt - 1;
+          const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), j));
+          const float wj = j0 + k < cnt ? w : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += wj == 0.f ? 0.f : wj * v[k][e];  // (an empty unit's slot holds stale data)
         }
       }
     }
@@ -555,8 +570,10 @@ DecodeArgs decode_args(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tens
   a.splits = splits;
   a.kvw = a.Hkv % 4 == 0 ? 4 : (a.Hkv % 2 == 0 ? 2 : 1);
   a.c = scale * kLog2e;
+  a.start = kDecodeStartPrice;
   if (splits > 1) {
     a.units = splits - 1;
+    a.unit_inv = 1.0 / ((double)a.B * a.units);
     a.part = workspace;
     a.prices = reinterpret_cast<int32_t*>(workspace + (int64_t)a.B * splits * a.Hq * (q->shape[2] + 4));
     // up to 1,024 sequences every decode wave sums the prices itself (16

@@ -10,8 +10,12 @@
 
 namespace {
 
+constexpr int32_t kFp4StartPrice = 6;
+
 struct Fp4DecodeArgs : DecodeArgs {
   ScaleSource ks, vs;
+  uint32_t page_inv;  // floor((2^32 - 1) / 16-key groups of a page)
+  int32_t R, hgroups;  // query heads of a kv head, and their groups of 16
 };
 
 // Decode: a workgroup is four waves, of 4 / KS kv heads (and up to 16 query heads of
@@ -24,7 +28,9 @@ struct Fp4DecodeArgs : DecodeArgs {
 // groups, which is where S^T leaves their probabilities, so V reaches the matrix
 // instruction without LDS: two numbers of a dim pair at a time are turned into 16
 // bits, and byte permutes pair them by keys.
-template <typename T, int D, int KS>
+//
+// ONE: pages of 16 keys, so a 16-key group is a page and starts at its slot 0.
+template <typename T, int D, int KS, bool ONE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_fp4_kernel(
     const Fp4DecodeArgs a) {
   typedef Mma<T> M;
@@ -35,6 +41,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   constexpr int NQ = CB / 8;              // k-steps per load
   constexpr int VE = D / 16;              // dims of V per lane
   constexpr int VW = VE > 8 ? 2 : 1;      // their words
+  constexpr int NT = 2;                   // tiles in flight
   constexpr int LDO = D + 4;
   __shared__ __align__(16) float ob[KS > 1 ? 4 * 16 * LDO : 4];
   __shared__ float ml[4][2][16];
@@ -42,9 +49,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, grp = lane >> 4, part = wv % KS;
   const int64_t cap = a.tab.cols * a.tab.page;
-  const int R = a.Hq / a.Hkv, hgroups = (R + 15) / 16;
-  const int kvh = (blockIdx.y / hgroups) * (4 / KS) + wv / KS;
-  const int h0 = (blockIdx.y % hgroups) * 16;
+  const int R = a.R, hgroups = a.hgroups, y = hgroups == 1 ? blockIdx.y : blockIdx.y / hgroups;
+  const int kvh = y * (4 / KS) + wv / KS;
+  const int h0 = ((int)blockIdx.y - y * hgroups) * 16;
   const bool hvalid = h0 + c16 < R;
   const int head = kvh * R + (hvalid ? h0 + c16 : 0);
   const char* const kbase = a.k.base + kvh * a.k.sh;
@@ -55,77 +62,118 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const uint64_t kssb = (uint32_t)a.ks.sb, vssb = (uint32_t)a.vs.sb;
   const uint32_t kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st, ksd = (uint32_t)a.ks.sd, vsd = (uint32_t)a.vs.sd;
   const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
-  const uint32_t gpp = (uint32_t)a.tab.page / 16u;
+  const uint32_t qkeep = hvalid && a.c != 0.f ? ~0u : 0u, qsign = a.c < 0.f ? 0x80008000u : 0u;
+  const uint32_t gpp = (uint32_t)a.tab.page / 16u, nblk = (uint32_t)a.tab.num_blocks;  // (below 2^31)
 
   struct Tile {
     uint32_t k[2][NI][CB / 8], ks[2][NI];
     uint32_t v[8][VW], vs[2];
+    bool named[2];
   };
+  // this lane's place in a group of 16 keys: codes of K, of V, scales of V
+  const uint32_t ko = c16 * kst + CB / 2 * grp, vso = VE * c16 / 32 * vsd + 4 * grp;
+  uint32_t kso[NI], vo[4];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) kso[i] = CB * (4 * i + grp) / 32 * ksd + c16;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) vo[e] = (4 * grp + e) * vst + VE / 2 * c16;
 
-  auto piece = [&](int64_t b, int64_t k_lo, int64_t k_hi, int64_t slot, int64_t) {
+  auto piece = [&](int64_t b_, int64_t lo_, int64_t hi_, int64_t slot_, int64_t) {
+    // (the same in all lanes, which the compiler does not see through the lengths'
+    // vector loads: descriptors made of it would be looped over)
+    const int32_t b = __builtin_amdgcn_readfirstlane((int32_t)b_), slot = __builtin_amdgcn_readfirstlane((int32_t)slot_);
+    const uint32_t k_lo = __builtin_amdgcn_readfirstlane((int32_t)lo_), k_hi = __builtin_amdgcn_readfirstlane((int32_t)hi_);
+    if (k_hi == 0) {  // no keys: zero rows (and no table column that could be read)
+      constexpr int LR = D / 4;
+      const int hd0 = kvh * R + h0;
+      for (int h = part * (16 / KS) + lane / LR; h < (part + 1) * (16 / KS); h += 64 / LR)
+        if (h0 + h < R)
+          *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)(hd0 + h) * a.o_sh +
+                                 4 * (lane % LR)) = v4{};
+      return;
+    }
     const int ntiles = (int)((k_hi - k_lo + 31) / 32);
     v8 qf[NI][NQ];
     {
-      const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_ss + (int64_t)head * a.q_sh;
+      const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_ss + (int64_t)head * a.q_sh;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          const v8 x = hvalid ? *reinterpret_cast<const v8*>(qp + CB * (4 * i + grp) + 8 * q) : v8{};
-          qf[i][q] = a.c > 0.f ? x : (a.c < 0.f ? -x : v8{});
+          // (a negative scale turns q's signs, a zero one clears q, as in the plain decode)
+          uint4 x = *reinterpret_cast<const uint4*>(qp + CB * (4 * i + grp) + 8 * q);
+          x.x = (x.x & qkeep) ^ qsign, x.y = (x.y & qkeep) ^ qsign, x.z = (x.z & qkeep) ^ qsign, x.w = (x.w & qkeep) ^ qsign;
+          qf[i][q] = __builtin_bit_cast(v8, x);
         }
     }
-    const void* trow = reinterpret_cast<const char*>(a.tab.table) + (a.tab.is64 ? 8 : 4) * (b * a.tab.row_stride);
-    const uint32_t g0 = (uint32_t)k_lo / 16u, gend = ((uint32_t)k_hi + 15u) / 16u;
-    auto block_of = [&](uint32_t g) -> int64_t {
-      if (g >= gend) return -1;
-      const int64_t blk = load_index_scalar(trow, gpp == 1u ? g : g / gpp, a.tab.is64);
-      return blk >= 0 && blk < a.tab.num_blocks ? blk : -1;
+    // 16-key group g of the sequence: its page's block, the slot in it, and whether the
+    // table names one.  Groups past the piece stand for its last one (their keys are
+    // masked), groups of foreign blocks for block 0 (their words become zero): every load is
+    // inside the caches, and none is behind a branch.
+    // (a table of 64-bit ids is read as pairs of words, one of 32-bit ids as each word
+    // twice: no branch, so the lookups of several groups wait together)
+    const uint32_t wide = a.tab.is64 ? 1u : 0u;
+    const const_i32_ptr trow = __builtin_bit_cast(const_i32_ptr, a.tab.table) + ((b * a.tab.row_stride) << wide);
+    const uint32_t g0 = k_lo / 16u, glast = (k_hi - 1u) / 16u;
+    struct Group {
+      uint32_t block, slot;
+      bool named;
     };
-    auto load = [&](int t, const int64_t* blk, Tile& x) {
+    auto group_of = [&](uint32_t g) -> Group {
+      g = g < glast ? g : glast;
+      uint32_t col = g, rem = 0;
+      if constexpr (!ONE) {
+        col = (uint32_t)(((uint64_t)g * a.page_inv) >> 32), rem = g - col * gpp;  // (at most one short)
+        if (rem >= gpp) ++col, rem -= gpp;
+      }
+      const uint32_t low = (uint32_t)trow[col << wide], high = (uint32_t)trow[(col << wide) + wide];
+      const bool named = low < nblk && (!wide || high == 0u);
+      return {named ? low : 0u, 16u * rem, named};
+    };
+    // (the offsets are made opaque where they are used: known to be the same in every
+    // round they are widened ahead, and each address is then a 64-bit vector sum)
+    auto at = [](const auto* base, uint32_t off) __attribute__((always_inline)) {
+      asm("" : "+v"(off));
+      return reinterpret_cast<const char*>(base) + off;
+    };
+    auto load = [&](const Group* gr, Tile& x) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t g = g0 + 2u * (uint32_t)t + h, j0 = 16u * g;
-        const uint32_t r0 = gpp == 1u ? 0u : 16u * (g - (g / gpp) * gpp);
-        const bool ok = blk[h] >= 0;
-        const uint64_t bb = ok ? (uint32_t)blk[h] : 0u;
-        // the ranges end after the group's keys, so codes past them read as 0
-        const uint32_t left = ok && j0 < (uint32_t)k_hi ? (uint32_t)k_hi - j0 : 0u;
-        const uint32_t rows = left > 0u ? r0 + (left < 16u ? left : 16u) : 0u;
-        const __amdgpu_buffer_rsrc_t rk =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + bb * ksb), 0, rows * kst, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rv =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + bb * vsb), 0, rows * vst, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)(ksbase + bb * kssb), 0,
-                                                                             left > 0u ? D / 32 * ksd : 0u, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)(vsbase + bb * vssb), 0,
-                                                                             left > 0u ? D / 32 * vsd : 0u, 0x00020000);
-        const uint32_t ko = (r0 + c16) * kst + CB / 2 * grp;
+        const uint64_t bb = gr[h].block;
+        x.named[h] = gr[h].named;
+        const char* kp = kbase + bb * ksb;
+        const char* vp = vbase + bb * vsb;
+        const uint8_t* ksp = ksbase + bb * kssb;
+        const uint8_t* vsp = vsbase + bb * vssb;
+        if constexpr (!ONE) {
+          const uint32_t r0 = gr[h].slot;
+          kp += r0 * kst, vp += r0 * vst, ksp += r0, vsp += r0;
+        }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
           if constexpr (CB == 32) {
-            const uint4 w = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + 64 * i, 0, 0));
+            const uint4 w = *reinterpret_cast<const uint4*>(at(kp, ko) + 64 * i);
             x.k[h][i][0] = w.x, x.k[h][i][1] = w.y, x.k[h][i][2] = w.z, x.k[h][i][3] = w.w;
           } else {
-            const uint2 w = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rk, ko, 0, 0));
+            const uint2 w = *reinterpret_cast<const uint2*>(at(kp, ko));
             x.k[h][i][0] = w.x, x.k[h][i][1] = w.y;
           }
-          x.ks[h][i] = __builtin_amdgcn_raw_buffer_load_b8(rks, CB * (4 * i + grp) / 32 * ksd + r0 + c16, 0, 0);
+          x.ks[h][i] = *reinterpret_cast<const uint8_t*>(at(ksp, kso[i]));
         }
-        const uint32_t vo = (r0 + 4 * grp) * vst + VE / 2 * c16;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t* const w = x.v[4 * h + e];
+          const char* const p = at(vp, vo[e]);
           if constexpr (VE == 16) {
-            const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rv, vo + e * vst, 0, 0));
+            const uint2 y = *reinterpret_cast<const uint2*>(p);
             w[0] = y.x, w[1] = y.y;
           } else if constexpr (VE == 8) {
-            w[0] = __builtin_amdgcn_raw_buffer_load_b32(rv, vo + e * vst, 0, 0);
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
           } else {
-            w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rv, vo + e * vst, 0, 0);
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
           }
         }
-        x.vs[h] = __builtin_amdgcn_raw_buffer_load_b32(rvs, VE * c16 / 32 * vsd + r0 + 4 * grp, 0, 0);
+        x.vs[h] = *reinterpret_cast<const uint32_t*>(at(vsp, vso));
       }
     };
 
@@ -134,7 +182,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     for (int d = 0; d < VE; ++d) oacc[d] = f32x4{};
     float m_used = -INFINITY, lsum = 0.f, nb = 0.f;  // (as in the plain decode)
 
-    auto compute = [&](int t, const Tile& x) {
+    auto compute = [&](int t, Tile& x) {
+      if (!(x.named[0] && x.named[1])) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t keep = x.named[h] ? ~0u : 0u;
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+#pragma unroll
+            for (int w = 0; w < CB / 8; ++w) x.k[h][i][w] &= keep;
+            x.ks[h][i] &= keep;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) x.v[4 * h + e][w] &= keep;
+          x.vs[h] &= keep;
+        }
+      }
       f32x4 s[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -147,14 +212,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
             s[h] = M::m16k32(__builtin_bit_cast(v8, fp4_eight<T>(x.k[h][i][q], sc)), qf[i][q], s[h]);
         }
       }
-      const uint32_t j0 = (uint32_t)k_lo + 32u * (uint32_t)t;
+      const uint32_t j0 = k_lo + 32u * (uint32_t)t;
       uint32_t vs[2] = {x.vs[0], x.vs[1]};
-      if (j0 + 32u > (uint32_t)k_hi) {
+      if (j0 + 32u > k_hi) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (j0 + 16u * h + 4u * grp + r >= (uint32_t)k_hi) {
+            if (j0 + 16u * h + 4u * grp + r >= k_hi) {
               s[h][r] = -INFINITY;
               vs[h] &= ~(255u << (8 * r));  // (a stale scale may stand for NaN)
             }
@@ -166,9 +231,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         mg = fmaxf(mg, __shfl_xor(mg, 32));
         const float mn = fmaxf(m_used, mg * c);
         const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m_used - mn);
+        if (__builtin_amdgcn_ballot_w64(m_used != -INFINITY) != 0) {  // (else nothing is summed yet)
 #pragma unroll
-        for (int d = 0; d < VE; ++d) oacc[d] *= alpha;
-        lsum *= alpha;
+          for (int d = 0; d < VE; ++d) oacc[d] *= alpha;
+          lsum *= alpha;
+        }
         m_used = mn;
         nb = mn == -INFINITY ? 0.f : -mn;
       }
@@ -181,9 +248,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
           lsum += p;
           pf[4 * h + r] = (T)p;
         }
+      // (a scale's byte is moved to the exponent; the conversion reads no other bits)
       float sc[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sc[e] = fp4_scale(vs[e >> 2] >> (8 * (e & 3)) & 255u);
+      for (int e = 0; e < 8; ++e)
+        sc[e] = __builtin_bit_cast(float, (e & 3) == 3 ? vs[e >> 2] >> 1 : vs[e >> 2] << (23 - 8 * (e & 3)));
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         constexpr int NP = VE > 8 ? 4 : VE / 2;  // pairs of dims in a word
@@ -211,27 +280,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
     };
 
-    // two tiles in flight, their blocks looked up one tile earlier still; loads are
-    // issued unconditionally (past the range they read zeros)
-    Tile xA, xB;
-    int64_t bA[2], bB[2];
-    auto blocks = [&](int t, int64_t* o) {
-      o[0] = block_of(g0 + 2u * (uint32_t)t);
-      o[1] = block_of(g0 + 2u * (uint32_t)t + 1u);
+    // NT tiles in flight, and the groups of the next one to load
+    Tile x[NT];
+    Group gr[2];
+    auto groups = [&](int t) {
+      gr[0] = group_of(g0 + 2u * (uint32_t)t);
+      gr[1] = group_of(g0 + 2u * (uint32_t)t + 1u);
     };
-    blocks(part, bA);
-    blocks(part + KS, bB);
-    load(part, bA, xA);
-    load(part + KS, bB, xB);
-    blocks(part + 2 * KS, bA);
-    blocks(part + 3 * KS, bB);
-    for (int t = part; t < ntiles; t += 2 * KS) {
-      compute(t, xA);
-      load(t + 2 * KS, bA, xA);
-      blocks(t + 4 * KS, bA);
-      if (t + KS < ntiles) compute(t + KS, xB);
-      load(t + 3 * KS, bB, xB);
-      blocks(t + 5 * KS, bB);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      groups(part + u * KS);
+      load(gr, x[u]);
+    }
+    groups(part + NT * KS);
+    for (int t = part; t < ntiles; t += NT * KS) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        compute(t + u * KS, x[u]);
+        load(gr, x[u]);
+        groups(t + (u + 1 + NT) * KS);
+      }
     }
 
     float lt = lsum + __shfl_xor(lsum, 16);
@@ -239,8 +307,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     if constexpr (KS == 1) {
       if (!hvalid) return;
       const float inv = lt > 0.f ? 1.f / lt : 0.f;
-      float* const pp = a.part + (slot * a.Hq + head) * (int64_t)(D + 4);
-      T* const op = reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)head * a.o_sh;
+      float* const pp = a.part + ((int64_t)slot * a.Hq + head) * (D + 4);
+      T* const op = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)head * a.o_sh;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -263,13 +331,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         ml[wv][1][c16] = lt;
       }
       __syncthreads();
-      auto top = [&](int h) {
-        float m = ml[w0][0][h];
+      float mt = ml[w0][0][c16];
 #pragma unroll
-        for (int p = 1; p < KS; ++p) m = fmaxf(m, ml[w0 + p][0][h]);
-        return m;
-      };
-      const float mt = top(c16), f = m_used == -INFINITY ? 0.f : exp2_fast(m_used - mt);
+      for (int p = 1; p < KS; ++p) mt = fmaxf(mt, ml[w0 + p][0][c16]);
+      auto weight = [&](float m) { return m == -INFINITY ? 0.f : exp2_fast(m - mt); };
+      float l = 0.f;
+#pragma unroll
+      for (int p = 0; p < KS; ++p) l += ml[w0 + p][1][c16] * weight(ml[w0 + p][0][c16]);
+      const float f = weight(m_used) * (slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f);
       float* const mine = ob + (wv * 16 + c16) * LDO;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -277,13 +346,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         for (int j = 0; j < VE; j += 4)
           *reinterpret_cast<f32x4*>(mine + VE * (4 * grp + r) + j) =
               f32x4{oacc[j][r] * f, oacc[j + 1][r] * f, oacc[j + 2][r] * f, oacc[j + 3][r] * f};
+      float* const pp = a.part + ((int64_t)slot * a.Hq + kvh * R + h0) * (D + 4);
+      if (slot >= 0 && part == 0 && grp == 0 && hvalid) {
+        pp[c16 * (D + 4) + D] = mt;
+        pp[c16 * (D + 4) + D + 1] = l;
+      }
       __syncthreads();
-      constexpr int LR = D / 4;         // lanes per row
-      constexpr int RW = 16 / KS;       // rows per wave
+      constexpr int LR = D / 4;    // lanes per row
+      constexpr int RW = 16 / KS;  // rows per wave
       static_assert(LR <= 64 && RW % (64 / LR) == 0, "rows of a wave");
-#pragma unroll
+      T* const op = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)(kvh * R + h0) * a.o_sh;
+#pragma unroll 1
       for (int i = 0; i < RW / (64 / LR); ++i) {
         const int h = part * RW + i * (64 / LR) + lane / LR, d = 4 * (lane % LR);
+        if (h0 + h >= R) break;
         f32x4 o = *reinterpret_cast<const f32x4*>(ob + (w0 * 16 + h) * LDO + d);
 #pragma unroll
         for (int p = 1; p < KS; ++p) {
@@ -291,27 +367,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] += y[e];
         }
-        const float m = top(h);
-        float l = 0.f;
-#pragma unroll
-        for (int p = 0; p < KS; ++p) {
-          const float mp = ml[w0 + p][0][h];
-          l += mp == -INFINITY ? 0.f : ml[w0 + p][1][h] * exp2_fast(mp - m);
-        }
-        if (h0 + h >= R) continue;
-        const int hd = kvh * R + h0 + h;
-        if (slot < 0) {
-          const float inv = l > 0.f ? 1.f / l : 0.f;
-          *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)hd * a.o_sh + d) =
-              v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
-        } else {
-          float* const pp = a.part + (slot * a.Hq + hd) * (int64_t)(D + 4);
-          *reinterpret_cast<f32x4*>(pp + d) = o;
-          if (d == 0) {
-            pp[D] = m;
-            pp[D + 1] = l;
-          }
-        }
+        if (slot < 0) *reinterpret_cast<v4*>(op + (int64_t)h * a.o_sh + d) = v4{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
+        else *reinterpret_cast<f32x4*>(pp + h * (D + 4) + d) = o;
       }
     }
   };
@@ -322,23 +379,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 // of, so that a line is read by one XCD (rows of 128, 64 and 32 bytes), if the
 // heads divide by that.
 int fp4_heads(int Hkv, int D) {
-  int n = 256 / D;
+  int n = D == 256 ? 1 : 4;
   while (Hkv % n) n /= 2;
   return n;
 }
 
+template <typename T, int D, bool ONE>
+void launch_decode_fp4_waves(const Fp4DecodeArgs& a, int heads, dim3 grid, hipStream_t st) {
+  if constexpr (D < 256) {
+    if (heads == 4) return attn_decode_fp4_kernel<T, D, 1, ONE><<<grid, dim3(256), 0, st>>>(a);
+    if (heads == 2) return attn_decode_fp4_kernel<T, D, 2, ONE><<<grid, dim3(256), 0, st>>>(a);
+  }
+  attn_decode_fp4_kernel<T, D, 4, ONE><<<grid, dim3(256), 0, st>>>(a);
+}
+
 template <typename T, int D>
 hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
-  const int heads = fp4_heads(a.Hkv, D), hgroups = (a.Hq / a.Hkv + 15) / 16;
+  const int heads = fp4_heads(a.Hkv, D), hgroups = a.hgroups;
   const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / heads * hgroups), (unsigned)a.B);
   if (a.splits > 1 && !a.prices_inline) {
     attn_decode_prices_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (heads == 1) attn_decode_fp4_kernel<T, D, 4><<<grid, dim3(256), 0, st>>>(a);
-  else if (heads == 2) attn_decode_fp4_kernel<T, D, 2><<<grid, dim3(256), 0, st>>>(a);
-  else attn_decode_fp4_kernel<T, D, 1><<<grid, dim3(256), 0, st>>>(a);
+  if (a.tab.page == 16) launch_decode_fp4_waves<T, D, true>(a, heads, grid, st);
+  else launch_decode_fp4_waves<T, D, false>(a, heads, grid, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   attn_decode_combine_kernel<T, D><<<dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st>>>(a);
@@ -374,6 +439,8 @@ hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_le
 
 }  // namespace
 
+int32_t attn_fp4_start_price() { return kFp4StartPrice; }
+
 hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                   const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
                                   const gdn_tensor* ctx, gdn_tensor* out, float* workspace, int32_t splits, float scale,
@@ -383,6 +450,11 @@ hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, con
   static_cast<DecodeArgs&>(a) = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
   a.ks = scale_source(ks);
   a.vs = scale_source(vs);
+  a.start = kFp4StartPrice;
+  a.R = a.Hq / a.Hkv;
+  a.hgroups = (a.R + 15) / 16;
+  a.page_inv = 0xFFFFFFFFu / (uint32_t)(a.tab.page / 16);
+  if (a.tab.num_blocks == 0) a.tab.cols = 0;  // (no page to read: lengths end at 0 keys)
   const int D = (int)q->shape[2];
   if (q->dtype == GDN_DTYPE_BF16) {
     if (D == 64) return launch_decode_fp4<bf16_t, 64>(a, st);

@@ -55,6 +55,7 @@ hipError_t attn_paged_decode_launch(const gdn_tensor* q, const gdn_tensor* kc, c
                                     int32_t splits, float scale, hipStream_t st);
 hipError_t attn_decode_scratch(hipStream_t st, float** ptr);
 int32_t attn_decode_start_price();
+int32_t attn_fp4_start_price();
 hipError_t attn_varlen_scored_launch(const gdn_tensor* q, const gdn_tensor* k, const gdn_tensor* v,
                                      const gdn_tensor* cu, gdn_tensor* out, const gdn_tensor* slopes,
                                      const gdn_tensor* pfx, int64_t max_seqlen, float scale, float cap, int causal,
@@ -790,7 +791,7 @@ int check_paged_decode(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn
   // the split decode prices the batch (16-key tiles plus a start price per
   // sequence) in 32 bits
   if (num_splits > 1 &&
-      B * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + attn_decode_start_price()) >= (int64_t(1) << 31))
+      B * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + (codes ? attn_fp4_start_price() : attn_decode_start_price())) >= (int64_t(1) << 31))
     return GDN_ERR_RANGE;
   // one page of one kv head is addressed with 32-bit byte offsets below 2^31
   const int64_t es = elem_size(k_cache->dtype);

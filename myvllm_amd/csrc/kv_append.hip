@@ -75,27 +75,13 @@ GDN_DEVICE int64_t find_seq(const AppendArgs& a, int64_t t, int lane) {
   return lo < a.nseq ? lo : -1;
 }
 
-// The pairs of a lane turned in R's precision, rounded once to T.
-template <typename R, typename T, typename V8>
-GDN_DEVICE void turn(V8& x, V8& y, const float* c, const float* s, bool interleaved) {
-  if (interleaved) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const R a0 = (R)(float)x[2 * j], b0 = (R)(float)x[2 * j + 1];
-      const R a1 = (R)(float)y[2 * j], b1 = (R)(float)y[2 * j + 1];
-      x[2 * j] = (T)(float)(a0 * (R)c[j] - b0 * (R)s[j]);
-      x[2 * j + 1] = (T)(float)(b0 * (R)c[j] + a0 * (R)s[j]);
-      y[2 * j] = (T)(float)(a1 * (R)c[j + 4] - b1 * (R)s[j + 4]);
-      y[2 * j + 1] = (T)(float)(b1 * (R)c[j + 4] + a1 * (R)s[j + 4]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const R p = (R)(float)x[j], q = (R)(float)y[j];
-      x[j] = (T)(float)(p * (R)c[j] - q * (R)s[j]);
-      y[j] = (T)(float)(q * (R)c[j] + p * (R)s[j]);
-    }
-  }
+// A pair turned in fp64, rounded through fp32 to T.
+template <typename T> struct Pair {
+  T a, b;
+};
+template <typename T> GDN_DEVICE Pair<T> turn_exactly(T a, T b, float c, float s) {
+  const double x = (float)a, y = (float)b, cd = c, sd = s;
+  return {(T)(float)(x * cd - y * sd), (T)(float)(y * cd + x * sd)};
 }
 
 template <typename T, int D, bool AXES = false, bool FP4 = false>
@@ -190,8 +176,40 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
     const int r = r0 + i * RPI;
     if (r >= nrows) continue;
     if (turns && r < nq + a.Hkv) {
-      if (FP4 && r >= nq) turn<double, T>(x[i], y[i], c, s, a.interleaved);
-      else turn<float, T>(x[i], y[i], c, s, a.interleaved);
+      if (FP4 && r >= nq) {
+        if (a.interleaved) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Pair<T> p = turn_exactly(x[i][2 * j], x[i][2 * j + 1], c[j], s[j]);
+            const Pair<T> q = turn_exactly(y[i][2 * j], y[i][2 * j + 1], c[j + 4], s[j + 4]);
+            x[i][2 * j] = p.a, x[i][2 * j + 1] = p.b;
+            y[i][2 * j] = q.a, y[i][2 * j + 1] = q.b;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const Pair<T> p = turn_exactly(x[i][j], y[i][j], c[j], s[j]);
+            x[i][j] = p.a, y[i][j] = p.b;
+          }
+        }
+      } else if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a0 = (float)x[i][2 * j], b0 = (float)x[i][2 * j + 1];
+          const float a1 = (float)y[i][2 * j], b1 = (float)y[i][2 * j + 1];
+          x[i][2 * j] = (T)(a0 * c[j] - b0 * s[j]);
+          x[i][2 * j + 1] = (T)(b0 * c[j] + a0 * s[j]);
+          y[i][2 * j] = (T)(a1 * c[j + 4] - b1 * s[j + 4]);
+          y[i][2 * j + 1] = (T)(b1 * c[j + 4] + a1 * s[j + 4]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float p = (float)x[i][j], q = (float)y[i][j];
+          x[i][j] = (T)(p * c[j] - q * s[j]);
+          y[i][j] = (T)(q * c[j] + p * s[j]);
+        }
+      }
     }
     if (FP4 && r >= nq) {
       uint32_t* const top = tops + (w * kAppendRows + i) * 32 + lane / U * (D / 32);

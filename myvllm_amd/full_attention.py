@@ -263,23 +263,28 @@ def _vec4(t: torch.Tensor) -> torch.Tensor:
 
 def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int) -> int:
     """:func:`decode_num_splits` of caches held in 4 bits, whose units are
-    workgroups of four waves on 256 / D kv heads (fewer where those do not
-    divide the heads)."""
-    heads = max(1, 256 // max(head_dim, 1))
+    workgroups of four waves: one kv head of 256 dims, else four (two or one where
+    four do not divide the heads).  One workgroup per CU streams best (64 sequences
+    of U[1024, 8192] keys, 2 kv heads of 256: 256 workgroups 46.7 us, 384 52.6, 512
+    49.8; 256 of U[512, 16384], 4 of 128: 256 workgroups 210, 512 225), with at least
+    256 keys each (one sequence of 2,943 keys: 12 units 13.4 us, 8 14.8, 32 15.0).
+    A batch of 1,024 rows is not split (512 sequences of U[512, 4096] keys, 2 kv
+    heads of 256: 143 us, 155 split), one of 512 not where its sequences are short
+    (512 of U[200, 1000] keys, 4 of 128: 47.6 and 53.9; of U[512, 8192] 306 and
+    248)."""
+    heads = 1 if head_dim > 128 else 4
     while num_kv_heads % heads:
         heads //= 2
     groups = max(num_kv_heads, 1) // heads * ((num_q_heads // max(num_kv_heads, 1) + 15) // 16)
     rows = max(1, num_seqs * groups)
-    if rows >= _FP4_SPLIT_ROWS:
+    if rows >= 1024 or (rows >= 512 and capacity <= 2048):
         return 1
     units = max(1, round(_FP4_TARGET_WORKGROUPS / rows))
-    by_keys = -(-max(capacity, 1) // _FP4_MIN_SPLIT_KEYS)
+    by_keys = -(-max(capacity, 1) // _DECODE_MIN_SPLIT_KEYS)
     return max(1, min(_DECODE_MAX_SPLITS, 1 + min(units, by_keys)))
 
 
-_FP4_TARGET_WORKGROUPS = 512
-_FP4_SPLIT_ROWS = 2048
-_FP4_MIN_SPLIT_KEYS = 256
+_FP4_TARGET_WORKGROUPS = 256
 
 
 def _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, scale, num_splits, out):
