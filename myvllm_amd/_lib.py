@@ -278,6 +278,24 @@ def vec16(t: torch.Tensor) -> torch.Tensor:
     return t if vec16_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def vec4_all(*tensors: torch.Tensor | None) -> bool:
+    """Whether the kernels can read all of them (None aside) with 4-byte accesses."""
+    ok = (_fast or _load_fast()).vec4_ok(*tensors)
+    if ok is not None:
+        return ok
+    return all(t is None or (t.stride(-1) == 1 and t.data_ptr() % 4 == 0 and all(
+        t.stride(i) * t.element_size() % 4 == 0 for i in range(t.dim() - 1))) for t in tensors)
+
+
+def copy_caches(caches, src, dst) -> bool:
+    """``cache_copy`` of lists or tuples in one native call; False where the caches
+    or numbers need a closer look."""
+    code = (_fast or _load_fast()).copy_caches(caches, src, dst)
+    if code:
+        raise GdnError("cache_copy", code, strerror(code))
+    return code is not None
+
+
 def same_device(*tensors: torch.Tensor) -> bool:
     """Whether all of them are plain tensors on one HIP device."""
     return (_fast or _load_fast()).same_device(*tensors) >= 0

@@ -43,10 +43,12 @@ def cache_copy(caches: torch.Tensor | Sequence[torch.Tensor], src: Sequence[int]
     ``src`` and ``dst`` are on the host (lists, CPU tensors or arrays of whole numbers),
     where a cache's allocator has them: they travel with the launch, and a captured
     call replays its own.  The places are distinct and none of them is a source, ids are
-    inside the caches; all of it is checked before anything is copied."""
+    inside the caches: checked before anything is copied."""
     caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
     if not caches:
         raise ValueError("no caches to copy in")
+    if _lib.copy_caches(caches, src, dst):
+        return
     _lib.require_device(*caches)
     pairs = _pairs(src, dst)
     rows = []

@@ -16,6 +16,7 @@
 
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "../../include/gdn_hip.h"
 
@@ -147,10 +148,10 @@ PyObject* same_device(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(dev);
 }
 
-// Whether the kernels can read tensors (None aside) with 16-byte accesses (unit
-// inner stride, 16-byte aligned data and outer strides); None if one is not a
+// Whether the kernels can read tensors (None aside) with accesses of `bytes`
+// (unit inner stride, aligned data and outer strides); None if one is not a
 // plain one.
-PyObject* vec16_ok(PyObject*, PyObject* const* args, Py_ssize_t count) {
+PyObject* aligned_ok(PyObject* const* args, Py_ssize_t count, int64_t bytes) {
   try {
     bool ok = true;
     for (Py_ssize_t k = 0; k < count; ++k) {
@@ -159,9 +160,9 @@ PyObject* vec16_ok(PyObject*, PyObject* const* args, Py_ssize_t count) {
       const at::Tensor& t = THPVariable_Unpack(args[k]);
       const int64_t n = t.dim();
       if (n == 0) Py_RETURN_NONE;
-      ok = ok && t.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+      ok = ok && t.stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % (uintptr_t)bytes == 0;
       const int64_t es = (int64_t)t.element_size();
-      for (int64_t i = 0; ok && i < n - 1; ++i) ok = t.stride(i) * es % 16 == 0;
+      for (int64_t i = 0; ok && i < n - 1; ++i) ok = t.stride(i) * es % bytes == 0;
     }
     return PyBool_FromLong(ok);
   } catch (const std::exception& e) {
@@ -169,6 +170,8 @@ PyObject* vec16_ok(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return nullptr;
   }
 }
+PyObject* vec16_ok(PyObject*, PyObject* const* args, Py_ssize_t count) { return aligned_ok(args, count, 16); }
+PyObject* vec4_ok(PyObject*, PyObject* const* args, Py_ssize_t count) { return aligned_ok(args, count, 4); }
 
 typedef Entry<0, 8, float> RecurrentStep;
 typedef Entry<1, 9, float, int32_t> ChunkPrefill;
@@ -199,6 +202,88 @@ typedef Entry<25, 9> KvRead;
 typedef Entry<26, 9, int32_t, float> PagedDecodeFp4;
 typedef Entry<27, 10, int64_t, float> PagedPrefillFp4;
 typedef Entry<28, 5> CacheCopy;
+
+// Whole numbers of a list or tuple; false if it is another object or one does not fit.
+bool ids_of(PyObject* o, std::vector<int32_t>& out) {
+  if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+  PyObject** const items = PySequence_Fast_ITEMS(o);
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); ++i) {
+    int over = 0;
+    const long v = PyLong_CheckExact(items[i]) ? PyLong_AsLongAndOverflow(items[i], &over) : 0;
+    if (!PyLong_CheckExact(items[i]) || over || v != (int32_t)v) return false;
+    out.push_back((int32_t)v);
+  }
+  return true;
+}
+
+// copy_caches(caches, src, dst): cache_copy on a list or tuple of caches (layers,
+// blocks, ...), as bytes; None where the caller has to look closer (other objects,
+// empty caches, blocks with gaps, too few or too large numbers).
+PyObject* copy_caches(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3 || !CacheCopy::fn) {
+    PyErr_SetString(PyExc_TypeError, "copy_caches(caches, src, dst)");
+    return nullptr;
+  }
+  if (!PyList_CheckExact(args[0]) && !PyTuple_CheckExact(args[0])) Py_RETURN_NONE;
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(args[0]);
+  PyObject** const items = PySequence_Fast_ITEMS(args[0]);
+  constexpr Py_ssize_t kMost = 64;
+  if (count < 1 || count > kMost) Py_RETURN_NONE;
+  try {
+    gdn_tensor d[kMost];
+    for (Py_ssize_t k = 0; k < count; ++k) {
+      if (!plain(items[k])) Py_RETURN_NONE;
+      const at::Tensor& t = THPVariable_Unpack(items[k]);
+      const at::Tensor& first = THPVariable_Unpack(items[0]);
+      if (t.dim() < 3 || t.numel() == 0 || !t.is_cuda() || t.device() != first.device() || t.size(1) != first.size(1))
+        Py_RETURN_NONE;
+      int64_t block = 1;
+      for (int64_t i = t.dim() - 1; i >= 2; --i) {
+        if (t.size(i) != 1 && t.stride(i) != block) Py_RETURN_NONE;
+        block *= t.size(i);
+      }
+      const int64_t es = (int64_t)t.element_size();
+      d[k] = gdn_tensor{};
+      d[k].data = t.data_ptr();
+      d[k].dtype = GDN_DTYPE_U8;
+      d[k].ndim = 3;
+      d[k].shape[0] = t.size(0);
+      d[k].shape[1] = t.size(1);
+      d[k].shape[2] = block * es;
+      d[k].stride[0] = t.stride(0) * es;
+      d[k].stride[1] = t.stride(1) * es;
+      d[k].stride[2] = 1;
+    }
+    std::vector<int32_t> ids;
+    if (!ids_of(args[1], ids)) Py_RETURN_NONE;
+    const size_t pairs = ids.size();
+    if (!ids_of(args[2], ids) || ids.size() != 2 * pairs) Py_RETURN_NONE;
+    if (pairs == 0) return PyLong_FromLong(0);
+    gdn_tensor p{};
+    p.data = ids.data();
+    p.dtype = GDN_DTYPE_I32;
+    p.ndim = 2;
+    p.shape[0] = 2;
+    p.shape[1] = p.stride[0] = (int64_t)pairs;
+    p.stride[1] = 1;
+    const at::Device dev = THPVariable_Unpack(items[0]).device();
+    const c10::DeviceGuard guard(dev);
+    void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    typedef gdn_tensor* Ptr;
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    for (Py_ssize_t k = 0; k < count && rc == 0; k += 4)
+      rc = reinterpret_cast<int (*)(Ptr, Ptr, Ptr, Ptr, Ptr, void*)>(CacheCopy::fn)(
+          &d[k], k + 1 < count ? &d[k + 1] : nullptr, k + 2 < count ? &d[k + 2] : nullptr,
+          k + 3 < count ? &d[k + 3] : nullptr, &p, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 typedef Size<0, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> ChunkPrefillSize;
 typedef Size<1, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t> PagedPrefillSize;
 typedef Size<2, int64_t, int64_t, int64_t, int32_t> PagedDecodeSize;
@@ -259,7 +344,7 @@ PyObject* bind(PyObject*, PyObject* dict) {
   Py_RETURN_NONE;
 }
 
-PyMethodDef g_methods[kNumBound + 4];
+PyMethodDef g_methods[kNumBound + 6];
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_gdn_binding", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -272,6 +357,8 @@ PyMODINIT_FUNC PyInit__gdn_binding() {
   for (const Bound& b : kBound) add(b.name, reinterpret_cast<void*>(b.call), METH_FASTCALL);
   add("same_device", reinterpret_cast<void*>(same_device), METH_FASTCALL);
   add("vec16_ok", reinterpret_cast<void*>(vec16_ok), METH_FASTCALL);
+  add("vec4_ok", reinterpret_cast<void*>(vec4_ok), METH_FASTCALL);
+  add("copy_caches", reinterpret_cast<void*>(copy_caches), METH_FASTCALL);
   add("bind", reinterpret_cast<void*>(bind), METH_O);
   g_methods[k] = PyMethodDef{nullptr, nullptr, 0, nullptr};
   return PyModule_Create(&g_module);

@@ -255,10 +255,14 @@ def _fp4(k_scales, v_scales, *forms) -> bool:
     return True
 
 
-def _vec4(t: torch.Tensor) -> torch.Tensor:
-    """Block scales as the kernels read them, four slots at once."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 4 == 0 and all(t.stride(i) % 4 == 0 for i in range(t.dim() - 1))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales):
+    """The tensors as the kernels read them: rows 16 bytes at a time, the scales of
+    four slots at once; misaligned ones as contiguous copies."""
+    if not _lib.vec16_all(q, k_cache, v_cache):
+        q, k_cache, v_cache = (t if t is None else _lib.vec16(t) for t in (q, k_cache, v_cache))
+    if not _lib.vec4_all(k_scales, v_scales):
+        k_scales, v_scales = (t.clone(memory_format=torch.contiguous_format) for t in (k_scales, v_scales))
+    return q, k_cache, v_cache, k_scales, v_scales
 
 
 def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int) -> int:
@@ -297,8 +301,8 @@ def _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_l
     if n_ws > 0:
         ws = torch.empty(n_ws, dtype=torch.float32, device=dev)
     o = _out_for(out, (B, Hq, Dh), q.dtype, dev)
-    _lib.call("paged_attention_decode_fp4", _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache), _vec4(k_scales),
-              _vec4(v_scales), block_tables, context_lens, o, ws, int(num_splits), float(scale))
+    _lib.call("paged_attention_decode_fp4", *_fp4_aligned(q, k_cache, v_cache, k_scales, v_scales), block_tables,
+              context_lens, o, ws, int(num_splits), float(scale))
     return _finish(out, o)
 
 
@@ -446,11 +450,11 @@ def _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, co
     dev = _lib.require_device(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens)
     if max_seqlen is None:
         max_seqlen = _max_seqlen(cu_seqlens)
-    q, k_cache, v_cache = _lib.vec16(q), _lib.vec16(k_cache), _lib.vec16(v_cache)
+    q, k_cache, v_cache, k_scales, v_scales = _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales)
     o = _out_for(out, q.shape, q.dtype, dev)
     ws = _prefill_workspace(q, k_cache, v_cache, block_tables, cu_seqlens, k_cache.shape[1])
-    _lib.call("paged_attention_prefill_fp4", q, k_cache, v_cache, _vec4(k_scales), _vec4(v_scales), block_tables,
-              context_lens, cu_seqlens, o, ws, int(max_seqlen), float(scale))
+    _lib.call("paged_attention_prefill_fp4", q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens,
+              cu_seqlens, o, ws, int(max_seqlen), float(scale))
     return _finish(out, o)
 
 
@@ -589,8 +593,6 @@ def paged_kv_read(
         num_tokens = int(cu_seqlens[-1].item()) if cu_seqlens is not None else block_tables.shape[0]
     shape = (num_tokens, k_cache.shape[2], k_cache.shape[3] * (2 if fp4 else 1))
     k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
-    if fp4:
-        k_scales, v_scales = _vec4(k_scales), _vec4(v_scales)
-    _lib.call("paged_kv_read", k, v, _lib.vec16(k_cache), _lib.vec16(v_cache), block_tables, context_lens, cu_seqlens,
-              k_scales, v_scales)
+    _, k_cache, v_cache, k_scales, v_scales = _fp4_aligned(None, k_cache, v_cache, k_scales, v_scales)
+    _lib.call("paged_kv_read", k, v, k_cache, v_cache, block_tables, context_lens, cu_seqlens, k_scales, v_scales)
     return k, v
