@@ -413,9 +413,10 @@ hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
 template <typename T, int D>
 hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
   constexpr int BN = 32;
-  if (nseq <= 0 || max_len <= 0) {
-    zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu,
-                                                                             a.cu64, a.nseq, a.T);
+  if (nseq <= 0 || max_len <= 0 || a.tab.num_blocks == 0) {
+    // (without a block to read every row is zero: those of no sequence are all of them)
+    zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(
+        a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu, a.cu64, a.tab.num_blocks == 0 ? 0 : a.nseq, a.T);
     return hipGetLastError();
   }
   // (the grids of the 16-bit caches, launch_prefill_t)

@@ -732,19 +732,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       *reinterpret_cast<uint4*>(&vs[buf][row * LDV + 8 * ch]) = vd[i];
     }
   };
-  // (kFp4) this thread's codes and scale of a row of keys or values
+  // (kFp4) this thread's codes and scale of a row of keys or values, and whether its
+  // 16-row group has keys (the wave's rows lie in one group)
   struct Codes {
     uint32_t w[QW], s;
+    bool named;
   };
   typedef std::conditional_t<Q4, Codes, uint4> Reg;
   constexpr int NREG = Q4 ? 1 : NLD;
+  const uint32_t qrow = (uint32_t)tid / QL8 & 15u, qch = (uint32_t)tid % QL8;
+  const uint32_t qko = qrow * kst + qch * (QE / 2), qvo = qrow * vst + qch * (QE / 2);
   auto load = [&](int t, Reg* kd, Reg* vd) __attribute__((always_inline)) {
     if constexpr (Q4) {
+      // Scalar bases and one offset per lane (descriptors of four tensors leave too few
+      // scalar registers: four chunks of up to 2,048 tokens over up to 16,384 keys took
+      // 1,154 us with them, 1,171 with addresses on the vector side, 1,083 so).  Rows past
+      // the range are read as the last one in it, a group without keys from block 0,
+      // whose codes and scales store() clears.
       uint32_t nlo[NG], nhi[NG], nsl[NG];
       bool nin[NG];
       load_ids(t + 1, nlo, nhi, nin, nsl);
-      // a wave's rows lie in one 16-row group
-      const uint32_t row = (uint32_t)tid / QL8, ch = (uint32_t)tid % QL8;
       static_assert(64 / QL8 <= 16, "a wave's rows");
       const int gu = w * (64 / QL8) / 16;
       uint32_t ulo = idlo[0], uhi = idhi[0], usl = slots[0];
@@ -754,36 +761,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         if (gu == g) ulo = idlo[g], uhi = idhi[g], usl = slots[g], uin = idin[g];
       const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)ulo);
       const uint32_t hi = T64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int32_t)uhi) : 0u;
-      const bool valid = uin && hi == 0u && lo < nblk;
-      const uint64_t bb = valid ? lo : 0u;
       const uint32_t j0 = (uint32_t)t * BN + 16u * gu;
-      const uint32_t ends = usl + (j0 < kend32 ? (kend32 - j0 < 16u ? kend32 - j0 : 16u) : 0u);
-      const __amdgpu_buffer_rsrc_t rk =
-          __builtin_amdgcn_make_buffer_rsrc((void*)(kbase + bb * ksb), 0, valid ? ends * kst : 0u, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rv =
-          __builtin_amdgcn_make_buffer_rsrc((void*)(vbase + bb * vsb), 0, valid ? ends * vst : 0u, 0x00020000);
-      // (the scales of rows past the range may be stale: they are read past the
-      // descriptor's end, as 0, or a NaN among them would reach the sums by 0 codes)
-      const uint32_t slot = usl + (row & 15), far = slot < ends ? 0u : 0x80000000u;
-      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(a.ks.base + bb * (uint32_t)a.ks.sb + kvh * a.ks.sh), 0, valid ? D / 32 * (uint32_t)a.ks.sd : 0u, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(a.vs.base + bb * (uint32_t)a.vs.sb + kvh * a.vs.sh), 0, valid ? D / 32 * (uint32_t)a.vs.sd : 0u, 0x00020000);
-      auto codes = [&](__amdgpu_buffer_rsrc_t r, uint32_t o, Codes& c) __attribute__((always_inline)) {
+      const bool named = uin && hi == 0u && lo < nblk;  // (uin: keys of the group lie in the range)
+      const uint64_t bb = named ? lo : 0u;
+      uint32_t ko = qko, vo = qvo, row = qrow;
+      if (named && kend32 - j0 < 16u) {
+        const uint32_t last = kend32 - j0 - 1u;
+        row = qrow < last ? qrow : last;
+        ko = row * kst + qch * (QE / 2), vo = row * vst + qch * (QE / 2);
+      }
+      uint32_t kso = qch * QE / 32 * (uint32_t)a.ks.sd + row, vso = qch * QE / 32 * (uint32_t)a.vs.sd + row;
+      asm("" : "+v"(ko), "+v"(vo), "+v"(kso), "+v"(vso));
+      const char* const kp = kbase + bb * ksb + (uint64_t)(usl * kst);
+      const char* const vp = vbase + bb * vsb + (uint64_t)(usl * vst);
+      const uint8_t* const ksp = a.ks.base + kvh * a.ks.sh + bb * (uint32_t)a.ks.sb + usl;
+      const uint8_t* const vsp = a.vs.base + kvh * a.vs.sh + bb * (uint32_t)a.vs.sb + usl;
+      auto codes = [](const char* p, Codes& c) __attribute__((always_inline)) {
         if constexpr (QW == 4) {
-          const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0));
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
           c.w[0] = x.x, c.w[1] = x.y, c.w[2] = x.z, c.w[3] = x.w;
         } else if constexpr (QW == 2) {
-          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
           c.w[0] = x.x, c.w[1] = x.y;
         } else {
-          c.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+          c.w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
       };
-      codes(rk, slot * kst + ch * (QE / 2), kd[0]);
-      codes(rv, slot * vst + ch * (QE / 2), vd[0]);
-      kd[0].s = __builtin_amdgcn_raw_buffer_load_b8(rks, (ch * QE / 32 * (uint32_t)a.ks.sd + slot) | far, 0, 0);
-      vd[0].s = __builtin_amdgcn_raw_buffer_load_b8(rvs, (ch * QE / 32 * (uint32_t)a.vs.sd + slot) | far, 0, 0);
+      codes(kp + ko, kd[0]);
+      codes(vp + vo, vd[0]);
+      kd[0].s = ksp[kso];
+      vd[0].s = vsp[vso];
+      kd[0].named = vd[0].named = named;
 #pragma unroll
       for (int g = 0; g < NG; ++g) idlo[g] = nlo[g], idhi[g] = nhi[g], idin[g] = nin[g], slots[g] = nsl[g];
     } else {
@@ -797,10 +805,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       // 16-byte stores, QE elements apart, fall on different banks
       const int turn = QW == 4 ? (ch + (ch >> 2)) & 3 : QW == 2 ? ch >> 2 & 1 : 0;
       auto put = [&](T* at, const Codes& c) __attribute__((always_inline)) {
-        const float s = fp4_scale(c.s);
-        uint32_t x[QW];
+        uint32_t x[QW], sb = c.s;
 #pragma unroll
         for (int i = 0; i < QW; ++i) x[i] = c.w[i];
+        if (!c.named) {
+          sb = 0u;
+#pragma unroll
+          for (int i = 0; i < QW; ++i) x[i] = 0u;
+        }
+        const float s = fp4_scale(sb);
         if constexpr (QW >= 2) {  // x[i] <- word (i ^ turn)
 #pragma unroll
           for (int i = 0; i < QW; i += 2) {
