@@ -553,6 +553,19 @@ int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, 
                                 int64_t max_seqlen, float scale, void* stream);
 
 /*
+ * paged_attention_prefill_fp4 for a few tokens of each sequence (at most max_seqlen, at
+ * least 1), by the decode's kernel: the query heads of all of a sequence's tokens
+ * share its reads of the keys.  workspace: 1-D fp32, 16-byte aligned, of
+ * paged_attention_decode_workspace_size(N, max_seqlen * Hq, D, num_splits) elements,
+ * overwritten; num_splits from 2 to 256 as for paged_attention_decode.  Rows of tokens
+ * past max_seqlen are not written.
+ */
+int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                            const gdn_tensor* k_scales, const gdn_tensor* v_scales, const gdn_tensor* block_tables,
+                            const gdn_tensor* context_lens, const gdn_tensor* cu_seqlens, gdn_tensor* out,
+                            gdn_tensor* workspace, int32_t num_splits, int64_t max_seqlen, float scale, void* stream);
+
+/*
  * Copies of blocks inside caches (no counterpart in the reference): in every layer of
  * each cache (layers, blocks, elements of a block), any type, block dst[i] <- block
  * src[i].  Up to four caches (NULL: none) of one number of blocks.

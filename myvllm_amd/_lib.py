@@ -70,6 +70,7 @@ EXPORTED_SYMBOLS = (
     "paged_attention_decode_fp4",
     "paged_attention_prefill_fp4",
     "cache_copy",
+    "paged_attention_few_fp4",
     "gdn_hbm_copy",
     "gdn_strerror",
     "gdn_abi_version",
@@ -188,6 +189,7 @@ def load() -> ctypes.CDLL:
             ("paged_attention_decode_fp4", [_PT] * 9 + [I, F, P]),
             ("paged_attention_prefill_fp4", [_PT] * 10 + [L, F, P]),
             ("cache_copy", [_PT] * 5 + [P]),
+            ("paged_attention_few_fp4", [_PT] * 10 + [I, L, F, P]),
         ):
             getattr(lib, fn).restype, getattr(lib, fn).argtypes = ctypes.c_int, types
         lib.paged_attention_decode_shared_workspace_size.restype = L

@@ -459,15 +459,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 // there, its row was written by that unit.  The pieces are taken 64 at a time, lane i
 // reading piece i's maximum and row sum, so their loads are in flight
 // together; the running maximum carries over between groups of 64.
+// `row` of the `rows` that a slot holds, to `op`.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArgs a) {
-  const int64_t bh = blockIdx.x;  // b * Hq + head
-  const int64_t b = bh / a.Hq;
-  const int head = (int)(bh % a.Hq);
+GDN_DEVICE void decode_combine(const DecodeArgs& a, int64_t b, int row, int rows, T* op) {
   const int lane = threadIdx.x;
   constexpr int PS = D + 4;
   constexpr int E = D / 64;
-  T* op = reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)head * a.o_sh + E * lane;
+  op += E * lane;
   const int64_t U = (int64_t)a.B * a.units;
   const int64_t Pt = load_index_scalar(a.prices, a.B, false), qb = load_index_scalar(a.prices, b, false),
                 qn = load_index_scalar(a.prices, b + 1, false);
@@ -478,8 +476,8 @@ __global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArg
     const int64_t u0 = floor_div((qb + a.start + 1) * U - 1, Pt, inv), u1 = floor_div(qn * U - 1, Pt, inv);
     if (u0 == u1) return;  // one unit held the whole sequence and wrote its row
     const bool all_units = Pt >= U;  // every unit has a price range
-    const float* base = a.part + ((b + u0) * a.Hq + head) * (int64_t)PS;
-    const int64_t rs = (int64_t)a.Hq * PS;  // one slot further
+    const float* base = a.part + ((b + u0) * rows + row) * (int64_t)PS;
+    const int64_t rs = (int64_t)rows * PS;  // one slot further
     float mx = -INFINITY;
     for (int64_t c0 = 0; c0 <= u1 - u0; c0 += 64) {
       const int64_t i = c0 + lane, u = u0 + i;
@@ -525,6 +523,14 @@ __global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArg
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) op[e] = (T)(acc[e] * inv);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attn_decode_combine_kernel(const DecodeArgs a) {
+  const int64_t bh = blockIdx.x;  // b * Hq + head
+  const int64_t b = bh / a.Hq;
+  const int head = (int)(bh % a.Hq);
+  decode_combine<T, D>(a, b, head, a.Hq, reinterpret_cast<T*>(a.o) + b * a.o_ss + (int64_t)head * a.o_sh);
 }
 
 template <typename T, int D, AttnForm FORM = kPlain>

@@ -16,6 +16,11 @@ struct Fp4DecodeArgs : DecodeArgs {
   ScaleSource ks, vs;
   uint32_t page_inv;  // floor((2^32 - 1) / 16-key groups of a page)
   int32_t R, hgroups;  // query heads of a kv head, and their groups of 16
+  // FEW: tokens of the sequences (offsets, their end, the most of one), and a slot's rows
+  const void* cu;
+  bool cu64;
+  int64_t T;
+  int32_t most, rows;
 };
 
 // Decode: a workgroup is four waves, of 4 / KS kv heads (and up to 16 query heads of
@@ -30,7 +35,9 @@ struct Fp4DecodeArgs : DecodeArgs {
 // bits, and byte permutes pair them by keys.
 //
 // ONE: pages of 16 keys, so a 16-key group is a page and starts at its slot 0.
-template <typename T, int D, int KS, bool ONE>
+// FEW: a few tokens of each sequence instead of one: the columns are the query heads
+// of one token after the other, each with its own last key.
+template <typename T, int D, int KS, bool ONE, bool FEW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_fp4_kernel(
     const Fp4DecodeArgs a) {
   typedef Mma<T> M;
@@ -52,8 +59,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int R = a.R, hgroups = a.hgroups, y = hgroups == 1 ? blockIdx.y : blockIdx.y / hgroups;
   const int kvh = y * (4 / KS) + wv / KS;
   const int h0 = ((int)blockIdx.y - y * hgroups) * 16;
-  const bool hvalid = h0 + c16 < R;
-  const int head = kvh * R + (hvalid ? h0 + c16 : 0);
+  // this lane's column: query head cr of the kv head, token ci
+  const int ci = FEW ? (int)((uint32_t)(h0 + c16) / (uint32_t)R) : 0, cr = h0 + c16 - ci * R;
   const char* const kbase = a.k.base + kvh * a.k.sh;
   const char* const vbase = a.v.base + kvh * a.v.sh;
   const uint8_t* const ksbase = a.ks.base + kvh * a.ks.sh;
@@ -62,7 +69,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const uint64_t kssb = (uint32_t)a.ks.sb, vssb = (uint32_t)a.vs.sb;
   const uint32_t kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st, ksd = (uint32_t)a.ks.sd, vsd = (uint32_t)a.vs.sd;
   const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
-  const uint32_t qkeep = hvalid && a.c != 0.f ? ~0u : 0u, qsign = a.c < 0.f ? 0x80008000u : 0u;
+  const uint32_t qsign = a.c < 0.f ? 0x80008000u : 0u;
   const uint32_t gpp = (uint32_t)a.tab.page / 16u, nblk = (uint32_t)a.tab.num_blocks;  // (below 2^31)
 
   struct Tile {
@@ -83,19 +90,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     // vector loads: descriptors made of it would be looped over)
     const int32_t b = __builtin_amdgcn_readfirstlane((int32_t)b_), slot = __builtin_amdgcn_readfirstlane((int32_t)slot_);
     const uint32_t k_lo = __builtin_amdgcn_readfirstlane((int32_t)lo_), k_hi = __builtin_amdgcn_readfirstlane((int32_t)hi_);
+    // columns of the sequence, its first row of q and out, the keys that this lane's
+    // column sees, and those that all of the group's see
+    int cols = R;
+    int64_t row0 = b;
+    uint32_t lim = k_hi, lim0 = k_hi;
+    if constexpr (FEW) {
+      int64_t s0, s1;
+      seq_range(a.cu, a.cu64, b, a.T, s0, s1);
+      const int len = __builtin_amdgcn_readfirstlane((int32_t)(s1 - s0 < a.most ? s1 - s0 : a.most));
+      cols = len * R;
+      if (cols <= h0) return;
+      row0 = s0;
+      const int64_t off = load_index(a.ctx, b, a.ctx64) - (s1 - s0) + 1;  // keys that token 0 sees
+      lim = (uint32_t)clamp64(off + ci, 0, k_hi);
+      lim0 = __builtin_amdgcn_readfirstlane((int32_t)clamp64(off + (int)((uint32_t)h0 / (uint32_t)R), 0, k_hi));
+    }
+    const bool hvalid = h0 + c16 < cols;
+    const uint32_t qkeep = hvalid && a.c != 0.f ? ~0u : 0u;
+    // column h of the group: its row in a slot, and in out
+    const int rows = FEW ? a.rows : a.Hq;
+    auto slot_row = [&](int h) __attribute__((always_inline)) {
+      const int i = FEW ? (int)((uint32_t)(h0 + h) / (uint32_t)R) : 0;
+      return i * a.Hq + kvh * R + h0 + h - i * R;
+    };
+    auto out_row = [&](int h) __attribute__((always_inline)) {
+      const int i = FEW ? (int)((uint32_t)(h0 + h) / (uint32_t)R) : 0;
+      return reinterpret_cast<T*>(a.o) + (row0 + i) * a.o_ss + (int64_t)(kvh * R + h0 + h - i * R) * a.o_sh;
+    };
     if (k_hi == 0) {  // no keys: zero rows (and no table column that could be read)
       constexpr int LR = D / 4;
-      const int hd0 = kvh * R + h0;
       for (int h = part * (16 / KS) + lane / LR; h < (part + 1) * (16 / KS); h += 64 / LR)
-        if (h0 + h < R)
-          *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)(hd0 + h) * a.o_sh +
-                                 4 * (lane % LR)) = v4{};
+        if (h0 + h < cols) *reinterpret_cast<v4*>(out_row(h) + 4 * (lane % LR)) = v4{};
       return;
     }
     const int ntiles = (int)((k_hi - k_lo + 31) / 32);
     v8 qf[NI][NQ];
     {
-      const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.q_ss + (int64_t)head * a.q_sh;
+      const T* qp = reinterpret_cast<const T*>(a.q) + (row0 + (hvalid ? ci : 0)) * a.q_ss +
+                    (int64_t)(kvh * R + (hvalid ? cr : 0)) * a.q_sh;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -214,15 +247,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
       const uint32_t j0 = k_lo + 32u * (uint32_t)t;
       uint32_t vs[2] = {x.vs[0], x.vs[1]};
-      if (j0 + 32u > k_hi) {
+      if (j0 + 32u > lim0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (j0 + 16u * h + 4u * grp + r >= k_hi) {
-              s[h][r] = -INFINITY;
-              vs[h] &= ~(255u << (8 * r));  // (a stale scale may stand for NaN)
-            }
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t j = j0 + 16u * h + 4u * grp + r;
+            if (j >= lim) s[h][r] = -INFINITY;
+            if (j >= k_hi) vs[h] &= ~(255u << (8 * r));  // (a stale scale may stand for NaN)
+          }
       }
       float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
       mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -307,8 +340,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     if constexpr (KS == 1) {
       if (!hvalid) return;
       const float inv = lt > 0.f ? 1.f / lt : 0.f;
-      float* const pp = a.part + ((int64_t)slot * a.Hq + head) * (D + 4);
-      T* const op = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)head * a.o_sh;
+      float* const pp = a.part + ((int64_t)slot * rows + slot_row(c16)) * (D + 4);
+      T* const op = out_row(c16);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -346,20 +379,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
         for (int j = 0; j < VE; j += 4)
           *reinterpret_cast<f32x4*>(mine + VE * (4 * grp + r) + j) =
               f32x4{oacc[j][r] * f, oacc[j + 1][r] * f, oacc[j + 2][r] * f, oacc[j + 3][r] * f};
-      float* const pp = a.part + ((int64_t)slot * a.Hq + kvh * R + h0) * (D + 4);
+      float* const pp = a.part + (int64_t)slot * rows * (D + 4);
       if (slot >= 0 && part == 0 && grp == 0 && hvalid) {
-        pp[c16 * (D + 4) + D] = mt;
-        pp[c16 * (D + 4) + D + 1] = l;
+        float* const mp = pp + (int64_t)slot_row(c16) * (D + 4) + D;
+        mp[0] = mt;
+        mp[1] = l;
       }
       __syncthreads();
       constexpr int LR = D / 4;    // lanes per row
       constexpr int RW = 16 / KS;  // rows per wave
       static_assert(LR <= 64 && RW % (64 / LR) == 0, "rows of a wave");
-      T* const op = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_ss + (int64_t)(kvh * R + h0) * a.o_sh;
 #pragma unroll 1
       for (int i = 0; i < RW / (64 / LR); ++i) {
         const int h = part * RW + i * (64 / LR) + lane / LR, d = 4 * (lane % LR);
-        if (h0 + h >= R) break;
+        if (h0 + h >= cols) break;
         f32x4 o = *reinterpret_cast<const f32x4*>(ob + (w0 * 16 + h) * LDO + d);
 #pragma unroll
         for (int p = 1; p < KS; ++p) {
@@ -367,8 +400,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] += y[e];
         }
-        if (slot < 0) *reinterpret_cast<v4*>(op + (int64_t)h * a.o_sh + d) = v4{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
-        else *reinterpret_cast<f32x4*>(pp + h * (D + 4) + d) = o;
+        if (slot < 0) *reinterpret_cast<v4*>(out_row(h) + d) = v4{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
+        else *reinterpret_cast<f32x4*>(pp + (int64_t)slot_row(h) * (D + 4) + d) = o;
       }
     }
   };
@@ -384,16 +417,36 @@ int fp4_heads(int Hkv, int D) {
   return n;
 }
 
-template <typename T, int D, bool ONE>
-void launch_decode_fp4_waves(const Fp4DecodeArgs& a, int heads, dim3 grid, hipStream_t st) {
-  if constexpr (D < 256) {
-    if (heads == 4) return attn_decode_fp4_kernel<T, D, 1, ONE><<<grid, dim3(256), 0, st>>>(a);
-    if (heads == 2) return attn_decode_fp4_kernel<T, D, 2, ONE><<<grid, dim3(256), 0, st>>>(a);
+// Merge of the pieces of one token and query head, and (the last kZeroBlocks
+// workgroups) the rows of out that no sequence covers, which are zero.
+constexpr int kZeroBlocks = 16;
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attn_few_combine_kernel(const Fp4DecodeArgs a) {
+  const int64_t all = (int64_t)a.B * a.rows, id = blockIdx.x;
+  if (id >= all) {
+    zero_uncovered_rows<(int)sizeof(T)>(a.o, a.o_ss, a.o_sh, a.Hq, D, a.cu, a.cu64, a.B, a.T, id - all, kZeroBlocks,
+                                        threadIdx.x, 64);
+    return;
   }
-  attn_decode_fp4_kernel<T, D, 4, ONE><<<grid, dim3(256), 0, st>>>(a);
+  const int64_t b = id / a.rows;
+  const int row = (int)(id - b * a.rows), i = row / a.Hq;
+  int64_t s0, s1;
+  seq_range(a.cu, a.cu64, b, a.T, s0, s1);
+  if (i >= s1 - s0) return;
+  decode_combine<T, D>(a, b, row, a.rows,
+                       reinterpret_cast<T*>(a.o) + (s0 + i) * a.o_ss + (int64_t)(row - i * a.Hq) * a.o_sh);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool ONE, bool FEW>
+void launch_decode_fp4_waves(const Fp4DecodeArgs& a, int heads, dim3 grid, hipStream_t st) {
+  if constexpr (D < 256) {
+    if (heads == 4) return attn_decode_fp4_kernel<T, D, 1, ONE, FEW><<<grid, dim3(256), 0, st>>>(a);
+    if (heads == 2) return attn_decode_fp4_kernel<T, D, 2, ONE, FEW><<<grid, dim3(256), 0, st>>>(a);
+  }
+  attn_decode_fp4_kernel<T, D, 4, ONE, FEW><<<grid, dim3(256), 0, st>>>(a);
+}
+
+template <typename T, int D, bool FEW>
 hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
   const int heads = fp4_heads(a.Hkv, D), hgroups = a.hgroups;
   const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / heads * hgroups), (unsigned)a.B);
@@ -402,11 +455,14 @@ hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (a.tab.page == 16) launch_decode_fp4_waves<T, D, true>(a, heads, grid, st);
-  else launch_decode_fp4_waves<T, D, false>(a, heads, grid, st);
+  if (a.tab.page == 16) launch_decode_fp4_waves<T, D, true, FEW>(a, heads, grid, st);
+  else launch_decode_fp4_waves<T, D, false, FEW>(a, heads, grid, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  attn_decode_combine_kernel<T, D><<<dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st>>>(a);
+  if constexpr (FEW)
+    attn_few_combine_kernel<T, D><<<dim3((unsigned)((int64_t)a.B * a.rows + kZeroBlocks)), dim3(64), 0, st>>>(a);
+  else
+    attn_decode_combine_kernel<T, D><<<dim3((unsigned)((int64_t)a.B * a.Hq)), dim3(64), 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -442,13 +498,20 @@ hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_le
 
 int32_t attn_fp4_start_price() { return kFp4StartPrice; }
 
-hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
-                                  const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
-                                  const gdn_tensor* ctx, gdn_tensor* out, float* workspace, int32_t splits, float scale,
-                                  hipStream_t st) {
-  if (q->shape[0] == 0) return hipSuccess;
-  Fp4DecodeArgs a{};
-  static_cast<DecodeArgs&>(a) = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
+namespace {
+template <bool FEW>
+hipError_t decode_fp4(const Fp4DecodeArgs& a, int dtype, int D, hipStream_t st) {
+  if (dtype == GDN_DTYPE_BF16) {
+    if (D == 64) return launch_decode_fp4<bf16_t, 64, FEW>(a, st);
+    if (D == 128) return launch_decode_fp4<bf16_t, 128, FEW>(a, st);
+    return launch_decode_fp4<bf16_t, 256, FEW>(a, st);
+  }
+  if (D == 64) return launch_decode_fp4<f16_t, 64, FEW>(a, st);
+  if (D == 128) return launch_decode_fp4<f16_t, 128, FEW>(a, st);
+  return launch_decode_fp4<f16_t, 256, FEW>(a, st);
+}
+
+void set_fp4(Fp4DecodeArgs& a, const gdn_tensor* ks, const gdn_tensor* vs) {
   a.ks = scale_source(ks);
   a.vs = scale_source(vs);
   a.start = kFp4StartPrice;
@@ -456,15 +519,42 @@ hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, con
   a.hgroups = (a.R + 15) / 16;
   a.page_inv = 0xFFFFFFFFu / (uint32_t)(a.tab.page / 16);
   if (a.tab.num_blocks == 0) a.tab.cols = 0;  // (no page to read: lengths end at 0 keys)
-  const int D = (int)q->shape[2];
-  if (q->dtype == GDN_DTYPE_BF16) {
-    if (D == 64) return launch_decode_fp4<bf16_t, 64>(a, st);
-    if (D == 128) return launch_decode_fp4<bf16_t, 128>(a, st);
-    return launch_decode_fp4<bf16_t, 256>(a, st);
-  }
-  if (D == 64) return launch_decode_fp4<f16_t, 64>(a, st);
-  if (D == 128) return launch_decode_fp4<f16_t, 128>(a, st);
-  return launch_decode_fp4<f16_t, 256>(a, st);
+}
+}  // namespace
+
+hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
+                                  const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
+                                  const gdn_tensor* ctx, gdn_tensor* out, float* workspace, int32_t splits, float scale,
+                                  hipStream_t st) {
+  if (q->shape[0] == 0) return hipSuccess;
+  Fp4DecodeArgs a{};
+  static_cast<DecodeArgs&>(a) = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
+  set_fp4(a, ks, vs);
+  return decode_fp4<false>(a, q->dtype, (int)q->shape[2], st);
+}
+
+// A few tokens (at most `most`) of each sequence by the decode's kernel, split
+// (splits >= 2).
+hipError_t attn_few_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* ks,
+                               const gdn_tensor* vs, const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* cu,
+                               gdn_tensor* out, float* workspace, int32_t splits, int32_t most, float scale,
+                               hipStream_t st) {
+  if (q->shape[0] == 0) return hipSuccess;
+  Fp4DecodeArgs a{};
+  static_cast<DecodeArgs&>(a) = decode_args(q, kc, vc, tab, ctx, out, workspace, splits, scale);
+  // (those count q's rows as sequences)
+  a.B = (int32_t)tab->shape[0];
+  a.rows = most * a.Hq;
+  a.unit_inv = 1.0 / ((double)a.B * a.units);
+  a.prices = reinterpret_cast<int32_t*>(workspace + (int64_t)a.B * splits * a.rows * (q->shape[2] + 4));
+  a.prices_inline = a.B <= 1024;
+  set_fp4(a, ks, vs);
+  a.hgroups = (int32_t)((most * a.R + 15) / 16);
+  a.cu = cu->data;
+  a.cu64 = cu->dtype == GDN_DTYPE_I64;
+  a.T = q->shape[0];
+  a.most = most;
+  return decode_fp4<true>(a, q->dtype, (int)q->shape[2], st);
 }
 
 hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,

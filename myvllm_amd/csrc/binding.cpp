@@ -202,6 +202,7 @@ typedef Entry<25, 9> KvRead;
 typedef Entry<26, 9, int32_t, float> PagedDecodeFp4;
 typedef Entry<27, 10, int64_t, float> PagedPrefillFp4;
 typedef Entry<28, 5> CacheCopy;
+typedef Entry<29, 10, int32_t, int64_t, float> PagedFewFp4;
 
 // Whole numbers of a list or tuple; false if it is another object or one does not fit.
 bool ids_of(PyObject* o, std::vector<int32_t>& out) {
@@ -325,6 +326,7 @@ const Bound kBound[] = {
     GDN_BOUND("paged_attention_decode_fp4", PagedDecodeFp4),
     GDN_BOUND("paged_attention_prefill_fp4", PagedPrefillFp4),
     GDN_BOUND("cache_copy", CacheCopy),
+    GDN_BOUND("paged_attention_few_fp4", PagedFewFp4),
     GDN_BOUND("paged_attention_decode_shared_workspace_size", PagedDecodeSharedSize),
     GDN_BOUND("gdn_chunk_prefill_workspace_size", ChunkPrefillSize),
     GDN_BOUND("paged_attention_prefill_workspace_size", PagedPrefillSize),

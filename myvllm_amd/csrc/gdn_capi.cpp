@@ -93,6 +93,10 @@ hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, co
                                    const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
                                    const gdn_tensor* ctx, const gdn_tensor* cu, gdn_tensor* out, float* workspace,
                                    int64_t max_seqlen, float scale, hipStream_t st);
+hipError_t attn_few_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* ks,
+                               const gdn_tensor* vs, const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* cu,
+                               gdn_tensor* out, float* workspace, int32_t splits, int32_t most, float scale,
+                               hipStream_t st);
 bool cache_copy_fits(gdn_tensor* const* t, const int64_t* es, int n, int64_t vec);
 hipError_t cache_copy_launch(gdn_tensor* const* t, const int64_t* es, int n, const int32_t* src, const int32_t* dst,
                              int64_t count, int64_t vec, hipStream_t st);
@@ -1083,6 +1087,30 @@ GDN_EXPORT int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor
   return launch_rc(attn_prefill_fp4_launch(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens,
                                            cu_seqlens, out, ws, max_seqlen, scale,
                                            reinterpret_cast<hipStream_t>(stream)));
+}
+
+GDN_EXPORT int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
+                                       const gdn_tensor* k_scales, const gdn_tensor* v_scales,
+                                       const gdn_tensor* block_tables, const gdn_tensor* context_lens,
+                                       const gdn_tensor* cu_seqlens, gdn_tensor* out, gdn_tensor* workspace,
+                                       int32_t num_splits, int64_t max_seqlen, float scale, void* stream) {
+  float* ws;
+  GDN_TRY(check_paged_prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, nullptr, max_seqlen,
+                              &ws, true));
+  GDN_TRY(check_scales(k_cache, v_cache, k_scales, v_scales, block_tables));
+  const int64_t N = block_tables->shape[0], Hq = q->shape[1], Hkv = k_cache->shape[2];
+  if (N < 1 || max_seqlen < 1) return GDN_ERR_SHAPE;
+  if (num_splits < 2 || num_splits > kMaxDecodeSplits) return GDN_ERR_RANGE;
+  // rows of the merge, groups of 16 columns and prices are counted in 31 bits
+  if (max_seqlen > kMaxGrid / Hq || N > (kMaxGrid - 64) / (max_seqlen * Hq) ||
+      Hkv * ((max_seqlen * (Hq / Hkv) + 15) / 16) > kMaxGridYZ ||
+      N * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + attn_fp4_start_price()) >= (int64_t(1) << 31))
+    return GDN_ERR_RANGE;
+  GDN_TRY(decode_workspace(workspace, paged_attention_decode_workspace_size(N, max_seqlen * Hq, q->shape[2], num_splits),
+                           num_splits, N, &ws));
+  return launch_rc(attn_few_fp4_launch(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens,
+                                       out, ws, num_splits, (int32_t)max_seqlen, scale,
+                                       reinterpret_cast<hipStream_t>(stream)));
 }
 
 namespace {

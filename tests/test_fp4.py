@@ -165,6 +165,27 @@ def test_attention_refused_sizes():
 
 
 @cpu_only
+def test_few_refusals():
+    def code(splits=2, most=3, ws=True, **change):
+        a = attention_args()
+        a.update(change)
+        n = _lib.workspace_size("paged_attention_decode_workspace_size", 2, max(most, 0) * 4, 128, splits)
+        a["ws"] = Z(n) if ws else None
+        return code_of("paged_attention_few_fp4", a.values(), splits, ctypes.c_int64(most), ctypes.c_float(1.0))
+
+    for change, want in SCALE_REFUSALS:
+        assert code(**change) == ERR[want], change
+    assert code(ws=False) == ERR["NULL"]
+    assert code(splits=1) == code(splits=257) == ERR["RANGE"]
+    assert code(most=0) == code(most=-1) == ERR["SHAPE"]
+    assert code(cu=Z(1, dtype=I32), tab=Z(0, 3, dtype=I32), ctx=Z(0, dtype=I32)) == ERR["SHAPE"]
+    a = attention_args()
+    a["ws"] = Z(8)
+    assert code_of("paged_attention_few_fp4", a.values(), 2, ctypes.c_int64(3), ctypes.c_float(1.0)) == ERR["SHAPE"]
+    assert code_of("paged_attention_few_fp4", a.values(), 2, ctypes.c_int64(2**30), ctypes.c_float(1.0)) == ERR["RANGE"]
+
+
+@cpu_only
 def test_read_refusals():
     def code(scales=True, **change):
         a = append_args()

@@ -205,6 +205,103 @@ def test_prefill_split(dev, Hq, Hkv, D, dtype):
     assert_within(o, ref, bound, "unsplit")
 
 
+def is_few(c, most):
+    from myvllm_amd.full_attention import _few_tokens
+
+    return _few_tokens(c["q"], c["kc"], c["tab"], most)
+
+
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", HEADS)
+@pytest.mark.parametrize("page, index", [(16, torch.int32), (48, torch.int64)])
+def test_few_tokens_heads(dev, Hq, Hkv, D, dtype, page, index):
+    """A few tokens of each sequence, as the decode's columns: groups that end inside a
+    token, empty sequences, tokens that see one key and whole contexts of new tokens."""
+    print(f"fp4 few {Hq}/{Hkv}x{D} {dtype} page={page}", flush=True)
+    most = 64 // (Hq // Hkv)
+    new = [1, 0, most, min(3, most), min(2, most), most, 1, min(5, most)]
+    ctx = [1, 20, most, 3 + 40, 33, most + 700, 300, 64 + 5]
+    ctx = [max(c, n) for c, n in zip(ctx, new)]
+    c = make(ctx, new, Hq, Hkv, D, page, dtype, index, seed=Hq + D, cols=60)
+    assert is_few(c, most) and not is_few(c, most + 64)
+    ref, bound = reference(c, new, D**-0.5)
+    a = prefill(c, dev, D**-0.5)
+    assert_within(a, ref, bound)
+    assert torch.equal(a, prefill(c, dev, D**-0.5))
+    d = {n: t.to(dev) for n, t in c.items()}
+    for splits in (2, 3, 40, 256):
+        ws = torch.full((_lib.workspace_size("paged_attention_decode_workspace_size", len(new), most * Hq, D, splits),),
+                        float("nan"), device=dev)
+        o = torch.full_like(d["q"], 7.0)
+        _lib.call("paged_attention_few_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"], d["cu"],
+                  o, ws, splits, most, D**-0.5)
+        assert_within(o, ref, bound, f"splits {splits}")
+
+
+@pytest.mark.parametrize("Hq, Hkv, D", [(8, 2, 128), (16, 2, 256), (4, 4, 64)])
+def test_few_tokens_edges(dev, Hq, Hkv, D):
+    """Rows outside the offsets and before position 0 are zero; lengths past the table; foreign blocks; NaN."""
+    c = make([30, 20], [8, 7], Hq, Hkv, D, cols=4)
+    c["cu"] = torch.tensor([2, 5, 10], dtype=torch.int32)
+    o = prefill(c, dev, 0.1)
+    assert is_few(c, 5) and not o[:2].any() and not o[10:].any()
+    assert_within(o[2:10], *reference(dict(c, q=c["q"][2:10]), [3, 5], 0.1))
+    c = make([3, 0], [5, 4], Hq, Hkv, D)
+    o = prefill(c, dev, 0.1)
+    assert not o[:2].any() and not o[5:].any()
+    assert_within(o[2:5], *reference(dict(c, q=c["q"][2:5], ctx=c["ctx"][:1]), [3], 0.1))
+    c = make([60, 100], [3, 4], Hq, Hkv, D, cols=8)
+    c["tab"][0, 1], c["tab"][1, 0], c["tab"][1, 5] = 10**6, -1, c["kc"].shape[0]
+    assert_within(prefill(c, dev, 0.1), *reference(c, [3, 4], 0.1))
+    c["ks"][int(c["tab"][0, 2]), 0, 0, 4] = 255  # key 36 of the first sequence, kv head 0
+    o = prefill(c, dev, 0.1).cpu()
+    R = Hq // Hkv
+    assert o[:3, :R].isnan().all() and not o[:3, R:].isnan().any() and not o[3:].isnan().any()
+    full = make([200, 30], [2, 3], Hq, Hkv, D)
+    short = dict(full, tab=full["tab"][:, :2].contiguous())  # 32 keys of the 200: queries past them see them all
+    k, v = (cache_values(full[x + "c"], full[x + "s"])[full["tab"][0, :2].long()].flatten(0, 1) for x in "kv")
+    ref, bound = ref_and_bound(full["q"][:2], k, v, torch.tensor([198, 199]), 0.1, BF)
+    assert_within(prefill(short, dev, 0.1)[:2], ref, bound)
+
+
+def test_few_tokens_batches(dev):
+    """More sequences than the waves price by themselves; scales of either sign and zero; one graph's replays."""
+    g = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 4, (1100,), generator=g).tolist()
+    ctx = [n + int(x) for n, x in zip(new, torch.randint(0, 60, (1100,), generator=g))]
+    c = make(ctx, new, 4, 2, 128)
+    assert_within(prefill(c, dev, 0.1), *reference(c, new, 0.1))
+    c = make([40, 100, 1000], [2, 3, 1], 4, 2, 128)
+    for scale in (-0.1, 0.0, 2.0):
+        assert_within(prefill(c, dev, scale), *reference(c, [2, 3, 1], scale))
+    d = {n: t.to(dev) for n, t in c.items()}
+    step = lambda: ops.paged_flash_attention_prefill(  # noqa: E731
+        d["q"], d["kc"], d["vc"], d["tab"], d["ctx"], d["cu"], None, 0.1, 16, max_seqlen=3, k_scales=d["ks"], v_scales=d["vs"])
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        d["q"].copy_(torch.randn(d["q"].shape, generator=torch.Generator().manual_seed(i)).to(BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = held.clone()
+        assert torch.equal(got, step())
+
+
+def test_empty_cache(dev):
+    """No blocks at all: every row is zero."""
+    c = make([30, 20], [3, 1], 4, 2, 128)
+    for n in ("kc", "vc", "ks", "vs"):
+        c[n] = c[n][:0]
+    assert not prefill(c, dev, 0.1).any()
+    wide = make([300, 20], [290, 1], 4, 2, 128)
+    assert not prefill(dict(wide, **{n: c[n] for n in ("kc", "vc", "ks", "vs")}), dev, 0.1).any()
+    one = make([30, 20], [1, 1], 4, 2, 128)
+    for splits in (1, 3):
+        assert not decode(dict(one, **{n: c[n] for n in ("kc", "vc", "ks", "vs")}), dev, 0.1, splits).any()
+
+
 def test_prefill_uncovered_rows(dev):
     """Rows outside the offsets, and queries before position 0, are zero."""
     c = make([30, 20], [10, 20])
@@ -214,6 +311,7 @@ def test_prefill_uncovered_rows(dev):
     sub = dict(c, q=c["q"][2:25])
     assert_within(o[2:25], *reference(sub, [8, 15], 0.1))
     c = make([3, 0], [10, 20])
+    assert not is_few(c, 20)
     o = prefill(c, dev, 0.1).cpu()
     assert not o[:7].any() and not o[10:].any()
     sub = dict(c, q=c["q"][7:10], ctx=c["ctx"][:1])
