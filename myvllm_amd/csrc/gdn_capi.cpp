@@ -97,7 +97,7 @@ hipError_t attn_few_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const 
                                const gdn_tensor* vs, const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* cu,
                                gdn_tensor* out, float* workspace, int32_t splits, int32_t most, float scale,
                                hipStream_t st);
-bool cache_copy_fits(gdn_tensor* const* t, const int64_t* es, int n, int64_t vec);
+bool cache_copy_fits(gdn_tensor* const* t, const int64_t* es, int n, int64_t vec, int64_t count);
 hipError_t cache_copy_launch(gdn_tensor* const* t, const int64_t* es, int n, const int32_t* src, const int32_t* dst,
                              int64_t count, int64_t vec, hipStream_t st);
 hipError_t hbm_stream_copy_launch(const void* src, void* dst, int64_t nbytes, int32_t blocks, hipStream_t st);
@@ -1158,7 +1158,7 @@ GDN_EXPORT int cache_copy(gdn_tensor* cache0, gdn_tensor* cache1, gdn_tensor* ca
     t[n++] = c;
   }
   if (n == 0) return GDN_ERR_NULL;
-  if (!cache_copy_fits(t, es, n, vec)) return GDN_ERR_RANGE;
+  if (!cache_copy_fits(t, es, n, vec, pairs->shape[1])) return GDN_ERR_RANGE;
   const int32_t* src = reinterpret_cast<const int32_t*>(pairs->data);
   const int32_t* dst = src + pairs->stride[0];
   GDN_TRY(check_pairs(src, dst, pairs->shape[1], t[0]->shape[1]));
