@@ -794,8 +794,9 @@ int check_paged_decode(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn
   if (B > kMaxGridYZ || Hkv * ((R + 15) / 16) > kMaxGridYZ) return GDN_ERR_RANGE;
   // the split decode prices the batch (16-key tiles plus a start price per
   // sequence) in 32 bits
+  const int32_t start = codes ? attn_fp4_start_price() : attn_decode_start_price();
   if (num_splits > 1 &&
-      B * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + (codes ? attn_fp4_start_price() : attn_decode_start_price())) >= (int64_t(1) << 31))
+      B * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + start) >= (int64_t(1) << 31))
     return GDN_ERR_RANGE;
   // one page of one kv head is addressed with 32-bit byte offsets below 2^31
   const int64_t es = elem_size(k_cache->dtype);

@@ -75,13 +75,17 @@ GDN_DEVICE int64_t find_seq(const AppendArgs& a, int64_t t, int lane) {
   return lo < a.nseq ? lo : -1;
 }
 
-// A pair turned in fp64, rounded through fp32 to T.
+// A pair turned in fp64, rounded to fp32 and that to T (the compiler, which sees two
+// roundings in a row, would round to odd first: other results next to a tie, and ten
+// instructions more each).
 template <typename T> struct Pair {
   T a, b;
 };
 template <typename T> GDN_DEVICE Pair<T> turn_exactly(T a, T b, float c, float s) {
   const double x = (float)a, y = (float)b, cd = c, sd = s;
-  return {(T)(float)(x * cd - y * sd), (T)(float)(y * cd + x * sd)};
+  float p = (float)(x * cd - y * sd), q = (float)(y * cd + x * sd);
+  asm("" : "+v"(p), "+v"(q));
+  return {(T)p, (T)q};
 }
 
 template <typename T, int D, bool AXES = false, bool FP4 = false>
@@ -282,10 +286,10 @@ __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
     const int64_t h = key ? h2 : h2 - a.Hkv;
     x[i] = y[i] = uint4{0, 0, 0, 0};
     sc[i] = 0;
-    if (t >= a.T) continue;
+    if (t >= a.T || a.nseq == 0) continue;
     int64_t n = n0, pos = -1;
     if (a.cu) {
-      if (n < 0) n = 0;
+      if (n < 0) n = 0;  // (tokens before the first sequence)
       while (n < a.nseq - 1 && load_index(a.cu, n + 1, a.cu64) <= t) ++n;
       int64_t s, e;
       seq_range(a.cu, a.cu64, n, a.T, s, e);

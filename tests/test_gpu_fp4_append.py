@@ -211,6 +211,24 @@ def test_every_kind_of_number(dev, dtype):
     assert ref.abs().nan_to_num(0).max() <= info.max
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_keys_are_rounded_through_fp32(dev, dtype, inter):
+    """A sum 2^-30 below the middle of two 16-bit numbers is that middle in fp32, so the even one of
+    them: 1.75, the border between 1.5 and 2, which becomes 2.  Rounded once it would be the lower
+    one, and 1.5.  (Magnitudes up to 4 give the scale 1.)"""
+    D, rot = 64, 64
+    c = make([40], [0], Hq=1, Hkv=1, D=D, dtype=dtype)
+    middle = 1.75 - torch.finfo(dtype).eps / 2
+    cos, sin = torch.full((40, rot // 2), middle), torch.full((40, rot // 2), 2.0**-30)
+    a, b = (slice(0, D, 2), slice(1, D, 2)) if inter else (slice(0, D // 2), slice(D // 2, D))
+    c["k"][:, :, a], c["k"][:, :, b] = 1.0, 1.0
+    c["k"][::2, 0, 6] = 2.0
+    c["k"][::2, 0, 7 + (25 if not inter else 0)] = 2.0
+    c["k"][1::2] *= -1
+    check(c, dev, cos=cos, sin=sin, interleaved=inter)
+
+
 def test_strides_streams_and_in_place(dev):
     """Caches as slices of a cache of layers with wider rows; q turned where it lies; another stream."""
     c = make([40, 3], [5, 70], D=256, Hq=8, Hkv=2)
@@ -295,6 +313,14 @@ def test_read_edges(dev):
         assert torch.equal(k, d["k"]) and torch.equal(v, d["v"])
     k, v = ops.paged_kv_read(d["kc"], d["vc"], d["tab"][:0], d["ctx"][:0], 16)
     assert k.shape == (0, 2, 128)
+
+
+def test_read_of_no_sequences(dev):
+    """Offsets of an empty batch: every row is one that nobody wrote."""
+    c = {n: t.to(dev) for n, t in make([3], [20]).items()}
+    k, v = ops.paged_kv_read(c["kc"], c["vc"], c["tab"][:0], c["ctx"][:0], 16, num_tokens=5, cu_seqlens=c["cu"][:1],
+                             k_scales=c["ks"], v_scales=c["vs"])
+    assert k.shape == (5, 2, 128) and not k.any() and not v.any()
 
 
 def test_append_and_read_in_a_graph(dev):
