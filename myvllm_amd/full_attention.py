@@ -265,27 +265,41 @@ def _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales):
     return q, k_cache, v_cache, k_scales, v_scales
 
 
-def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int) -> int:
+def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int,
+                          few: bool = False) -> int:
     """:func:`decode_num_splits` of caches held in 4 bits, whose units are
     workgroups of four waves: one kv head of 256 dims, else four (two or one where
-    four do not divide the heads).  One workgroup per CU streams best (64 sequences
+    four do not divide the heads).
+
+    One workgroup per CU streams best where a tile holds enough bytes (64 sequences
     of U[1024, 8192] keys, 2 kv heads of 256: 256 workgroups 46.7 us, 384 52.6, 512
-    49.8; 256 of U[512, 16384], 4 of 128: 256 workgroups 210, 512 225), with at least
-    256 keys each (one sequence of 2,943 keys: 12 units 13.4 us, 8 14.8, 32 15.0).
-    A batch of 1,024 rows is not split (512 sequences of U[512, 4096] keys, 2 kv
-    heads of 256: 143 us, 155 split), one of 512 not where its sequences are short
-    (512 of U[200, 1000] keys, 4 of 128: 47.6 and 53.9; of U[512, 8192] 306 and
-    248)."""
+    49.8; 256 of U[512, 16384], 4 of 128: 256 workgroups 210, 512 225); heads of 64
+    dims want three (16 of U[1000, 8000], 16 heads: 256 workgroups 35.3, 768 28.8; 48
+    of U[300, 3000]: 47.6 and 32.5), and so do a few tokens a sequence (``few``),
+    whose shorter sequences leave some of their groups of columns empty (12 sequences
+    of 3 to 9 tokens over 6,000 keys, 16 heads of 64: 256 workgroups 32.8, 768 26.8; 32
+    of them, 16 / 4 of 128: 63.0 and 42.6).  At least 256 keys a unit (one sequence of
+    2,943 keys, 2 heads of 256: 12 units 13.4 us, 8 14.8, 32 15.0), of 128 dims or
+    fewer 128 (of 1,000 keys, 4 heads of 128: 4 units 15.8, 8 13.4); at most 64 a
+    sequence (one of 16,000 keys, 16 heads of 64: 64 units 18.8, 125 23.4), 32 of the
+    few (4 sequences, 16 / 4 of 128: 32 units 22.7, 47 25.7).
+
+    Not split: with heads of 256, batches of 1,024 rows (512 sequences of U[512, 4096]
+    keys, 2 kv heads: 143 us, 155 split) and of 512 short ones; else 2,048 rows, or 512
+    of up to 1,024 keys (512 sequences of U[200, 1000] keys, 4 of 128: 47.6 and
+    53.9; 1,024 rows of U[200, 2000], 16 of 64: 117.7 and 110.7)."""
     heads = 1 if head_dim > 128 else 4
     while num_kv_heads % heads:
         heads //= 2
     groups = max(num_kv_heads, 1) // heads * ((num_q_heads // max(num_kv_heads, 1) + 15) // 16)
     rows = max(1, num_seqs * groups)
-    if rows >= 1024 or (rows >= 512 and capacity <= 2048):
+    wide = head_dim > 128
+    if rows >= (1024 if wide else 2048) or (rows >= 512 and capacity <= (2048 if wide else 1024)):
         return 1
-    units = max(1, round(_FP4_TARGET_WORKGROUPS / rows))
-    by_keys = -(-max(capacity, 1) // _DECODE_MIN_SPLIT_KEYS)
-    return max(1, min(_DECODE_MAX_SPLITS, 1 + min(units, by_keys)))
+    target = 768 if head_dim <= 64 or (few and not wide) else _FP4_TARGET_WORKGROUPS
+    units = max(1, round(target / rows))
+    by_keys = -(-max(capacity, 1) // (256 if wide else 128))
+    return 1 + min(units, by_keys, 32 if few else 64)
 
 
 _FP4_TARGET_WORKGROUPS = 256
@@ -300,7 +314,9 @@ def _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_l
     n_ws = _lib.workspace_size("paged_attention_decode_workspace_size", B, Hq, Dh, int(num_splits))
     if n_ws > 0:
         ws = torch.empty(n_ws, dtype=torch.float32, device=dev)
-    o = _out_for(out, (B, Hq, Dh), q.dtype, dev)
+    # (empty_like takes 1.1 us, empty 1.6)
+    o = _out_for(out, q.shape, q.dtype, dev) if out is not None else \
+        torch.empty_like(q, memory_format=torch.contiguous_format)
     _lib.call("paged_attention_decode_fp4", *_fp4_aligned(q, k_cache, v_cache, k_scales, v_scales), block_tables,
               context_lens, o, ws, int(num_splits), float(scale))
     return _finish(out, o)
@@ -481,7 +497,7 @@ def _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, co
     if _few_tokens(q, k_cache, block_tables, int(max_seqlen)):
         N, most, cap = block_tables.shape[0], int(max_seqlen), block_tables.shape[1] * k_cache.shape[1]
         # (its groups of 16 columns are so many more workgroups)
-        splits = max(2, fp4_decode_num_splits(N, most * q.shape[1], k_cache.shape[2], q.shape[2], cap))
+        splits = max(2, fp4_decode_num_splits(N, most * q.shape[1], k_cache.shape[2], q.shape[2], cap, few=True))
         ws = _few_workspace(N, most * q.shape[1], q.shape[2], splits, dev)
         if ws is not None:
             _lib.call("paged_attention_few_fp4", q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens,
@@ -627,7 +643,8 @@ def paged_kv_read(
     if num_tokens is None:
         num_tokens = int(cu_seqlens[-1].item()) if cu_seqlens is not None else block_tables.shape[0]
     shape = (num_tokens, k_cache.shape[2], k_cache.shape[3] * (2 if fp4 else 1))
-    k, v = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty(shape, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     _, k_cache, v_cache, k_scales, v_scales = _fp4_aligned(None, k_cache, v_cache, k_scales, v_scales)
     _lib.call("paged_kv_read", k, v, k_cache, v_cache, block_tables, context_lens, cu_seqlens, k_scales, v_scales)
     return k, v
