@@ -23,11 +23,14 @@
 // height and width of an image's patches), and every frequency turns by the
 // position of its own axis: c[j] = cos[p[axis(j)]][j].  The axes of all
 // frequencies are two bits each in the arguments; a lane reads the rows of the
-// axes that its eight frequencies have.
+// axes that its eight frequencies have.  17,653 tokens of 16 / 4 heads of 128, three axes
+// (226 MB) 47 us, one axis of context_lens 42: the positions are one more load that the
+// tables' rows wait for (all axes' rows at once, without the branch, 47).
 // FP4: the caches hold codes and block scales (fp4.h) of the rows that the
 // 16-bit cache would hold.  A block's 32 numbers lie in two to four lanes,
 // wherever the rotation's pairs put them, so its largest magnitude is taken by an
-// LDS maximum of the wave.  Keys are rotated in 64 bits there (products of a
+// LDS maximum of the wave (30,447 tokens of 16 / 2 heads of 256, 608 MB, 104 us, 5.8
+// TB/s, 99 % of a streaming copy; the 16-bit cache 112).  Keys are rotated in 64 bits there (products of a
 // 16-bit and a 32-bit number are exact in them): next to a border between two
 // codes the last bit of a fp32 sum would choose another one now and then.
 #include "fp4.h"
@@ -257,13 +260,17 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
 // their places: one wave per kReadRows x (1024 / D) rows, k and v heads of a
 // token in turn, a lane 16 dims of a row.  Rows without a place are zero, and
 // so are those of a table entry outside [0, num_blocks).
+//
+// Bound: HBM, and the chain of offsets, length, table and codes: 30,447 tokens of 2 heads of
+// 256 in 4 bits (79 MB) 18 us, 13.5 at the copy's rate; with 1, 4 and 8 rows a lane 18.8,
+// 19.6 and 24.2, and 23.1 where each row waits for its own lookup.
 struct ReadArgs {
   AppendArgs in;  // caches, tables, lengths; T, nseq, Hkv
   void *k, *v;
   int64_t k_st, k_sh, v_st, v_sh;
 };
 
-constexpr int kReadRows = 4;
+constexpr int kReadRows = 2;
 
 template <typename T, int D, bool FP4>
 __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
@@ -273,12 +280,50 @@ __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
   const uint32_t first = (blockIdx.x * 4 + w) * (kReadRows * RPI), per = 2 * (uint32_t)a.Hkv;  // (rows below 2^31)
   const uint32_t t0 = first / per;
   if (t0 >= a.T) return;
-  // the sequence of the wave's first token; a lane whose token is past its end goes on
-  int64_t n0 = t0;
-  if (a.cu) n0 = find_seq(a, t0, lane);
+  // The rows' tokens and places, then their blocks, then their codes: loads of one
+  // kind wait together.  As a rule all tokens of the wave are of one sequence.
+  int64_t n0 = -1, s0 = 0, e0 = 0, off = 0;
+  bool same = false;
+  if (a.cu) {
+    n0 = find_seq(a, t0, lane);
+    if (n0 >= 0) {
+      seq_range(a.cu, a.cu64, n0, a.T, s0, e0);
+      off = load_index(a.ctx, n0, a.ctx64) - e0;
+      same = (first + kReadRows * RPI - 1) / per < (uint64_t)e0;
+    }
+  }
   const int u = lane % U;
   uint4 x[kReadRows], y[kReadRows];
   uint32_t sc[kReadRows];
+  int64_t n[kReadRows], pos[kReadRows], block[kReadRows];
+  const int64_t nfirst = n0 < 0 ? 0 : n0;  // (tokens before the first sequence)
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    const uint32_t t = (first + i * RPI + lane / U) / per;
+    n[i] = same ? n0 : t;
+    pos[i] = same ? off + t : -1;
+    if (!a.cu && t < a.T) pos[i] = load_index(a.ctx, t, a.ctx64) - 1;
+  }
+  if (a.cu && !same && a.nseq > 0) {
+#pragma unroll 1
+    for (int i = 0; i < kReadRows; ++i) {
+      const uint32_t t = (first + i * RPI + lane / U) / per;
+      if (t >= a.T) break;
+      int64_t m = nfirst, s, e;
+      while (m < a.nseq - 1 && load_index(a.cu, m + 1, a.cu64) <= t) ++m;
+      seq_range(a.cu, a.cu64, m, a.T, s, e);
+      const int64_t p = t >= s && t < e ? load_index(a.ctx, m, a.ctx64) - e + t : -1;
+#pragma unroll
+      for (int k = 0; k < kReadRows; ++k)
+        if (k == i) n[k] = m, pos[k] = p;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    block[i] = -1;
+    if (pos[i] >= 0 && pos[i] < a.limit)
+      block[i] = load_index(a.tab, n[i] * a.tab_st + (uint32_t)pos[i] / (uint32_t)a.page, a.tab64);
+  }
 #pragma unroll
   for (int i = 0; i < kReadRows; ++i) {
     const uint32_t row = first + i * RPI + lane / U, t = row / per, h2 = row - t * per;
@@ -286,30 +331,16 @@ __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
     const int64_t h = key ? h2 : h2 - a.Hkv;
     x[i] = y[i] = uint4{0, 0, 0, 0};
     sc[i] = 0;
-    if (t >= a.T || a.nseq == 0) continue;
-    int64_t n = n0, pos = -1;
-    if (a.cu) {
-      if (n < 0) n = 0;  // (tokens before the first sequence)
-      while (n < a.nseq - 1 && load_index(a.cu, n + 1, a.cu64) <= t) ++n;
-      int64_t s, e;
-      seq_range(a.cu, a.cu64, n, a.T, s, e);
-      if (t >= s && t < e) pos = load_index(a.ctx, n, a.ctx64) - e + t;
-    } else {
-      n = t;
-      pos = load_index(a.ctx, n, a.ctx64) - 1;
-    }
-    if (pos < 0 || pos >= a.limit) continue;
-    const int64_t col = (uint32_t)pos / (uint32_t)a.page, slot = pos - col * a.page;
-    const int64_t block = load_index(a.tab, n * a.tab_st + col, a.tab64);
-    if (block < 0 || block >= a.num_blocks) continue;
-    const char* p = key ? reinterpret_cast<const char*>(a.kc) + block * a.kc_sb + slot * a.kc_st + h * a.kc_sh
-                        : reinterpret_cast<const char*>(a.vc) + block * a.vc_sb + slot * a.vc_st + h * a.vc_sh;
+    if (block[i] < 0 || block[i] >= a.num_blocks) continue;
+    const int64_t slot = (uint32_t)pos[i] % (uint32_t)a.page, at = block[i];
+    const char* p = key ? reinterpret_cast<const char*>(a.kc) + at * a.kc_sb + slot * a.kc_st + h * a.kc_sh
+                        : reinterpret_cast<const char*>(a.vc) + at * a.vc_sb + slot * a.vc_st + h * a.vc_sh;
     if constexpr (FP4) {
       const uint2 c = *reinterpret_cast<const uint2*>(p + 8 * u);
       x[i].x = c.x;
       x[i].y = c.y;
       const ScaleSource& ss = key ? a.ks : a.vs;
-      sc[i] = ss.base[block * ss.sb + h * ss.sh + (u / 2) * ss.sd + slot];
+      sc[i] = ss.base[at * ss.sb + h * ss.sh + (u / 2) * ss.sd + slot];
     } else {
       x[i] = *reinterpret_cast<const uint4*>(p + 32 * u);
       y[i] = *reinterpret_cast<const uint4*>(p + 32 * u + 16);
