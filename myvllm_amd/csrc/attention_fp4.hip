@@ -5,6 +5,16 @@
 // instructions, so the result is that of the 16-bit attention over the values that
 // the codes stand for.  The scales of a page lie slot by slot for each 32 dims
 // (blocks, heads, D / 32, page): one load gives a lane those of four keys.
+//
+// Bound: HBM in long batches, where each byte of codes and scales is read once: 256
+// sequences of U[512, 16384] keys, 16 / 4 heads of 128 (1,106 MB) 205 us and 6 of the
+// merge, 5.2 TB/s, 90 % of a streaming copy (16-bit caches 690); 64 of U[1024, 8192], 16 / 2
+// of 256 (174 MB) 42.7 + 4.8, against 128.  There a start of 9 us shows, which a lone
+// sequence takes almost whole (2,943 keys 9.4 + 4.9): instruction fetch, lengths, table,
+// codes, the product's chain, the merge.  Heads of 64 dims reach 3.1 TB/s: a tile is 2 KB
+// and its conversions and products the work of one of 4 KB.  The scaled products of
+// 4-bit operands were not taken: their sums are short of fp32 (7e-5 of the summands'
+// magnitudes).
 #include "attention_decode.h"
 #include "attention_prefill.h"
 
@@ -408,11 +418,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   decode_deal(a, cap, lane, wv == 0, piece);
 }
 
-// Kv heads of a decode workgroup: as many as a 128-byte line of the cache holds rows
-// of, so that a line is read by one XCD (rows of 128, 64 and 32 bytes), if the
-// heads divide by that.
-int fp4_heads(int Hkv, int D) {
-  int n = D == 256 ? 1 : 4;
+// Kv heads of a decode workgroup: one, whose keys its four waves deal among them, for heads
+// of 256 dims (a line of the cache a row), and for small batches, where a key split inside
+// the workgroup costs less than one that goes through the merge (one sequence of 9,000
+// keys, 16 / 4 heads of 128: 14.2 us, with a wave a head 17.0; 8 of 3,000: 12.8 and 15.9; but
+// 12 of 9,000 28.8 and 22.2: rows counts sequences, kv heads and groups of 16 columns).
+// Else four (or two, or one, as the heads divide), whose rows of a slot share lines (256
+// sequences of U[512, 16384] keys, 4 of 128: 230 us, two heads a workgroup 255, one 370).
+int fp4_heads(int64_t rows, int Hkv, int D) {
+  int n = D == 256 || rows <= 32 ? 1 : 4;
   while (Hkv % n) n /= 2;
   return n;
 }
@@ -448,7 +462,7 @@ void launch_decode_fp4_waves(const Fp4DecodeArgs& a, int heads, dim3 grid, hipSt
 
 template <typename T, int D, bool FEW>
 hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
-  const int heads = fp4_heads(a.Hkv, D), hgroups = a.hgroups;
+  const int hgroups = a.hgroups, heads = fp4_heads((int64_t)a.B * a.Hkv * hgroups, a.Hkv, D);
   const dim3 grid((unsigned)(a.splits > 1 ? a.units : 1), (unsigned)(a.Hkv / heads * hgroups), (unsigned)a.B);
   if (a.splits > 1 && !a.prices_inline) {
     attn_decode_prices_kernel<<<dim3(1), dim3(1024), 0, st>>>(a);

@@ -268,8 +268,9 @@ def _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales):
 def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, capacity: int,
                           few: bool = False) -> int:
     """:func:`decode_num_splits` of caches held in 4 bits, whose units are
-    workgroups of four waves: one kv head of 256 dims, else four (two or one where
-    four do not divide the heads).
+    workgroups of four waves: one kv head of 256 dims and in batches of up to 32 rows
+    (sequences times kv heads, and groups of 16 query heads), else four (two or one
+    where four do not divide the heads).
 
     One workgroup per CU streams best where a tile holds enough bytes (64 sequences
     of U[1024, 8192] keys, 2 kv heads of 256: 256 workgroups 46.7 us, 384 52.6, 512
@@ -278,28 +279,29 @@ def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, he
     of U[300, 3000]: 47.6 and 32.5), and so do a few tokens a sequence (``few``),
     whose shorter sequences leave some of their groups of columns empty (12 sequences
     of 3 to 9 tokens over 6,000 keys, 16 heads of 64: 256 workgroups 32.8, 768 26.8; 32
-    of them, 16 / 4 of 128: 63.0 and 42.6).  At least 256 keys a unit (one sequence of
-    2,943 keys, 2 heads of 256: 12 units 13.4 us, 8 14.8, 32 15.0), of 128 dims or
-    fewer 128 (of 1,000 keys, 4 heads of 128: 4 units 15.8, 8 13.4); at most 64 a
-    sequence (one of 16,000 keys, 16 heads of 64: 64 units 18.8, 125 23.4), 32 of the
-    few (4 sequences, 16 / 4 of 128: 32 units 22.7, 47 25.7).
+    of them, 16 / 4 of 128: 63.0 and 42.6).  At least 256 keys a unit of heads of 256
+    (one sequence of 2,943 keys, 2 heads: 12 units 13.4 us, 8 14.8, 32 15.0), 192 of
+    smaller ones (of 3,000 keys, 4 heads of 128: 16 units 11.5, 12 12.7, 24 12.6); at
+    most 64 a sequence, 32 in small batches (one of 9,000 keys: 32 units 14.3, 48
+    14.6) and of the few (4 sequences, 16 / 4 of 128: 32 units 22.7, 47 25.7).
 
     Not split: with heads of 256, batches of 1,024 rows (512 sequences of U[512, 4096]
     keys, 2 kv heads: 143 us, 155 split) and of 512 short ones; else 2,048 rows, or 512
     of up to 1,024 keys (512 sequences of U[200, 1000] keys, 4 of 128: 47.6 and
     53.9; 1,024 rows of U[200, 2000], 16 of 64: 117.7 and 110.7)."""
-    heads = 1 if head_dim > 128 else 4
-    while num_kv_heads % heads:
+    wide, kv = head_dim > 128, max(num_kv_heads, 1)
+    groups = (num_q_heads // kv + 15) // 16
+    small = num_seqs * kv * groups <= 32
+    heads = 1 if wide or small else 4
+    while kv % heads:
         heads //= 2
-    groups = max(num_kv_heads, 1) // heads * ((num_q_heads // max(num_kv_heads, 1) + 15) // 16)
-    rows = max(1, num_seqs * groups)
-    wide = head_dim > 128
+    rows = max(1, num_seqs * (kv // heads) * groups)
     if rows >= (1024 if wide else 2048) or (rows >= 512 and capacity <= (2048 if wide else 1024)):
         return 1
-    target = 768 if head_dim <= 64 or (few and not wide) else _FP4_TARGET_WORKGROUPS
+    target = 768 if not wide and not small and (few or head_dim <= 64) else _FP4_TARGET_WORKGROUPS
     units = max(1, round(target / rows))
-    by_keys = -(-max(capacity, 1) // (256 if wide else 128))
-    return 1 + min(units, by_keys, 32 if few else 64)
+    by_keys = -(-max(capacity, 1) // (256 if wide else 192))
+    return 1 + min(units, by_keys, 32 if few or small and not wide else 64)
 
 
 _FP4_TARGET_WORKGROUPS = 256
