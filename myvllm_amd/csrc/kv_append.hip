@@ -50,6 +50,10 @@ struct AppendArgs {
   int64_t T, nseq, tab_st, cols, num_blocks, limit;  // limit: positions that have a place and an angle
   int32_t page, Hq, Hkv, rot, chunks;                // chunks: waves per token
   bool tab64, ctx64, cu64, interleaved;
+};
+
+// (apart: a launch of the plain form copies no more arguments than it needs)
+struct AppendExArgs : AppendArgs {
   // AXES: positions (axes, T), their rows of cos and sin, and the axis of each
   // frequency, eight frequencies a 16-bit half
   const void* pos;
@@ -92,7 +96,8 @@ template <typename T> GDN_DEVICE Pair<T> turn_exactly(T a, T b, float c, float s
 }
 
 template <typename T, int D, bool AXES = false, bool FP4 = false>
-__global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(256) void paged_kv_append_kernel(
+    const std::conditional_t<AXES || FP4, AppendExArgs, AppendArgs> a) {
   typedef T v8 __attribute__((ext_vector_type(8)));
   constexpr int U = D / 16;    // lanes per row
   constexpr int RPI = 64 / U;  // rows per wave and step
@@ -218,28 +223,30 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
         }
       }
     }
-    if (FP4 && r >= nq) {
-      uint32_t* const top = tops + (w * kAppendRows + i) * 32 + lane / U * (D / 32);
-      top[e0 / 32] = 0u;  // (LDS operations of a wave complete in order; both are written by every lane of a row)
-      top[e1 / 32] = 0u;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __hip_atomic_fetch_max(top + e0 / 32, top_of_eight(x[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-      __hip_atomic_fetch_max(top + e1 / 32, top_of_eight(y[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (block < 0) continue;
-      const uint32_t s0 = fp4_scale_byte<T>(top[e0 / 32]), s1 = fp4_scale_byte<T>(top[e1 / 32]);
-      const bool key = r < nq + a.Hkv;
-      const int h = r - nq - (key ? 0 : a.Hkv);
-      uint8_t* const p = reinterpret_cast<uint8_t*>(key ? a.kc : a.vc) + block * (key ? a.kc_sb : a.vc_sb) +
-                         slot * (key ? a.kc_st : a.vc_st) + h * (key ? a.kc_sh : a.vc_sh);
-      const uint32_t w0 = fp4_codes<T>(x[i], s0), w1 = fp4_codes<T>(y[i], s1);
-      *reinterpret_cast<uint32_t*>(p + e0 / 2) = w0;
-      *reinterpret_cast<uint32_t*>(p + e1 / 2) = w1;
-      const ScaleSource& sc = key ? a.ks : a.vs;
-      uint8_t* const q = sc.base + block * sc.sb + h * sc.sh + slot;
-      if (e0 % 32 == 0) q[e0 / 32 * sc.sd] = (uint8_t)s0;
-      if (e1 % 32 == 0) q[e1 / 32 * sc.sd] = (uint8_t)s1;
-      continue;
+    if constexpr (FP4) {
+      if (r >= nq) {
+        uint32_t* const top = tops + (w * kAppendRows + i) * 32 + lane / U * (D / 32);
+        top[e0 / 32] = 0u;  // (LDS operations of a wave complete in order; both are written by every lane of a row)
+        top[e1 / 32] = 0u;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __hip_atomic_fetch_max(top + e0 / 32, top_of_eight(x[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        __hip_atomic_fetch_max(top + e1 / 32, top_of_eight(y[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (block < 0) continue;
+        const uint32_t s0 = fp4_scale_byte<T>(top[e0 / 32]), s1 = fp4_scale_byte<T>(top[e1 / 32]);
+        const bool key = r < nq + a.Hkv;
+        const int h = r - nq - (key ? 0 : a.Hkv);
+        uint8_t* const p = reinterpret_cast<uint8_t*>(key ? a.kc : a.vc) + block * (key ? a.kc_sb : a.vc_sb) +
+                           slot * (key ? a.kc_st : a.vc_st) + h * (key ? a.kc_sh : a.vc_sh);
+        const uint32_t w0 = fp4_codes<T>(x[i], s0), w1 = fp4_codes<T>(y[i], s1);
+        *reinterpret_cast<uint32_t*>(p + e0 / 2) = w0;
+        *reinterpret_cast<uint32_t*>(p + e1 / 2) = w1;
+        const ScaleSource& sc = key ? a.ks : a.vs;
+        uint8_t* const q = sc.base + block * sc.sb + h * sc.sh + slot;
+        if (e0 % 32 == 0) q[e0 / 32 * sc.sd] = (uint8_t)s0;
+        if (e1 % 32 == 0) q[e1 / 32 * sc.sd] = (uint8_t)s1;
+        continue;
+      }
     }
     T* p;
     if (r < nq) {
@@ -265,7 +272,7 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(const AppendArgs a
 // 256 in 4 bits (79 MB) 18 us, 13.5 at the copy's rate; with 1, 4 and 8 rows a lane 18.8,
 // 19.6 and 24.2, and 23.1 where each row waits for its own lookup.
 struct ReadArgs {
-  AppendArgs in;  // caches, tables, lengths; T, nseq, Hkv
+  AppendExArgs in;  // caches, tables, lengths; T, nseq, Hkv
   void *k, *v;
   int64_t k_st, k_sh, v_st, v_sh;
 };
@@ -274,7 +281,7 @@ constexpr int kReadRows = 2;
 
 template <typename T, int D, bool FP4>
 __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
-  const AppendArgs& a = g.in;
+  const AppendExArgs& a = g.in;
   constexpr int U = D / 16, RPI = 64 / U;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t first = (blockIdx.x * 4 + w) * (kReadRows * RPI), per = 2 * (uint32_t)a.Hkv;  // (rows below 2^31)
@@ -364,7 +371,7 @@ __global__ __launch_bounds__(256) void paged_kv_read_kernel(const ReadArgs g) {
 }
 
 template <typename T, int D>
-hipError_t launch_append(const AppendArgs& a, bool fp4, hipStream_t st) {
+hipError_t launch_append(const AppendExArgs& a, bool fp4, hipStream_t st) {
   const dim3 grid((unsigned)((a.T * a.chunks + 3) / 4)), block(256);
   if (fp4) {
     if (a.pos) paged_kv_append_kernel<T, D, true, true><<<grid, block, 0, st>>>(a);
@@ -376,7 +383,7 @@ hipError_t launch_append(const AppendArgs& a, bool fp4, hipStream_t st) {
   return hipGetLastError();
 }
 template <typename T>
-hipError_t launch_append(const AppendArgs& a, int D, bool fp4, hipStream_t st) {
+hipError_t launch_append(const AppendExArgs& a, int D, bool fp4, hipStream_t st) {
   if (D == 64) return launch_append<T, 64>(a, fp4, st);
   if (D == 128) return launch_append<T, 128>(a, fp4, st);
   return launch_append<T, 256>(a, fp4, st);
@@ -442,7 +449,7 @@ hipError_t paged_kv_append_launch(const gdn_tensor* k, const gdn_tensor* v, gdn_
                                   const int32_t* sections, bool dealt, hipStream_t st) {
   if (k->shape[0] == 0) return hipSuccess;
   const int D = (int)k->shape[2];
-  AppendArgs a{};
+  AppendExArgs a{};
   a.k = k->data;
   a.k_st = k->stride[0];
   a.k_sh = k->stride[1];

@@ -223,7 +223,8 @@ def paged_flash_attention_decode(
     scores only."""
     if k_cache.shape[1] != block_size:
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
-    if _fp4(k_scales, v_scales, softcap, alibi_slopes):
+    if k_scales is not None or v_scales is not None:
+        _check_fp4(k_scales, v_scales, softcap, alibi_slopes)
         return _decode_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, scale, num_splits, out)
     dev = _lib.require_device(q, k_cache, v_cache, block_tables, context_lens, alibi_slopes)
     B, Hq, Dh = q.shape
@@ -244,15 +245,12 @@ def paged_flash_attention_decode(
     return _finish(out, o)
 
 
-def _fp4(k_scales, v_scales, *forms) -> bool:
-    """Whether a call is over caches held in 4 bits."""
-    if k_scales is None and v_scales is None:
-        return False
+def _check_fp4(k_scales, v_scales, *forms) -> None:
+    """The arguments of a call over caches held in 4 bits."""
     if k_scales is None or v_scales is None:
         raise ValueError("k_scales and v_scales come together")
     if any(f is not None for f in forms):
         raise ValueError("caches held in 4 bits take plain scores: no softcap, alibi_slopes or prefix_lens")
-    return True
 
 
 def _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales):
@@ -441,7 +439,8 @@ def paged_flash_attention_prefill(
     (:func:`paged_kv_append`), for plain scores only."""
     if k_cache.shape[1] != page_block_size:
         raise ValueError(f"page_block_size {page_block_size} != k_cache.shape[1] {k_cache.shape[1]}")
-    if _fp4(k_scales, v_scales, softcap, alibi_slopes, prefix_lens):
+    if k_scales is not None or v_scales is not None:
+        _check_fp4(k_scales, v_scales, softcap, alibi_slopes, prefix_lens)
         return _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, page_block_tables, context_lens, cu_seqlens,
                                   scale, max_seqlen, out)
     dev = _lib.require_device(q, k_cache, v_cache, page_block_tables, context_lens, cu_seqlens, alibi_slopes,
@@ -568,13 +567,13 @@ def paged_kv_append(
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     if q is None and out is not None:
         raise ValueError("out is the rotated q's: none without q")
-    extended = _fp4(k_scales, v_scales) or positions is not None
+    extended = k_scales is not None or v_scales is not None or positions is not None or sections is not None
+    tensors = (k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin)
     if extended:
+        if k_scales is not None or v_scales is not None:
+            _check_fp4(k_scales, v_scales)
         positions, axes = _axes(positions, sections, cos)
-    elif sections is not None:
-        raise ValueError("sections are those of positions")
-    tensors = (k, v, k_cache, v_cache, block_tables, context_lens, q, out, cu_seqlens, cos, sin, positions, k_scales,
-               v_scales)
+        tensors += (positions, k_scales, v_scales)
     if not _lib.same_device(*tensors):
         _lib.require_device(*tensors)
     if not _lib.vec16_all(q, k, v, cos, sin):
@@ -637,7 +636,9 @@ def paged_kv_read(
     if k_cache.shape[1] != block_size:
         raise ValueError(f"block_size {block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     dev = _lib.require_device(k_cache, v_cache, block_tables, context_lens, cu_seqlens, k_scales, v_scales)
-    fp4 = _fp4(k_scales, v_scales)
+    fp4 = k_scales is not None or v_scales is not None
+    if fp4:
+        _check_fp4(k_scales, v_scales)
     if dtype is None:
         dtype = torch.bfloat16 if fp4 else k_cache.dtype
     elif not fp4 and dtype != k_cache.dtype:
