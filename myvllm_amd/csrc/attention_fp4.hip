@@ -480,21 +480,14 @@ hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <typename T, int D>
-hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
+template <typename T, int D, int PG>
+hipError_t launch_prefill_fp4_tiles(const Fp4AttnArgs& a, int64_t nseq, hipStream_t st) {
   constexpr int BN = 32;
-  if (nseq <= 0 || max_len <= 0 || a.tab.num_blocks == 0) {
-    // (without a block to read every row is zero: those of no sequence are all of them)
-    zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(
-        a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu, a.cu64, a.tab.num_blocks == 0 ? 0 : a.nseq, a.T);
-    return hipGetLastError();
-  }
   // (the grids of the 16-bit caches, launch_prefill_t)
   const int64_t tiles = a.T / (32 * (4 / a.gh)) + nseq + 1;
   if (a.extra > 0) {
     const dim3 grid((unsigned)(a.rows + a.Hq / a.gh + a.extra));
-    if (a.tab.is64) attn_prefill_kernel<T, D, BN, 3, true, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
-    else attn_prefill_kernel<T, D, BN, 2, true, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+    attn_prefill_kernel<T, D, BN, PG, true, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     constexpr int DG = D == 256 ? 2 : 1;
@@ -503,9 +496,23 @@ hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_le
     return hipGetLastError();
   }
   const dim3 grid((unsigned)(tiles * (a.Hq / a.gh)));
-  if (a.tab.is64) attn_prefill_kernel<T, D, BN, 3, false, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
-  else attn_prefill_kernel<T, D, BN, 2, false, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
+  attn_prefill_kernel<T, D, BN, PG, false, 0, kFp4><<<grid, dim3(256), 0, st>>>(a);
   return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
+  if (nseq <= 0 || max_len <= 0 || a.tab.num_blocks == 0) {
+    // (without a block to read every row is zero: those of no sequence are all of them)
+    zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(
+        a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu, a.cu64, a.tab.num_blocks == 0 ? 0 : a.nseq, a.T);
+    return hipGetLastError();
+  }
+  if (a.tab.is64) return launch_prefill_fp4_tiles<T, D, 3>(a, nseq, st);
+  const bool alike = a.k.sb == a.v.sb && a.k.st == a.v.st && a.ks.sb == a.vs.sb && a.ks.sh == a.vs.sh &&
+                     a.ks.sd == a.vs.sd;
+  if (a.tab.page == 16 && alike) return launch_prefill_fp4_tiles<T, D, 4>(a, nseq, st);
+  return launch_prefill_fp4_tiles<T, D, 2>(a, nseq, st);
 }
 
 }  // namespace

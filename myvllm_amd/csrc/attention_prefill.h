@@ -84,7 +84,11 @@ constexpr bool q_pieces_inside(int dq) {
 // the four waves.
 // PG: 0 packed rows, 1 paged (any page size: a table lookup per row),
 // 2 / 3 paged with a page size that is a multiple of 16 and an int32 / int64
-// block table (one lookup per 16 rows, a tile ahead, 32-bit arithmetic)
+// block table (one lookup per 16 rows, a tile ahead, 32-bit arithmetic); kFp4 also 4,
+// an int32 table, pages of 16 keys, and v's strides those of k, which holds fewer scalar
+// registers: four chunks of up to 2,048 tokens over up to 16,384 keys, 16 / 2 heads of
+// 256 945 us, by PG 2 1,090 (16-bit caches 997); 16 prompts of up to 4,096 774 and 822;
+// the four chunks with 16 heads of 64 300 and 352
 // Workgroup id -> (sequence, query tile): tiles of tile_len queries (a power
 // of two), laid out sequence after sequence over the tiles that exist (no
 // workgroup of a padded grid exits idle).  Below D = 256 batches of up to 64
@@ -605,7 +609,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   bool idin[NG];                // its groups lie inside the range and the table
   uint32_t slots[NG];           // their first page slot
   constexpr bool G16 = PG >= 2, T64 = PG == 3;  // 16-row groups per page lookup; int64 table
-  const uint32_t gpp = G16 ? (uint32_t)a.tab.page / 16 : 1u;  // 16-row groups per page
+  constexpr bool ONE = PG == 4;                               // a page is a 16-row group
+  const uint32_t gpp = G16 && !ONE ? (uint32_t)a.tab.page / 16 : 1u;  // 16-row groups per page
   uint32_t gcol = 0, grem = 0;  // table column and group within the page of the next group
   // (G16) this sequence's row of the block table as 32-bit words; the table
   // has columns, and key positions (columns x page), block ids and block
@@ -628,8 +633,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         lo[g] = trow[e];
         hi[g] = 0u;
       }
-      sl[g] = 16 * grem;
-      if (++grem == gpp) {
+      sl[g] = ONE ? 0u : 16 * grem;
+      if (ONE) {
+        ++gcol;
+      } else if (++grem == gpp) {
         grem = 0;
         ++gcol;
       }
@@ -640,10 +647,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     grem = (uint32_t)tile0 * NG - gcol * gpp;
   }
   if (G16) load_ids(tile0, idlo, idhi, idin, slots);
-  const uint32_t kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st;  // row strides in bytes (below 2^31)
+  const uint32_t kst = (uint32_t)a.k.st, vst = ONE ? kst : (uint32_t)a.v.st;  // row strides in bytes (below 2^31)
   const char* kbase = a.k.base + kvh * a.k.sh;
   const char* vbase = a.v.base + kvh * a.v.sh;
-  const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;
+  const uint64_t ksb = (uint32_t)a.k.sb, vsb = ONE ? ksb : (uint32_t)a.v.sb;
   const uint32_t nblk = (uint32_t)(a.tab.num_blocks < 0x7fffffff ? a.tab.num_blocks : 0x7fffffff);
   auto load_tile = [&](int t, uint4* kd, uint4* vd) {
     __amdgpu_buffer_rsrc_t rkg[NG], rvg[NG], rkt, rvt;
@@ -746,7 +753,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     if constexpr (Q4) {
       // Scalar bases and one offset per lane (descriptors of four tensors leave too few
       // scalar registers: four chunks of up to 2,048 tokens over up to 16,384 keys took
-      // 1,154 us with them, 1,171 with addresses on the vector side, 1,083 so).  Rows past
+      // 1,154 us with them, 1,171 with addresses on the vector side, 1,083 so, by PG 2).  Rows past
       // the range are read as the last one in it, a group without keys from block 0,
       // whose codes and scales store() clears.
       uint32_t nlo[NG], nhi[NG], nsl[NG];
@@ -770,12 +777,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         row = qrow < last ? qrow : last;
         ko = row * kst + qch * (QE / 2), vo = row * vst + qch * (QE / 2);
       }
-      uint32_t kso = qch * QE / 32 * (uint32_t)a.ks.sd + row, vso = qch * QE / 32 * (uint32_t)a.vs.sd + row;
-      asm("" : "+v"(ko), "+v"(vo), "+v"(kso), "+v"(vso));
+      const ScaleSource& vss = ONE ? a.ks : a.vs;  // (its strides)
+      uint32_t kso = qch * QE / 32 * (uint32_t)a.ks.sd + row, vso = qch * QE / 32 * (uint32_t)vss.sd + row;
+      asm("" : "+v"(ko), "+v"(kso));
+      if (ONE) vo = ko, vso = kso;
+      else asm("" : "+v"(vo), "+v"(vso));
       const char* const kp = kbase + bb * ksb + (uint64_t)(usl * kst);
       const char* const vp = vbase + bb * vsb + (uint64_t)(usl * vst);
       const uint8_t* const ksp = a.ks.base + kvh * a.ks.sh + bb * (uint32_t)a.ks.sb + usl;
-      const uint8_t* const vsp = a.vs.base + kvh * a.vs.sh + bb * (uint32_t)a.vs.sb + usl;
+      const uint8_t* const vsp = a.vs.base + kvh * vss.sh + bb * (uint32_t)vss.sb + usl;
       auto codes = [](const char* p, Codes& c) __attribute__((always_inline)) {
         if constexpr (QW == 4) {
           const uint4 x = *reinterpret_cast<const uint4*>(p);

@@ -205,6 +205,35 @@ def test_prefill_split(dev, Hq, Hkv, D, dtype):
     assert_within(o, ref, bound, "unsplit")
 
 
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(16, 2, 256, BF), (8, 4, 128, HF), (4, 4, 64, BF)])
+@pytest.mark.parametrize("page, apart", [(16, ""), (32, ""), (16, "vc"), (16, "ks"), (16, "vs"), (16, "kc")])
+def test_prefill_layouts(dev, Hq, Hkv, D, dtype, page, apart):
+    """Pages of 16 keys with k and v laid out alike, and every other layout, whole and split."""
+    print(f"fp4 prefill {Hq}/{Hkv}x{D} {dtype} page={page} apart={apart}", flush=True)
+
+    def put(n, t):
+        if n != apart:
+            return t.to(dev)
+        w = torch.full((t.shape[0] + 1, t.shape[1] + 1, t.shape[2] + 1, t.shape[3] + 32), 255, dtype=t.dtype,
+                       device=dev)
+        w = w[1:, :t.shape[1], :t.shape[2], :t.shape[3]]
+        w.copy_(t)
+        return w
+
+    new, ctx = [70, 0, 129, 1, 33, 64], [70, 40, 300, 1000, 800, 64]
+    for few in (False, True):
+        if few:
+            new, ctx = new[3:5], [3000, 2000]
+        c = make(ctx, new, Hq, Hkv, D, page, dtype, seed=D + page)
+        ref, bound = reference(c, new, D**-0.5)
+        assert_within(prefill(c, dev, D**-0.5, put=put), ref, bound)
+        d = {n: put(n, t) for n, t in c.items()}
+        o = torch.empty_like(d["q"])
+        _lib.call("paged_attention_prefill_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"],
+                  d["cu"], o, None, max(new), D**-0.5)
+        assert_within(o, ref, bound, "unsplit")
+
+
 def is_few(c, most):
     from myvllm_amd.full_attention import _few_tokens
 
