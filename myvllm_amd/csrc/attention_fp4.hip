@@ -22,6 +22,11 @@ namespace {
 
 constexpr int32_t kFp4StartPrice = 6;
 
+// Whether v and its scales lie as k and its do.
+template <typename A> bool alike(const A& a) {
+  return a.k.sb == a.v.sb && a.k.st == a.v.st && a.ks.sb == a.vs.sb && a.ks.sh == a.vs.sh && a.ks.sd == a.vs.sd;
+}
+
 struct Fp4DecodeArgs : DecodeArgs {
   ScaleSource ks, vs;
   uint32_t page_inv;  // floor((2^32 - 1) / 16-key groups of a page)
@@ -44,7 +49,8 @@ struct Fp4DecodeArgs : DecodeArgs {
 // instruction without LDS: two numbers of a dim pair at a time are turned into 16
 // bits, and byte permutes pair them by keys.
 //
-// ONE: pages of 16 keys, so a 16-key group is a page and starts at its slot 0.
+// ONE: pages of 16 keys, so a 16-key group is a page and starts at its slot 0, and v's
+// strides those of k.
 // FEW: a few tokens of each sequence instead of one: the columns are the query heads
 // of one token after the other, each with its own last key.
 template <typename T, int D, int KS, bool ONE, bool FEW>
@@ -75,9 +81,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const char* const vbase = a.v.base + kvh * a.v.sh;
   const uint8_t* const ksbase = a.ks.base + kvh * a.ks.sh;
   const uint8_t* const vsbase = a.vs.base + kvh * a.vs.sh;
-  const uint64_t ksb = (uint32_t)a.k.sb, vsb = (uint32_t)a.v.sb;  // (below 2^32, as all of them, checked by the entry)
-  const uint64_t kssb = (uint32_t)a.ks.sb, vssb = (uint32_t)a.vs.sb;
-  const uint32_t kst = (uint32_t)a.k.st, vst = (uint32_t)a.v.st, ksd = (uint32_t)a.ks.sd, vsd = (uint32_t)a.vs.sd;
+  const uint64_t ksb = (uint32_t)a.k.sb, vsb = ONE ? ksb : (uint32_t)a.v.sb;  // (below 2^32, as all of them, checked by the entry)
+  const uint64_t kssb = (uint32_t)a.ks.sb, vssb = ONE ? kssb : (uint32_t)a.vs.sb;
+  const uint32_t kst = (uint32_t)a.k.st, vst = ONE ? kst : (uint32_t)a.v.st;
+  const uint32_t ksd = (uint32_t)a.ks.sd, vsd = ONE ? ksd : (uint32_t)a.vs.sd;
   const float c = a.c > 0.f ? a.c : (a.c < 0.f ? -a.c : 1.f);
   const uint32_t qsign = a.c < 0.f ? 0x80008000u : 0u;
   const uint32_t gpp = (uint32_t)a.tab.page / 16u, nblk = (uint32_t)a.tab.num_blocks;  // (below 2^31)
@@ -469,7 +476,7 @@ hipError_t launch_decode_fp4(const Fp4DecodeArgs& a, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (a.tab.page == 16) launch_decode_fp4_waves<T, D, true, FEW>(a, heads, grid, st);
+  if (a.tab.page == 16 && alike(a)) launch_decode_fp4_waves<T, D, true, FEW>(a, heads, grid, st);
   else launch_decode_fp4_waves<T, D, false, FEW>(a, heads, grid, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
@@ -509,9 +516,7 @@ hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_le
     return hipGetLastError();
   }
   if (a.tab.is64) return launch_prefill_fp4_tiles<T, D, 3>(a, nseq, st);
-  const bool alike = a.k.sb == a.v.sb && a.k.st == a.v.st && a.ks.sb == a.vs.sb && a.ks.sh == a.vs.sh &&
-                     a.ks.sd == a.vs.sd;
-  if (a.tab.page == 16 && alike) return launch_prefill_fp4_tiles<T, D, 4>(a, nseq, st);
+  if (a.tab.page == 16 && alike(a)) return launch_prefill_fp4_tiles<T, D, 4>(a, nseq, st);
   return launch_prefill_fp4_tiles<T, D, 2>(a, nseq, st);
 }
 

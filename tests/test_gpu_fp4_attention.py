@@ -205,12 +205,11 @@ def test_prefill_split(dev, Hq, Hkv, D, dtype):
     assert_within(o, ref, bound, "unsplit")
 
 
-@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(16, 2, 256, BF), (8, 4, 128, HF), (4, 4, 64, BF)])
-@pytest.mark.parametrize("page, apart", [(16, ""), (32, ""), (16, "vc"), (16, "ks"), (16, "vs"), (16, "kc")])
-def test_prefill_layouts(dev, Hq, Hkv, D, dtype, page, apart):
-    """Pages of 16 keys with k and v laid out alike, and every other layout, whole and split."""
-    print(f"fp4 prefill {Hq}/{Hkv}x{D} {dtype} page={page} apart={apart}", flush=True)
+LAYOUTS = [(16, ""), (32, ""), (16, "vc"), (16, "ks"), (16, "vs"), (16, "kc")]
 
+
+def laid_out(dev, apart):
+    """Tensors on the GPU, the one called `apart` with larger strides than the others."""
     def put(n, t):
         if n != apart:
             return t.to(dev)
@@ -220,10 +219,17 @@ def test_prefill_layouts(dev, Hq, Hkv, D, dtype, page, apart):
         w.copy_(t)
         return w
 
-    new, ctx = [70, 0, 129, 1, 33, 64], [70, 40, 300, 1000, 800, 64]
-    for few in (False, True):
-        if few:
-            new, ctx = new[3:5], [3000, 2000]
+    return put
+
+
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(16, 2, 256, BF), (8, 4, 128, HF), (4, 4, 64, BF)])
+@pytest.mark.parametrize("page, apart", LAYOUTS)
+def test_layouts(dev, Hq, Hkv, D, dtype, page, apart):
+    """Pages of 16 keys with k and v laid out alike, and every other layout: prefill whole and split,
+    a few tokens, decode."""
+    print(f"fp4 layouts {Hq}/{Hkv}x{D} {dtype} page={page} apart={apart}", flush=True)
+    put = laid_out(dev, apart)
+    for new, ctx in (([70, 0, 129, 1, 33, 64], [70, 40, 300, 1000, 800, 64]), ([1, 33], [3000, 2000])):
         c = make(ctx, new, Hq, Hkv, D, page, dtype, seed=D + page)
         ref, bound = reference(c, new, D**-0.5)
         assert_within(prefill(c, dev, D**-0.5, put=put), ref, bound)
@@ -232,6 +238,15 @@ def test_prefill_layouts(dev, Hq, Hkv, D, dtype, page, apart):
         _lib.call("paged_attention_prefill_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"],
                   d["cu"], o, None, max(new), D**-0.5)
         assert_within(o, ref, bound, "unsplit")
+    for new, ctx in (([1, 3, 0, 4], [900, 70, 5, 4]), ([2] * 20, [50 + 7 * i for i in range(20)])):
+        c = make(ctx, new, Hq, Hkv, D, page, dtype, seed=D + page)
+        assert is_few(c, max(new))
+        assert_within(prefill(c, dev, D**-0.5, put=put), *reference(c, new, D**-0.5))
+    for ctx in ([900, 70, 0, 4], [50 + 7 * i for i in range(20)]):
+        c = make(ctx, [1] * len(ctx), Hq, Hkv, D, page, dtype, seed=D + page)
+        ref, bound = reference(c, [1] * len(ctx), D**-0.5)
+        for splits in (None, 1, 4):
+            assert_within(decode(c, dev, D**-0.5, splits, put=put), ref, bound)
 
 
 def is_few(c, most):
