@@ -8,8 +8,8 @@
 //
 // Bound: HBM in long batches, where each byte of codes and scales is read once: 256
 // sequences of U[512, 16384] keys, 16 / 4 heads of 128 (1,106 MB) 205 us and 6 of the
-// merge, 5.2 TB/s, 90 % of a streaming copy (16-bit caches 690); 64 of U[1024, 8192], 16 / 2
-// of 256 (174 MB) 42.7 + 4.8, against 128.  There a start of 9 us shows, which a lone
+// merge, 5.2 TB/s, 90 % of a streaming copy (by 16-bit caches 690); 64 of U[1024, 8192], 16 / 2
+// of 256 (174 MB) 42.3 + 4.8, against 128.  There a start of 9 us shows, which a lone
 // sequence takes almost whole (2,943 keys 9.4 + 4.9): instruction fetch, lengths, table,
 // codes, the product's chain, the merge.  Heads of 64 dims reach 3.1 TB/s: a tile is 2 KB
 // and its conversions and products the work of one of 4 KB.  The scaled products of
