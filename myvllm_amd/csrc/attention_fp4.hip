@@ -11,7 +11,7 @@
 // merge, 5.2 TB/s, 90 % of a streaming copy (by 16-bit caches 690); 64 of U[1024, 8192], 16 / 2
 // of 256 (174 MB) 42.3 + 4.8, against 128.  There a start of 9 us shows, which a lone
 // sequence takes almost whole (2,943 keys 9.4 + 4.9): instruction fetch, lengths, table,
-// codes, the product's chain, the merge.  Heads of 64 dims reach 3.1 TB/s: a tile is 2 KB
+// codes, the product's chain, the merge.  Heads of 64 dims reach 3.7 TB/s: a tile is 2 KB
 // and its conversions and products the work of one of 4 KB.  The scaled products of
 // 4-bit operands were not taken: their sums are short of fp32 (7e-5 of the summands'
 // magnitudes).
@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int32_t kFp4StartPrice = 6;
+constexpr int32_t kFp4StartPrice = 6;  // of a piece's start, in 16-key groups
 
 // Whether v and its scales lie as k and its do.
 template <typename A> bool alike(const A& a) {
