@@ -226,12 +226,19 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(
     if constexpr (FP4) {
       if (r >= nq) {
         uint32_t* const top = tops + (w * kAppendRows + i) * 32 + lane / U * (D / 32);
-        top[e0 / 32] = 0u;  // (LDS operations of a wave complete in order; both are written by every lane of a row)
+        // (LDS operations of a wave complete in order; the lanes of a row, which all write
+        // the zeros and take part in the maxima, meet between the steps)
+        auto meet = []() __attribute__((always_inline)) {
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        top[e0 / 32] = 0u;
         top[e1 / 32] = 0u;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        meet();
         __hip_atomic_fetch_max(top + e0 / 32, top_of_eight(x[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
         __hip_atomic_fetch_max(top + e1 / 32, top_of_eight(y[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        meet();
         if (block < 0) continue;
         const uint32_t s0 = fp4_scale_byte<T>(top[e0 / 32]), s1 = fp4_scale_byte<T>(top[e1 / 32]);
         const bool key = r < nq + a.Hkv;

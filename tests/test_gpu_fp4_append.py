@@ -350,3 +350,23 @@ def test_append_and_read_in_a_graph(dev):
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert torch.equal(cache[0], d["kc"]) and torch.equal(cache[1], d["ks"])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rot, inter", [(0, False), (16, False), (48, True), (64, False)])
+def test_block_maxima(dev, D, rot, inter):
+    """A block's scale is its own largest magnitude's, whichever lane has it and whatever the
+    wave's other rows and earlier steps left: each of the block's places in turn, blocks
+    2^20 apart next to each other and after each other.  (A block of 16 of turned and 16 of other numbers
+    is shared by lanes of both halves.)"""
+    T, Hkv = 96, 8
+    c = make([T], [0], Hq=1, Hkv=Hkv, D=D, seed=rot)
+    t, h, b = torch.meshgrid(torch.arange(T), torch.arange(Hkv), torch.arange(D // 32), indexing="ij")
+    size = 2.0 ** (20.0 * ((t + h + b) % 2) - 10.0 * (h % 3))
+    for x, shift in (("k", 0), ("v", 7)):
+        rows = c[x].float().clamp(-0.4, 0.4).unflatten(-1, (-1, 32))
+        at = ((t + 5 * h + 11 * b + shift) % 32)[..., None]
+        rows = rows.scatter(-1, at, (1.0 + t / 128)[..., None].float() * (1 - 2 * (t % 2))[..., None])
+        c[x] = (rows * size[..., None]).flatten(-2).to(BF)
+    cos, sin = rope(T, rot) if rot else (None, None)
+    check(c, dev, cos=cos, sin=sin, interleaved=inter)
