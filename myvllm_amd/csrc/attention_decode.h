@@ -459,6 +459,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 // there, its row was written by that unit.  The pieces are taken 64 at a time, lane i
 // reading piece i's maximum and row sum, so their loads are in flight
 // together; the running maximum carries over between groups of 64.
+// NaN scores leave a piece's maximum as it was, -inf where it has no others, but
+// not its row sum: a piece is without weight where both say so, and one NaN sum makes
+// the row NaN, as in a sequence of one piece.
 // `row` of the `rows` that a slot holds, to `op`.
 template <typename T, int D>
 GDN_DEVICE void decode_combine(const DecodeArgs& a, int64_t b, int row, int rows, T* op) {
@@ -488,7 +491,11 @@ GDN_DEVICE void decode_combine(const DecodeArgs& a, int64_t b, int row, int rows
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) cm = fmaxf(cm, __shfl_xor(cm, d));
       const float mn = fmaxf(mx, cm);
+      if (__builtin_amdgcn_ballot_w64(li != li) != 0) l = __builtin_nanf("");
       if (mn == -INFINITY) continue;
+      // (pieces of this row: an empty unit's slot holds stale data, and one whose keys the
+      // row does not see whatever their values made of its zero weights)
+      const uint64_t in = __builtin_amdgcn_ballot_w64(mi != -INFINITY || li != 0.f);
       const float sc = exp2_fast(mx - mn);  // (0 while mx is -inf)
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] *= sc;
@@ -513,14 +520,14 @@ GDN_DEVICE void decode_combine(const DecodeArgs& a, int64_t b, int row, int rows
         for (int k = 0; k < 8; ++k) {
           const int j = j0 + k < cnt ? j0 + k : cnt - 1;
           const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wi), j));
-          const float wj = j0 + k < cnt ? w : 0.f;
+          const bool counts = j0 + k < cnt && (in >> j & 1u);
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += wj == 0.f ? 0.f : wj * v[k][e];  // (an empty unit's slot holds stale data)
+          for (int e = 0; e < E; ++e) acc[e] += counts ? w * v[k][e] : 0.f;
         }
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int e = 0; e < E; ++e) op[e] = (T)(acc[e] * inv);
 }
