@@ -558,8 +558,9 @@ int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, 
  * least 1), by the decode's kernel: the query heads of all of a sequence's tokens
  * share its reads of the keys.  workspace: 1-D fp32, 16-byte aligned, of
  * paged_attention_decode_workspace_size(N, max_seqlen * Hq, D, num_splits) elements,
- * overwritten; num_splits from 2 to 256 as for paged_attention_decode.  Rows of tokens
- * past max_seqlen are not written.
+ * overwritten; num_splits from 2 to 256 as for paged_attention_decode.  A sequence of more
+ * than max_seqlen tokens gets its rows too, not split, so slower.  Rows of q times Hq
+ * below 2^30 (GDN_ERR_RANGE).
  */
 int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                             const gdn_tensor* k_scales, const gdn_tensor* v_scales, const gdn_tensor* block_tables,

@@ -2,6 +2,8 @@
 // tiles, and their launch.
 #pragma once
 
+#include <type_traits>
+
 #include "attention_common.h"
 
 namespace {
@@ -111,13 +113,21 @@ GDN_DEVICE int32_t floor_div(int64_t n, int64_t d, double inv) {
 // The pieces of a decode workgroup's unit, one after the other:
 // piece(sequence, first key, end of its keys, workspace slot or -1 where it is the
 // whole sequence, the sequence's last key).  first_wave: of the workgroup.
-template <typename Piece>
-GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool first_wave, Piece&& piece) {
+// further(): asked after the unit, whether there are further pieces, each of the whole
+// sequence blockIdx.z (of other columns, which it chooses).
+struct NothingFurther {
+  GDN_DEVICE bool operator()() const { return false; }
+};
+template <typename Piece, typename Further = NothingFurther>
+GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool first_wave, Piece&& piece,
+                            Further&& further = NothingFurther()) {
+  constexpr bool FURTHER = !std::is_same<std::decay_t<Further>, NothingFurther>::value;
   // with one split, unit z is sequence z; else unit u holds the batch's
   // prices [x0, x1) (they fit 31 bits, which the entry point checks)
   const int32_t SP = a.start;
   int32_t b = blockIdx.z, x0 = 0, x1 = 0, qb = 0;
-  if (a.splits > 1) {
+  // (false: an empty unit, of a smaller total than U: no piece)
+  auto find = [&]() __attribute__((always_inline)) {
     const int64_t U = (int64_t)a.B * a.units;
     const int64_t u = (int64_t)blockIdx.z * a.units + blockIdx.x;
     if (a.prices_inline) {
@@ -138,7 +148,7 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
       x1 = floor_div((u + 1) * tot, U, a.unit_inv);
       const bool writer = u == 0 && blockIdx.y == 0 && first_wave;
       if (writer && lane == 0) a.prices[a.B] = tot;
-      if (x0 >= x1 && !writer) return;  // an empty unit (a smaller total than U): no piece
+      if (x0 >= x1 && !writer) return false;
       int32_t run = 0;
       for (int32_t c0 = 0; c0 < a.B; c0 += 64) {
         const int32_t p = c0 == 0 ? p0 : price(c0 + lane);
@@ -154,12 +164,12 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
         run += __builtin_amdgcn_readlane(inc, 63);
         if (cnt < 64 && !writer) break;  // (the answer is in this chunk)
       }
-      if (x0 >= x1) return;
+      if (x0 >= x1) return false;
     } else {
       const int64_t Pt = load_index_scalar(a.prices, a.B, false);
       x0 = floor_div(u * Pt, U, a.unit_inv);
       x1 = floor_div((u + 1) * Pt, U, a.unit_inv);
-      if (x0 >= x1) return;  // an empty unit (a smaller total than U): no piece
+      if (x0 >= x1) return false;
       // the sequence holding price x0: the last b < B with Q[b] <= x0 (Q[0] =
       // 0), by a 64-ary search over the prefix (one probe per lane per
       // round, Q[lo] <= x0 throughout)
@@ -176,6 +186,14 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
       b = __builtin_amdgcn_readfirstlane(lo + (int32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(le)) - 1);
       qb = (int32_t)load_index_scalar(a.prices, b, false);
     }
+    return true;
+  };
+  bool dealt = true;  // pieces of the unit, not further ones
+  if (a.splits > 1 && !find()) {
+    if constexpr (!FURTHER) return;
+    if (!further()) return;
+    dealt = false;
+    b = blockIdx.z;
   }
   for (;;) {
     const int64_t L = clamp64(load_index(a.ctx, b, a.ctx64), 0, cap);
@@ -187,7 +205,7 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
     int32_t qn = 0;
     int64_t k_lo = 0, k_hi = L, slot = -1;
     bool any = true;
-    if (a.splits > 1) {
+    if (a.splits > 1 && (!FURTHER || dealt)) {
       const int32_t tb = (int32_t)((L + 15) / 16);  // the sequence's tiles
       qn = qb + (tb > 0 ? tb + SP : 0);
       const int32_t r0 = x0 - qb - SP, r1 = x1 - qb - SP;
@@ -198,7 +216,16 @@ GDN_DEVICE void decode_deal(const DecodeArgs& a, int64_t cap, int lane, bool fir
       if (t0 > 0 || t1 < tb) slot = (int64_t)b + (int64_t)blockIdx.z * a.units + blockIdx.x;
     }
     if (any) piece(b, k_lo, k_hi, slot, L - 1);
-    if (a.splits == 1 || qn >= x1) break;
+    if constexpr (FURTHER) {
+      if (!dealt || a.splits == 1 || qn >= x1) {
+        if (!further()) break;
+        dealt = false;
+        b = blockIdx.z;
+        continue;
+      }
+    } else {
+      if (a.splits == 1 || qn >= x1) break;
+    }
     ++b;
     qb = qn;
   }

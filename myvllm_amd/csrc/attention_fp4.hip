@@ -52,7 +52,10 @@ struct Fp4DecodeArgs : DecodeArgs {
 // ONE: pages of 16 keys, so a 16-key group is a page and starts at its slot 0, and v's
 // strides those of k.
 // FEW: a few tokens of each sequence instead of one: the columns are the query heads
-// of one token after the other, each with its own last key.
+// of one token after the other, each with its own last key.  The grid and the slots hold
+// the columns of `most` tokens; a sequence that has more of them all the same (the
+// caller's number was too small, or is a captured graph's) is read once more for each
+// further group of columns, by the workgroups of its first unit.
 template <typename T, int D, int KS, bool ONE, bool FEW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_decode_fp4_kernel(
     const Fp4DecodeArgs a) {
@@ -74,9 +77,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int64_t cap = a.tab.cols * a.tab.page;
   const int R = a.R, hgroups = a.hgroups, y = hgroups == 1 ? blockIdx.y : blockIdx.y / hgroups;
   const int kvh = y * (4 / KS) + wv / KS;
-  const int h0 = ((int)blockIdx.y - y * hgroups) * 16;
-  // this lane's column: query head cr of the kv head, token ci
-  const int ci = FEW ? (int)((uint32_t)(h0 + c16) / (uint32_t)R) : 0, cr = h0 + c16 - ci * R;
+  int h0 = ((int)blockIdx.y - y * hgroups) * 16;  // the first column
+  int most = FEW ? a.most : 0;                    // tokens whose columns are taken
   const char* const kbase = a.k.base + kvh * a.k.sh;
   const char* const vbase = a.v.base + kvh * a.v.sh;
   const uint8_t* const ksbase = a.ks.base + kvh * a.ks.sh;
@@ -105,6 +107,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   auto piece = [&](int64_t b_, int64_t lo_, int64_t hi_, int64_t slot_, int64_t) {
     // (the same in all lanes, which the compiler does not see through the lengths'
     // vector loads: descriptors made of it would be looped over)
+    // this lane's column: query head cr of the kv head, token ci
+    const int ci = FEW ? (int)((uint32_t)(h0 + c16) / (uint32_t)R) : 0, cr = h0 + c16 - ci * R;
     const int32_t b = __builtin_amdgcn_readfirstlane((int32_t)b_), slot = __builtin_amdgcn_readfirstlane((int32_t)slot_);
     const uint32_t k_lo = __builtin_amdgcn_readfirstlane((int32_t)lo_), k_hi = __builtin_amdgcn_readfirstlane((int32_t)hi_);
     // columns of the sequence, its first row of q and out, the keys that this lane's
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
     if constexpr (FEW) {
       int64_t s0, s1;
       seq_range(a.cu, a.cu64, b, a.T, s0, s1);
-      const int len = __builtin_amdgcn_readfirstlane((int32_t)(s1 - s0 < a.most ? s1 - s0 : a.most));
+      const int len = __builtin_amdgcn_readfirstlane((int32_t)(s1 - s0 < most ? s1 - s0 : most));
       cols = len * R;
       if (cols <= h0) return;
       row0 = s0;
@@ -422,7 +426,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
     }
   };
-  decode_deal(a, cap, lane, wv == 0, piece);
+  if constexpr (FEW) {
+    decode_deal(a, cap, lane, wv == 0, piece, [&]() __attribute__((always_inline)) {
+      if (blockIdx.x != 0) return false;
+      // (the arguments once more, so that none is held for this in the loops before)
+      typedef const Fp4DecodeArgs __attribute__((address_space(4))) * ArgsPtr;
+      ArgsPtr args = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      const int64_t s = clamp64(load_index_scalar(args->cu, blockIdx.z, args->cu64), 0, args->T);
+      const int64_t e = clamp64(load_index_scalar(args->cu, (int64_t)blockIdx.z + 1, args->cu64), s, args->T);
+      h0 += most != INT32_MAX ? args->most * args->R : args->hgroups * 16;
+      most = INT32_MAX;
+      return h0 < (int)(e - s) * args->R;
+    });
+  } else {
+    decode_deal(a, cap, lane, wv == 0, piece);
+  }
 }
 
 // Kv heads of a decode workgroup: one, whose keys its four waves deal among them, for heads

@@ -1102,8 +1102,8 @@ GDN_EXPORT int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_
   const int64_t N = block_tables->shape[0], Hq = q->shape[1], Hkv = k_cache->shape[2];
   if (N < 1 || max_seqlen < 1) return GDN_ERR_SHAPE;
   if (num_splits < 2 || num_splits > kMaxDecodeSplits) return GDN_ERR_RANGE;
-  // rows of the merge, groups of 16 columns and prices are counted in 31 bits
-  if (max_seqlen > kMaxGrid / Hq || N > (kMaxGrid - 64) / (max_seqlen * Hq) ||
+  // rows of the merge, columns, groups of 16 of them and prices are counted in 31 bits
+  if (q->shape[0] > (kMaxGrid / 2) / Hq || max_seqlen > kMaxGrid / Hq || N > (kMaxGrid - 64) / (max_seqlen * Hq) ||
       Hkv * ((max_seqlen * (Hq / Hkv) + 15) / 16) > kMaxGridYZ ||
       N * ((block_tables->shape[1] * k_cache->shape[1] + 15) / 16 + attn_fp4_start_price()) >= (int64_t(1) << 31))
     return GDN_ERR_RANGE;

@@ -436,7 +436,10 @@ def paged_flash_attention_prefill(
     ``softcap``, ``alibi_slopes`` and ``prefix_lens`` as in
     :func:`flash_attention_prefill`, positions and keys counted over the cache;
     with ``k_scales`` and ``v_scales`` the caches are held in 4 bits
-    (:func:`paged_kv_append`), for plain scores only."""
+    (:func:`paged_kv_append`), for plain scores only.  ``max_seqlen`` (the most
+    tokens of a sequence, read from ``cu_seqlens`` when not given, one host sync)
+    chooses among kernels and their sizes; a sequence of more tokens, as one of a
+    captured graph's later replays, has its rows all the same."""
     if k_cache.shape[1] != page_block_size:
         raise ValueError(f"page_block_size {page_block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     if k_scales is not None or v_scales is not None:
@@ -475,7 +478,7 @@ def _few_tokens(q, k_cache, block_tables, most) -> bool:
     44.1."""
     if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2 or q.shape[0] == 0 or most < 1:
         return False
-    if block_tables.shape[0] < 1 or k_cache.shape[2] < 1:
+    if block_tables.shape[0] < 1 or k_cache.shape[2] < 1 or q.shape[0] * q.shape[1] >= 2**30:
         return False
     return most * (q.shape[1] // k_cache.shape[2]) <= _FEW_COLUMNS
 

@@ -512,3 +512,60 @@ def test_graphs_share_no_workspace(dev):
     b = step(ds[0])
     torch.cuda.synchronize()
     assert torch.equal(a, want[1]) and torch.equal(b, want[0])
+
+
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", HEADS)
+@pytest.mark.parametrize("most", [1, 2, 3])
+def test_more_tokens_than_said(dev, Hq, Hkv, D, dtype, most):
+    """Sequences of more tokens than max_seqlen: every row is written, and right (as over 16-bit caches)."""
+    print(f"fp4 few, more than {most}, {Hq}/{Hkv}x{D} {dtype}", flush=True)
+    new = [most, 0, most + 1, 40, 1, most + 16]
+    ctx = [300, 20, 70, 40, 9, 900]
+    c = make(ctx, new, Hq, Hkv, D, dtype=dtype, seed=D + Hq)
+    ref, bound = reference(c, new, D**-0.5)
+    d = {n: t.to(dev) for n, t in c.items()}
+    for splits in (2, 3, 40):
+        ws = torch.full((_lib.workspace_size("paged_attention_decode_workspace_size", 6, most * Hq, D, splits),),
+                        float("nan"), device=dev)
+        o = torch.full_like(d["q"], float("nan"))
+        _lib.call("paged_attention_few_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"], d["cu"],
+                  o, ws, splits, most, D**-0.5)
+        assert_within(o, ref, bound, f"splits {splits}")
+    if is_few(c, most):
+        out = torch.full_like(d["q"], float("nan"))
+        assert_within(prefill(c, dev, D**-0.5, max_seqlen=most, out=out), ref, bound)
+
+
+def test_more_tokens_in_a_later_replay(dev):
+    """A captured graph whose offsets, lengths and table then hold other batches: longer sequences, empty ones, a
+    lone one, rows of no sequence."""
+    Hq, Hkv, D = 8, 2, 128
+    c = make([300, 200, 90, 500], [6] * 4, Hq, Hkv, D, cols=40)
+    d = {n: t.to(dev) for n, t in c.items()}
+    out = torch.empty_like(d["q"])
+    step = lambda: ops.paged_flash_attention_prefill(  # noqa: E731
+        d["q"], d["kc"], d["vc"], d["tab"], d["ctx"], d["cu"], None, 0.1, 16, max_seqlen=6, out=out, k_scales=d["ks"],
+        v_scales=d["vs"])
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for ctx, new in (([300, 200, 90, 500], [6] * 4), ([24, 7, 60, 600], [20, 0, 1, 3]), ([0, 0, 640, 0], [0, 0, 24, 0]),
+                     ([5, 31, 16, 2], [5, 7, 8, 2])):
+        x = make(ctx, new, Hq, Hkv, D, seed=sum(ctx))
+        rows = sum(new)
+        d["q"][:rows] = x["q"].to(dev)
+        d["cu"].copy_(x["cu"])
+        d["ctx"].copy_(x["ctx"])
+        d["tab"].fill_(-1)
+        d["tab"][:, :x["tab"].shape[1]] = x["tab"].to(dev)
+        for n in ("kc", "vc", "ks", "vs"):
+            m = min(x[n].shape[0], c[n].shape[0])
+            d[n][:m] = x[n][:m].to(dev)
+            x[n] = d[n].cpu()
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_within(out[:rows], *reference(x, new, 0.1))
+        assert not out[rows:].any()
