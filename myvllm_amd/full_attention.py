@@ -483,10 +483,17 @@ def _few_tokens(q, k_cache, block_tables, most) -> bool:
     return most * (q.shape[1] // k_cache.shape[2]) <= _FEW_COLUMNS
 
 
+_FEW_WORKSPACE = 2**27  # floats, 512 MiB
+
+
 def _few_workspace(N, rows, head_dim, splits, dev):
+    """The workspace, whose slots are sized by the longest sequence; None (the prefill goes in tiles) where
+    it would take more than the prefill's 512 MiB or is not to be had."""
+    n = _lib.workspace_size("paged_attention_decode_workspace_size", N, rows, head_dim, splits)
+    if n > _FEW_WORKSPACE:
+        return None
     try:
-        return torch.empty(_lib.workspace_size("paged_attention_decode_workspace_size", N, rows, head_dim, splits),
-                           dtype=torch.float32, device=dev)
+        return torch.empty(n, dtype=torch.float32, device=dev)
     except torch.OutOfMemoryError:
         return None
 

@@ -232,3 +232,17 @@ def test_python_refusals():
         ops.paged_kv_read(*caches, 16, cu_seqlens=a["cu"], **scales)
     with pytest.raises(ValueError, match="block_size"):
         ops.paged_kv_read(*caches, 32, **scales)
+
+
+def test_few_tokens_workspace():
+    """At most 512 MiB, as the prefill's docstring says: one long sequence among many sizes all slots."""
+    from myvllm_amd.full_attention import _few_workspace
+
+    size = lambda *s: _lib.workspace_size("paged_attention_decode_workspace_size", *s)  # noqa: E731
+    for N, rows, D, splits in ((1024, 64 * 16, 64, 2), (4096, 8 * 16, 256, 2)):
+        assert size(N, rows, D, splits) > 2**27
+        assert _few_workspace(N, rows, D, splits, "meta") is None
+    for N in range(950, 1000):
+        n, ws = size(N, 1024, 64, 2), _few_workspace(N, 1024, 64, 2, "meta")
+        assert (ws is None) == (n > 2**27) and (ws is None or ws.numel() == n)
+    assert size(950, 1024, 64, 2) <= 2**27 < size(999, 1024, 64, 2)

@@ -569,3 +569,21 @@ def test_more_tokens_in_a_later_replay(dev):
         torch.cuda.synchronize()
         assert_within(out[:rows], *reference(x, new, 0.1))
         assert not out[rows:].any()
+
+
+def test_few_tokens_of_many(dev):
+    """One sequence of 64 tokens among 1,023 of one: the few-tokens form's slots would take 544 MiB, so it goes in
+    tiles, within the 512 MiB."""
+    Hq = Hkv = 16
+    D, new = 64, [1] * 700 + [64] + [1] * 323
+    g = torch.Generator().manual_seed(4)
+    ctx = [n + int(x) for n, x in zip(new, torch.randint(0, 12, (1024,), generator=g))]
+    c = make(ctx, new, Hq, Hkv, D)
+    assert is_few(c, 64)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(dev)
+    torch.cuda.reset_peak_memory_stats(dev)
+    o = prefill(c, dev, 0.1, max_seqlen=64)
+    inputs = sum(t.numel() * t.element_size() for t in c.values())
+    assert torch.cuda.max_memory_allocated(dev) - before < 2**29 + 2 * inputs
+    assert_within(o, *reference(c, new, 0.1))
