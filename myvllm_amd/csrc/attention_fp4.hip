@@ -527,8 +527,8 @@ hipError_t launch_prefill_fp4_tiles(const Fp4AttnArgs& a, int64_t nseq, hipStrea
 }
 
 template <typename T, int D>
-hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, int64_t max_len, hipStream_t st) {
-  if (nseq <= 0 || max_len <= 0 || a.tab.num_blocks == 0) {
+hipError_t launch_prefill_fp4(const Fp4AttnArgs& a, int64_t nseq, hipStream_t st) {
+  if (nseq <= 0 || a.tab.num_blocks == 0) {
     // (without a block to read every row is zero: those of no sequence are all of them)
     zero_uncovered_rows_kernel<(int)sizeof(T)><<<dim3(64), dim3(256), 0, st>>>(
         a.o, a.o_st, a.o_sh, a.Hq, a.dim, a.cu, a.cu64, a.tab.num_blocks == 0 ? 0 : a.nseq, a.T);
@@ -605,7 +605,7 @@ hipError_t attn_few_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const 
 hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                    const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
                                    const gdn_tensor* ctx, const gdn_tensor* cu, gdn_tensor* out, float* workspace,
-                                   int64_t max_seqlen, float scale, hipStream_t st) {
+                                   float scale, hipStream_t st) {
   if (q->shape[0] == 0) return hipSuccess;
   Fp4AttnArgs a{};
   static_cast<AttnArgs&>(a) = paged_args(q, kc, vc, tab, ctx, cu, out, workspace, scale);
@@ -614,11 +614,11 @@ hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, co
   const int D = (int)q->shape[2];
   const int64_t N = cu->shape[0] - 1;
   if (q->dtype == GDN_DTYPE_BF16) {
-    if (D == 64) return launch_prefill_fp4<bf16_t, 64>(a, N, max_seqlen, st);
-    if (D == 128) return launch_prefill_fp4<bf16_t, 128>(a, N, max_seqlen, st);
-    return launch_prefill_fp4<bf16_t, 256>(a, N, max_seqlen, st);
+    if (D == 64) return launch_prefill_fp4<bf16_t, 64>(a, N, st);
+    if (D == 128) return launch_prefill_fp4<bf16_t, 128>(a, N, st);
+    return launch_prefill_fp4<bf16_t, 256>(a, N, st);
   }
-  if (D == 64) return launch_prefill_fp4<f16_t, 64>(a, N, max_seqlen, st);
-  if (D == 128) return launch_prefill_fp4<f16_t, 128>(a, N, max_seqlen, st);
-  return launch_prefill_fp4<f16_t, 256>(a, N, max_seqlen, st);
+  if (D == 64) return launch_prefill_fp4<f16_t, 64>(a, N, st);
+  if (D == 128) return launch_prefill_fp4<f16_t, 128>(a, N, st);
+  return launch_prefill_fp4<f16_t, 256>(a, N, st);
 }

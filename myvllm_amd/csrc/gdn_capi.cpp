@@ -92,7 +92,7 @@ hipError_t attn_decode_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, con
 hipError_t attn_prefill_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc,
                                    const gdn_tensor* ks, const gdn_tensor* vs, const gdn_tensor* tab,
                                    const gdn_tensor* ctx, const gdn_tensor* cu, gdn_tensor* out, float* workspace,
-                                   int64_t max_seqlen, float scale, hipStream_t st);
+                                   float scale, hipStream_t st);
 hipError_t attn_few_fp4_launch(const gdn_tensor* q, const gdn_tensor* kc, const gdn_tensor* vc, const gdn_tensor* ks,
                                const gdn_tensor* vs, const gdn_tensor* tab, const gdn_tensor* ctx, const gdn_tensor* cu,
                                gdn_tensor* out, float* workspace, int32_t splits, int32_t most, float scale,
@@ -1086,8 +1086,7 @@ GDN_EXPORT int paged_attention_prefill_fp4(const gdn_tensor* q, const gdn_tensor
   // (the kernel reads the first column of every sequence)
   if (block_tables->shape[0] > 0 && block_tables->shape[1] == 0) return GDN_ERR_SHAPE;
   return launch_rc(attn_prefill_fp4_launch(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens,
-                                           cu_seqlens, out, ws, max_seqlen, scale,
-                                           reinterpret_cast<hipStream_t>(stream)));
+                                           cu_seqlens, out, ws, scale, reinterpret_cast<hipStream_t>(stream)));
 }
 
 GDN_EXPORT int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,

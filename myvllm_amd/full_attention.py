@@ -439,7 +439,8 @@ def paged_flash_attention_prefill(
     (:func:`paged_kv_append`), for plain scores only.  ``max_seqlen`` (the most
     tokens of a sequence, read from ``cu_seqlens`` when not given, one host sync)
     chooses among kernels and their sizes; a sequence of more tokens, as one of a
-    captured graph's later replays, has its rows all the same."""
+    captured graph's later replays, has its rows all the same (over 16-bit caches 0
+    says that there are none)."""
     if k_cache.shape[1] != page_block_size:
         raise ValueError(f"page_block_size {page_block_size} != k_cache.shape[1] {k_cache.shape[1]}")
     if k_scales is not None or v_scales is not None:

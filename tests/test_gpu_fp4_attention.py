@@ -587,3 +587,20 @@ def test_few_tokens_of_many(dev):
     inputs = sum(t.numel() * t.element_size() for t in c.values())
     assert torch.cuda.max_memory_allocated(dev) - before < 2**29 + 2 * inputs
     assert_within(o, *reference(c, new, 0.1))
+
+
+@pytest.mark.parametrize("most", [0, 1])
+def test_tiles_of_more_tokens_than_said(dev, most):
+    """The prefill in tiles takes its sequences from the offsets alone; with empty ones only, every row is zero."""
+    new = [70, 0, 1, 33]
+    for Hq, Hkv, D, dtype in HEADS[:4]:
+        c = make([90, 4, 300, 33], new, Hq, Hkv, D, dtype=dtype)
+        d = {n: t.to(dev) for n, t in c.items()}
+        o = torch.full_like(d["q"], float("nan"))
+        _lib.call("paged_attention_prefill_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"], d["cu"],
+                  o, None, most, 0.1)
+        assert_within(o, *reference(c, new, 0.1))
+        if most == 0:
+            assert_within(prefill(c, dev, 0.1, max_seqlen=0), *reference(c, new, 0.1))
+        out = torch.full_like(d["q"], float("nan"))
+        assert not prefill(dict(c, cu=torch.zeros_like(c["cu"])), dev, 0.1, out=out).any()
