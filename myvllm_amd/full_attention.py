@@ -617,8 +617,8 @@ def _axes(positions, sections, cos):
         raise ValueError("positions are (T,) or (axes, T) with one to four axes and as many sections")
     if sum(sections) != cos.shape[1] or min(sections) < 0:
         raise ValueError(f"sections {tuple(sections)} are not the {cos.shape[1]} frequencies of cos and sin")
-    if positions.stride(1) != 1:
-        positions = positions.contiguous()
+    if positions.stride(1) != 1:  # (contiguous() leaves a lone token's stride as it is)
+        positions = positions.clone(memory_format=torch.contiguous_format)
     return positions, tuple(int(n) for n in sections) + (0,) * (4 - len(sections))
 
 

@@ -246,3 +246,18 @@ def test_few_tokens_workspace():
         n, ws = size(N, 1024, 64, 2), _few_workspace(N, 1024, 64, 2, "meta")
         assert (ws is None) == (n > 2**27) and (ws is None or ws.numel() == n)
     assert size(950, 1024, 64, 2) <= 2**27 < size(999, 1024, 64, 2)
+
+
+@pytest.mark.parametrize("T", [1, 2, 5])
+@pytest.mark.parametrize("axes", [1, 3])
+def test_positions_of_any_stride(T, axes):
+    """Positions kept token by token, (T, axes) turned over, and every other one of a longer list: copied, one token
+    as several."""
+    from myvllm_amd.full_attention import _axes
+
+    cos = Z(48, 32)
+    wide = torch.arange(8 * 4 * axes, dtype=I32).view(8, 4 * axes)
+    for p in (wide[:T, :axes].t(), wide[:T, ::4].t(), wide.t()[::4, :2 * T:2]) + ((wide[:T, 0],) if axes == 1 else ()):
+        rows = p if p.dim() == 2 else p[None]
+        got, of = _axes(p, (32,) if axes == 1 else (12, 10, 10), cos)
+        assert torch.equal(got, rows) and got.stride(1) == 1 and sum(of) == 32

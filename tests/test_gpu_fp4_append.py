@@ -370,3 +370,20 @@ def test_block_maxima(dev, D, rot, inter):
         c[x] = (rows * size[..., None]).flatten(-2).to(BF)
     cos, sin = rope(T, rot) if rot else (None, None)
     check(c, dev, cos=cos, sin=sin, interleaved=inter)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_one_token_with_positions_kept_token_by_token(dev, bits):
+    """One token's positions as a column of (T, axes), whose tokens lie `axes` apart, as of several tokens."""
+    cos, sin = rope(64, 128)
+    wide = torch.randint(0, 64, (6, 3), generator=torch.Generator().manual_seed(1)).int().to(dev)
+    for n in (1, 2, 6):
+        c = make([n], [40], bits=bits, seed=n)
+        d = {x: t.to(dev) for x, t in c.items()}
+        q = append(d, 16, cos=cos.to(dev), sin=sin.to(dev), positions=wide[:n].t(), sections=(22, 21, 21))
+        e = {x: t.to(dev) for x, t in c.items()}
+        want, _ = check(c, dev, cos=cos, sin=sin, positions=wide[:n].t().cpu().contiguous(), sections=(22, 21, 21))
+        turned = append(e, 16, cos=cos.to(dev), sin=sin.to(dev), positions=wide[:n].cpu().t().contiguous().to(dev),
+                        sections=(22, 21, 21))
+        torch.cuda.synchronize()
+        assert torch.equal(q, turned) and all(torch.equal(d[x], want[x]) for x in ("kc", "vc"))
