@@ -127,3 +127,23 @@ def test_paged_cache_compaction(dev, bits):
     for s, was in rows.items():
         assert all(torch.equal(t[:, c.blocks[s]], x) for t, x in zip(c._tensors(), was))
     assert c.compact() == 0
+
+
+@pytest.mark.parametrize("n, streams", [(779, False), (780, True), (1300, True)])
+def test_large_copies(dev, n, streams):
+    """32 MiB and more go by stores past the caches: two caches, several launches of 448 pairs, blocks that end inside a
+    workgroup's 4 KB, and a kernel that reads the blocks straight after the copy."""
+    print(f"cache copy of {n} large blocks", flush=True)
+    blocks = 2 * n + 5
+    a = torch.randint(-128, 127, (4, blocks, 4352), dtype=torch.int16, device=dev)  # blocks of 8,704 bytes
+    b = torch.randint(0, 256, (2, blocks, 257, 16), dtype=torch.uint8, device=dev)  # of 4,112
+    assert (n * (4 * 8704 + 2 * 4112) >= 2**25) == streams
+    src, dst = pairs(blocks, n, n)
+    s, d = (torch.tensor(x, device=dev) for x in (src, dst))
+    want = [t.clone().index_copy_(1, d, t[:, s]) for t in (a, b)]
+    torch.cuda.synchronize()
+    cache_copy([a, b], src, dst)
+    read = [t[:, d] + 1 for t in (a, b)]
+    torch.cuda.synchronize()
+    for t, w, r in zip((a, b), want, read):
+        assert torch.equal(t, w) and torch.equal(r, w[:, d] + 1)
