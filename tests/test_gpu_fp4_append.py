@@ -387,3 +387,31 @@ def test_one_token_with_positions_kept_token_by_token(dev, bits):
                         sections=(22, 21, 21))
         torch.cuda.synchronize()
         assert torch.equal(q, turned) and all(torch.equal(d[x], want[x]) for x in ("kc", "vc"))
+
+
+def test_append_past_4_gib(dev):
+    """Rows other than those that are there, into blocks whose bytes lie past 2^32 of the cache's start; the blocks at
+    those addresses less 2^32 stay as they were."""
+    page, Hkv, D = 16, 2, 256
+    per = page * Hkv * D // 2
+    blocks = (2**32 + 2**28) // per
+    low = 2**32 // per
+    g = torch.Generator().manual_seed(9)
+    kc, vc = (torch.zeros(blocks, page, Hkv, D // 2, dtype=torch.uint8, device=dev) for _ in range(2))
+    ks, vs = (torch.full((blocks, Hkv, D // 32, page), 127, dtype=torch.uint8, device=dev) for _ in range(2))
+    at = [blocks - 1, low, low + 77]
+    tab, ctx = torch.tensor([at], dtype=torch.int32, device=dev), torch.tensor([41], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 41], dtype=torch.int32, device=dev)
+    for turn in range(2):
+        k, v = (torch.randn(41, Hkv, D, generator=g).to(BF) for _ in range(2))
+        ops.paged_kv_append(None, k.to(dev), v.to(dev), kc, vc, tab, ctx, page, cu_seqlens=cu, k_scales=ks, v_scales=vs)
+        got = ops.paged_kv_read(kc, vc, tab, ctx, page, 41, cu, k_scales=ks, v_scales=vs)
+        torch.cuda.synchronize()
+        for mine, rows, codes, scales in ((got[0], k, kc, ks), (got[1], v, vc, vs)):
+            c, s = pack_ref(rows)
+            assert torch.equal(mine.cpu().double(), unpack_ref(c, s))
+            for i, b in enumerate(at):
+                m = min(41 - 16 * i, 16)
+                assert torch.equal(codes[b, :m].cpu(), c[16 * i:16 * i + m])
+                assert torch.equal(scales[b, :, :, :m].cpu(), s[16 * i:16 * i + m].permute(1, 2, 0))
+                assert not codes[b - low].any() and (scales[b - low] == 127).all()
