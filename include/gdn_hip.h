@@ -540,8 +540,8 @@ int paged_kv_read(gdn_tensor* k, gdn_tensor* v, const gdn_tensor* k_cache, const
  * to be the type that was appended.  Workspaces and their sizes are the 16-bit ops'; a
  * NULL workspace leaves the prefill unsplit.  Page strides below 2^32 bytes, and tables
  * below 2^31 keys (GDN_ERR_RANGE); the prefill's table has a column at least
- * (GDN_ERR_SHAPE).  Sums are fp32: 2^8 keys max|v| is to stay below 2^128.  A NaN among a
- * prefill's values may reach all queries of its key tile.
+ * (GDN_ERR_SHAPE).  Sums are fp32: 2^8 keys max|v| is to stay below 2^128.  A NaN (scale
+ * byte 255) reaches the queries that see its key, and no others.
  */
 int paged_attention_decode_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, const gdn_tensor* v_cache,
                                const gdn_tensor* k_scales, const gdn_tensor* v_scales, const gdn_tensor* block_tables,

@@ -54,6 +54,14 @@ GDN_DEVICE float max_lane_pair32(float x) {
   return a > b ? a : b;
 }
 
+// The lane's number worked out where it is asked for: for rare branches, whose
+// addresses would otherwise be worked out ahead of the loop and held in registers.
+GDN_DEVICE uint32_t lane_anew() {
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));
+  return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
+
 GDN_DEVICE int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
 // An index at a wave-uniform position read through the scalar data cache (a

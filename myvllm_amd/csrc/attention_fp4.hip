@@ -71,6 +71,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   constexpr int LDO = D + 4;
   __shared__ __align__(16) float ob[KS > 1 ? 4 * 16 * LDO : 4];
   __shared__ float ml[4][2][16];
+  // FEW: of each wave, the first key whose value is NaN in each 32 dims among those that only
+  // some columns see: a probability of 0 would not keep it from the others, so its
+  // scale is cleared and the columns that see it get their NaN at the end
+  __shared__ uint32_t nan_at[FEW ? 4 * (D / 32) : 1];
 
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, grp = lane >> 4, part = wv % KS;
@@ -139,6 +143,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       const int i = FEW ? (int)((uint32_t)(h0 + h) / (uint32_t)R) : 0;
       return reinterpret_cast<T*>(a.o) + (row0 + i) * a.o_ss + (int64_t)(kvh * R + h0 + h - i * R) * a.o_sh;
     };
+    if constexpr (FEW) {
+      if (lane < D / 32) nan_at[wv * (D / 32) + lane] = UINT32_MAX;
+    }
     if (k_hi == 0) {  // no keys: zero rows (and no table column that could be read)
       constexpr int LR = D / 4;
       for (int h = part * (16 / KS) + lane / LR; h < (part + 1) * (16 / KS); h += 64 / LR)
@@ -277,6 +284,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
             if (j >= lim) s[h][r] = -INFINITY;
             if (j >= k_hi) vs[h] &= ~(255u << (8 * r));  // (a stale scale may stand for NaN)
           }
+        if constexpr (FEW) {
+          // (bytes of 255)
+          auto full = [](uint32_t x) { return ((x & 0x7F7F7F7Fu) + 0x01010101u) & x & 0x80808080u; };
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64((full(vs[0]) | full(vs[1])) != 0) != 0, 0)) {
+            const uint32_t l = lane_anew();
+            uint32_t at = UINT32_MAX;
+#pragma unroll
+            for (int h = 1; h >= 0; --h) {
+              const uint32_t j = j0 + 16u * h + 4u * (l >> 4);  // the word's first key
+              const uint32_t all = lim0 > j ? lim0 - j : 0u;    // of its keys, those that all columns see
+              const uint32_t some = all < 4u ? full(vs[h]) >> 7 & ~0u << (8 * all) : 0u;
+              at = some != 0u ? j + __builtin_ctz(some) / 8 : at;
+              vs[h] &= ~(255u * some);
+            }
+            __hip_atomic_fetch_min(&nan_at[wv * (D / 32) + VE * (l & 15u) / 32], at, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_WAVEFRONT);
+          }
+        }
       }
       float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
       mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -356,6 +381,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       }
     }
 
+    if constexpr (FEW) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      const uint32_t l = lane_anew();
+      const uint32_t* const at = nan_at + wv * (D / 32) + VE * 4 * (l >> 4) / 32;
+      const uint32_t at0 = at[0], at1 = VE == 16 ? at[1] : at0;  // of this lane's rows 0, 1 and 2, 3
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64((at0 < at1 ? at0 : at1) < lim) != 0, 0)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int d = 0; d < VE; ++d) oacc[d][r] = (r < 2 ? at0 : at1) < lim ? __builtin_nanf("") : oacc[d][r];
+      }
+    }
     float lt = lsum + __shfl_xor(lsum, 16);
     lt += __shfl_xor(lt, 32);
     if constexpr (KS == 1) {

@@ -429,6 +429,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   // CUs each) in turn, so every sequence spreads over all of them, and a
   // sequence's workgroups run together and share its K/V rows in L2.
   __shared__ int32_t lookup[8];
+  // (kFp4) the first key whose value is NaN in each 32 dims: a probability of 0 would
+  // not keep it from the queries before it, so its numbers go to LDS as finite ones
+  // and the queries that see it get their NaN at the end (16 prompts of 1,024 tokens, 16 / 2 heads
+  // of 256 287 -> 294 us, four chunks of 1,500 behind 7,500 keys 978 -> 989; a branch
+  // that writes to LDS at once 298 and 994)
+  __shared__ uint32_t nan_at[Q4 ? NDT : 1];
+  if (Q4 && tid < NDT) nan_at[tid] = UINT32_MAX;
   const int hg = a.Hq / gh;  // head groups
   // (the grid's rows end with one tile's head groups more than the sequences
   // can have; a split grid's extra workgroups come after them)
@@ -808,14 +815,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
       load_tile(t, kd, vd);
     }
   };
-  auto store = [&](int buf, const Reg* kd, const Reg* vd) __attribute__((always_inline)) {
+  uint32_t nan_tile = UINT32_MAX;  // (kFp4) the first tile in which this thread's numbers of a value are NaN
+  auto store = [&](int t, int buf, const Reg* kd, const Reg* vd) __attribute__((always_inline)) {
     if constexpr (Q4) {
       const int row = tid / QL8, ch = tid % QL8;
       // neighbouring lanes write their words in another order each, so that their
       // 16-byte stores, QE elements apart, fall on different banks
       const int turn = QW == 4 ? (ch + (ch >> 2)) & 3 : QW == 2 ? ch >> 2 & 1 : 0;
-      auto put = [&](T* at, const Codes& c) __attribute__((always_inline)) {
-        uint32_t x[QW], sb = c.s;
+      auto put = [&](T* at, const Codes& c, uint32_t scale) __attribute__((always_inline)) {
+        uint32_t x[QW], sb = scale;
 #pragma unroll
         for (int i = 0; i < QW; ++i) x[i] = c.w[i];
         if (!c.named) {
@@ -843,8 +851,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
 #pragma unroll
         for (int i = 0; i < QW; ++i) *reinterpret_cast<uint4*>(at + QE * ch + 8 * (i ^ turn)) = fp4_eight<T>(x[i], s);
       };
-      put(&ks[buf][row * LDK], kd[0]);
-      put(&vs[buf][row * LDV], vd[0]);
+      put(&ks[buf][row * LDK], kd[0], kd[0].s);
+      const bool nan = vd[0].named && vd[0].s == 255u;
+      const uint32_t in = nan ? (uint32_t)t : UINT32_MAX;
+      nan_tile = in < nan_tile ? in : nan_tile;
+      put(&vs[buf][row * LDV], vd[0], nan ? 0u : vd[0].s);
     } else {
       store_tile(buf, kd, vd);
     }
@@ -1067,7 +1078,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   const int ntiles = (int)((kend + BN - 1) / BN);
   stage_q();  // (waits for the query loads with tile 0's loads in flight)
   if constexpr (FORM == kScored) score_consts();
-  store(0, kA, vA);
+  store(tile0, 0, kA, vA);
   load(tile0 + 1, kB, vB);
   load(tile0 + 2, kA, vA);
   __syncthreads();
@@ -1077,28 +1088,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
   for (int t = tile0; t < ntiles; t += 2) {
     if constexpr (PG == 0) {
       compute(t, 0, [&]() __attribute__((always_inline)) {
-        store(1, kB, vB);
+        store(t + 1, 1, kB, vB);
         load(t + 3, kB, vB);
       });
       __syncthreads();
       compute(t + 1, 1, [&]() __attribute__((always_inline)) {
-        store(0, kA, vA);
+        store(t + 2, 0, kA, vA);
         load(t + 4, kA, vA);
       });
       __syncthreads();
     } else {
       const auto after = []() {};  // (one instantiation of compute for both calls)
       compute(t, 0, after);
-      store(1, kB, vB);
+      store(t + 1, 1, kB, vB);
       load(t + 3, kB, vB);
       __syncthreads();
       compute(t + 1, 1, after);
-      store(0, kA, vA);
+      store(t + 2, 0, kA, vA);
       load(t + 4, kA, vA);
       __syncthreads();
     }
   }
 
+  if constexpr (Q4) {
+    const uint32_t u = 64 * w + lane_anew();
+    if (nan_tile != UINT32_MAX)
+      __hip_atomic_fetch_min(&nan_at[u % QL8 * QE / 32], nan_tile * BN + u / QL8, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_WORKGROUP);
+    __syncthreads();
+    const uint32_t keys = (uint32_t)seen(q0 + (u & 31u) + 1);  // that this lane's query sees
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) {
+      const bool nan = nan_at[d] < keys;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(nan) != 0, 0)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[d][r] = nan ? __builtin_nanf("") : oacc[d][r];
+      }
+    }
+  }
   const float lt = lsum + __shfl_xor(lsum, 32);
   if constexpr (SPLIT || FORM == kShared) {
     if (FORM == kShared || !whole) {

@@ -6,6 +6,7 @@ import torch
 
 import myvllm_amd as ops
 from attention_bounds import assert_within
+from myvllm_amd import _lib
 from oracle.fp4 import cache_values
 from test_gpu_fp4_attention import decode, is_few, make, prefill, reference
 
@@ -115,3 +116,68 @@ def test_prefill_fp4(dev, Hq, Hkv, D, dtype, few):
     nan[at[4] - 2:at[4], :R] = True
     print(f"fp4 prefill NaN {Hq}/{Hkv}x{D} few {few}", flush=True)
     check(prefill(c, dev, D**-0.5), ref, bound, nan)
+
+
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", SHAPES)
+@pytest.mark.parametrize("new, ctx", [([4, 3, 1, 0, 4], [700, 35, 481, 20, 4]), ([70, 3, 130, 0, 33], [700, 35, 130, 20, 4000]),
+                                      ([2, 9, 70], [4000, 2001, 1500])])
+def test_values_that_only_later_queries_see(dev, Hq, Hkv, D, dtype, new, ctx):
+    """NaN among the values of the new tokens: rows before them are as without it (a weight of 0 would not keep it
+    out), in the few-tokens form and in tiles, split and not."""
+    R, far = Hq // Hkv, len(new) == 3
+    c = make(ctx, new, Hq, Hkv, D, dtype=dtype, seed=D, cols=1000 if far else 0)
+    few = is_few(c, max(new))
+    assert few == (max(new) * R <= 64)
+    ref, bound = reference(c, new, D**-0.5)
+    nan = torch.zeros(ref.shape, dtype=torch.bool)
+    at = [sum(new[:i]) for i in range(len(new) + 1)]
+
+    def bad(n, j, h, blocks):  # key j: the rows from position j on see it
+        set_nan(c, "v", n, j, h, blocks)
+        row = at[n] + max(0, j - (ctx[n] - new[n]))
+        for b in blocks:
+            nan[row:at[n + 1], h * R:(h + 1) * R, 32 * b:32 * b + 32] = True
+
+    bad(0, ctx[0] - 1, 0, [0])
+    bad(0, ctx[0] - 2, 1, [1])
+    bad(1, ctx[1] - 2, 0, range(D // 32))
+    bad(1, 7, 1, [0])  # all rows see it
+    bad(1, ctx[1] - 1, 1, [0, 1])
+    bad(2, ctx[2] - 1, 1, [D // 32 - 1])
+    if new[2] > 20:
+        bad(2, ctx[2] - 17, 1, [0])
+        bad(2, ctx[2] - 33, 0, [0])
+        bad(2, ctx[2] - 20, 0, [0, 1])
+    if len(new) > 4:
+        bad(4, ctx[4] - 1, 0, [1])
+        bad(4, ctx[4] - 3, 0, [1])
+    print(f"fp4 NaN values {Hq}/{Hkv}x{D} new={new} few={few}", flush=True)
+    check(prefill(c, dev, D**-0.5), ref, bound, nan)
+    d = {n: t.to(dev) for n, t in c.items()}
+    o = torch.empty_like(d["q"])
+    _lib.call("paged_attention_prefill_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"], d["cu"], o,
+              None, max(new), D**-0.5)
+    check(o, ref, bound, nan)
+    for splits in (2, 40):
+        ws = torch.empty(_lib.workspace_size("paged_attention_decode_workspace_size", len(new), 4 * Hq, D, splits),
+                         device=dev)
+        o.fill_(float("inf"))
+        _lib.call("paged_attention_few_fp4", d["q"], d["kc"], d["vc"], d["ks"], d["vs"], d["tab"], d["ctx"], d["cu"], o,
+                  ws, splits, 4, D**-0.5)
+        check(o, ref, bound, nan)
+
+
+@pytest.mark.parametrize("few", [True, False])
+def test_rows_that_see_no_key(dev, few):
+    """Queries before position 0 are zero whatever the values, and the stale ones past the length, hold."""
+    Hq, Hkv, D = 8, 2, 128
+    new, ctx = ([6, 4], [3, 2]) if few else ([60, 40], [33, 2])
+    c = make(ctx, new, Hq, Hkv, D)
+    assert is_few(c, max(new)) == few
+    set_nan(c, "v", 0, slice(None), 0)
+    set_nan(c, "v", 1, 1, 1)
+    o = prefill(c, dev, 0.1).cpu()
+    a, b = new[0] - ctx[0], new[0] + new[1] - ctx[1]
+    assert not o[:a].any() and o[a:new[0], :4].isnan().all() and not o[a:new[0], 4:].isnan().any()
+    assert not o[new[0]:b].any() and not o[b:, :4].isnan().any() and not o[b, 4:].isnan().any()
+    assert o[b + 1, 4:].isnan().all()
