@@ -505,6 +505,9 @@ def _paged_prefill_fp4(q, k_cache, v_cache, k_scales, v_scales, block_tables, co
     if max_seqlen is None:
         max_seqlen = _max_seqlen(cu_seqlens)
     q, k_cache, v_cache, k_scales, v_scales = _fp4_aligned(q, k_cache, v_cache, k_scales, v_scales)
+    if block_tables.dim() == 2 and block_tables.shape[1] == 0:
+        # (no keys, so zero rows; the tiles' kernel reads a column, which then names no block)
+        block_tables = torch.nn.functional.pad(block_tables, (0, 1), value=-1)
     o = _out_for(out, q.shape, q.dtype, dev)
     if _few_tokens(q, k_cache, block_tables, int(max_seqlen)):
         N, most, cap = block_tables.shape[0], int(max_seqlen), block_tables.shape[1] * k_cache.shape[1]

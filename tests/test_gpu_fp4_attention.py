@@ -604,3 +604,17 @@ def test_tiles_of_more_tokens_than_said(dev, most):
             assert_within(prefill(c, dev, 0.1, max_seqlen=0), *reference(c, new, 0.1))
         out = torch.full_like(d["q"], float("nan"))
         assert not prefill(dict(c, cu=torch.zeros_like(c["cu"])), dev, 0.1, out=out).any()
+
+
+@pytest.mark.parametrize("new", [[3, 1], [290, 1]])
+def test_tables_without_columns(dev, new):
+    """No keys at all: zero rows, in a few tokens and in tiles, as over 16-bit caches."""
+    c = make([300, 20], new, 4, 2, 128)
+    c["tab"] = c["tab"][:, :0]
+    out = torch.full_like(c["q"], float("nan")).to(dev)
+    assert not prefill(c, dev, 0.1, out=out).any()
+    k, v = (cache_values(c[x + "c"], c[x + "s"]).nan_to_num(0).to(BF).to(dev) for x in "kv")
+    o = ops.paged_flash_attention_prefill(c["q"].to(dev), k, v, c["tab"].to(dev), c["ctx"].to(dev), c["cu"].to(dev), None,
+                                          0.1, 16)
+    torch.cuda.synchronize()
+    assert not o.any()
