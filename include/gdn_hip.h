@@ -509,9 +509,10 @@ int paged_kv_append(const gdn_tensor* k, const gdn_tensor* v, gdn_tensor* k_cach
  *   plus 8 for the sign) of the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times the scale,
  *   of two as near the one with the even code, past 6 scales of 6; the first of two
  *   codes is in the low half of their byte.  32 numbers with an infinity or a NaN among
- *   them get the scale byte 255, which reads as NaN.  The numbers are those that a
- *   16-bit cache would hold; keys are rotated in fp64 for it.  Pages of a multiple of
- *   16 slots (GDN_ERR_SHAPE); rows of codes 16-byte, scales 4-byte aligned.
+ *   them get the scale byte 255, which reads as NaN.  The numbers are values as they
+ *   are, and keys rotated in fp64 and rounded through fp32 to their type, which may be the
+ *   neighbours of those that a 16-bit cache, rotated in fp32, would hold.  Pages of a
+ *   multiple of 16 slots (GDN_ERR_SHAPE); rows of codes 16-byte, scales 4-byte aligned.
  * All else as for paged_kv_append.  GDN_ERR_ARG for negative sections and sections
  * that do not add up to rot / 2.
  */

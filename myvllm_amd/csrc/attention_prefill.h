@@ -87,8 +87,8 @@ constexpr bool q_pieces_inside(int dq) {
 // block table (one lookup per 16 rows, a tile ahead, 32-bit arithmetic); kFp4 also 4,
 // an int32 table, pages of 16 keys, and v's strides those of k, which holds fewer scalar
 // registers: four chunks of up to 2,048 tokens over up to 16,384 keys, 16 / 2 heads of
-// 256 945 us, by PG 2 1,090 (16-bit caches 997); 16 prompts of up to 4,096 774 and 822;
-// the four chunks with 16 heads of 64 300 and 352
+// 256 950 us, by PG 2 1,110 (16-bit caches 1,005); 16 prompts of up to 4,096 785 and 851;
+// the four chunks with 16 heads of 64 293 and 343
 // Workgroup id -> (sequence, query tile): tiles of tile_len queries (a power
 // of two), laid out sequence after sequence over the tiles that exist (no
 // workgroup of a padded grid exits idle).  Below D = 256 batches of up to 64

@@ -29,8 +29,8 @@
 // FP4: the caches hold codes and block scales (fp4.h) of the rows that the
 // 16-bit cache would hold.  A block's 32 numbers lie in two to four lanes,
 // wherever the rotation's pairs put them, so its largest magnitude is taken by an
-// LDS maximum of the wave (30,447 tokens of 16 / 2 heads of 256, 608 MB, 104 us, 5.8
-// TB/s, 99 % of a streaming copy; the 16-bit cache 112).  Keys are rotated in 64 bits there (products of a
+// LDS maximum of the wave (30,447 tokens of 16 / 2 heads of 256, 608 MB, 105 us by itself, 5.8
+// TB/s, 98 % of a streaming copy, 108 in turn with a read; the 16-bit cache 112; with three axes 121).  Keys are rotated in 64 bits there (products of a
 // 16-bit and a 32-bit number are exact in them): next to a border between two
 // codes the last bit of a fp32 sum would choose another one now and then.
 #include "fp4.h"
@@ -276,8 +276,9 @@ __global__ __launch_bounds__(256) void paged_kv_append_kernel(
 // so are those of a table entry outside [0, num_blocks).
 //
 // Bound: HBM, and the chain of offsets, length, table and codes: 30,447 tokens of 2 heads of
-// 256 in 4 bits (79 MB) 18 us, 13.5 at the copy's rate; with 1, 4 and 8 rows a lane 18.8,
-// 19.6 and 24.2, and 23.1 where each row waits for its own lookup.
+// 256 in 4 bits (79 MB) 18 us by itself, 22 in turn with the append, 13.5 at the copy's rate; by
+// itself with 1, 4 and 8 rows a lane 18.8, 19.6 and 24.2, and 23.1 where each row waits for
+// its own lookup.  From 16-bit caches (125 MB) 21.5, the copy's rate.
 struct ReadArgs {
   AppendExArgs in;  // caches, tables, lengths; T, nseq, Hkv
   void *k, *v;

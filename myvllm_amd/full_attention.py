@@ -276,7 +276,7 @@ def fp4_decode_num_splits(num_seqs: int, num_q_heads: int, num_kv_heads: int, he
     dims want three (16 of U[1000, 8000], 16 heads: 256 workgroups 35.3, 768 28.8; 48
     of U[300, 3000]: 47.6 and 32.5), and so do a few tokens a sequence (``few``),
     whose shorter sequences leave some of their groups of columns empty (12 sequences
-    of 3 to 9 tokens over 6,000 keys, 16 heads of 64: 256 workgroups 32.8, 768 26.8; 32
+    of 3 to 9 tokens over 6,000 keys, 16 heads of 64: 256 workgroups 34.3, 768 27.5; 32
     of them, 16 / 4 of 128: 63.0 and 42.6).  At least 256 keys a unit of heads of 256
     (one sequence of 2,943 keys, 2 heads: 12 units 13.4 us, 8 14.8, 32 15.0), 192 of
     smaller ones (of 3,000 keys, 4 heads of 128: 16 units 11.5, 12 12.7, 24 12.6); at
@@ -472,11 +472,12 @@ _FEW_COLUMNS = 64
 def _few_tokens(q, k_cache, block_tables, most) -> bool:
     """Whether a prefill over caches held in 4 bits goes by the decode's kernel, whose
     groups of 16 columns (query heads of a kv head, times tokens) each pass over the
-    keys, or in tiles of 32 queries.  Over 6,000 keys, few / tiles: 12 sequences of 8
-    tokens, 16 / 2 heads of 256 (64 columns) 44.5 / 72.6 us, 16 tokens 63.7 / 73.6, 32
-    88.2 / 75.9; 16 / 4 of 128, 16 tokens (64 columns) 36.5 / 49.2, 32 65.4 / 50.2;
-    16 / 16 of 64, 16 tokens 31.4 / 68.2; one sequence of 8, 16 / 2 of 256, 19.1 /
-    44.1."""
+    keys, or in tiles of 32 queries.  Over 6,000 keys, few / tiles, 64 columns: 12 sequences
+    of 8 tokens, 16 / 2 heads of 256, 45.6 / 101 us, 32 of them 73 / 135, one 19.6 / 40;
+    12 of 16, 16 / 4 of 128, 36.7 / 56.4; 32 of 64 tokens, 16 heads of 64, 170 / 154 (12 of 16,
+    16 columns, 29.8 / 61.6).  With 128 columns either wins: 16 tokens, 16 / 2 of 256, 12
+    sequences 67.3 / 70.3, 64 of 1,500 keys 89 / 64; 32 tokens, 16 / 4 of 128, 12
+    sequences 51.5 / 58.0, 32 of them 131 / 86; 128 tokens, 16 of 64, 32 sequences 322 / 178."""
     if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2 or q.shape[0] == 0 or most < 1:
         return False
     if block_tables.shape[0] < 1 or k_cache.shape[2] < 1 or q.shape[0] * q.shape[1] >= 2**30:
