@@ -181,3 +181,41 @@ def test_rows_that_see_no_key(dev, few):
     assert not o[:a].any() and o[a:new[0], :4].isnan().all() and not o[a:new[0], 4:].isnan().any()
     assert not o[new[0]:b].any() and not o[b:, :4].isnan().any() and not o[b, 4:].isnan().any()
     assert o[b + 1, 4:].isnan().all()
+
+
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", SHAPES)
+def test_other_forms(dev, Hq, Hkv, D, dtype):
+    """Capped and biased scores, sequences that share their first keys, a split prefill: over 16-bit caches."""
+    R, page = Hq // Hkv, 16
+    ctx = [700, 16 * 30 + 1, 2000, 33, 1]
+    c = make(ctx, [1] * 5, Hq, Hkv, D, dtype=dtype, seed=D, stale=False)
+    kc, vc = (cache_values(c[x + "c"], c[x + "s"]).to(dtype) for x in "kv")
+    q = c["q"].clone()
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    q[0, 0, 5], nan[0, 0] = NAN, True
+    for n, h, keys in ((2, 1, range(2000)), (1, 0, [480]), (3, 1, [32])):
+        for j in keys:
+            kc[int(c["tab"][n, j // page]), j % page, h, 7] = NAN
+        nan[n, h * R:(h + 1) * R] = True
+    d = [t.to(dev) for t in (q, kc, vc, c["tab"], c["ctx"])]
+    for kw in (dict(softcap=20.0), dict(alibi_slopes=torch.full((Hq,), 0.01, device=dev))):
+        for splits in SPLITS:
+            o = ops.paged_flash_attention_decode(*d, D**-0.5, page, num_splits=splits, **kw).cpu()
+            assert o[nan].isnan().all() and not o[~nan].isnan().any(), (kw, splits)
+    cu = torch.arange(6, dtype=torch.int32, device=dev)
+    o = ops.paged_flash_attention_prefill(*d, cu, None, D**-0.5, page).cpu()
+    assert o[nan].isnan().all() and not o[~nan].isnan().any()
+    # four sequences that share 32 keys; the last one's own keys of head 1 are all NaN
+    tab = torch.full((4, 20), -1, dtype=torch.int32)
+    tab[:, :2] = c["tab"][0, :2]
+    tab[0, 2:20], tab[1, 2:20], tab[2, 2:4], tab[3, 2:20] = (c["tab"][2, a:b] for a, b in ((4, 22), (24, 42), (44, 46), (48, 66)))
+    k = cache_values(c["kc"], c["ks"]).to(dtype)
+    k[tab[3, 2:].long(), :, 1, 3] = NAN
+    q = c["q"][:4].clone()
+    q[1, 2, 9] = NAN
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    nan[1, 2], nan[3, R:2 * R] = True, True
+    lens = torch.tensor([320, 300, 50, 311], dtype=torch.int32)
+    o = ops.paged_flash_attention_decode_shared(q.to(dev), k.to(dev), d[2], tab.to(dev), lens.to(dev),
+                                                torch.tensor([32], dtype=torch.int32, device=dev), D**-0.5, page).cpu()
+    assert o[nan].isnan().all() and not o[~nan].isnan().any()
