@@ -571,7 +571,8 @@ int paged_attention_few_fp4(const gdn_tensor* q, const gdn_tensor* k_cache, cons
 /*
  * Copies of blocks inside caches (no counterpart in the reference): in every layer of
  * each cache (layers, blocks, elements of a block), any type, block dst[i] <- block
- * src[i].  Up to four caches (NULL: none) of one number of blocks.
+ * src[i].  Up to four caches (NULL: none) of one number of blocks; blocks of a cache that
+ * overlap (an expanded view) are GDN_ERR_STRIDE.
  *   pairs (2, n) i32 in HOST memory, read before the call returns: the sources, then
  *   the places.  Places are distinct and none is a source (GDN_ERR_ARG); ids outside
  *   the caches are GDN_ERR_RANGE.

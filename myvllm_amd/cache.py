@@ -38,7 +38,7 @@ def cache_copy(caches: torch.Tensor | Sequence[torch.Tensor], src: Sequence[int]
     """Copies blocks inside caches, in place: in every layer of every cache
     (layers, blocks, ...), block ``dst[i]`` becomes block ``src[i]``; the step behind a
     fork or a compaction.  Any element type; the caches have one number of blocks,
-    and the elements of a block lie side by side.
+    the elements of a block lie side by side, and no two blocks overlap (an expanded view).
 
     ``src`` and ``dst`` are on the host (lists, CPU tensors or arrays of whole numbers),
     where a cache's allocator has them: they travel with the launch, and a captured

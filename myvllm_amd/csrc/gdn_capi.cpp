@@ -1137,6 +1137,20 @@ int check_pairs(const int32_t* src, const int32_t* dst, int64_t n, int64_t block
   }
   return GDN_OK;
 }
+
+// Whether the blocks of a cache (layers, blocks, elements) lie apart: copies between
+// overlapping ones would race.
+bool blocks_apart(const gdn_tensor* t) {
+  if (numel(t) == 0) return true;
+  int64_t span = t->shape[2];
+  const int inner = t->shape[0] <= 1 || (t->shape[1] > 1 && t->stride[1] <= t->stride[0]) ? 1 : 0;
+  for (const int d : {inner, 1 - inner}) {
+    if (t->shape[d] <= 1) continue;
+    if (t->stride[d] < span) return false;
+    span += (t->shape[d] - 1) * t->stride[d];
+  }
+  return true;
+}
 }  // namespace
 
 GDN_EXPORT int cache_copy(gdn_tensor* cache0, gdn_tensor* cache1, gdn_tensor* cache2, gdn_tensor* cache3,
@@ -1159,6 +1173,8 @@ GDN_EXPORT int cache_copy(gdn_tensor* cache0, gdn_tensor* cache1, gdn_tensor* ca
   }
   if (n == 0) return GDN_ERR_NULL;
   if (!cache_copy_fits(t, es, n, vec, pairs->shape[1])) return GDN_ERR_RANGE;
+  for (int i = 0; i < n; ++i)
+    if (!blocks_apart(t[i])) return GDN_ERR_STRIDE;
   const int32_t* src = reinterpret_cast<const int32_t*>(pairs->data);
   const int32_t* dst = src + pairs->stride[0];
   GDN_TRY(check_pairs(src, dst, pairs->shape[1], t[0]->shape[1]));

@@ -226,3 +226,19 @@ def test_copy_python_refusals():
         _pairs([2**31], [1])
     assert _pairs(torch.tensor([4, 5]), [6, 7]).tolist() == [[4, 5], [6, 7]]
     assert _pairs([], []).shape == (2, 0)
+
+
+@cpu_only
+def test_copy_of_overlapping_blocks():
+    """Blocks that share memory are refused (their copies would race); any order of layers and blocks is not."""
+    w = torch.zeros(4000)
+    none = torch.zeros(2, 0, dtype=torch.int32)
+    pairs = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32)
+    for size, stride in (((2, 6, 32), (192, 0, 1)), ((2, 6, 32), (0, 32, 1)), ((1, 6, 32), (0, 31, 1)),
+                         ((2, 6, 32), (191, 32, 1)), ((3, 6, 32), (32, 95, 1)), ((2, 6, 32), (31, 64, 1)), ((2, 2, 32), (32, 32, 1))):
+        t = w.as_strided(size, stride)
+        assert call([t], none) == call([t], pairs) == ERR["STRIDE"], stride
+        assert call([torch.zeros(2, size[1], 32), t], none) == ERR["STRIDE"]
+    for size, stride in (((2, 6, 32), (192, 32, 1)), ((2, 6, 32), (32, 64, 1)), ((1, 6, 32), (0, 32, 1)),
+                         ((3, 1, 32), (40, 0, 1)), ((2, 6, 32), (32, 70, 1)), ((2, 6, 0), (0, 0, 1)), ((1, 1, 32), (0, 0, 1))):
+        assert call([w.as_strided(size, stride)], none) == 0, stride
